@@ -580,7 +580,7 @@ __global__ __launch_bounds__(256) void fewin_conv_kernel(const GConvArgs a, int 
     for (int tl = 0; tl < tn; ++tl) {
       const int t = t0 + tl;
       const int ty = t / tw, tx = t - ty * tw;
-      // wc: this thread's 4 output channels for input channel c (vector x scalar FMAs: v_pk_fma_f32 pairs)
+      // wc: this thread's 4 output channels for input channel c (vector x scalar FMAs)
       const f32x4 w0 = Wl[(tl * 4 + 0) * 16 + q], w1 = Wl[(tl * 4 + 1) * 16 + q], w2 = Wl[(tl * 4 + 2) * 16 + q], w3 = Wl[(tl * 4 + 3) * 16 + q];
       const f32x4* xp = X + (ty * ph.dys - dyl) * lds_w + cx + tx * ph.dxs;
       const int xstep = a.isy * lds_w;
