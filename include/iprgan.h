@@ -34,7 +34,7 @@
 extern "C" {
 #endif
 
-#define IPRGAN_VERSION 226
+#define IPRGAN_VERSION 227
 
 enum { IPRGAN_ACT_NONE = 0, IPRGAN_ACT_RELU = 1, IPRGAN_ACT_LRELU = 2, IPRGAN_ACT_TANH = 3,
        IPRGAN_ACT_SIGMOID_PM1 = 4 };   /* sigmoid(x)*2-1: nn.Sigmoid + Decoder32.Normalize (networks/decoder.py:14-16,31-32) */
@@ -480,6 +480,51 @@ int iprgan_debug_force_splitk(int splits);
 #define IPRGAN_TUNE_RECORD_INTS 17
 int iprgan_tune_export(int* records, size_t cap_records, size_t* count);
 int iprgan_tune_import(const int* records, size_t n_records, int replace);
+
+/* ---- activation checkpoints in 8 bits (csrc/mx8.hip): what a pass keeps of an activation for its backward pass -----------------
+ * Microscaled blocks of 32 consecutive elements in memory order (the last one may be partial): int8 codes, one a element, and
+ * one E8M0 exponent byte a block.  m = max |x| of the block; e = floor(log2 m) - 6, one more when m * 2^-e >= 127.5, clamped to
+ * [-127, 121]; code = rint(x * 2^-e) (ties to even), scale byte = e + 127, value = code * 2^e.  Off by at most half a step
+ * 2^(e-1) <= m / 127.5 (above 127.5 * 2^121 an element saturates: less than one step).  A block that holds a NaN or an infinity
+ * stores scale byte 255 and reads back as NaN.  codes: n bytes, 16-byte aligned; scales: ceil(n / 32) bytes.
+ * kind / pstride: storage kind of the tensor (IPRGAN_ST_F32 / _BF16 / _X3) and plane stride of a three-plane one (0 = n). */
+int iprgan_mx8_quant(const void* x, void* codes, void* scales, size_t n, int kind, size_t pstride, void* stream);
+int iprgan_mx8_dequant(const void* codes, const void* scales, void* y, size_t n, int kind, size_t pstride, void* stream);
+/* dz = dy * act'(out), out read from its checkpoint (iprgan_act_bwd; dy and dz fp32 or bf16) */
+int iprgan_mx8_act_bwd(const void* dy, const void* codes, const void* scales, void* dz, size_t n, int act, float slope, int kind,
+                       size_t dy_pstride, size_t dz_pstride, void* stream);
+/* Norm backward with the layer's INPUT read from its checkpoint: iprgan_bn_bwd (G = 1), iprgan_instnorm_bwd (G = batch, M = HW;
+ * mean / invstd [G][C]), iprgan_bn_prelu_bwd (slope_dev: the PReLU slope on the device, dslope its gradient; act LRELU).  Activation none,
+ * ReLU or LeakyReLU: the mask gamma * (x - mean) * invstd + beta > 0 is one comparison of x with a threshold formed in 64 bits.
+ * gamma / beta (when there is an activation) and dgamma / dbeta: both or neither.  dx_kind = dy_kind, or three planes from an fp32 dy.  ws: 16-byte aligned,
+ * iprgan_mx8_norm_bwd_ws_floats(G, M, C) floats.  dbias_prev / dbias_n / dbias_beta as for iprgan_bn_bwd. */
+size_t iprgan_mx8_norm_bwd_ws_floats(int G, int M, int C);
+int iprgan_mx8_norm_bwd(const void* codes, const void* scales, const void* dy, const float* gamma, const float* beta,
+                        const float* save_mean, const float* save_invstd, const float* slope_dev, void* dx, float* dgamma,
+                        float* dbeta, float* dslope, float* ws, int G, int M, int C, int act, float slope, float* dbias_prev,
+                        int dbias_n, float dbias_beta, int dy_kind, size_t dy_pstride, int dx_kind, size_t dx_pstride, void* stream);
+
+/* ---- microscaled 4-bit floating point (csrc/mx4.hip): compressed weights and their product -----------------------------------
+ * A matrix [rows][cols] in blocks of 32 elements along a row: E2M1 codes (0, .5, 1, 1.5, 2, 3, 4, 6 and a sign), one E8M0
+ * exponent byte a block.  e = floor(log2 max|x|) - 2, one more when max|x| * 2^-e >= 7, clamped to [-127, 125]; round to nearest,
+ * ties to the even code.  A block that holds a NaN or an infinity stores scale byte 255 and reads back as NaN.  Rows are padded with
+ * zero codes to whole groups of 128 elements: KB = iprgan_mx4_pitch(cols) = 4 * ceil(cols / 128) blocks a row; codes
+ * [rows][KB * 16] bytes (element 2i in the low half of byte i; 16-byte aligned), scales [rows][KB] bytes (4-byte aligned). */
+int iprgan_mx4_pitch(int cols);
+int iprgan_mx4_quant(const void* x, void* codes, void* scales, int rows, int cols, int x_bf16, void* stream);
+int iprgan_mx4_dequant(const void* codes, const void* scales, void* y, int rows, int cols, int y_bf16, void* stream);
+/* y [M][N] = act(x W^T + bias), W [N][K] in 4 bits.  x [M][K]: fp32 (multiplied as three bf16 planes: products exact, fp32
+ * accumulation), bf16, or 4-bit itself (x = codes with K columns, x_scales; the scaled matrix instruction).  bias [N] fp32 or
+ * NULL; y fp32 or bf16, rounded once.  ws: 16-byte aligned, iprgan_mx4_linear_ws_floats floats (0: may be NULL); sums over a
+ * split K are added in fixed order. */
+enum { IPRGAN_X_F32 = 0, IPRGAN_X_BF16 = 1, IPRGAN_X_MX4 = 2 };
+size_t iprgan_mx4_linear_ws_floats(int M, int N, int K, int x_kind);
+int iprgan_mx4_linear(const void* x, const void* x_scales, const void* w_codes, const void* w_scales, const float* bias, void* y,
+                      float* ws, int M, int N, int K, int x_kind, int act, float slope, int y_bf16, void* stream);
+/* dx [M][K] = dy [M][N] W: the gradient with respect to x through the frozen 4-bit weights */
+size_t iprgan_mx4_linear_bwd_ws_floats(int M, int N, int K);
+int iprgan_mx4_linear_bwd(const void* dy, const void* w_codes, const void* w_scales, void* dx, float* ws, int M, int N, int K,
+                          int dy_bf16, int dx_bf16, void* stream);
 
 /* ---- misc elementwise ----------------------------------------------------------------------- */
 int iprgan_fill(float* p, float v, size_t n, void* stream);

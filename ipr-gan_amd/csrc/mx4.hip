@@ -1,0 +1,660 @@
+// Microscaled 4-bit floating point: quantisation, reading back, the product y = act(x W^T + b) with 4-bit weights, and the
+// product's gradient with respect to x.
+//
+// Format: blocks of 32 elements along a row, one E8M0 exponent byte a block, elements E2M1 (sign, 2 exponent bits, 1 mantissa
+// bit: 0, .5, 1, 1.5, 2, 3, 4, 6).  Rows are padded with zero codes to whole groups of 128 elements, so a row is KB = 4 *
+// ceil(cols / 128) blocks: KB * 16 bytes of codes (element 2i in the low half of byte i) and KB scale bytes - every block is 16 aligned
+// bytes, every 128 elements' scales one aligned word, and no kernel has a tail along K on its 4-bit operands.
+//   e = floor(log2 max|x|) - 2, one more when max|x| * 2^-e >= 7, clamped to [-127, 125]; round to nearest, ties to the even code
+// e is the smallest exponent for which nothing rounds past 6: an element is off by at most half the distance of its neighbours.
+// x * 2^-e is exact, so this is ONE rounding.  A block with a NaN or an infinity stores scale byte 255 and reads back as NaN.
+#include "common.h"
+
+namespace iprgan {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+// scale byte from the bit pattern of the largest magnitude; see mx8.hip for the same rule with 8-bit codes
+__device__ __forceinline__ unsigned mx4_scale(unsigned amax) {
+  if (amax >= 0x7f800000u) return 255u;
+  const int s = (int)(amax >> 23) - 2 + ((amax & 0x7fffffu) >= 0x600000u ? 1 : 0);
+  return (unsigned)(s < 0 ? 0 : s > 252 ? 252 : s);
+}
+__device__ __forceinline__ float mx4_inv(unsigned s) { return __uint_as_float((254u - s) << 23); }
+__device__ __forceinline__ float mx4_step(unsigned s) {
+  return __uint_as_float(s == 0 ? 0x00400000u : s == 255u ? 0x7fc00000u : s << 23);
+}
+
+// 8 consecutive elements of row `r` from column c on; zero behind the row's end.  VEC: rows start on 16 bytes and 8 elements never straddle an end
+template <bool BF, bool VEC>
+__device__ __forceinline__ void ld8(const void* base, size_t r, int ld, int c, float* v) {
+  if (VEC) {
+    if (c + 8 <= ld) {
+      if (BF) {
+        const bf16x8 h = *(const bf16x8*)((const __bf16*)base + r * ld + c);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = (float)h[k];
+      } else {
+        const float* p = (const float*)base + r * ld + c;
+        const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) { v[k] = a[k]; v[k + 4] = b[k]; }
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    v[k] = 0.f;
+    if (c + k < ld) v[k] = BF ? (float)((const __bf16*)base)[r * ld + c + k] : ((const float*)base)[r * ld + c + k];
+  }
+}
+
+// A thread owns 8 consecutive elements (4 bytes of codes); 4 neighbouring lanes share a block.  HBM-bound.
+template <bool BF, bool VEC>
+__global__ __launch_bounds__(256) void mx4_quant_kernel(const void* __restrict__ x, unsigned* __restrict__ codes,
+                                                        uint8_t* __restrict__ scales, unsigned groups, int cols, FastDiv d_row) {
+  const unsigned stride = gridDim.x * 256;
+  for (unsigned i = blockIdx.x * 256 + threadIdx.x; i < groups; i += stride) {       // groups % 16 == 0: a block's lanes stay together
+    const unsigned r = fdiv(i, d_row), c = (i - r * d_row.d) * 8;
+    float v[8];
+    ld8<BF, VEC>(x, r, cols, (int)c, v);
+    unsigned m = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const unsigned b = __float_as_uint(v[k]) & 0x7fffffffu;
+      m = b > m ? b : m;
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      const unsigned b = __shfl_xor(m, o, 64);
+      m = b > m ? b : m;
+    }
+    const unsigned s = mx4_scale(m);
+    unsigned w = 0;
+    if (s != 255u) {
+      const float inv = mx4_inv(s);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = fminf(fmaxf(v[k] * inv, -6.f), 6.f);       // (the clamp acts at the exponent cap only)
+      w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[0], v[1], 1.f, 0);
+      w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2], v[3], 1.f, 1);
+      w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[4], v[5], 1.f, 2);
+      w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[6], v[7], 1.f, 3);
+    }
+    codes[i] = w;
+    if ((i & 3) == 0) scales[i >> 2] = (uint8_t)s;
+  }
+}
+
+template <bool BF, bool VEC>
+__global__ __launch_bounds__(256) void mx4_dequant_kernel(const unsigned* __restrict__ codes, const uint8_t* __restrict__ scales,
+                                                          void* __restrict__ y, unsigned groups, int cols, FastDiv d_row) {
+  const unsigned stride = gridDim.x * 256;
+  for (unsigned i = blockIdx.x * 256 + threadIdx.x; i < groups; i += stride) {
+    const unsigned r = fdiv(i, d_row), c = (i - r * d_row.d) * 8;
+    if ((int)c >= cols) continue;
+    const unsigned w = codes[i];
+    const float step = mx4_step(scales[i >> 2]);
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 1),
+                p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 2), q = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 3);
+    const float v[8] = {a.x * step, a.y * step, b.x * step, b.y * step, p.x * step, p.y * step, q.x * step, q.y * step};
+    if (VEC && (int)c + 8 <= cols) {
+      if (BF) {
+        bf16x8 h;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) h[k] = (__bf16)v[k];
+        *(bf16x8*)((__bf16*)y + (size_t)r * cols + c) = h;
+      } else {
+        float* o = (float*)y + (size_t)r * cols + c;
+        const f32x4 lo = {v[0], v[1], v[2], v[3]}, hi = {v[4], v[5], v[6], v[7]};
+        *(f32x4*)o = lo;
+        *(f32x4*)(o + 4) = hi;
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if ((int)c + k >= cols) break;
+        if (BF) ((__bf16*)y)[(size_t)r * cols + c + k] = (__bf16)v[k];
+        else ((float*)y)[(size_t)r * cols + c + k] = v[k];
+      }
+    }
+  }
+}
+
+// ---- the product ---------------------------------------------------------------------------------------------------------------
+// Both forms compute the TRANSPOSED tile: the weights are the matrix instruction's first operand (its rows = output columns n), x is the
+// second (its columns = output rows m), so a lane's four results are four consecutive n of one row m: 16-byte fp32 or 8-byte bf16 stores.
+struct LinArgs {
+  const void* x;                 // [M][K] fp32 / bf16, or 4-bit codes
+  const uint8_t* xs;             // scales of a 4-bit x
+  const uint8_t *w, *ws;         // weights' codes [N][KB * 16] and scales [N][KB]
+  const float* bias;
+  void* y;
+  float* slab;                   // [splits][M][N] when the K axis is split
+  int M, N, K, KB, steps_per_split;      // a step is 128 elements of K
+  int act, y_bf16, vec_x, vec_y;
+  float slope;
+};
+
+__device__ __forceinline__ void store4(const LinArgs& a, int m, int n, f32x4 v) {
+  if (m >= a.M || n >= a.N) return;
+  if (a.slab) {
+    float* o = a.slab + ((size_t)blockIdx.z * a.M + m) * a.N + n;
+    if (a.vec_y) {
+      *(f32x4*)o = v;
+    } else {
+      for (int k = 0; k < 4 && n + k < a.N; ++k) o[k] = v[k];
+    }
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) v[k] = act_apply(v[k] + (a.bias && n + k < a.N ? a.bias[n + k] : 0.f), a.act, a.slope);
+  const size_t o = (size_t)m * a.N + n;
+  if (a.y_bf16) {
+    bf16x4 h;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) h[k] = (__bf16)v[k];
+    if (a.vec_y) {
+      *(bf16x4*)((__bf16*)a.y + o) = h;
+    } else {
+      for (int k = 0; k < 4 && n + k < a.N; ++k) ((__bf16*)a.y)[o + k] = h[k];
+    }
+  } else if (a.vec_y) {
+    *(f32x4*)((float*)a.y + o) = v;
+  } else {
+    for (int k = 0; k < 4 && n + k < a.N; ++k) ((float*)a.y)[o + k] = v[k];
+  }
+}
+
+// 8 fp4 elements (one word) of a block -> bf16, exact (a 4-bit value times a power of two)
+__device__ __forceinline__ bf16x8 widen_fp4(unsigned w, float scale) {
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1),
+               c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3);
+  const bf16x8 r = {a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+  return r;
+}
+__device__ __forceinline__ bf16x8 nan8() {
+  const __bf16 q = __builtin_bit_cast(__bf16, (unsigned short)0x7fc0);
+  const bf16x8 r = {q, q, q, q, q, q, q, q};
+  return r;
+}
+// x in PL bf16 planes: one (bf16 input) or three (fp32 input: x = h + m + l exactly, so the products with the exactly widened weights
+// are exact and only the fp32 accumulation rounds)
+template <int PL>
+__device__ __forceinline__ void split_planes(const float* v, bf16x8* p) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) p[0][k] = (__bf16)v[k];
+  if (PL == 3) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float r = v[k] - (float)p[0][k];
+      p[1][k] = (__bf16)r;
+      p[2][k] = (__bf16)(r - (float)p[1][k]);
+    }
+  }
+}
+
+// fp32 / bf16 x.  A block is 4 waves: each owns 16 * NF output columns (weights straight from memory to its registers: a lane reads
+// whole 16-byte blocks, lane group g block g of the step, and the step's four instructions take 8 elements of each block - the order of
+// K is free as long as both operands agree); the 16 * MF rows of x are shared through LDS, split into planes on the way in.
+template <int MF, int NF, int PL>
+__global__ __launch_bounds__(256) void mx4_linear_kernel(const LinArgs a) {
+  constexpr int XP = 136;                                   // LDS row pitch in bf16: 16 rows x 4-bank offset, conflict-free fragment reads
+  __shared__ __bf16 xs[2][PL][MF * 16][XP];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * 64 * NF + wave * 16 * NF, m0 = blockIdx.y * 16 * MF;
+  const int s0 = blockIdx.z * a.steps_per_split, s1 = min(a.KB / 4, s0 + a.steps_per_split);
+  const int xr = threadIdx.x >> 4, xc = (threadIdx.x & 15) * 8;
+  f32x4 acc[NF][MF];
+#pragma unroll
+  for (int n = 0; n < NF; ++n)
+#pragma unroll
+    for (int m = 0; m < MF; ++m) acc[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const u32x4* wp[NF];
+  const uint8_t* sp[NF];
+#pragma unroll
+  for (int n = 0; n < NF; ++n) {
+    const int row = min(n0 + n * 16 + i, a.N - 1);          // columns past N repeat the last row; their results are not stored
+    wp[n] = (const u32x4*)(a.w + (size_t)row * a.KB * 16) + g;
+    sp[n] = a.ws + (size_t)row * a.KB + g;
+  }
+  auto load_x = [&](int s, int t, float* v) {
+    const int m = m0 + xr + t * 16, c = s * 128 + xc;
+    if (m < a.M) {
+      if (a.vec_x) ld8<PL == 1, true>(a.x, m, a.K, c, v);
+      else ld8<PL == 1, false>(a.x, m, a.K, c, v);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = 0.f;
+    }
+  };
+  auto put_x = [&](int buf, int t, const float* v) {
+    bf16x8 p[PL];
+    split_planes<PL>(v, p);
+#pragma unroll
+    for (int q = 0; q < PL; ++q) *(bf16x8*)&xs[buf][q][xr + t * 16][xc] = p[q];
+  };
+  u32x4 wq[NF], wn[NF];
+  unsigned sq[NF], sn[NF];
+  float xv[MF][8];
+  if (s0 < s1) {
+#pragma unroll
+    for (int n = 0; n < NF; ++n) { wq[n] = wp[n][s0 * 4]; sq[n] = sp[n][s0 * 4]; }
+#pragma unroll
+    for (int t = 0; t < MF; ++t) { load_x(s0, t, xv[t]); put_x(0, t, xv[t]); }
+  }
+  __syncthreads();
+  for (int s = s0; s < s1; ++s) {
+    const int buf = (s - s0) & 1;
+    const bool more = s + 1 < s1;
+    if (more) {
+#pragma unroll
+      for (int n = 0; n < NF; ++n) { wn[n] = wp[n][(s + 1) * 4]; sn[n] = sp[n][(s + 1) * 4]; }
+#pragma unroll
+      for (int t = 0; t < MF; ++t) load_x(s + 1, t, xv[t]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      bf16x8 wf[NF];
+#pragma unroll
+      for (int n = 0; n < NF; ++n) {
+        wf[n] = widen_fp4(wq[n][j], mx4_step(sq[n]));
+        if (sq[n] == 255u) wf[n] = nan8();
+      }
+#pragma unroll
+      for (int q = PL - 1; q >= 0; --q)
+#pragma unroll
+        for (int m = 0; m < MF; ++m) {
+          const bf16x8 xf = *(const bf16x8*)&xs[buf][q][m * 16 + i][g * 32 + j * 8];
+#pragma unroll
+          for (int n = 0; n < NF; ++n) acc[n][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[n], xf, acc[n][m], 0, 0, 0);
+        }
+    }
+    if (more) {
+#pragma unroll
+      for (int t = 0; t < MF; ++t) put_x(buf ^ 1, t, xv[t]);
+#pragma unroll
+      for (int n = 0; n < NF; ++n) { wq[n] = wn[n]; sq[n] = sn[n]; }
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int n = 0; n < NF; ++n)
+#pragma unroll
+    for (int m = 0; m < MF; ++m) store4(a, m0 + m * 16 + i, n0 + n * 16 + g * 4, acc[n][m]);
+}
+
+// 4-bit x: the scaled matrix instruction multiplies 128 elements of K at once, one scale byte a lane and operand.
+__global__ __launch_bounds__(256) void mx4_linear4_kernel(const LinArgs a) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * 128 + (wave & 1) * 64, m0 = blockIdx.y * 128 + (wave >> 1) * 64;
+  const int s0 = blockIdx.z * a.steps_per_split, s1 = min(a.KB / 4, s0 + a.steps_per_split);
+  f32x4 acc[4][4];
+#pragma unroll
+  for (int n = 0; n < 4; ++n)
+#pragma unroll
+    for (int m = 0; m < 4; ++m) acc[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const i32x4 *wp[4], *xp[4];
+  const unsigned *wsp[4], *xsp[4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const size_t rn = min(n0 + t * 16 + i, a.N - 1), rm = min(m0 + t * 16 + i, a.M - 1);
+    wp[t] = (const i32x4*)(a.w + rn * a.KB * 16) + g;
+    xp[t] = (const i32x4*)((const uint8_t*)a.x + rm * a.KB * 16) + g;
+    wsp[t] = (const unsigned*)(a.ws + rn * a.KB);
+    xsp[t] = (const unsigned*)(a.xs + rm * a.KB);
+  }
+  for (int s = s0; s < s1; ++s) {
+    i32x8 wf[4], xf[4];
+    int wsc[4], xsc[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const i32x4 p = wp[t][s * 4], q = xp[t][s * 4];
+      wf[t] = i32x8{p[0], p[1], p[2], p[3], 0, 0, 0, 0};
+      xf[t] = i32x8{q[0], q[1], q[2], q[3], 0, 0, 0, 0};
+      wsc[t] = (int)(wsp[t][s] >> 8 * g);
+      xsc[t] = (int)(xsp[t][s] >> 8 * g);
+    }
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int m = 0; m < 4; ++m)
+        acc[n][m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[n], xf[m], acc[n][m], 4, 4, 0, wsc[n], 0, xsc[m]);
+  }
+#pragma unroll
+  for (int n = 0; n < 4; ++n)
+#pragma unroll
+    for (int m = 0; m < 4; ++m) store4(a, m0 + m * 16 + i, n0 + n * 16 + g * 4, acc[n][m]);
+}
+
+// out[m][n] = act(sum over the splits, in order, + bias[n])
+__global__ __launch_bounds__(256) void mx4_slab_reduce_kernel(const float* __restrict__ slab, int splits, size_t total, int N,
+                                                              const float* __restrict__ bias, void* __restrict__ out, int act,
+                                                              float slope, int out_bf16, int vec) {
+  const int V = vec ? 4 : 1;
+  const size_t e = ((size_t)blockIdx.x * 256 + threadIdx.x) * V;
+  if (e >= total) return;
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  if (vec) {
+    for (int z = 0; z < splits; ++z) s += *(const f32x4*)(slab + (size_t)z * total + e);
+  } else {
+    for (int z = 0; z < splits; ++z) s.x += slab[(size_t)z * total + e];
+  }
+  const int n = (int)(e % (size_t)N);
+  for (int k = 0; k < V; ++k) {
+    const float v = act_apply(s[k] + (bias ? bias[n + k] : 0.f), act, slope);
+    if (out_bf16) ((__bf16*)out)[e + k] = (__bf16)v;
+    else ((float*)out)[e + k] = v;
+  }
+}
+
+// ---- gradient with respect to x: dx[m][k] = sum_n dy[m][n] W[n][k] -----------------------------------------------------------------
+// The reduction runs along the rows of W, so a lane needs 8 rows' values of one k.  It reads one word (8 k) of each of its 8 rows,
+// widens them with the rows' scales and interleaves row pairs: the eight vectors it then holds are its operands for EIGHT instructions
+// j = 0..7, whose row i stands for k = 8 i + j - the 8 x 8 transposition costs 32 permutes and no LDS.  A wave covers 128 k; the
+// block's 4 waves split the rows n and add their tiles through LDS.  The lane's results over j are 8 consecutive k.
+struct BwdArgs {
+  const void* dy;
+  const uint8_t *w, *ws;
+  void* dx;
+  float* slab;                 // [splits][M][K] when the rows n are split over blocks
+  int M, N, K, KB, steps_per_wave, dx_bf16, vec_dy, vec_dx;       // a step is 32 rows of W
+};
+template <int MF, int PL>
+__global__ __launch_bounds__(256) void mx4_linear_bwd_kernel(const BwdArgs a) {
+  __shared__ float tile[4][16][132];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+  const int k0 = blockIdx.x * 128, m0 = blockIdx.y * 16 * MF;
+  const int steps = (a.N + 31) / 32;
+  const int s0 = (blockIdx.z * 4 + wave) * a.steps_per_wave, s1 = min(steps, s0 + a.steps_per_wave);
+  f32x4 acc[8][MF];
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+#pragma unroll
+    for (int m = 0; m < MF; ++m) acc[j][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int s = s0; s < s1; ++s) {
+    const int nb = s * 32 + g * 8;
+    unsigned wq[8], sc[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const size_t row = min(nb + r, a.N - 1);              // rows past N meet a zero of dy
+      wq[r] = *(const unsigned*)(a.w + row * a.KB * 16 + k0 / 2 + i * 4);
+      sc[r] = a.ws[row * a.KB + k0 / 32 + (i >> 2)];
+    }
+    bf16x8 xf[MF][PL];
+#pragma unroll
+    for (int m = 0; m < MF; ++m) {
+      float v[8];
+      const int mm = m0 + m * 16 + i;
+      if (mm < a.M) {
+        if (a.vec_dy) ld8<PL == 1, true>(a.dy, mm, a.N, nb, v);
+        else ld8<PL == 1, false>(a.dy, mm, a.N, nb, v);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = 0.f;
+      }
+      split_planes<PL>(v, xf[m]);
+    }
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      unsigned p[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        const float step = mx4_step(sc[r]);
+        bf16x2 t;
+        switch (b) {                                        // (the byte number is an immediate)
+          case 0: t = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(wq[r], step, 0); break;
+          case 1: t = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(wq[r], step, 1); break;
+          case 2: t = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(wq[r], step, 2); break;
+          default: t = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(wq[r], step, 3); break;
+        }
+        p[r] = sc[r] == 255u ? 0x7fc07fc0u : __builtin_bit_cast(unsigned, t);
+      }
+      u32x4 lo, hi;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        lo[r] = __builtin_amdgcn_perm(p[2 * r + 1], p[2 * r], 0x05040100u);
+        hi[r] = __builtin_amdgcn_perm(p[2 * r + 1], p[2 * r], 0x07060302u);
+      }
+      const bf16x8 wl = __builtin_bit_cast(bf16x8, lo), wh = __builtin_bit_cast(bf16x8, hi);
+#pragma unroll
+      for (int m = 0; m < MF; ++m)
+#pragma unroll
+        for (int q = PL - 1; q >= 0; --q) {
+          acc[2 * b][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wl, xf[m][q], acc[2 * b][m], 0, 0, 0);
+          acc[2 * b + 1][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wh, xf[m][q], acc[2 * b + 1][m], 0, 0, 0);
+        }
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < MF; ++m) {
+    if (m) __syncthreads();
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const f32x4 lo = {acc[0][m][r], acc[1][m][r], acc[2][m][r], acc[3][m][r]}, hi = {acc[4][m][r], acc[5][m][r], acc[6][m][r], acc[7][m][r]};
+      *(f32x4*)&tile[wave][i][8 * (g * 4 + r)] = lo;
+      *(f32x4*)&tile[wave][i][8 * (g * 4 + r) + 4] = hi;
+    }
+    __syncthreads();
+    const int mm = threadIdx.x >> 4, kk = (threadIdx.x & 15) * 8, row = m0 + m * 16 + mm, k = k0 + kk;
+    if (row < a.M && k < a.K) {
+      float v[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] = (tile[0][mm][kk + q] + tile[1][mm][kk + q]) + (tile[2][mm][kk + q] + tile[3][mm][kk + q]);
+      const size_t o = ((size_t)(a.slab ? blockIdx.z : 0) * a.M + row) * a.K + k;
+      if (a.slab || !a.dx_bf16) {
+        float* d = a.slab ? a.slab : (float*)a.dx;
+        if (a.vec_dx && k + 8 <= a.K) {
+          const f32x4 lo = {v[0], v[1], v[2], v[3]}, hi = {v[4], v[5], v[6], v[7]};
+          *(f32x4*)(d + o) = lo;
+          *(f32x4*)(d + o + 4) = hi;
+        } else {
+          for (int q = 0; q < 8 && k + q < a.K; ++q) d[o + q] = v[q];
+        }
+      } else {
+        bf16x8 h;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) h[q] = (__bf16)v[q];
+        if (a.vec_dx && k + 8 <= a.K) {
+          *(bf16x8*)((__bf16*)a.dx + o) = h;
+        } else {
+          for (int q = 0; q < 8 && k + q < a.K; ++q) ((__bf16*)a.dx)[o + q] = h[q];
+        }
+      }
+    }
+  }
+}
+
+static inline bool aligned(const void* p, unsigned a) { return ((uintptr_t)p & (a - 1)) == 0; }
+static inline int kb_of(int cols) { return 4 * cdiv(cols, 128); }
+
+static int slab_reduce(const float* slab, int splits, int M, int N, const float* bias, void* out, int act, float slope, int out_bf16,
+                       hipStream_t st) {
+  const size_t total = (size_t)M * N;
+  const int vec = N % 4 == 0;
+  const size_t blocks = cdivz(total, vec ? 1024 : 256);
+  IPR_CHECK(blocks < 0x7fffffffull, "mx4: %zu outputs are too many", total);
+  hipLaunchKernelGGL(mx4_slab_reduce_kernel, dim3((unsigned)blocks), dim3(256), 0, st, slab, splits, total, N, bias, out, act, slope, out_bf16, vec);
+  IPR_LAUNCH_CHECK();
+  return 0;
+}
+
+// how the product is cut: 16 * mf rows x 64 * nf columns a block (fp32 / bf16 x) or 128 x 128 (4-bit x), K over `splits` blocks
+struct LinPlan {
+  int mf, nf, tm, tn, splits, steps_per_split;
+};
+static LinPlan lin_plan(int M, int N, int K, int x_kind) {
+  LinPlan p;
+  const int steps = kb_of(K) / 4;
+  if (x_kind == IPRGAN_X_MX4) {
+    p.mf = p.nf = 4;
+    p.tm = cdiv(M, 128);
+    p.tn = cdiv(N, 128);
+  } else {
+    p.mf = M <= 16 ? 1 : M <= 32 ? 2 : 4;
+    p.nf = p.mf == 1 ? 1 : 2;
+    p.tm = cdiv(M, 16 * p.mf);
+    p.tn = cdiv(N, 64 * p.nf);
+  }
+  const long long tiles = (long long)p.tm * p.tn;
+  int want = tiles >= 512 ? 1 : (int)(512 / tiles);           // two blocks a CU
+  if (want > 64) want = 64;
+  if (want > steps) want = steps;
+  if (want < 1) want = 1;
+  p.steps_per_split = cdiv(steps, want);
+  p.splits = cdiv(steps, p.steps_per_split);
+  return p;
+}
+struct BwdPlan {
+  int mf, tm, tk, splits, steps_per_wave;
+};
+static BwdPlan bwd_plan(int M, int N, int K) {
+  BwdPlan p;
+  p.mf = M <= 16 ? 1 : 2;
+  p.tm = cdiv(M, 16 * p.mf);
+  p.tk = cdiv(K, 128);
+  const int steps = cdiv(N, 32);
+  const long long tiles = (long long)p.tm * p.tk;
+  int want = tiles >= 512 ? 1 : (int)(512 / tiles);
+  if (want > 64) want = 64;
+  if (want > cdiv(steps, 4)) want = cdiv(steps, 4);
+  if (want < 1) want = 1;
+  p.steps_per_wave = cdiv(steps, want * 4);
+  p.splits = cdiv(steps, p.steps_per_wave * 4);
+  return p;
+}
+
+}  // namespace iprgan
+
+using namespace iprgan;
+
+extern "C" {
+
+int iprgan_mx4_pitch(int cols) { return cols > 0 && cols <= 0x7fffff80 ? kb_of(cols) : 0; }
+
+static int mx4_rows_check(const char* who, int rows, int cols, unsigned* groups) {
+  IPR_CHECK(rows > 0 && cols > 0, "%s: empty input (%d rows of %d)", who, rows, cols);
+  const size_t g = (size_t)rows * cdivz((size_t)cols, 128) * 16;
+  IPR_CHECK(g < 0x7fff0000ull, "%s: %d rows of %d are too many elements", who, rows, cols);
+  *groups = (unsigned)g;
+  return 0;
+}
+
+int iprgan_mx4_quant(const void* x, void* codes, void* scales, int rows, int cols, int x_bf16, void* stream) {
+  unsigned groups;
+  if (mx4_rows_check("mx4_quant", rows, cols, &groups)) return 1;
+  IPR_CHECK(x && codes && scales, "mx4_quant: null operand");
+  IPR_CHECK(x_bf16 == 0 || x_bf16 == 1, "mx4_quant: storage kind %d (fp32 or bf16)", x_bf16);
+  IPR_CHECK(aligned(codes, 16) && aligned(scales, 4) && aligned(x, x_bf16 ? 2 : 4), "mx4_quant: codes must be 16-byte, scales 4-byte aligned");
+  const bool vec = cols % (x_bf16 ? 8 : 4) == 0 && aligned(x, 16);
+  auto k = x_bf16 ? (vec ? mx4_quant_kernel<true, true> : mx4_quant_kernel<true, false>)
+                  : (vec ? mx4_quant_kernel<false, true> : mx4_quant_kernel<false, false>);
+  const unsigned blocks = (groups + 255) / 256;
+  hipLaunchKernelGGL(k, dim3(blocks < 8192 ? blocks : 8192), dim3(256), 0, (hipStream_t)stream, x, (unsigned*)codes, (uint8_t*)scales,
+                     groups, cols, make_fastdiv((uint32_t)kb_of(cols) * 4));
+  IPR_LAUNCH_CHECK();
+  return 0;
+}
+
+int iprgan_mx4_dequant(const void* codes, const void* scales, void* y, int rows, int cols, int y_bf16, void* stream) {
+  unsigned groups;
+  if (mx4_rows_check("mx4_dequant", rows, cols, &groups)) return 1;
+  IPR_CHECK(y && codes && scales, "mx4_dequant: null operand");
+  IPR_CHECK(y_bf16 == 0 || y_bf16 == 1, "mx4_dequant: storage kind %d (fp32 or bf16)", y_bf16);
+  IPR_CHECK(aligned(codes, 16) && aligned(scales, 4) && aligned(y, y_bf16 ? 2 : 4), "mx4_dequant: codes must be 16-byte, scales 4-byte aligned");
+  const bool vec = cols % (y_bf16 ? 8 : 4) == 0 && aligned(y, 16);
+  auto k = y_bf16 ? (vec ? mx4_dequant_kernel<true, true> : mx4_dequant_kernel<true, false>)
+                  : (vec ? mx4_dequant_kernel<false, true> : mx4_dequant_kernel<false, false>);
+  const unsigned blocks = (groups + 255) / 256;
+  hipLaunchKernelGGL(k, dim3(blocks < 8192 ? blocks : 8192), dim3(256), 0, (hipStream_t)stream, (const unsigned*)codes,
+                     (const uint8_t*)scales, y, groups, cols, make_fastdiv((uint32_t)kb_of(cols) * 4));
+  IPR_LAUNCH_CHECK();
+  return 0;
+}
+
+static int lin_check(const char* who, int M, int N, int K) {
+  IPR_CHECK(M > 0 && N > 0 && K > 0, "%s: empty product (M=%d, N=%d, K=%d)", who, M, N, K);
+  IPR_CHECK(K <= (1 << 24) && M <= (1 << 20) && N <= (1 << 28), "%s: M=%d, N=%d, K=%d (at most 2^20, 2^28, 2^24)", who, M, N, K);
+  return 0;
+}
+
+size_t iprgan_mx4_linear_ws_floats(int M, int N, int K, int x_kind) {
+  if (M < 1 || N < 1 || K < 1) return 0;
+  const LinPlan p = lin_plan(M, N, K, x_kind);
+  return p.splits > 1 ? (size_t)p.splits * M * N : 0;
+}
+
+int iprgan_mx4_linear(const void* x, const void* x_scales, const void* w_codes, const void* w_scales, const float* bias, void* y,
+                      float* ws, int M, int N, int K, int x_kind, int act, float slope, int y_bf16, void* stream) {
+  if (lin_check("mx4_linear", M, N, K)) return 1;
+  IPR_CHECK(x_kind == IPRGAN_X_F32 || x_kind == IPRGAN_X_BF16 || x_kind == IPRGAN_X_MX4, "mx4_linear: kind %d of x", x_kind);
+  IPR_CHECK(x && w_codes && w_scales && y && (x_kind != IPRGAN_X_MX4 || x_scales), "mx4_linear: null operand");
+  IPR_CHECK(y_bf16 == 0 || y_bf16 == 1, "mx4_linear: storage kind %d of y (fp32 or bf16)", y_bf16);
+  IPR_CHECK(act >= IPRGAN_ACT_NONE && act <= IPRGAN_ACT_SIGMOID_PM1, "mx4_linear: activation %d", act);
+  IPR_CHECK(aligned(w_codes, 16) && aligned(w_scales, 4) && aligned(x, x_kind == IPRGAN_X_MX4 ? 16 : x_kind == IPRGAN_X_BF16 ? 2 : 4) &&
+                (x_kind != IPRGAN_X_MX4 || aligned(x_scales, 4)) && aligned(y, y_bf16 ? 2 : 4),
+            "mx4_linear: codes must be 16-byte, scales 4-byte aligned");
+  const LinPlan p = lin_plan(M, N, K, x_kind);
+  IPR_CHECK(p.tm <= 65535, "mx4_linear: M=%d", M);
+  IPR_CHECK(p.splits == 1 || (ws && aligned(ws, 16)), "mx4_linear: the workspace of iprgan_mx4_linear_ws_floats is missing");
+  hipStream_t st = (hipStream_t)stream;
+  LinArgs a;
+  a.x = x; a.xs = (const uint8_t*)x_scales; a.w = (const uint8_t*)w_codes; a.ws = (const uint8_t*)w_scales; a.bias = bias; a.y = y;
+  a.slab = p.splits > 1 ? ws : nullptr;
+  a.M = M; a.N = N; a.K = K; a.KB = kb_of(K); a.steps_per_split = p.steps_per_split;
+  a.act = act; a.slope = slope; a.y_bf16 = y_bf16;
+  a.vec_x = K % (x_kind == IPRGAN_X_BF16 ? 8 : 4) == 0 && aligned(x, 16);
+  a.vec_y = N % 4 == 0 && (a.slab || aligned(y, y_bf16 ? 8 : 16));
+  const dim3 grid(p.tn, p.tm, p.splits), blk(256);
+  if (x_kind == IPRGAN_X_MX4) {
+    hipLaunchKernelGGL(mx4_linear4_kernel, grid, blk, 0, st, a);
+  } else if (x_kind == IPRGAN_X_BF16) {
+    auto k = p.mf == 1 ? mx4_linear_kernel<1, 1, 1> : p.mf == 2 ? mx4_linear_kernel<2, 2, 1> : mx4_linear_kernel<4, 2, 1>;
+    hipLaunchKernelGGL(k, grid, blk, 0, st, a);
+  } else {
+    auto k = p.mf == 1 ? mx4_linear_kernel<1, 1, 3> : p.mf == 2 ? mx4_linear_kernel<2, 2, 3> : mx4_linear_kernel<4, 2, 3>;
+    hipLaunchKernelGGL(k, grid, blk, 0, st, a);
+  }
+  IPR_LAUNCH_CHECK();
+  return p.splits > 1 ? slab_reduce(ws, p.splits, M, N, bias, y, act, slope, y_bf16, st) : 0;
+}
+
+size_t iprgan_mx4_linear_bwd_ws_floats(int M, int N, int K) {
+  if (M < 1 || N < 1 || K < 1) return 0;
+  const BwdPlan p = bwd_plan(M, N, K);
+  return p.splits > 1 ? (size_t)p.splits * M * K : 0;
+}
+
+int iprgan_mx4_linear_bwd(const void* dy, const void* w_codes, const void* w_scales, void* dx, float* ws, int M, int N, int K,
+                          int dy_bf16, int dx_bf16, void* stream) {
+  if (lin_check("mx4_linear_bwd", M, N, K)) return 1;
+  IPR_CHECK(dy && w_codes && w_scales && dx, "mx4_linear_bwd: null operand");
+  IPR_CHECK((dy_bf16 == 0 || dy_bf16 == 1) && (dx_bf16 == 0 || dx_bf16 == 1), "mx4_linear_bwd: storage kinds %d, %d (fp32 or bf16)", dy_bf16, dx_bf16);
+  IPR_CHECK(aligned(w_codes, 16) && aligned(w_scales, 4) && aligned(dy, dy_bf16 ? 2 : 4) && aligned(dx, dx_bf16 ? 2 : 4),
+            "mx4_linear_bwd: codes must be 16-byte, scales 4-byte aligned");
+  const BwdPlan p = bwd_plan(M, N, K);
+  IPR_CHECK(p.tm <= 65535, "mx4_linear_bwd: M=%d", M);
+  IPR_CHECK(p.splits == 1 || (ws && aligned(ws, 16)), "mx4_linear_bwd: the workspace of iprgan_mx4_linear_bwd_ws_floats is missing");
+  hipStream_t st = (hipStream_t)stream;
+  BwdArgs a;
+  a.dy = dy; a.w = (const uint8_t*)w_codes; a.ws = (const uint8_t*)w_scales; a.dx = dx;
+  a.slab = p.splits > 1 ? ws : nullptr;
+  a.M = M; a.N = N; a.K = K; a.KB = kb_of(K); a.steps_per_wave = p.steps_per_wave; a.dx_bf16 = dx_bf16;
+  a.vec_dy = N % (dy_bf16 ? 8 : 4) == 0 && aligned(dy, 16);
+  a.vec_dx = K % (a.slab || !dx_bf16 ? 4 : 8) == 0 && (a.slab || aligned(dx, 16));
+  const dim3 grid(p.tk, p.tm, p.splits), blk(256);
+  auto k = dy_bf16 ? (p.mf == 1 ? mx4_linear_bwd_kernel<1, 1> : mx4_linear_bwd_kernel<2, 1>)
+                   : (p.mf == 1 ? mx4_linear_bwd_kernel<1, 3> : mx4_linear_bwd_kernel<2, 3>);
+  hipLaunchKernelGGL(k, grid, blk, 0, st, a);
+  IPR_LAUNCH_CHECK();
+  return p.splits > 1 ? slab_reduce(ws, p.splits, M, K, nullptr, dx, IPRGAN_ACT_NONE, 0.f, dx_bf16, st) : 0;
+}
+
+}  // extern "C"

@@ -134,6 +134,18 @@ SIGNATURES = {
     'iprgan_prof_get': (_I, [_I, C.c_char_p, _I, C.POINTER(C.c_longlong), C.POINTER(C.c_double), C.POINTER(C.c_double)]),
     'iprgan_prof_num_layers': (_I, []),
     'iprgan_prof_get_layer': (_I, [_I, C.c_char_p, _I, C.POINTER(C.c_longlong), C.POINTER(C.c_double), C.POINTER(C.c_double)]),
+    'iprgan_mx8_quant': (_I, [_P, _P, _P, _Z, _I, _Z, _P]),
+    'iprgan_mx8_dequant': (_I, [_P, _P, _P, _Z, _I, _Z, _P]),
+    'iprgan_mx8_act_bwd': (_I, [_P, _P, _P, _P, _Z, _I, _F, _I, _Z, _Z, _P]),
+    'iprgan_mx8_norm_bwd_ws_floats': (_Z, [_I, _I, _I]),
+    'iprgan_mx8_norm_bwd': (_I, [_P] * 13 + [_I, _I, _I, _I, _F, _P, _I, _F, _I, _Z, _I, _Z, _P]),
+    'iprgan_mx4_pitch': (_I, [_I]),
+    'iprgan_mx4_quant': (_I, [_P, _P, _P, _I, _I, _I, _P]),
+    'iprgan_mx4_dequant': (_I, [_P, _P, _P, _I, _I, _I, _P]),
+    'iprgan_mx4_linear_ws_floats': (_Z, [_I, _I, _I, _I]),
+    'iprgan_mx4_linear': (_I, [_P] * 7 + [_I, _I, _I, _I, _I, _F, _I, _P]),
+    'iprgan_mx4_linear_bwd_ws_floats': (_Z, [_I, _I, _I]),
+    'iprgan_mx4_linear_bwd': (_I, [_P] * 5 + [_I, _I, _I, _I, _I, _P]),
     'iprgan_fill': (_I, [_P, _F, _Z, _P]),
     'iprgan_axpy': (_I, [_P, _P, _F, _Z, _P]),
     'iprgan_axpy_multi': (_I, [_P, _P, _P, _I, _F, _P]),
@@ -281,6 +293,17 @@ def stream():
     if _raw_stream is not None:
         return _raw_stream(_cur_device())
     return torch.cuda.current_stream().cuda_stream
+
+
+def bptr(t, dtype):
+    """Device pointer of a contiguous byte tensor (codes, scales) of ``dtype``."""
+    if not t.is_cuda:
+        raise RuntimeError('iprgan kernels need GPU tensors (got a CPU tensor); there is no CPU path')
+    if t.dtype != dtype or not t.is_contiguous():
+        raise RuntimeError(f'this iprgan kernel argument must be a contiguous {dtype} tensor (got {t.dtype}, contiguous={t.is_contiguous()})')
+    if _acct is not None:
+        _acct_note(t)
+    return t.data_ptr()
 
 
 def ptr_table(tensors):

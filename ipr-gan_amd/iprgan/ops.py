@@ -163,6 +163,226 @@ def dquery(name, d, *extra):
     return v
 
 
+# ---- activation checkpoints in 8 bits (csrc/mx8.hip) ---------------------------------------------
+class Mx8:
+    """An activation kept in 8 bits: int8 ``codes`` (one an element, memory order) and uint8 E8M0 ``scales`` (one per 32
+    consecutive elements); value = code * 2^(scale - 127), scale 255 = NaN (include/iprgan.h: iprgan_mx8_quant).  ``kind`` is the
+    storage kind it is restored to.  The norm layers' backward passes and ``act_bwd`` take it in the place of the saved tensor."""
+    __slots__ = ('codes', 'scales', 'shape', 'kind')
+
+    def __init__(self, codes, scales, shape, kind=ST_F32):
+        shape = tuple(int(v) for v in shape)
+        n = 1
+        for v in shape:
+            n *= v
+        if codes.dtype != torch.int8 or scales.dtype != torch.uint8:
+            raise RuntimeError(f'Mx8: int8 codes and uint8 scales expected (got {codes.dtype}, {scales.dtype})')
+        if codes.numel() != n or scales.numel() != (n + 31) // 32:
+            raise RuntimeError(f'Mx8: {codes.numel()} codes and {scales.numel()} scales for a tensor of shape {shape}')
+        if codes.device != scales.device:
+            raise RuntimeError(f'Mx8: codes on {codes.device}, scales on {scales.device}')
+        if kind not in (ST_F32, ST_BF16, ST_X3):
+            raise RuntimeError(f'Mx8: storage kind {kind}')
+        self.codes, self.scales, self.shape, self.kind = codes, scales, shape, kind
+
+    @property
+    def dtype(self):
+        """dtype of the tensor it stands for (a three-plane tensor is its bf16 h plane)."""
+        return torch.float32 if self.kind == ST_F32 else torch.bfloat16
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def dim(self):
+        return len(self.shape)
+
+    def numel(self):
+        return self.codes.numel()
+
+    def view(self, *shape):
+        shape = shape[0] if len(shape) == 1 and not isinstance(shape[0], int) else shape
+        return Mx8(self.codes, self.scales, shape, self.kind)
+
+
+def _one_device(who, *tensors):
+    """All operands on the current device: the launch goes to ITS stream."""
+    cur = torch.cuda.current_device() if torch.cuda.is_available() else None
+    for t in tensors:
+        if t is None:
+            continue
+        if t.device.type != 'cuda':
+            raise RuntimeError(f'{who}: iprgan kernels need GPU tensors (got a CPU tensor); there is no CPU path')
+        if t.device.index != cur:
+            raise RuntimeError(f'{who}: operand on {t.device}, current device is cuda:{cur}')
+
+
+def _aligned(t):
+    """``t``, or a copy where a contiguous view starts off a 16-byte boundary (a row of an odd-sized tensor, a slice of a flat
+    buffer): the kernels use vector accesses.  Three-plane slices stay: their 8-byte form is the kernels' own."""
+    if t is None or t.data_ptr() % 16 == 0 or is16(t) == ST_X3:
+        return t
+    return t.clone()
+
+
+def mx8_quant(x):
+    """``x`` (any storage kind) saved in 8 bits."""
+    _one_device('mx8_quant', x)
+    if x.is_contiguous():
+        x = _aligned(x)
+    n = x.numel()
+    codes = torch.empty((n,), dtype=torch.int8, device=x.device)
+    scales = torch.empty(((n + 31) // 32,), dtype=torch.uint8, device=x.device)
+    k = is16(x)
+    call('iprgan_mx8_quant', ptr(x), L.bptr(codes, torch.int8), L.bptr(scales, torch.uint8), n, k, pstride(x), stream())
+    return Mx8(codes, scales, x.shape, k)
+
+
+def mx8_dequant(q, kind=None):
+    """The saved activation in storage kind ``kind`` (default: the kind it was saved from).  bf16 and three planes are exact."""
+    _one_device('mx8_dequant', q)
+    k = q.kind if kind is None else kind
+    y = empty_kind(q.shape, q, k)
+    call('iprgan_mx8_dequant', L.bptr(q.codes, torch.int8), L.bptr(q.scales, torch.uint8), ptr(y), q.numel(), k, pstride(y), stream())
+    return y
+
+
+def _mx8_norm_bwd(q, dy, gamma, beta, mean, invstd, act, slope, groups, slope_t=None, want_params=True, dbias=None, dbias_beta=0.0):
+    """Norm backward with the layer's input read from its checkpoint: (dx, dgamma, dbeta, dslope)."""
+    C_ = q.shape[-1]
+    M = q.numel() // max(1, C_ * groups)
+    if tuple(dy.shape) != q.shape:
+        raise RuntimeError(f'norm backward: checkpoint of shape {q.shape}, gradient of shape {tuple(dy.shape)}')
+    for t, n in ((gamma, C_), (beta, C_), (mean, groups * C_), (invstd, groups * C_)):
+        if t is not None and t.numel() != n:
+            raise RuntimeError(f'norm backward: a parameter or statistic has {t.numel()} values, {n} expected')
+    _one_device('norm backward', q, dy, gamma, beta, mean, invstd, slope_t, dbias)
+    dy, gamma, beta, mean, invstd = (t if t is None or not t.is_contiguous() else _aligned(t) for t in (dy, gamma, beta, mean, invstd))
+    k = is16(dy)
+    splits = q.kind == ST_X3 or (q.kind == ST_F32 and _NORM_DYF32 and _norm_splits_here(q))
+    kx = ST_X3 if (k == ST_F32 and L.act_x3() and splits) else k
+    dx = empty_kind(dy.shape, dy, kx)
+    dgamma = empty((C_,), mean) if want_params else None
+    dbeta = empty((C_,), mean) if want_params else None
+    dslope = empty((1,), mean) if slope_t is not None else None
+    ws = scratch(query('iprgan_mx8_norm_bwd_ws_floats', groups, M, C_), mean)
+    call('iprgan_mx8_norm_bwd', L.bptr(q.codes, torch.int8), L.bptr(q.scales, torch.uint8), ptr(dy), ptr32(gamma), ptr32(beta),
+         ptr32(mean), ptr32(invstd), ptr32(slope_t), ptr(dx), ptr(dgamma), ptr(dbeta), ptr(dslope), ptr(ws), groups, M, C_, act,
+         float(slope), ptr32(dbias), dbias.numel() if dbias is not None else 0, float(dbias_beta), k, pstride(dy), kx, pstride(dx),
+         stream())
+    return _out(dx), dgamma, dbeta, dslope
+
+
+# ---- microscaled 4-bit weights (csrc/mx4.hip) ------------------------------------------------------
+class Mx4:
+    """A matrix of shape (rows, cols) in 4-bit floating point: uint8 ``codes`` [rows, KB * 16] (element 2i in the low half of
+    byte i) and uint8 E8M0 ``scales`` [rows, KB], KB = 4 * ceil(cols / 128) blocks of 32 a row (include/iprgan.h:
+    iprgan_mx4_quant).  0.53 bytes an element."""
+    __slots__ = ('codes', 'scales', 'shape')
+
+    def __init__(self, codes, scales, shape):
+        rows, cols = (int(v) for v in shape)
+        kb = 4 * ((cols + 127) // 128)
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+            raise RuntimeError(f'Mx4: uint8 codes and scales expected (got {codes.dtype}, {scales.dtype})')
+        if codes.numel() != rows * kb * 16 or scales.numel() != rows * kb:
+            raise RuntimeError(f'Mx4: {codes.numel()} bytes of codes and {scales.numel()} scales for a ({rows}, {cols}) matrix: '
+                               f'{rows * kb * 16} and {rows * kb} expected')
+        if codes.device != scales.device:
+            raise RuntimeError(f'Mx4: codes on {codes.device}, scales on {scales.device}')
+        self.codes, self.scales, self.shape = codes, scales, (rows, cols)
+
+    @property
+    def device(self):
+        return self.codes.device
+
+
+def mx4_quant(x):
+    """A matrix (or a tensor seen as [shape[0], rest]) rounded to 4 bits; fp32 or bf16."""
+    _one_device('mx4_quant', x)
+    x = f32(x) if is16(x) == ST_X3 else x
+    if x.dim() < 1 or x.numel() == 0:
+        raise RuntimeError(f'mx4_quant: empty input of shape {tuple(x.shape)}')
+    rows, cols = x.shape[0], x.numel() // x.shape[0]
+    kb = query('iprgan_mx4_pitch', cols)
+    codes = torch.empty((rows, kb * 16), dtype=torch.uint8, device=x.device)
+    scales = torch.empty((rows, kb), dtype=torch.uint8, device=x.device)
+    call('iprgan_mx4_quant', ptr(x), L.bptr(codes, torch.uint8), L.bptr(scales, torch.uint8), rows, cols, is16(x), stream())
+    return Mx4(codes, scales, (rows, cols))
+
+
+def _mx4_out_kind(who, dtype):
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise RuntimeError(f'{who}: float32 or bfloat16 results (got {dtype})')
+    if dtype == torch.bfloat16 and L.act_x3():
+        raise RuntimeError(f'{who}: a bfloat16 result would be taken for three planes in this math mode (ask for float32, then to_kind)')
+    return 1 if dtype == torch.bfloat16 else 0
+
+
+def mx4_dequant(q, dtype=torch.float32):
+    """The values of a 4-bit matrix as float32 or bfloat16 (both exact) [rows, cols]."""
+    _one_device('mx4_dequant', q)
+    k = _mx4_out_kind('mx4_dequant', dtype)
+    y = empty(q.shape, q, dtype)
+    call('iprgan_mx4_dequant', L.bptr(q.codes, torch.uint8), L.bptr(q.scales, torch.uint8), ptr(y), q.shape[0], q.shape[1], k, stream())
+    return y
+
+
+X_MX4 = 2           # include/iprgan.h: IPRGAN_X_MX4
+
+
+def mx4_linear(x, w, bias=None, act=L.ACT_NONE, slope=0.0, dtype=None):
+    """y = act(x W^T + bias): ``w`` an Mx4 of shape (N, K); ``x`` [..., K] fp32 or bf16 (unrounded: fp32 goes through three bf16
+    planes) or an Mx4 of shape (M, K).  y in ``dtype`` (default: x's; float32 for a 4-bit x)."""
+    if not isinstance(w, Mx4):
+        raise RuntimeError('mx4_linear: the weights must be an Mx4 (mx4_quant)')
+    N, K = w.shape
+    if not isinstance(x, Mx4) and is16(x) == ST_X3:
+        x = f32(x)
+    if x.shape[-1] != K or len(x.shape) < 1:
+        raise RuntimeError(f'mx4_linear: x of shape {tuple(x.shape)} against weights of shape {w.shape}')
+    if bias is not None and bias.numel() != N:
+        raise RuntimeError(f'mx4_linear: {bias.numel()} bias values for {N} columns')
+    _one_device('mx4_linear', x, w, bias)
+    if isinstance(x, Mx4):
+        lead, M, k, dtype = (x.shape[0],), x.shape[0], X_MX4, torch.float32 if dtype is None else dtype
+        xp, xsp = L.bptr(x.codes, torch.uint8), L.bptr(x.scales, torch.uint8)
+    else:
+        lead, M, k, dtype = tuple(x.shape[:-1]), x.numel() // K, is16(x), x.dtype if dtype is None else dtype
+        xp, xsp = ptr(x), None
+    y = empty(lead + (N,), x, dtype)
+    ky = _mx4_out_kind('mx4_linear', dtype)
+    nws = query('iprgan_mx4_linear_ws_floats', M, N, K, k)
+    ws = scratch(nws, x) if nws else None
+    L.acct_flops(2.0 * M * N * K)
+    call('iprgan_mx4_linear', xp, xsp, L.bptr(w.codes, torch.uint8), L.bptr(w.scales, torch.uint8), ptr32(bias), ptr(y), ptr(ws),
+         M, N, K, k, act, float(slope), ky, stream())
+    return y
+
+
+def mx4_linear_bwd(dy, w, dtype=None):
+    """dx = dy W: the gradient with respect to x through the frozen 4-bit weights; dy [..., N] fp32 or bf16, dx in ``dtype``
+    (default: dy's)."""
+    if not isinstance(w, Mx4):
+        raise RuntimeError('mx4_linear_bwd: the weights must be an Mx4 (mx4_quant)')
+    N, K = w.shape
+    if is16(dy) == ST_X3:
+        dy = f32(dy)
+    if dy.dim() < 1 or dy.shape[-1] != N:
+        raise RuntimeError(f'mx4_linear_bwd: dy of shape {tuple(dy.shape)} against weights of shape {w.shape}')
+    _one_device('mx4_linear_bwd', dy, w)
+    dtype = dy.dtype if dtype is None else dtype
+    M = dy.numel() // N
+    dx = empty(tuple(dy.shape[:-1]) + (K,), dy, dtype)
+    kx = _mx4_out_kind('mx4_linear_bwd', dtype)
+    nws = query('iprgan_mx4_linear_bwd_ws_floats', M, N, K)
+    ws = scratch(nws, dy) if nws else None
+    L.acct_flops(2.0 * M * N * K)
+    call('iprgan_mx4_linear_bwd', ptr(dy), L.bptr(w.codes, torch.uint8), L.bptr(w.scales, torch.uint8), ptr(dx), ptr(ws), M, N, K,
+         is16(dy), kx, stream())
+    return dx
+
+
 # ---- layout ---------------------------------------------------------------------------------
 def nchw_to_nhwc(x):
     _f32(x)
@@ -189,6 +409,16 @@ def permute_021(src, A, Bd, K, out=None, beta=0.0):
 
 
 def act_bwd(dy, out, act, slope=0.0):
+    """dz = dy * act'(out); ``out`` may be its 8-bit checkpoint (Mx8)."""
+    if isinstance(out, Mx8):
+        if tuple(dy.shape) != out.shape and dy.numel() != out.numel():
+            raise RuntimeError(f'act_bwd: checkpoint of shape {out.shape}, gradient of shape {tuple(dy.shape)}')
+        _one_device('act_bwd', dy, out)
+        dy = f32(dy) if is16(dy) == ST_X3 else _aligned(dy) if dy.is_contiguous() else dy
+        dz = _empty_like(dy)
+        call('iprgan_mx8_act_bwd', ptr(dy), L.bptr(out.codes, torch.int8), L.bptr(out.scales, torch.uint8), ptr(dz), dy.numel(), act,
+             float(slope), is16(dy), 0, 0, stream())
+        return dz
     if ST_X3 in (is16(dy), is16(out)):          # (no three-plane form: a stand-alone activation backward is rare)
         dy, out = f32(dy), f32(out)
     if dy.dtype != out.dtype:
@@ -598,7 +828,9 @@ def bn_fwd(x, gamma, beta, running_mean, running_var, eps, momentum, training, a
 
 def bn_bwd(x, y, dy, gamma, mean, invstd, act, slope=0.0, beta=None, dbias=None, dbias_beta=0.0):
     """dbias: a tensor that receives (beta-accumulates) the column sums of dx = the bias gradient of the convolution
-    that produced x."""
+    that produced x.  ``x`` may be its 8-bit checkpoint (Mx8; activation none, ReLU or LeakyReLU, ``y`` is not read)."""
+    if isinstance(x, Mx8):
+        return _mx8_norm_bwd(x, dy, gamma, beta, mean, invstd, act, slope, 1, dbias=dbias, dbias_beta=dbias_beta)[:3]
     C_ = x.shape[-1]
     M = x.numel() // C_
     st, dy, y = _norm_bwd_kinds(x, dy, y)
@@ -633,6 +865,9 @@ def bn_prelu_fwd(x, gamma, beta, running_mean, running_var, eps, momentum, train
 
 
 def bn_prelu_bwd(x, dy, gamma, beta, mean, invstd, slope_t, dbias=None, dbias_beta=0.0):
+    """(dx, dgamma, dbeta, dslope); ``x`` may be its 8-bit checkpoint (Mx8)."""
+    if isinstance(x, Mx8):
+        return _mx8_norm_bwd(x, dy, gamma, beta, mean, invstd, L.ACT_LRELU, 0.0, 1, slope_t=slope_t, dbias=dbias, dbias_beta=dbias_beta)
     C_ = x.shape[-1]
     M = x.numel() // C_
     st, dy, _ = _norm_bwd_kinds(x, dy)
@@ -892,6 +1127,10 @@ def instnorm_fwd(x, gamma, beta, eps, act, slope=0.0, conv_stats=None, conv_bias
 
 
 def instnorm_bwd(x, y, dy, gamma, mean, invstd, act, slope=0.0, beta=None, dbias=None, dbias_beta=0.0):
+    """(dx, dgamma, dbeta), the latter None without affine parameters; ``x`` may be its 8-bit checkpoint (Mx8)."""
+    if isinstance(x, Mx8):
+        return _mx8_norm_bwd(x, dy, gamma, beta, mean, invstd, act, slope, x.shape[0], want_params=gamma is not None, dbias=dbias,
+                             dbias_beta=dbias_beta)[:3]
     B, H, W, C_ = x.shape
     st, dy, y = _norm_bwd_kinds(x, dy, y)
     dx = empty_kind(dy.shape, dy, ST_X3) if st == ST_X3_XDF32 else _empty_like(dy)

@@ -1,0 +1,78 @@
+"""Plain CPU forms of the microscaled formats (csrc/mx8.hip, csrc/mx4.hip) in float64: what the tests compare against."""
+import torch
+
+LEVELS = torch.tensor([0., .5, 1., 1.5, 2., 3., 4., 6.], dtype=torch.float64)
+
+
+def exponents(amax, half_open, cap):
+    """Smallest e in [-127, cap] with amax < half_open * 2^e (half_open: where rounding would pass the largest code)."""
+    e = torch.full(amax.shape, -127, dtype=torch.int64)
+    for v in range(-127, cap):                                   # counting up, not a logarithm: exact and independent
+        e += (amax >= half_open * 2.0 ** v).long() * (e == v).long()
+    return e
+
+
+def mx8_encode(x):
+    """float32 / bfloat16 tensor -> (codes int8 [n], scales uint8 [ceil(n / 32)])"""
+    v = x.detach().cpu().double().reshape(-1)
+    n = v.numel()
+    p = torch.zeros(-(-n // 32) * 32, dtype=torch.float64)
+    p[:n] = v
+    p = p.view(-1, 32)
+    bad = ~torch.isfinite(p).all(1)
+    p = torch.where(bad[:, None], torch.zeros_like(p), p)
+    e = exponents(p.abs().amax(1), 127.5, 121)
+    q = torch.round(p * torch.exp2(-e.double())[:, None]).clamp(-127, 127)        # torch.round: ties to even
+    s = torch.where(bad, torch.full_like(e, 255), e + 127)
+    return q.view(-1)[:n].to(torch.int8), s.to(torch.uint8)
+
+
+def mx8_decode(codes, scales):
+    """-> float64 [n]"""
+    n = codes.numel()
+    step = torch.exp2(scales.double() - 127)
+    step[scales == 255] = float('nan')
+    return codes.double() * step.repeat_interleave(32)[:n]
+
+
+def mx4_encode(x):
+    """[R, C] -> (codes uint8 [R, KB * 16], scales uint8 [R, KB])"""
+    x = x.detach().cpu().double()
+    r, c = x.shape
+    p = torch.zeros(r, -(-c // 128) * 128, dtype=torch.float64)
+    p[:, :c] = x
+    p = p.view(r, -1, 32)
+    bad = ~torch.isfinite(p).all(2)
+    p = torch.where(bad[..., None], torch.zeros_like(p), p)
+    e = exponents(p.abs().amax(2), 7.0, 125)
+    y = p * torch.exp2(-e.double())[..., None]
+    a = y.abs()
+    idx = torch.zeros(a.shape, dtype=torch.int64)
+    for i in range(1, 8):
+        mid = (LEVELS[i - 1] + LEVELS[i]) / 2
+        idx += (a >= mid).long() if i % 2 == 0 else (a > mid).long()       # a tie goes to the even code
+    nib = (idx | (torch.signbit(y).long() << 3)).view(r, -1, 2)
+    s = torch.where(bad, torch.full_like(e, 255), e + 127)
+    return (nib[..., 0] | (nib[..., 1] << 4)).to(torch.uint8), s.to(torch.uint8)
+
+
+def mx4_decode(codes, scales, cols):
+    """-> float64 [R, cols]"""
+    lut = torch.cat([LEVELS, -LEVELS])
+    c = codes.cpu().long()
+    v = torch.stack([lut[c & 15], lut[c >> 4]], 2).view(c.shape[0], -1, 32)
+    step = torch.exp2(scales.cpu().double() - 127)
+    step[scales.cpu() == 255] = float('nan')
+    return (v * step[..., None]).reshape(c.shape[0], -1)[:, :cols]
+
+
+def act(v, kind, slope):
+    if kind == 1:
+        return torch.where(v > 0, v, torch.zeros_like(v))
+    if kind == 2:
+        return torch.where(v > 0, v, v * slope)
+    if kind == 3:
+        return torch.tanh(v)
+    if kind == 4:
+        return torch.sigmoid(v) * 2 - 1
+    return v

@@ -1,0 +1,116 @@
+"""CPU: refusals of the microscaled operators (their C entries check before they launch) and the checks of their containers."""
+import ctypes as C
+
+import pytest
+import torch
+
+from iprgan import _lib as L
+from iprgan import ops
+
+P = C.c_void_p(4096)            # a non-null, aligned address: every call below is refused before anything is launched
+ODD = C.c_void_p(4096 + 8)
+
+
+def refused(name, *args):
+    with pytest.raises(RuntimeError, match=name):
+        L.call(name, *args)
+
+
+def test_mx8_entries_refuse_bad_calls():
+    refused('iprgan_mx8_quant', P, P, P, 0, 0, 0, None)
+    refused('iprgan_mx8_quant', None, P, P, 8, 0, 0, None)
+    refused('iprgan_mx8_quant', ODD, P, P, 8, 0, 0, None)
+    refused('iprgan_mx8_quant', P, P, P, 8, 3, 0, None)
+    refused('iprgan_mx8_quant', P, P, P, 8, 2, 4, None)
+    refused('iprgan_mx8_dequant', P, P, P, 0, 0, 0, None)
+    refused('iprgan_mx8_dequant', P, P, ODD, 8, 0, 0, None)
+    refused('iprgan_mx8_dequant', P, P, P, 8, 2, 6, None)
+    refused('iprgan_mx8_act_bwd', P, P, P, P, 8, 1, 0.0, 2, 0, 0, None)
+    refused('iprgan_mx8_act_bwd', P, P, P, P, 0, 1, 0.0, 0, 0, 0, None)
+
+
+def norm(codes=P, dy=P, gamma=P, beta=P, slope=None, dx=P, dgamma=P, dbeta=P, dslope=None, ws=P, G=1, M=8, C_=8, act=1, dbias=None, nb=0,
+         kd=0, kx=0):
+    return ('iprgan_mx8_norm_bwd', codes, P, dy, gamma, beta, P, P, slope, dx, dgamma, dbeta, dslope, ws, G, M, C_, act, 0.1, dbias, nb, 0.0,
+            kd, 0, kx, 0, None)
+
+
+@pytest.mark.parametrize('bad', [dict(M=0), dict(G=0), dict(C_=6), dict(codes=None), dict(ws=None), dict(dx=ODD), dict(act=3), dict(beta=None),
+                                 dict(gamma=None, act=0), dict(dbeta=None), dict(dslope=P), dict(slope=P, act=1), dict(dslope=P, slope=P, act=2, G=2),
+                                 dict(kd=1, kx=0), dict(kd=5, kx=5), dict(dbias=P, nb=9), dict(G=70000)])
+def test_norm_backward_refuses(bad):
+    refused(*norm(**bad))
+
+
+def test_mx4_entries_refuse_bad_calls():
+    assert L.query('iprgan_mx4_pitch', 1) == 4 and L.query('iprgan_mx4_pitch', 129) == 8 and L.query('iprgan_mx4_pitch', 0) == 0
+    refused('iprgan_mx4_quant', P, P, P, 0, 4, 0, None)
+    refused('iprgan_mx4_quant', P, P, P, 4, 0, 0, None)
+    refused('iprgan_mx4_quant', P, ODD, P, 4, 4, 0, None)
+    refused('iprgan_mx4_quant', P, P, P, 4, 4, 2, None)
+    refused('iprgan_mx4_quant', P, P, P, 1 << 30, 1 << 10, 0, None)
+    refused('iprgan_mx4_dequant', P, P, None, 4, 4, 0, None)
+    lin = lambda *a: ('iprgan_mx4_linear',) + a
+    refused(*lin(P, None, P, P, None, P, P, 0, 8, 8, 0, 0, 0.0, 0, None))
+    refused(*lin(P, None, P, P, None, P, P, 8, 8, 0, 0, 0, 0.0, 0, None))
+    refused(*lin(P, None, P, P, None, P, P, 8, 8, 8, 2, 0, 0.0, 0, None))            # a 4-bit x without scales
+    refused(*lin(P, None, P, P, None, P, P, 8, 8, 8, 3, 0, 0.0, 0, None))
+    refused(*lin(P, None, P, P, None, P, P, 8, 8, 8, 0, 9, 0.0, 0, None))
+    refused(*lin(P, None, ODD, P, None, P, P, 8, 8, 8, 0, 0, 0.0, 0, None))
+    refused(*lin(P, None, P, P, None, P, P, 8, 8, 8, 0, 0, 0.0, 2, None))
+    refused(*lin(P, None, P, P, None, P, None, 4, 64, 8192, 0, 0, 0.0, 0, None))      # a split K needs its workspace
+    refused('iprgan_mx4_linear_bwd', P, P, P, P, P, 8, 0, 8, 0, 0, None)
+    refused('iprgan_mx4_linear_bwd', P, P, P, None, P, 8, 8, 8, 0, 0, None)
+    refused('iprgan_mx4_linear_bwd', P, P, P, P, None, 4, 8192, 64, 0, 0, None)
+
+
+def test_workspace_sizes():
+    assert L.query('iprgan_mx4_linear_ws_floats', 0, 8, 8, 0) == 0
+    assert L.query('iprgan_mx4_linear_ws_floats', 4, 64, 8192, 0) % (4 * 64) == 0
+    assert L.query('iprgan_mx8_norm_bwd_ws_floats', 1, 100, 64) >= 5 * 64
+    assert L.query('iprgan_mx8_norm_bwd_ws_floats', 0, 100, 64) == 0
+
+
+def test_containers_refuse_what_does_not_fit():
+    c8, s8 = torch.zeros(70, dtype=torch.int8), torch.zeros(3, dtype=torch.uint8)
+    q = ops.Mx8(c8, s8, (2, 35))
+    assert q.shape == (2, 35) and q.numel() == 70 and q.dim() == 2 and q.dtype == torch.float32
+    assert q.view(7, 10).shape == (7, 10) and q.view((70,)).shape == (70,)
+    for codes, scales, shape in ((c8, s8, (2, 36)), (c8, s8[:2], (70,)), (c8.int(), s8, (70,)), (c8, s8.int(), (70,))):
+        with pytest.raises(RuntimeError, match='Mx8'):
+            ops.Mx8(codes, scales, shape)
+    with pytest.raises(RuntimeError, match='Mx8'):
+        ops.Mx8(c8, s8, (70,), kind=3)
+    c4, s4 = torch.zeros(3, 64, dtype=torch.uint8), torch.zeros(3, 4, dtype=torch.uint8)
+    assert ops.Mx4(c4, s4, (3, 100)).shape == (3, 100)
+    for codes, scales, shape in ((c4, s4, (3, 129)), (c4, s4, (2, 100)), (c4.int(), s4, (3, 100)), (c4, s4[:, :3], (3, 100))):
+        with pytest.raises(RuntimeError, match='Mx4'):
+            ops.Mx4(codes, scales, shape)
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.zeros(4, 32)
+    w4 = ops.Mx4(torch.zeros(3, 64, dtype=torch.uint8), torch.zeros(3, 4, dtype=torch.uint8), (3, 32))
+    q = ops.Mx8(torch.zeros(128, dtype=torch.int8), torch.zeros(4, dtype=torch.uint8), (4, 32))
+    for f in (lambda: ops.mx8_quant(x), lambda: ops.mx8_dequant(q), lambda: ops.mx4_quant(x), lambda: ops.mx4_dequant(w4),
+              lambda: ops.mx4_linear(x, w4), lambda: ops.mx4_linear_bwd(torch.zeros(4, 3), w4), lambda: ops.act_bwd(x, q, 1),
+              lambda: ops.bn_bwd(q, None, x, None, torch.zeros(32), torch.zeros(32), 0)):
+        with pytest.raises(RuntimeError, match='GPU tensors'):
+            f()
+
+
+def test_shapes_are_checked():
+    w4 = ops.Mx4(torch.zeros(3, 64, dtype=torch.uint8), torch.zeros(3, 4, dtype=torch.uint8), (3, 32))
+    with pytest.raises(RuntimeError, match='mx4_linear'):
+        ops.mx4_linear(torch.zeros(4, 33), w4)
+    with pytest.raises(RuntimeError, match='mx4_linear'):
+        ops.mx4_linear(torch.zeros(4, 32), torch.zeros(3, 32))
+    with pytest.raises(RuntimeError, match='bias'):
+        ops.mx4_linear(torch.zeros(4, 32), w4, torch.zeros(4))
+    with pytest.raises(RuntimeError, match='mx4_linear_bwd'):
+        ops.mx4_linear_bwd(torch.zeros(4, 32), w4)
+    q = ops.Mx8(torch.zeros(128, dtype=torch.int8), torch.zeros(4, dtype=torch.uint8), (4, 32))
+    with pytest.raises(RuntimeError, match='norm backward'):
+        ops.bn_bwd(q, None, torch.zeros(4, 31), None, torch.zeros(32), torch.zeros(32), 0)
+    with pytest.raises(RuntimeError, match='norm backward'):
+        ops.bn_bwd(q, None, torch.zeros(4, 32), torch.zeros(31), torch.zeros(32), torch.zeros(32), 0)
