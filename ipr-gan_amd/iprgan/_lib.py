@@ -295,17 +295,6 @@ def stream():
     return torch.cuda.current_stream().cuda_stream
 
 
-def bptr(t, dtype):
-    """Device pointer of a contiguous byte tensor (codes, scales) of ``dtype``."""
-    if not t.is_cuda:
-        raise RuntimeError('iprgan kernels need GPU tensors (got a CPU tensor); there is no CPU path')
-    if t.dtype != dtype or not t.is_contiguous():
-        raise RuntimeError(f'this iprgan kernel argument must be a contiguous {dtype} tensor (got {t.dtype}, contiguous={t.is_contiguous()})')
-    if _acct is not None:
-        _acct_note(t)
-    return t.data_ptr()
-
-
 def ptr_table(tensors):
     arr = (C.c_void_p * len(tensors))()
     for i, t in enumerate(tensors):

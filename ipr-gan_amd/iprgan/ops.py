@@ -163,12 +163,82 @@ def dquery(name, d, *extra):
     return v
 
 
+# ---- microscaled storage: what both formats share ---------------------------------------------------
+# The small calls of these operators are host-bound (a launch costs 2-3 us on the device, the first version of these wrappers
+# 10-17 us a call): one allocation for codes and scales, containers built without re-checking what a kernel just wrote, and size
+# queries answered from a dict.
+def _new(shape, like, dtype):
+    """empty() from anything with a .device, without its argument handling."""
+    if _POISON and dtype.is_floating_point:
+        return torch.full(shape if isinstance(shape, tuple) else (shape,), float('nan'), dtype=dtype, device=like.device)
+    return torch.empty(shape, dtype=dtype, device=like.device)
+
+
+def _one_device(who, first, *rest):
+    """All operands on the current device: the launch goes to ITS stream."""
+    d = first.get_device()
+    for t in rest:
+        if t is not None and t.get_device() != d:
+            raise RuntimeError(f'{who}: iprgan kernels need GPU tensors of one device (got {first.device} and {t.device}); there is no CPU path')
+    if d < 0:
+        raise RuntimeError(f'{who}: iprgan kernels need GPU tensors (got a CPU tensor); there is no CPU path')
+    if d != (L._cur_device() if L._cur_device is not None else torch.cuda.current_device()):
+        raise RuntimeError(f'{who}: operands on cuda:{d}, which is not the current device')
+
+
+def _vptr(t, keep):
+    """ptr() for vector accesses: a contiguous view that starts off a 16-byte boundary (a row of an odd-sized tensor, a slice of a
+    flat buffer) is copied; the copy lives in ``keep`` until the launch is enqueued.  (Three-plane tensors stay: a copy of the h plane
+    alone would not be one; their kernels accept 8 bytes.)"""
+    if t is None:
+        return None
+    p = ptr(t)
+    if p & 15 and is16(t) != ST_X3:
+        t = t.clone()
+        keep.append(t)
+        p = t.data_ptr()
+    return p
+
+
+class _Packed:
+    """Codes and scales of a quantised tensor: two tensors handed in by the caller, or one buffer a kernel wrote (codes, then
+    the scales at the next multiple of 16)."""
+    __slots__ = ('_codes', '_scales', '_buf', '_split', 'shape', '_dev')
+
+    def _adopt(self, codes, scales):
+        for t in (codes, scales):
+            if not t.is_contiguous():
+                raise RuntimeError(f'{type(self).__name__}: contiguous codes and scales expected')
+        if codes.device != scales.device:
+            raise RuntimeError(f'{type(self).__name__}: codes on {codes.device}, scales on {scales.device}')
+        self._codes, self._scales, self._buf, self._dev = codes, scales, None, codes.get_device()
+
+    @property
+    def device(self):
+        return (self._codes if self._buf is None else self._buf).device
+
+    def get_device(self):
+        return self._dev
+
+    def ptrs(self):
+        """(codes, scales) as device pointers."""
+        if self._buf is None:
+            c, s = self._codes, self._scales
+            if L._acct is not None:
+                L._acct_note(c), L._acct_note(s)
+            return c.data_ptr(), s.data_ptr()
+        if L._acct is not None:
+            L._acct_note(self._buf)
+        p = self._buf.data_ptr()
+        return p, p + self._split
+
+
 # ---- activation checkpoints in 8 bits (csrc/mx8.hip) ---------------------------------------------
-class Mx8:
+class Mx8(_Packed):
     """An activation kept in 8 bits: int8 ``codes`` (one an element, memory order) and uint8 E8M0 ``scales`` (one per 32
     consecutive elements); value = code * 2^(scale - 127), scale 255 = NaN (include/iprgan.h: iprgan_mx8_quant).  ``kind`` is the
     storage kind it is restored to.  The norm layers' backward passes and ``act_bwd`` take it in the place of the saved tensor."""
-    __slots__ = ('codes', 'scales', 'shape', 'kind')
+    __slots__ = ('kind', '_n')
 
     def __init__(self, codes, scales, shape, kind=ST_F32):
         shape = tuple(int(v) for v in shape)
@@ -179,106 +249,128 @@ class Mx8:
             raise RuntimeError(f'Mx8: int8 codes and uint8 scales expected (got {codes.dtype}, {scales.dtype})')
         if codes.numel() != n or scales.numel() != (n + 31) // 32:
             raise RuntimeError(f'Mx8: {codes.numel()} codes and {scales.numel()} scales for a tensor of shape {shape}')
-        if codes.device != scales.device:
-            raise RuntimeError(f'Mx8: codes on {codes.device}, scales on {scales.device}')
         if kind not in (ST_F32, ST_BF16, ST_X3):
             raise RuntimeError(f'Mx8: storage kind {kind}')
-        self.codes, self.scales, self.shape, self.kind = codes, scales, shape, kind
+        self._adopt(codes, scales)
+        self.shape, self.kind, self._n = shape, kind, n
+
+    @property
+    def codes(self):
+        return self._codes if self._buf is None else self._buf[:self._n].view(torch.int8)
+
+    @property
+    def scales(self):
+        return self._scales if self._buf is None else self._buf[self._split:]
 
     @property
     def dtype(self):
         """dtype of the tensor it stands for (a three-plane tensor is its bf16 h plane)."""
         return torch.float32 if self.kind == ST_F32 else torch.bfloat16
 
-    @property
-    def device(self):
-        return self.codes.device
-
     def dim(self):
         return len(self.shape)
 
     def numel(self):
-        return self.codes.numel()
+        return self._n
 
     def view(self, *shape):
-        shape = shape[0] if len(shape) == 1 and not isinstance(shape[0], int) else shape
-        return Mx8(self.codes, self.scales, shape, self.kind)
-
-
-def _one_device(who, *tensors):
-    """All operands on the current device: the launch goes to ITS stream."""
-    cur = torch.cuda.current_device() if torch.cuda.is_available() else None
-    for t in tensors:
-        if t is None:
-            continue
-        if t.device.type != 'cuda':
-            raise RuntimeError(f'{who}: iprgan kernels need GPU tensors (got a CPU tensor); there is no CPU path')
-        if t.device.index != cur:
-            raise RuntimeError(f'{who}: operand on {t.device}, current device is cuda:{cur}')
-
-
-def _aligned(t):
-    """``t``, or a copy where a contiguous view starts off a 16-byte boundary (a row of an odd-sized tensor, a slice of a flat
-    buffer): the kernels use vector accesses.  Three-plane slices stay: their 8-byte form is the kernels' own."""
-    if t is None or t.data_ptr() % 16 == 0 or is16(t) == ST_X3:
-        return t
-    return t.clone()
+        """The same codes under another shape of as many elements."""
+        shape = tuple(int(v) for v in (shape[0] if len(shape) == 1 and not isinstance(shape[0], int) else shape))
+        n = 1
+        for v in shape:
+            n *= v
+        if n != self._n:
+            raise RuntimeError(f'Mx8: {self._n} elements seen as {shape}')
+        q = object.__new__(Mx8)
+        q._codes, q._scales, q._buf, q._split, q._dev = (None, None, self._buf, self._split, self._dev) if self._buf is not None \
+            else (self._codes, self._scales, None, 0, self._dev)
+        q.shape, q.kind, q._n = shape, self.kind, n
+        return q
 
 
 def mx8_quant(x):
     """``x`` (any storage kind) saved in 8 bits."""
     _one_device('mx8_quant', x)
-    if x.is_contiguous():
-        x = _aligned(x)
-    n = x.numel()
-    codes = torch.empty((n,), dtype=torch.int8, device=x.device)
-    scales = torch.empty(((n + 31) // 32,), dtype=torch.uint8, device=x.device)
-    k = is16(x)
-    call('iprgan_mx8_quant', ptr(x), L.bptr(codes, torch.int8), L.bptr(scales, torch.uint8), n, k, pstride(x), stream())
-    return Mx8(codes, scales, x.shape, k)
+    keep = []
+    p, n, k = _vptr(x, keep), x.numel(), is16(x)
+    split = (n + 15) & ~15
+    q = object.__new__(Mx8)
+    q._buf = buf = torch.empty(split + (n + 31) // 32, dtype=torch.uint8, device=x.device)
+    q._codes = q._scales = None
+    q._split, q._dev, q.shape, q.kind, q._n = split, x.get_device(), tuple(x.shape), k, n
+    c = buf.data_ptr()
+    if L._acct is not None:
+        L._acct_note(buf)
+    call('iprgan_mx8_quant', p, c, c + split, n, k, pstride(x) if k == ST_X3 else 0, stream())
+    return q
 
 
 def mx8_dequant(q, kind=None):
     """The saved activation in storage kind ``kind`` (default: the kind it was saved from).  bf16 and three planes are exact."""
+    if not isinstance(q, Mx8):
+        raise RuntimeError('mx8_dequant: an Mx8 (mx8_quant) expected')
     _one_device('mx8_dequant', q)
     k = q.kind if kind is None else kind
-    y = empty_kind(q.shape, q, k)
-    call('iprgan_mx8_dequant', L.bptr(q.codes, torch.int8), L.bptr(q.scales, torch.uint8), ptr(y), q.numel(), k, pstride(y), stream())
+    y = empty_kind(q.shape, q, k) if k == ST_X3 else _new(q.shape, q, torch.float32 if k == ST_F32 else torch.bfloat16)
+    c, s = q.ptrs()
+    call('iprgan_mx8_dequant', c, s, ptr(y), q._n, k, pstride(y) if k == ST_X3 else 0, stream())
     return y
+
+
+_wsq = {}
+
+
+def _ws_floats(*key):
+    """A workspace-size query (entry point, sizes): a pure function, asked of the library once."""
+    v = _wsq.get(key)
+    if v is None:
+        if len(_wsq) > 4096:
+            _wsq.clear()
+        v = _wsq[key] = query(*key)
+    return v
 
 
 def _mx8_norm_bwd(q, dy, gamma, beta, mean, invstd, act, slope, groups, slope_t=None, want_params=True, dbias=None, dbias_beta=0.0):
     """Norm backward with the layer's input read from its checkpoint: (dx, dgamma, dbeta, dslope)."""
     C_ = q.shape[-1]
-    M = q.numel() // max(1, C_ * groups)
-    if tuple(dy.shape) != q.shape:
+    M = q._n // (C_ * groups) if C_ * groups else 0
+    if dy.shape != q.shape:
         raise RuntimeError(f'norm backward: checkpoint of shape {q.shape}, gradient of shape {tuple(dy.shape)}')
-    for t, n in ((gamma, C_), (beta, C_), (mean, groups * C_), (invstd, groups * C_)):
-        if t is not None and t.numel() != n:
-            raise RuntimeError(f'norm backward: a parameter or statistic has {t.numel()} values, {n} expected')
+    if mean.numel() != groups * C_ or invstd.numel() != groups * C_ or (gamma is not None and gamma.numel() != C_) \
+            or (beta is not None and beta.numel() != C_):
+        raise RuntimeError(f'norm backward: a parameter or statistic does not fit {groups} group(s) of {C_} channels')
     _one_device('norm backward', q, dy, gamma, beta, mean, invstd, slope_t, dbias)
-    dy, gamma, beta, mean, invstd = (t if t is None or not t.is_contiguous() else _aligned(t) for t in (dy, gamma, beta, mean, invstd))
     k = is16(dy)
-    splits = q.kind == ST_X3 or (q.kind == ST_F32 and _NORM_DYF32 and _norm_splits_here(q))
-    kx = ST_X3 if (k == ST_F32 and L.act_x3() and splits) else k
-    dx = empty_kind(dy.shape, dy, kx)
-    dgamma = empty((C_,), mean) if want_params else None
-    dbeta = empty((C_,), mean) if want_params else None
-    dslope = empty((1,), mean) if slope_t is not None else None
-    ws = scratch(query('iprgan_mx8_norm_bwd_ws_floats', groups, M, C_), mean)
-    call('iprgan_mx8_norm_bwd', L.bptr(q.codes, torch.int8), L.bptr(q.scales, torch.uint8), ptr(dy), ptr32(gamma), ptr32(beta),
-         ptr32(mean), ptr32(invstd), ptr32(slope_t), ptr(dx), ptr(dgamma), ptr(dbeta), ptr(dslope), ptr(ws), groups, M, C_, act,
-         float(slope), ptr32(dbias), dbias.numel() if dbias is not None else 0, float(dbias_beta), k, pstride(dy), kx, pstride(dx),
-         stream())
+    kx = k
+    if k == ST_F32 and L.act_x3() and (q.kind == ST_X3 or (q.kind == ST_F32 and _NORM_DYF32 and _norm_splits_here(q))):
+        kx = ST_X3
+    keep = []
+    pdy = _vptr(dy, keep)
+    for t in (gamma, beta, mean, invstd):
+        if t is not None and t.dtype != torch.float32:
+            raise RuntimeError(f'this iprgan kernel argument must be float32 (got {t.dtype})')
+    dx = empty_kind(dy.shape, dy, kx) if kx == ST_X3 else _new(q.shape, dy, dy.dtype)
+    dgamma = dbeta = dslope = None
+    if want_params:
+        dgamma, dbeta = _new((2, (C_ + 3) & ~3), mean, torch.float32).unbind(0)      # (C_ % 4 == 0: two rows of one allocation)
+    if slope_t is not None:
+        dslope = _new((1,), mean, torch.float32)
+    nws = _ws_floats('iprgan_mx8_norm_bwd_ws_floats', groups, M, C_)
+    ws = L.acct_scratch(_new(nws, mean, torch.float32))
+    c, s = q.ptrs()
+    call('iprgan_mx8_norm_bwd', c, s, pdy, _vptr(gamma, keep), _vptr(beta, keep), _vptr(mean, keep), _vptr(invstd, keep), ptr32(slope_t),
+         ptr(dx), ptr(dgamma), ptr(dbeta), ptr(dslope), ws.data_ptr(), groups, M, C_, act, float(slope), ptr32(dbias),
+         dbias.numel() if dbias is not None else 0, float(dbias_beta), k, pstride(dy) if k == ST_X3 else 0, kx,
+         pstride(dx) if kx == ST_X3 else 0, stream())
     return _out(dx), dgamma, dbeta, dslope
 
 
 # ---- microscaled 4-bit weights (csrc/mx4.hip) ------------------------------------------------------
-class Mx4:
+class Mx4(_Packed):
     """A matrix of shape (rows, cols) in 4-bit floating point: uint8 ``codes`` [rows, KB * 16] (element 2i in the low half of
     byte i) and uint8 E8M0 ``scales`` [rows, KB], KB = 4 * ceil(cols / 128) blocks of 32 a row (include/iprgan.h:
     iprgan_mx4_quant).  0.53 bytes an element."""
-    __slots__ = ('codes', 'scales', 'shape')
+    __slots__ = ()
 
     def __init__(self, codes, scales, shape):
         rows, cols = (int(v) for v in shape)
@@ -288,43 +380,61 @@ class Mx4:
         if codes.numel() != rows * kb * 16 or scales.numel() != rows * kb:
             raise RuntimeError(f'Mx4: {codes.numel()} bytes of codes and {scales.numel()} scales for a ({rows}, {cols}) matrix: '
                                f'{rows * kb * 16} and {rows * kb} expected')
-        if codes.device != scales.device:
-            raise RuntimeError(f'Mx4: codes on {codes.device}, scales on {scales.device}')
-        self.codes, self.scales, self.shape = codes, scales, (rows, cols)
+        self._adopt(codes, scales)
+        self.shape = (rows, cols)
 
     @property
-    def device(self):
-        return self.codes.device
+    def codes(self):
+        return self._codes if self._buf is None else self._buf[:self._split].view(self.shape[0], -1)
+
+    @property
+    def scales(self):
+        return self._scales if self._buf is None else self._buf[self._split:].view(self.shape[0], -1)
 
 
 def mx4_quant(x):
     """A matrix (or a tensor seen as [shape[0], rest]) rounded to 4 bits; fp32 or bf16."""
     _one_device('mx4_quant', x)
-    x = f32(x) if is16(x) == ST_X3 else x
-    if x.dim() < 1 or x.numel() == 0:
-        raise RuntimeError(f'mx4_quant: empty input of shape {tuple(x.shape)}')
-    rows, cols = x.shape[0], x.numel() // x.shape[0]
-    kb = query('iprgan_mx4_pitch', cols)
-    codes = torch.empty((rows, kb * 16), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((rows, kb), dtype=torch.uint8, device=x.device)
-    call('iprgan_mx4_quant', ptr(x), L.bptr(codes, torch.uint8), L.bptr(scales, torch.uint8), rows, cols, is16(x), stream())
-    return Mx4(codes, scales, (rows, cols))
+    k = is16(x)
+    if k == ST_X3:
+        x, k = f32(x), ST_F32
+    n = x.numel()
+    if n == 0 or x.dim() < 1:
+        raise RuntimeError(f'mx4_quant: a matrix expected (got shape {tuple(x.shape)})')
+    rows = x.shape[0]
+    cols = n // rows
+    kb = 4 * ((cols + 127) // 128)
+    split = rows * kb * 16
+    q = object.__new__(Mx4)
+    q._buf = buf = torch.empty(split + rows * kb, dtype=torch.uint8, device=x.device)
+    q._codes = q._scales = None
+    q._split, q._dev, q.shape = split, x.get_device(), (rows, cols)
+    c = buf.data_ptr()
+    if L._acct is not None:
+        L._acct_note(buf)
+    call('iprgan_mx4_quant', ptr(x), c, c + split, rows, cols, k, stream())
+    return q
 
 
 def _mx4_out_kind(who, dtype):
-    if dtype not in (torch.float32, torch.bfloat16):
+    if dtype is torch.float32:
+        return 0
+    if dtype is not torch.bfloat16:
         raise RuntimeError(f'{who}: float32 or bfloat16 results (got {dtype})')
-    if dtype == torch.bfloat16 and L.act_x3():
+    if L.act_x3():
         raise RuntimeError(f'{who}: a bfloat16 result would be taken for three planes in this math mode (ask for float32, then to_kind)')
-    return 1 if dtype == torch.bfloat16 else 0
+    return 1
 
 
 def mx4_dequant(q, dtype=torch.float32):
     """The values of a 4-bit matrix as float32 or bfloat16 (both exact) [rows, cols]."""
+    if not isinstance(q, Mx4):
+        raise RuntimeError('mx4_dequant: an Mx4 (mx4_quant) expected')
     _one_device('mx4_dequant', q)
     k = _mx4_out_kind('mx4_dequant', dtype)
-    y = empty(q.shape, q, dtype)
-    call('iprgan_mx4_dequant', L.bptr(q.codes, torch.uint8), L.bptr(q.scales, torch.uint8), ptr(y), q.shape[0], q.shape[1], k, stream())
+    y = _new(q.shape, q, dtype)
+    c, s = q.ptrs()
+    call('iprgan_mx4_dequant', c, s, ptr(y), q.shape[0], q.shape[1], k, stream())
     return y
 
 
@@ -337,26 +447,32 @@ def mx4_linear(x, w, bias=None, act=L.ACT_NONE, slope=0.0, dtype=None):
     if not isinstance(w, Mx4):
         raise RuntimeError('mx4_linear: the weights must be an Mx4 (mx4_quant)')
     N, K = w.shape
-    if not isinstance(x, Mx4) and is16(x) == ST_X3:
-        x = f32(x)
-    if x.shape[-1] != K or len(x.shape) < 1:
+    quantised = isinstance(x, Mx4)
+    k = X_MX4 if quantised else is16(x)
+    if k == ST_X3 and not quantised:
+        x, k = f32(x), ST_F32
+    if len(x.shape) < 1 or x.shape[-1] != K:
         raise RuntimeError(f'mx4_linear: x of shape {tuple(x.shape)} against weights of shape {w.shape}')
     if bias is not None and bias.numel() != N:
         raise RuntimeError(f'mx4_linear: {bias.numel()} bias values for {N} columns')
     _one_device('mx4_linear', x, w, bias)
-    if isinstance(x, Mx4):
-        lead, M, k, dtype = (x.shape[0],), x.shape[0], X_MX4, torch.float32 if dtype is None else dtype
-        xp, xsp = L.bptr(x.codes, torch.uint8), L.bptr(x.scales, torch.uint8)
+    if quantised:
+        M = x.shape[0]
+        shape = (M, N)
+        dtype = torch.float32 if dtype is None else dtype
+        xp, xsp = x.ptrs()
     else:
-        lead, M, k, dtype = tuple(x.shape[:-1]), x.numel() // K, is16(x), x.dtype if dtype is None else dtype
+        M = x.numel() // K
+        shape = (M, N) if x.dim() == 2 else tuple(x.shape[:-1]) + (N,)
+        dtype = x.dtype if dtype is None else dtype
         xp, xsp = ptr(x), None
-    y = empty(lead + (N,), x, dtype)
     ky = _mx4_out_kind('mx4_linear', dtype)
-    nws = query('iprgan_mx4_linear_ws_floats', M, N, K, k)
-    ws = scratch(nws, x) if nws else None
+    y = _new(shape, x, dtype)
+    nws = _ws_floats('iprgan_mx4_linear_ws_floats', M, N, K, k)
+    ws = L.acct_scratch(_new(nws, x, torch.float32)) if nws else None
     L.acct_flops(2.0 * M * N * K)
-    call('iprgan_mx4_linear', xp, xsp, L.bptr(w.codes, torch.uint8), L.bptr(w.scales, torch.uint8), ptr32(bias), ptr(y), ptr(ws),
-         M, N, K, k, act, float(slope), ky, stream())
+    wc, wsc = w.ptrs()
+    call('iprgan_mx4_linear', xp, xsp, wc, wsc, ptr32(bias), ptr(y), ptr(ws), M, N, K, k, act, float(slope), ky, stream())
     return y
 
 
@@ -366,20 +482,21 @@ def mx4_linear_bwd(dy, w, dtype=None):
     if not isinstance(w, Mx4):
         raise RuntimeError('mx4_linear_bwd: the weights must be an Mx4 (mx4_quant)')
     N, K = w.shape
-    if is16(dy) == ST_X3:
-        dy = f32(dy)
+    k = is16(dy)
+    if k == ST_X3:
+        dy, k = f32(dy), ST_F32
     if dy.dim() < 1 or dy.shape[-1] != N:
         raise RuntimeError(f'mx4_linear_bwd: dy of shape {tuple(dy.shape)} against weights of shape {w.shape}')
     _one_device('mx4_linear_bwd', dy, w)
     dtype = dy.dtype if dtype is None else dtype
     M = dy.numel() // N
-    dx = empty(tuple(dy.shape[:-1]) + (K,), dy, dtype)
     kx = _mx4_out_kind('mx4_linear_bwd', dtype)
-    nws = query('iprgan_mx4_linear_bwd_ws_floats', M, N, K)
-    ws = scratch(nws, dy) if nws else None
+    dx = _new((M, K) if dy.dim() == 2 else tuple(dy.shape[:-1]) + (K,), dy, dtype)
+    nws = _ws_floats('iprgan_mx4_linear_bwd_ws_floats', M, N, K)
+    ws = L.acct_scratch(_new(nws, dy, torch.float32)) if nws else None
     L.acct_flops(2.0 * M * N * K)
-    call('iprgan_mx4_linear_bwd', ptr(dy), L.bptr(w.codes, torch.uint8), L.bptr(w.scales, torch.uint8), ptr(dx), ptr(ws), M, N, K,
-         is16(dy), kx, stream())
+    wc, wsc = w.ptrs()
+    call('iprgan_mx4_linear_bwd', ptr(dy), wc, wsc, ptr(dx), ptr(ws), M, N, K, k, kx, stream())
     return dx
 
 
@@ -411,13 +528,14 @@ def permute_021(src, A, Bd, K, out=None, beta=0.0):
 def act_bwd(dy, out, act, slope=0.0):
     """dz = dy * act'(out); ``out`` may be its 8-bit checkpoint (Mx8)."""
     if isinstance(out, Mx8):
-        if tuple(dy.shape) != out.shape and dy.numel() != out.numel():
+        if dy.numel() != out.numel():
             raise RuntimeError(f'act_bwd: checkpoint of shape {out.shape}, gradient of shape {tuple(dy.shape)}')
         _one_device('act_bwd', dy, out)
-        dy = f32(dy) if is16(dy) == ST_X3 else _aligned(dy) if dy.is_contiguous() else dy
-        dz = _empty_like(dy)
-        call('iprgan_mx8_act_bwd', ptr(dy), L.bptr(out.codes, torch.int8), L.bptr(out.scales, torch.uint8), ptr(dz), dy.numel(), act,
-             float(slope), is16(dy), 0, 0, stream())
+        dy = f32(dy) if is16(dy) == ST_X3 else dy
+        keep = []
+        pdy, dz = _vptr(dy, keep), _new(dy.shape, dy, dy.dtype)
+        c, s = out.ptrs()
+        call('iprgan_mx8_act_bwd', pdy, c, s, ptr(dz), dy.numel(), act, float(slope), is16(dy), 0, 0, stream())
         return dz
     if ST_X3 in (is16(dy), is16(out)):          # (no three-plane form: a stand-alone activation backward is rare)
         dy, out = f32(dy), f32(out)
