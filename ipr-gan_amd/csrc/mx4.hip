@@ -10,6 +10,8 @@
 // x * 2^-e is exact, so this is ONE rounding.  A block with a NaN or an infinity stores scale byte 255 and reads back as NaN.
 #include "common.h"
 
+#include <atomic>
+
 namespace iprgan {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -291,67 +293,214 @@ __global__ __launch_bounds__(256) void mx4_linear_kernel(const LinArgs a) {
     for (int m = 0; m < MF; ++m) store4(a, m0 + m * 16 + i, n0 + n * 16 + g * 4, acc[n][m]);
 }
 
-// 4-bit x: the scaled matrix instruction multiplies 128 elements of K at once, one scale byte a lane and operand.
+// ---- 4-bit x -------------------------------------------------------------------------------------------------------------------
+// The scaled matrix instruction multiplies 128 elements of K at once: a lane holds one 16-byte block of its row (i = lane & 15, block
+// g = lane >> 4 of the step) and that block's scale byte, for each operand.
+
+// Few rows (M <= 64): both operands straight from memory, the block's waves side by side along n, K split over blocks.
+template <int MF, int NF>
 __global__ __launch_bounds__(256) void mx4_linear4_kernel(const LinArgs a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * 128 + (wave & 1) * 64, m0 = blockIdx.y * 128 + (wave >> 1) * 64;
+  const int n0 = (blockIdx.x * 4 + wave) * 16 * NF, m0 = blockIdx.y * 16 * MF;
   const int s0 = blockIdx.z * a.steps_per_split, s1 = min(a.KB / 4, s0 + a.steps_per_split);
-  f32x4 acc[4][4];
+  f32x4 acc[NF][MF];
 #pragma unroll
-  for (int n = 0; n < 4; ++n)
+  for (int n = 0; n < NF; ++n)
 #pragma unroll
-    for (int m = 0; m < 4; ++m) acc[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const i32x4 *wp[4], *xp[4];
-  const unsigned *wsp[4], *xsp[4];
+    for (int m = 0; m < MF; ++m) acc[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const i32x4 *wp[NF], *xp[MF];
+  const uint8_t *wsp[NF], *xsp[MF];
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const size_t rn = min(n0 + t * 16 + i, a.N - 1), rm = min(m0 + t * 16 + i, a.M - 1);
-    wp[t] = (const i32x4*)(a.w + rn * a.KB * 16) + g;
-    xp[t] = (const i32x4*)((const uint8_t*)a.x + rm * a.KB * 16) + g;
-    wsp[t] = (const unsigned*)(a.ws + rn * a.KB);
-    xsp[t] = (const unsigned*)(a.xs + rm * a.KB);
+  for (int t = 0; t < NF; ++t) {
+    const size_t r = min(n0 + t * 16 + i, a.N - 1);          // rows past the end repeat the last one; their results are not stored
+    wp[t] = (const i32x4*)(a.w + r * a.KB * 16) + g;
+    wsp[t] = a.ws + r * a.KB + g;
   }
-  for (int s = s0; s < s1; ++s) {
-    i32x8 wf[4], xf[4];
-    int wsc[4], xsc[4];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const i32x4 p = wp[t][s * 4], q = xp[t][s * 4];
+  for (int t = 0; t < MF; ++t) {
+    const size_t r = min(m0 + t * 16 + i, a.M - 1);
+    xp[t] = (const i32x4*)((const uint8_t*)a.x + r * a.KB * 16) + g;
+    xsp[t] = a.xs + r * a.KB + g;
+  }
+#pragma unroll 2
+  for (int s = s0; s < s1; ++s) {
+    i32x8 wf[NF], xf[MF];
+    int wsc[NF], xsc[MF];
+#pragma unroll
+    for (int t = 0; t < NF; ++t) {
+      const i32x4 p = wp[t][s * 4];
       wf[t] = i32x8{p[0], p[1], p[2], p[3], 0, 0, 0, 0};
-      xf[t] = i32x8{q[0], q[1], q[2], q[3], 0, 0, 0, 0};
-      wsc[t] = (int)(wsp[t][s] >> 8 * g);
-      xsc[t] = (int)(xsp[t][s] >> 8 * g);
+      wsc[t] = wsp[t][s * 4];
     }
 #pragma unroll
-    for (int n = 0; n < 4; ++n)
+    for (int t = 0; t < MF; ++t) {
+      const i32x4 p = xp[t][s * 4];
+      xf[t] = i32x8{p[0], p[1], p[2], p[3], 0, 0, 0, 0};
+      xsc[t] = xsp[t][s * 4];
+    }
 #pragma unroll
-      for (int m = 0; m < 4; ++m)
+    for (int n = 0; n < NF; ++n)
+#pragma unroll
+      for (int m = 0; m < MF; ++m)
         acc[n][m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[n], xf[m], acc[n][m], 4, 4, 0, wsc[n], 0, xsc[m]);
   }
 #pragma unroll
-  for (int n = 0; n < 4; ++n)
+  for (int n = 0; n < NF; ++n)
 #pragma unroll
-    for (int m = 0; m < 4; ++m) store4(a, m0 + m * 16 + i, n0 + n * 16 + g * 4, acc[n][m]);
+    for (int m = 0; m < MF; ++m) store4(a, m0 + m * 16 + i, n0 + n * 16 + g * 4, acc[n][m]);
 }
 
-// out[m][n] = act(sum over the splits, in order, + bias[n])
+typedef __attribute__((address_space(3))) void lds_void;
+template <int BYTES>
+__device__ __forceinline__ void lds_dma(__amdgpu_buffer_rsrc_t rs, unsigned lds, unsigned voff, unsigned soff) {
+#if defined(__HIP_DEVICE_COMPILE__)      // (an error that the host pass defers silently, dropping the kernel's stub)
+  if constexpr (BYTES == 16) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(uintptr_t)lds, 16, voff, soff, 0, 0);
+  else __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(uintptr_t)lds, 4, voff, soff, 0, 0);
+#endif
+}
+template <int L>
+__device__ __forceinline__ void wait_ring(int stages) {
+  static_assert(2 * L <= 63, "vmcnt is a 6-bit field");
+  if (stages >= 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * L) : "memory");
+  else if (stages == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(L) : "memory");
+  else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
+// Many rows: a TN x TM tile, WN x WM waves, codes and scales of both operands through an LDS ring of four stages (128 elements of K each),
+// filled by LDS-DMA two stages ahead; ONE counted wait and ONE barrier a stage.  Rows are 64 bytes a stage = 4 blocks; block c of row r
+// sits at position c ^ ((r >> 2) & 3), so the 16 rows of a fragment read touch all banks (unswizzled: 4-way conflicts); a DMA lane's
+// place in LDS is fixed, so the swizzle is in its global address.  The first half of the waves loads W, the second half x.
+template <int TN, int TM, int WN, int WM>
+__global__ __launch_bounds__(WN* WM * 64) void mx4_gemm4_kernel(const LinArgs a, int tn, int tm) {
+  constexpr int WAVES = WN * WM, NT = TN / WN / 16, MT = TM / WM / 16, NST = 4;
+  constexpr int PC = (TN + TM) / 16 / WAVES, PS = (TN + TM) / 64 / WAVES, L = PC + PS;       // DMA pieces a wave and stage
+  constexpr int XC = TN * 64, WS = XC + TM * 64, XS = WS + TN * 4, STAGE = XS + TM * 4;
+  static_assert(TN == TM && WAVES % 2 == 0 && PS >= 1, "each half of the waves loads one operand");
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  const unsigned ring = (unsigned)(uintptr_t)(lds_void*)smem;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
+  // tile order: the XCDs take contiguous runs (each has its own L2), and a run walks 4 tiles along n, then down m, so the tiles that run
+  // together share rows of W and of x
+  const unsigned total = (unsigned)tn * tm, per = total / 8, rem = total % 8, xcd = blockIdx.x % 8;
+  const unsigned id = xcd * per + min(xcd, rem) + blockIdx.x / 8;
+  const unsigned grp = id / (4u * tm), in = id - grp * 4u * tm, gw = min(4u, tn - grp * 4u);
+  const int n0 = (int)(grp * 4 + in % gw) * TN, m0 = (int)(in / gw) * TM;
+  const int s0 = blockIdx.z * a.steps_per_split, steps = min(a.KB / 4, s0 + a.steps_per_split) - s0;
+
+  // this wave's DMA pieces: PC of 16 rows x 64 bytes of codes, PS of 64 rows x 4 scale bytes, of ONE operand
+  const bool mine_w = wave < WAVES / 2;
+  const int sub = mine_w ? wave : wave - WAVES / 2;
+  const int base = mine_w ? n0 : m0, last = (mine_w ? a.N : a.M) - 1 - base;                // rows past the end repeat the last one
+  const uint8_t* cb = (mine_w ? a.w : (const uint8_t*)a.x) + (size_t)base * a.KB * 16;
+  const uint8_t* sb = (mine_w ? a.ws : a.xs) + (size_t)base * a.KB;
+  const __amdgpu_buffer_rsrc_t rc = __builtin_amdgcn_make_buffer_rsrc((void*)cb, 0, -1, 0x00020000);
+  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)sb, 0, -1, 0x00020000);
+  unsigned vc[PC], vs[PS];
+#pragma unroll
+  for (int p = 0; p < PC; ++p) {
+    const int r = (sub * PC + p) * 16 + (lane >> 2);
+    vc[p] = (unsigned)min(r, last) * a.KB * 16 + (((lane & 3) ^ ((r >> 2) & 3)) * 16);
+  }
+#pragma unroll
+  for (int p = 0; p < PS; ++p) vs[p] = (unsigned)min((sub * PS + p) * 64 + lane, last) * a.KB;
+  const unsigned lc = ring + (mine_w ? 0 : XC) + sub * PC * 1024, ls = ring + (mine_w ? WS : XS) + sub * PS * 256;
+  auto issue = [&](int t) {
+    const unsigned slot = (unsigned)(t % NST) * STAGE, s = s0 + t;
+#pragma unroll
+    for (int p = 0; p < PC; ++p) lds_dma<16>(rc, lc + slot + p * 1024, vc[p], s * 64);
+#pragma unroll
+    for (int p = 0; p < PS; ++p) lds_dma<4>(rs, ls + slot + p * 256, vs[p], s * 4);
+  };
+  const int wn = wave % WN, wm = wave / WN;
+  const int fr = i * 64 + (g ^ ((i >> 2) & 3)) * 16;                                        // fragment read: row i, block g
+  f32x4 acc[NT][MT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int t = 0; t < NST - 1; ++t)
+    if (t < steps) issue(t);
+  for (int t = 0; t < steps; ++t) {
+    wait_ring<L>(min(NST - 2, steps - 1 - t));            // stage t has landed (this wave's share) ...
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");    // ... and this wave's reads of stage t - 1 are done
+    __builtin_amdgcn_s_barrier();                         // ... in every wave: stage t - 1's slot is free
+    if (t + NST - 1 < steps) issue(t + NST - 1);
+    const uint8_t* st = smem + (t % NST) * STAGE;
+    const uint8_t *wl = st + wn * (NT * 16 * 64) + fr, *xl = st + XC + wm * (MT * 16 * 64) + fr;
+    const uint8_t *wsl = st + WS + (wn * NT * 16 + i) * 4 + g, *xsl = st + XS + (wm * MT * 16 + i) * 4 + g;
+    i32x8 xf[MT];
+    int xsc[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const i32x4 p = *(const i32x4*)(xl + m * 1024);
+      xf[m] = i32x8{p[0], p[1], p[2], p[3], 0, 0, 0, 0};
+      xsc[m] = xsl[m * 64];
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const i32x4 p = *(const i32x4*)(wl + n * 1024);
+      const i32x8 wf = {p[0], p[1], p[2], p[3], 0, 0, 0, 0};
+      const int wsc = wsl[n * 64];
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+        acc[n][m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf, xf[m], acc[n][m], 4, 4, 0, wsc, 0, xsc[m]);
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) store4(a, m0 + (wm * MT + m) * 16 + i, n0 + (wn * NT + n) * 16 + g * 4, acc[n][m]);
+}
+
+// out[m][n] = act(sum over the splits + bias[n]).  A block covers 256 / LZ groups of V elements; LZ lanes of each group add every
+// LZ-th split and are then added in lane order: a fixed order whatever the launch, and the loads of 64 splits are not one chain.
+template <int V, int LZ>
 __global__ __launch_bounds__(256) void mx4_slab_reduce_kernel(const float* __restrict__ slab, int splits, size_t total, int N,
                                                               const float* __restrict__ bias, void* __restrict__ out, int act,
-                                                              float slope, int out_bf16, int vec) {
-  const int V = vec ? 4 : 1;
-  const size_t e = ((size_t)blockIdx.x * 256 + threadIdx.x) * V;
-  if (e >= total) return;
-  f32x4 s = {0.f, 0.f, 0.f, 0.f};
-  if (vec) {
-    for (int z = 0; z < splits; ++z) s += *(const f32x4*)(slab + (size_t)z * total + e);
-  } else {
-    for (int z = 0; z < splits; ++z) s.x += slab[(size_t)z * total + e];
+                                                              float slope, int out_bf16) {
+  constexpr int GR = 256 / LZ;
+  __shared__ float sh[LZ][GR][V + (V > 1)];
+  const int gr = threadIdx.x % GR, lz = threadIdx.x / GR;
+  const size_t e = ((size_t)blockIdx.x * GR + gr) * V;
+  float s[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) s[k] = 0.f;
+  if (e < total) {
+#pragma unroll 4
+    for (int z = lz; z < splits; z += LZ) {
+      const float* p = slab + (size_t)z * total + e;
+      if constexpr (V == 4) {
+        const f32x4 q = *(const f32x4*)p;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s[k] += q[k];
+      } else {
+        s[0] += p[0];
+      }
+    }
   }
+#pragma unroll
+  for (int k = 0; k < V; ++k) sh[lz][gr][k] = s[k];
+  __syncthreads();
+  if (lz || e >= total) return;
   const int n = (int)(e % (size_t)N);
+#pragma unroll
   for (int k = 0; k < V; ++k) {
-    const float v = act_apply(s[k] + (bias ? bias[n + k] : 0.f), act, slope);
-    if (out_bf16) ((__bf16*)out)[e + k] = (__bf16)v;
-    else ((float*)out)[e + k] = v;
+    float v = 0.f;
+#pragma unroll
+    for (int z = 0; z < LZ; ++z) v += sh[z][gr][k];
+    s[k] = act_apply(v + (bias ? bias[n + k] : 0.f), act, slope);
+  }
+  if constexpr (V == 4) {
+    if (out_bf16) {
+      const bf16x4 h = {(__bf16)s[0], (__bf16)s[1], (__bf16)s[2], (__bf16)s[3]};
+      *(bf16x4*)((__bf16*)out + e) = h;
+    } else {
+      const f32x4 q = {s[0], s[1], s[2], s[3]};
+      *(f32x4*)((float*)out + e) = q;
+    }
+  } else {
+    if (out_bf16) ((__bf16*)out)[e] = (__bf16)s[0];
+    else ((float*)out)[e] = s[0];
   }
 }
 
@@ -478,33 +627,55 @@ static inline int kb_of(int cols) { return 4 * cdiv(cols, 128); }
 static int slab_reduce(const float* slab, int splits, int M, int N, const float* bias, void* out, int act, float slope, int out_bf16,
                        hipStream_t st) {
   const size_t total = (size_t)M * N;
-  const int vec = N % 4 == 0;
-  const size_t blocks = cdivz(total, vec ? 1024 : 256);
+  const bool vec = N % 4 == 0 && aligned(out, out_bf16 ? 8 : 16);
+  const bool deep = splits >= 8;                             // 8 lanes a group pay for themselves from 8 splits on
+  const size_t blocks = cdivz(total, (vec ? 4 : 1) * (deep ? 32 : 256));
   IPR_CHECK(blocks < 0x7fffffffull, "mx4: %zu outputs are too many", total);
-  hipLaunchKernelGGL(mx4_slab_reduce_kernel, dim3((unsigned)blocks), dim3(256), 0, st, slab, splits, total, N, bias, out, act, slope, out_bf16, vec);
+  auto k = vec ? (deep ? mx4_slab_reduce_kernel<4, 8> : mx4_slab_reduce_kernel<4, 1>) : (deep ? mx4_slab_reduce_kernel<1, 8> : mx4_slab_reduce_kernel<1, 1>);
+  hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(256), 0, st, slab, splits, total, N, bias, out, act, slope, out_bf16);
   IPR_LAUNCH_CHECK();
   return 0;
 }
 
-// how the product is cut: 16 * mf rows x 64 * nf columns a block (fp32 / bf16 x) or 128 x 128 (4-bit x), K over `splits` blocks
+template <int TN, int TM, int WN, int WM>
+static int gemm4_go(const LinArgs& a, int tn, int tm, int splits, hipStream_t st) {
+  constexpr int LDS = 4 * (TN + TM) * 68;
+  auto k = mx4_gemm4_kernel<TN, TM, WN, WM>;
+  static std::atomic<unsigned long long> ready{0};           // one bit a device: more than 64 KB of dynamic LDS has to be allowed once
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e == hipSuccess && (dev >= 64 || !(ready.load() >> dev & 1))) {
+    e = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    if (e == hipSuccess && dev < 64) ready.fetch_or(1ull << dev);
+  }
+  IPR_CHECK(e == hipSuccess, "mx4_linear: %d bytes of LDS: %s", LDS, hipGetErrorString(e));
+  hipLaunchKernelGGL(k, dim3((unsigned)tn * tm, 1, splits), dim3(WN * WM * 64), LDS, st, a, tn, tm);
+  IPR_LAUNCH_CHECK();
+  return 0;
+}
+
+// how the product is cut: 16 * mf rows x 64 * nf columns a block, or (4-bit x of more than 64 rows) square tiles of `tile`; K over `splits` blocks
 struct LinPlan {
-  int mf, nf, tm, tn, splits, steps_per_split;
+  int mf, nf, tile, tm, tn, splits, steps_per_split;
 };
 static LinPlan lin_plan(int M, int N, int K, int x_kind) {
   LinPlan p;
   const int steps = kb_of(K) / 4;
-  if (x_kind == IPRGAN_X_MX4) {
-    p.mf = p.nf = 4;
-    p.tm = cdiv(M, 128);
-    p.tn = cdiv(N, 128);
+  p.mf = M <= 16 ? 1 : M <= 32 ? 2 : 4;
+  p.nf = p.mf == 1 ? 1 : 2;
+  p.tile = 0;
+  long long full = 512;                                       // blocks that fill the chip: two a CU
+  if (x_kind == IPRGAN_X_MX4 && M > 64) {
+    p.tile = (long long)cdiv(M, 256) * cdiv(N, 256) >= 192 ? 256 : 128;
+    p.tm = cdiv(M, p.tile);
+    p.tn = cdiv(N, p.tile);
+    if (p.tile == 256) full = 1;
   } else {
-    p.mf = M <= 16 ? 1 : M <= 32 ? 2 : 4;
-    p.nf = p.mf == 1 ? 1 : 2;
     p.tm = cdiv(M, 16 * p.mf);
     p.tn = cdiv(N, 64 * p.nf);
   }
   const long long tiles = (long long)p.tm * p.tn;
-  int want = tiles >= 512 ? 1 : (int)(512 / tiles);           // two blocks a CU
+  int want = tiles >= full ? 1 : (int)(full / tiles);
   if (want > 64) want = 64;
   if (want > steps) want = steps;
   if (want < 1) want = 1;
@@ -602,7 +773,7 @@ int iprgan_mx4_linear(const void* x, const void* x_scales, const void* w_codes, 
                 (x_kind != IPRGAN_X_MX4 || aligned(x_scales, 4)) && aligned(y, y_bf16 ? 2 : 4),
             "mx4_linear: codes must be 16-byte, scales 4-byte aligned");
   const LinPlan p = lin_plan(M, N, K, x_kind);
-  IPR_CHECK(p.tm <= 65535, "mx4_linear: M=%d", M);
+  IPR_CHECK(p.tm <= 65535 && (long long)p.tm * p.tn < 0x7fffffffll, "mx4_linear: M=%d, N=%d", M, N);
   IPR_CHECK(p.splits == 1 || (ws && aligned(ws, 16)), "mx4_linear: the workspace of iprgan_mx4_linear_ws_floats is missing");
   hipStream_t st = (hipStream_t)stream;
   LinArgs a;
@@ -614,7 +785,13 @@ int iprgan_mx4_linear(const void* x, const void* x_scales, const void* w_codes, 
   a.vec_y = N % 4 == 0 && (a.slab || aligned(y, y_bf16 ? 8 : 16));
   const dim3 grid(p.tn, p.tm, p.splits), blk(256);
   if (x_kind == IPRGAN_X_MX4) {
-    hipLaunchKernelGGL(mx4_linear4_kernel, grid, blk, 0, st, a);
+    if (p.tile) {
+      const int rc = p.tile == 256 ? gemm4_go<256, 256, 2, 4>(a, p.tn, p.tm, p.splits, st) : gemm4_go<128, 128, 2, 2>(a, p.tn, p.tm, p.splits, st);
+      if (rc) return rc;
+    } else {
+      auto k = p.mf == 1 ? mx4_linear4_kernel<1, 1> : p.mf == 2 ? mx4_linear4_kernel<2, 2> : mx4_linear4_kernel<4, 2>;
+      hipLaunchKernelGGL(k, grid, blk, 0, st, a);
+    }
   } else if (x_kind == IPRGAN_X_BF16) {
     auto k = p.mf == 1 ? mx4_linear_kernel<1, 1, 1> : p.mf == 2 ? mx4_linear_kernel<2, 2, 1> : mx4_linear_kernel<4, 2, 1>;
     hipLaunchKernelGGL(k, grid, blk, 0, st, a);

@@ -381,6 +381,18 @@ def test_mx4_linear_gradient_against_differences(dev):
     assert abs(float(num - ana)) <= 2.0 ** -23 * 100 * float(scale)
 
 
+@pytest.mark.parametrize('M,K,N', [(4099, 300, 3101), (2304, 1700, 5888)])
+def test_mx4_product_of_many_rows(dev, M, K, N):
+    """More tiles than the chip runs at once, ragged edges, both operands in 4 bits (float64 on the device)."""
+    from iprgan import ops
+    x, w = rnd(M, K, seed=1).to(dev), rnd(N, K, seed=2).to(dev) / K ** 0.5
+    xq, wq = ops.mx4_quant(x), ops.mx4_quant(w)
+    y = ops.mx4_linear(xq, wq, dtype=torch.float32).double()
+    xd, wd = ops.mx4_dequant(xq).double(), ops.mx4_dequant(wq).double().t().contiguous()
+    err, tol = (y - xd @ wd).abs(), lin_bound(xd.abs(), wd.abs(), K, 1)
+    assert bool((err <= tol).all()), float((err / tol).max())
+
+
 def test_mx4_linear_leading_dimensions_and_unaligned_views(dev):
     from iprgan import ops
     w4 = ops.mx4_quant(rnd(24, 64, seed=2).to(dev))
