@@ -209,7 +209,7 @@ __device__ __forceinline__ void split_planes(const float* v, bf16x8* p) {
 template <int MF, int NF, int PL>
 __global__ __launch_bounds__(256) void mx4_linear_kernel(const LinArgs a) {
   constexpr int XP = 136;                                   // LDS row pitch in bf16: 16 rows x 4-bank offset, conflict-free fragment reads
-  __shared__ __bf16 xs[2][PL][MF * 16][XP];
+  __shared__ __bf16 xs[PL][MF * 16][XP];                    // one buffer: 52 KB at most, three blocks a CU hide each other's barriers
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
   const int n0 = blockIdx.x * 64 * NF + wave * 16 * NF, m0 = blockIdx.y * 16 * MF;
   const int s0 = blockIdx.z * a.steps_per_split, s1 = min(a.KB / 4, s0 + a.steps_per_split);
@@ -237,31 +237,29 @@ __global__ __launch_bounds__(256) void mx4_linear_kernel(const LinArgs a) {
       for (int k = 0; k < 8; ++k) v[k] = 0.f;
     }
   };
-  auto put_x = [&](int buf, int t, const float* v) {
-    bf16x8 p[PL];
-    split_planes<PL>(v, p);
-#pragma unroll
-    for (int q = 0; q < PL; ++q) *(bf16x8*)&xs[buf][q][xr + t * 16][xc] = p[q];
-  };
   u32x4 wq[NF], wn[NF];
   unsigned sq[NF], sn[NF];
   float xv[MF][8];
-  if (s0 < s1) {
+  auto load = [&](int s) {
 #pragma unroll
-    for (int n = 0; n < NF; ++n) { wq[n] = wp[n][s0 * 4]; sq[n] = sp[n][s0 * 4]; }
+    for (int n = 0; n < NF; ++n) { wn[n] = wp[n][s * 4]; sn[n] = sp[n][s * 4]; }
 #pragma unroll
-    for (int t = 0; t < MF; ++t) { load_x(s0, t, xv[t]); put_x(0, t, xv[t]); }
-  }
-  __syncthreads();
+    for (int t = 0; t < MF; ++t) load_x(s, t, xv[t]);
+  };
+  if (s0 < s1) load(s0);
   for (int s = s0; s < s1; ++s) {
-    const int buf = (s - s0) & 1;
-    const bool more = s + 1 < s1;
-    if (more) {
+    if (s > s0) __syncthreads();                            // every wave has read the last step's planes
 #pragma unroll
-      for (int n = 0; n < NF; ++n) { wn[n] = wp[n][(s + 1) * 4]; sn[n] = sp[n][(s + 1) * 4]; }
+    for (int t = 0; t < MF; ++t) {
+      bf16x8 p[PL];
+      split_planes<PL>(xv[t], p);
 #pragma unroll
-      for (int t = 0; t < MF; ++t) load_x(s + 1, t, xv[t]);
+      for (int q = 0; q < PL; ++q) *(bf16x8*)&xs[q][xr + t * 16][xc] = p[q];
     }
+#pragma unroll
+    for (int n = 0; n < NF; ++n) { wq[n] = wn[n]; sq[n] = sn[n]; }
+    __syncthreads();
+    if (s + 1 < s1) load(s + 1);                            // in flight while this step is multiplied
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       bf16x8 wf[NF];
@@ -274,18 +272,11 @@ __global__ __launch_bounds__(256) void mx4_linear_kernel(const LinArgs a) {
       for (int q = PL - 1; q >= 0; --q)
 #pragma unroll
         for (int m = 0; m < MF; ++m) {
-          const bf16x8 xf = *(const bf16x8*)&xs[buf][q][m * 16 + i][g * 32 + j * 8];
+          const bf16x8 xf = *(const bf16x8*)&xs[q][m * 16 + i][g * 32 + j * 8];
 #pragma unroll
           for (int n = 0; n < NF; ++n) acc[n][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[n], xf, acc[n][m], 0, 0, 0);
         }
     }
-    if (more) {
-#pragma unroll
-      for (int t = 0; t < MF; ++t) put_x(buf ^ 1, t, xv[t]);
-#pragma unroll
-      for (int n = 0; n < NF; ++n) { wq[n] = wn[n]; sq[n] = sn[n]; }
-    }
-    __syncthreads();
   }
 #pragma unroll
   for (int n = 0; n < NF; ++n)
