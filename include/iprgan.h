@@ -518,7 +518,7 @@ int iprgan_mx4_dequant(const void* codes, const void* scales, void* y, int rows,
  * NULL; y fp32 or bf16, rounded once.  ws: 16-byte aligned, iprgan_mx4_linear_ws_floats floats (0: may be NULL); sums over a
  * split K are added in fixed order. */
 enum { IPRGAN_X_F32 = 0, IPRGAN_X_BF16 = 1, IPRGAN_X_MX4 = 2 };
-size_t iprgan_mx4_linear_ws_floats(int M, int N, int K, int x_kind);
+size_t iprgan_mx4_linear_ws_floats(int M, int N, int K, int x_kind, int act);
 int iprgan_mx4_linear(const void* x, const void* x_scales, const void* w_codes, const void* w_scales, const float* bias, void* y,
                       float* ws, int M, int N, int K, int x_kind, int act, float slope, int y_bf16, void* stream);
 /* dx [M][K] = dy [M][N] W: the gradient with respect to x through the frozen 4-bit weights */

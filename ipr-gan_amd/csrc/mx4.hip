@@ -141,10 +141,15 @@ struct LinArgs {
   void* y;
   float* slab;                   // [splits][M][N] when the K axis is split
   int M, N, K, KB, steps_per_split;      // a step is 128 elements of K
-  int act, y_bf16, vec_x, vec_y;
+  int act, y_bf16, vec_x, vec_y, vec8;      // vec_y: 4 columns at once, vec8: 8 bf16 columns
   float slope;
 };
 
+// none, ReLU, LeakyReLU (none: slope 1).  tanh and the sigmoid go through the slab pass: their code, once an accumulator, would make the
+// product kernels' epilogues several times their loops.
+__device__ __forceinline__ float lin_act(float v, int act, float slope) {
+  return v > 0.f ? v : act == IPRGAN_ACT_RELU ? 0.f : v * slope;
+}
 __device__ __forceinline__ void store4(const LinArgs& a, int m, int n, f32x4 v) {
   if (m >= a.M || n >= a.N) return;
   if (a.slab) {
@@ -152,26 +157,32 @@ __device__ __forceinline__ void store4(const LinArgs& a, int m, int n, f32x4 v) 
     if (a.vec_y) {
       *(f32x4*)o = v;
     } else {
-      for (int k = 0; k < 4 && n + k < a.N; ++k) o[k] = v[k];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (n + k < a.N) o[k] = v[k];
+    }
+    return;
+  }
+  const size_t o = (size_t)m * a.N + n;
+  if (a.vec_y) {
+    f32x4 b = {0.f, 0.f, 0.f, 0.f};
+    if (a.bias) b = f32x4{a.bias[n], a.bias[n + 1], a.bias[n + 2], a.bias[n + 3]};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = lin_act(v[k] + b[k], a.act, a.slope);
+    if (a.y_bf16) {
+      const bf16x4 h = {(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+      *(bf16x4*)((__bf16*)a.y + o) = h;
+    } else {
+      *(f32x4*)((float*)a.y + o) = v;
     }
     return;
   }
 #pragma unroll
-  for (int k = 0; k < 4; ++k) v[k] = act_apply(v[k] + (a.bias && n + k < a.N ? a.bias[n + k] : 0.f), a.act, a.slope);
-  const size_t o = (size_t)m * a.N + n;
-  if (a.y_bf16) {
-    bf16x4 h;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) h[k] = (__bf16)v[k];
-    if (a.vec_y) {
-      *(bf16x4*)((__bf16*)a.y + o) = h;
-    } else {
-      for (int k = 0; k < 4 && n + k < a.N; ++k) ((__bf16*)a.y)[o + k] = h[k];
-    }
-  } else if (a.vec_y) {
-    *(f32x4*)((float*)a.y + o) = v;
-  } else {
-    for (int k = 0; k < 4 && n + k < a.N; ++k) ((float*)a.y)[o + k] = v[k];
+  for (int k = 0; k < 4; ++k) {
+    if (n + k >= a.N) continue;
+    const float r = lin_act(v[k] + (a.bias ? a.bias[n + k] : 0.f), a.act, a.slope);
+    if (a.y_bf16) ((__bf16*)a.y)[o + k] = (__bf16)r;
+    else ((float*)a.y)[o + k] = r;
   }
 }
 
@@ -351,96 +362,167 @@ __device__ __forceinline__ void lds_dma(__amdgpu_buffer_rsrc_t rs, unsigned lds,
 }
 template <int L>
 __device__ __forceinline__ void wait_ring(int stages) {
-  static_assert(2 * L <= 63, "vmcnt is a 6-bit field");
-  if (stages >= 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * L) : "memory");
-  else if (stages == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(L) : "memory");
+  if (stages >= 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(L) : "memory");
   else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-// Many rows: a TN x TM tile, WN x WM waves, codes and scales of both operands through an LDS ring of four stages (128 elements of K each),
-// filled by LDS-DMA two stages ahead; ONE counted wait and ONE barrier a stage.  Rows are 64 bytes a stage = 4 blocks; block c of row r
-// sits at position c ^ ((r >> 2) & 3), so the 16 rows of a fragment read touch all banks (unswizzled: 4-way conflicts); a DMA lane's
-// place in LDS is fixed, so the swizzle is in its global address.  The first half of the waves loads W, the second half x.
-template <int TN, int TM, int WN, int WM>
-__global__ __launch_bounds__(WN* WM * 64) void mx4_gemm4_kernel(const LinArgs a, int tn, int tm) {
-  constexpr int WAVES = WN * WM, NT = TN / WN / 16, MT = TM / WM / 16, NST = 4;
-  constexpr int PC = (TN + TM) / 16 / WAVES, PS = (TN + TM) / 64 / WAVES, L = PC + PS;       // DMA pieces a wave and stage
-  constexpr int XC = TN * 64, WS = XC + TM * 64, XS = WS + TN * 4, STAGE = XS + TM * 4;
-  static_assert(TN == TM && WAVES % 2 == 0 && PS >= 1, "each half of the waves loads one operand");
+// Many rows: TN x TM tiles, WN x WM waves, codes and scales of both operands through an LDS ring of four stages (128 elements of K each)
+// filled by LDS-DMA; the first half of the waves loads W, the second half x.
+//   * The stages of ALL tiles a block computes form one stream (a block walks tiles blockIdx.x, + gridDim.x, ..): the next tile's first
+//     stages are in flight while a tile's results are stored.  In the middle of a stage's multiplications a wave waits for its share of
+//     the next stage (counted; a full drain behind an epilogue, whose stores share the counter), then ONE barrier - every wave's share
+//     has landed, and every wave is done with the previous stage, whose slot is refilled.
+//   * Rows are 64 bytes a stage = 4 blocks; block c of row r sits at position c ^ ((r >> 1) & 3): 8 lanes of a fragment read then touch all 32
+//     banks (at r >> 2 the conflicts doubled the LDS time).  A DMA lane's place in LDS is fixed, so the swizzle is in its address.
+//   * S16 (rows of whole 512-element groups): the scales of four stages travel as one 16-byte piece a row; one 4-byte piece a row and
+//     stage costs the intake as much as a third of the codes (64 cache lines an instruction): 375 -> 352 us at 8192^3.
+//   * Tile order: the XCDs take contiguous runs (each has its own L2), and a run walks 4 tiles along n, then down m.
+// What bounds it: 256 x 256, 8192^3: the DMA intake alone takes 0.63 us a stage, the multiplications 0.67 at the sustained clock.
+template <int TN, int TM, int WN, int WM, bool S16>
+__global__ __launch_bounds__(WN* WM * 64, 2) void mx4_gemm4_kernel(const LinArgs a, int tn, int tm) {
+  constexpr int WAVES = WN * WM, NT = TN / WN / 16, MT = TM / WM / 16, NST = 4, D = 2;        // D: W fragments read ahead
+  constexpr int PC = (TN + TM) / 16 / WAVES, PS = (TN + TM) / 64 / WAVES, L = PC + (S16 ? 0 : PS);      // DMA pieces a wave and stage
+  constexpr int XC = TN * 64, WS = XC + TM * 64, XS = WS + (S16 ? 0 : TN * 4), STAGE = XS + (S16 ? 0 : TM * 4);
+  constexpr int RING = NST * STAGE, SSLOT = (TN + TM) * 16, SR = S16 ? 16 : 4;                 // SR: scale bytes of a row in LDS
+  static_assert(TN == TM && WAVES % 2 == 0 && PS >= 1 && NST == 4, "each half of the waves loads one operand");
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   const unsigned ring = (unsigned)(uintptr_t)(lds_void*)smem;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
-  // tile order: the XCDs take contiguous runs (each has its own L2), and a run walks 4 tiles along n, then down m, so the tiles that run
-  // together share rows of W and of x
-  const unsigned total = (unsigned)tn * tm, per = total / 8, rem = total % 8, xcd = blockIdx.x % 8;
-  const unsigned id = xcd * per + min(xcd, rem) + blockIdx.x / 8;
-  const unsigned grp = id / (4u * tm), in = id - grp * 4u * tm, gw = min(4u, tn - grp * 4u);
-  const int n0 = (int)(grp * 4 + in % gw) * TN, m0 = (int)(in / gw) * TM;
   const int s0 = blockIdx.z * a.steps_per_split, steps = min(a.KB / 4, s0 + a.steps_per_split) - s0;
+  const unsigned total = (unsigned)tn * tm, per = total / 8, rem = total % 8;
+  auto tile_at = [&](unsigned b, int& n0, int& m0) {
+    const unsigned xcd = b % 8, id = xcd * per + min(xcd, rem) + b / 8;
+    const unsigned grp = id / (4u * tm), in = id - grp * 4u * tm, gw = min(4u, tn - grp * 4u);
+    n0 = (int)(grp * 4 + in % gw) * TN;
+    m0 = (int)(in / gw) * TM;
+  };
+  const int tiles = (int)((total - blockIdx.x + gridDim.x - 1) / gridDim.x), stages = tiles * steps;      // blockIdx.x < total
 
-  // this wave's DMA pieces: PC of 16 rows x 64 bytes of codes, PS of 64 rows x 4 scale bytes, of ONE operand
+  // the loading side: cursor (it, is) = tile and stage of the next piece, the tile's addresses
   const bool mine_w = wave < WAVES / 2;
   const int sub = mine_w ? wave : wave - WAVES / 2;
-  const int base = mine_w ? n0 : m0, last = (mine_w ? a.N : a.M) - 1 - base;                // rows past the end repeat the last one
-  const uint8_t* cb = (mine_w ? a.w : (const uint8_t*)a.x) + (size_t)base * a.KB * 16;
-  const uint8_t* sb = (mine_w ? a.ws : a.xs) + (size_t)base * a.KB;
-  const __amdgpu_buffer_rsrc_t rc = __builtin_amdgcn_make_buffer_rsrc((void*)cb, 0, -1, 0x00020000);
-  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)sb, 0, -1, 0x00020000);
+  __amdgpu_buffer_rsrc_t rc, rs;
   unsigned vc[PC], vs[PS];
+  int it = 0, is = 0;
+  auto aim = [&](int k) {
+    int n0, m0;
+    tile_at(blockIdx.x + k * gridDim.x, n0, m0);
+    const int base = mine_w ? n0 : m0, last = (mine_w ? a.N : a.M) - 1 - base;              // rows past the end repeat the last one
+    rc = __builtin_amdgcn_make_buffer_rsrc((void*)((mine_w ? a.w : (const uint8_t*)a.x) + (size_t)base * a.KB * 16), 0, -1, 0x00020000);
+    rs = __builtin_amdgcn_make_buffer_rsrc((void*)((mine_w ? a.ws : a.xs) + (size_t)base * a.KB), 0, -1, 0x00020000);
 #pragma unroll
-  for (int p = 0; p < PC; ++p) {
-    const int r = (sub * PC + p) * 16 + (lane >> 2);
-    vc[p] = (unsigned)min(r, last) * a.KB * 16 + (((lane & 3) ^ ((r >> 2) & 3)) * 16);
-  }
+    for (int p = 0; p < PC; ++p) {
+      const int r = (sub * PC + p) * 16 + (lane >> 2);
+      vc[p] = (unsigned)min(r, last) * a.KB * 16 + (((lane & 3) ^ ((r >> 1) & 3)) * 16);
+    }
 #pragma unroll
-  for (int p = 0; p < PS; ++p) vs[p] = (unsigned)min((sub * PS + p) * 64 + lane, last) * a.KB;
-  const unsigned lc = ring + (mine_w ? 0 : XC) + sub * PC * 1024, ls = ring + (mine_w ? WS : XS) + sub * PS * 256;
-  auto issue = [&](int t) {
-    const unsigned slot = (unsigned)(t % NST) * STAGE, s = s0 + t;
+    for (int p = 0; p < PS; ++p) vs[p] = (unsigned)min((sub * PS + p) * 64 + lane, last) * a.KB;
+  };
+  const unsigned lc = ring + (mine_w ? 0 : XC) + sub * PC * 1024;
+  const unsigned ls = S16 ? ring + RING + (mine_w ? 0 : TN * 16) + sub * PS * 1024 : ring + (mine_w ? WS : XS) + sub * PS * 256;
+  auto issue = [&](int q) {                             // stage q of the stream (S16: every tile has a multiple of 4 stages)
+    const unsigned slot = (unsigned)(q & 3) * STAGE, s = s0 + is;
+    if constexpr (S16) {
+      if ((q & 3) == 0) {
+#pragma unroll
+        for (int p = 0; p < PS; ++p) lds_dma<16>(rs, ls + ((q >> 2) & 1) * SSLOT + p * 1024, vs[p], s * 4);
+      }
+    }
 #pragma unroll
     for (int p = 0; p < PC; ++p) lds_dma<16>(rc, lc + slot + p * 1024, vc[p], s * 64);
+    if constexpr (!S16) {
 #pragma unroll
-    for (int p = 0; p < PS; ++p) lds_dma<4>(rs, ls + slot + p * 256, vs[p], s * 4);
+      for (int p = 0; p < PS; ++p) lds_dma<4>(rs, ls + slot + p * 256, vs[p], s * 4);
+    }
+    if (++is == steps) {
+      is = 0;
+      if (++it < tiles) aim(it);
+    }
   };
   const int wn = wave % WN, wm = wave / WN;
-  const int fr = i * 64 + (g ^ ((i >> 2) & 3)) * 16;                                        // fragment read: row i, block g
-  f32x4 acc[NT][MT];
+  const int fr = i * 64 + (g ^ ((i >> 1) & 3)) * 16;                                        // fragment read: row i, block g
+  aim(0);
+  for (int q = 0; q < NST - 1 && q < stages; ++q) issue(q);
+  if (stages >= 3) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * L) : "memory");             // (S16: the scale piece is issued first)
+  else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  int q = 0;
+#pragma unroll 1
+  for (int k = 0; k < tiles; ++k) {
+    f32x4 acc[NT][MT];
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int m = 0; m < MT; ++m) acc[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int t = 0; t < NST - 1; ++t)
-    if (t < steps) issue(t);
-  for (int t = 0; t < steps; ++t) {
-    wait_ring<L>(min(NST - 2, steps - 1 - t));            // stage t has landed (this wave's share) ...
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");    // ... and this wave's reads of stage t - 1 are done
-    __builtin_amdgcn_s_barrier();                         // ... in every wave: stage t - 1's slot is free
-    if (t + NST - 1 < steps) issue(t + NST - 1);
-    const uint8_t* st = smem + (t % NST) * STAGE;
-    const uint8_t *wl = st + wn * (NT * 16 * 64) + fr, *xl = st + XC + wm * (MT * 16 * 64) + fr;
-    const uint8_t *wsl = st + WS + (wn * NT * 16 + i) * 4 + g, *xsl = st + XS + (wm * MT * 16 + i) * 4 + g;
-    i32x8 xf[MT];
-    int xsc[MT];
+      for (int m = 0; m < MT; ++m) acc[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int t = 0; t < steps; ++t, ++q) {
+      const uint8_t* st = smem + (q & 3) * STAGE;
+      const uint8_t *wl = st + wn * (NT * 16 * 64) + fr, *xl = st + XC + wm * (MT * 16 * 64) + fr;
+      const uint8_t* sc = S16 ? smem + RING + ((q >> 2) & 1) * SSLOT + (q & 3) * 4 + g : st + WS + g;
+      const uint8_t *wsl = sc + (wn * NT * 16 + i) * SR, *xsl = sc + TN * SR + (wm * MT * 16 + i) * SR;
+      i32x4 xf[MT], wf[D + 1];
+      int xsc[MT], wsc[D + 1];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const i32x4 p = *(const i32x4*)(xl + m * 1024);
-      xf[m] = i32x8{p[0], p[1], p[2], p[3], 0, 0, 0, 0};
-      xsc[m] = xsl[m * 64];
+      for (int m = 0; m < MT; ++m) { xf[m] = *(const i32x4*)(xl + m * 1024); xsc[m] = xsl[m * 16 * SR]; }
+#pragma unroll
+      for (int n = 0; n < D; ++n) { wf[n] = *(const i32x4*)(wl + n * 1024); wsc[n] = wsl[n * 16 * SR]; }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        if (n == NT / 2 - 1 && q + 1 < stages) {
+          if (t == 0 && k) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+          else wait_ring<L>(stages - 2 - q);
+          __builtin_amdgcn_s_barrier();
+          if (q + NST - 1 < stages) issue(q + NST - 1);
+        }
+        if (n + D < NT) { wf[(n + D) % (D + 1)] = *(const i32x4*)(wl + (n + D) * 1024); wsc[(n + D) % (D + 1)] = wsl[(n + D) * 16 * SR]; }
+        const i32x4 wq = wf[n % (D + 1)];
+        const i32x8 w8 = {wq[0], wq[1], wq[2], wq[3], 0, 0, 0, 0};
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const i32x8 x8 = {xf[m][0], xf[m][1], xf[m][2], xf[m][3], 0, 0, 0, 0};
+          acc[n][m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w8, x8, acc[n][m], 4, 4, 0, wsc[n % (D + 1)], 0, xsc[m]);
+        }
+        __builtin_amdgcn_sched_barrier(0);              // the reads stay D fragments ahead of the multiplications
+      }
     }
+    int n0, m0;
+    tile_at(blockIdx.x + k * gridDim.x, n0, m0);
+    n0 += wn * NT * 16;
+    m0 += wm * MT * 16 + i;
+    if (a.vec8 && !a.slab) {
+      // bf16, 16 bytes a lane: lane groups g and g ^ 1 trade halves of two neighbouring fragments, so that a lane holds 8 columns
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const i32x4 p = *(const i32x4*)(wl + n * 1024);
-      const i32x8 wf = {p[0], p[1], p[2], p[3], 0, 0, 0, 0};
-      const int wsc = wsl[n * 64];
+      for (int n = 0; n < NT; n += 2) {
+        const int col = n0 + (n + (g & 1)) * 16 + (g >> 1) * 8;
+        float b0[4], b1[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int ca = n0 + n * 16 + g * 4 + c;
+          b0[c] = a.bias && ca < a.N ? a.bias[ca] : 0.f;
+          b1[c] = a.bias && ca + 16 < a.N ? a.bias[ca + 16] : 0.f;
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          bf16x2 p[4];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            p[c] = bf16x2{(__bf16)lin_act(acc[n][m][2 * c] + b0[2 * c], a.act, a.slope), (__bf16)lin_act(acc[n][m][2 * c + 1] + b0[2 * c + 1], a.act, a.slope)};
+            p[2 + c] = bf16x2{(__bf16)lin_act(acc[n + 1][m][2 * c] + b1[2 * c], a.act, a.slope),
+                              (__bf16)lin_act(acc[n + 1][m][2 * c + 1] + b1[2 * c + 1], a.act, a.slope)};
+          }
+          const auto lo = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, p[0]), __builtin_bit_cast(unsigned, p[2]), false, false);
+          const auto hi = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, p[1]), __builtin_bit_cast(unsigned, p[3]), false, false);
+          const u32x4 o = {lo[0], hi[0], lo[1], hi[1]};
+          if (m0 + m * 16 < a.M && col < a.N) *(u32x4*)((__bf16*)a.y + (size_t)(m0 + m * 16) * a.N + col) = o;
+        }
+      }
+    } else {
 #pragma unroll
       for (int m = 0; m < MT; ++m)
-        acc[n][m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf, xf[m], acc[n][m], 4, 4, 0, wsc, 0, xsc[m]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) store4(a, m0 + m * 16, n0 + n * 16 + g * 4, acc[n][m]);
     }
   }
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int n = 0; n < NT; ++n) store4(a, m0 + (wm * MT + m) * 16 + i, n0 + (wn * NT + n) * 16 + g * 4, acc[n][m]);
 }
 
 // out[m][n] = act(sum over the splits + bias[n]).  A block covers 256 / LZ groups of V elements; LZ lanes of each group add every
@@ -628,10 +710,10 @@ static int slab_reduce(const float* slab, int splits, int M, int N, const float*
   return 0;
 }
 
-template <int TN, int TM, int WN, int WM>
+template <int TN, int TM, int WN, int WM, bool S16>
 static int gemm4_go(const LinArgs& a, int tn, int tm, int splits, hipStream_t st) {
-  constexpr int LDS = 4 * (TN + TM) * 68;
-  auto k = mx4_gemm4_kernel<TN, TM, WN, WM>;
+  constexpr int LDS = S16 ? (TN + TM) * (4 * 64 + 2 * 16) : (TN + TM) * 4 * 68;
+  auto k = mx4_gemm4_kernel<TN, TM, WN, WM, S16>;
   static std::atomic<unsigned long long> ready{0};           // one bit a device: more than 64 KB of dynamic LDS has to be allowed once
   int dev = 0;
   hipError_t e = hipGetDevice(&dev);
@@ -640,21 +722,22 @@ static int gemm4_go(const LinArgs& a, int tn, int tm, int splits, hipStream_t st
     if (e == hipSuccess && dev < 64) ready.fetch_or(1ull << dev);
   }
   IPR_CHECK(e == hipSuccess, "mx4_linear: %d bytes of LDS: %s", LDS, hipGetErrorString(e));
-  hipLaunchKernelGGL(k, dim3((unsigned)tn * tm, 1, splits), dim3(WN * WM * 64), LDS, st, a, tn, tm);
+  const unsigned total = (unsigned)tn * tm, resident = TN == 256 ? 256 : 512;       // blocks the chip holds at once
+  hipLaunchKernelGGL(k, dim3(total < resident ? total : resident, 1, splits), dim3(WN * WM * 64), LDS, st, a, tn, tm);
   IPR_LAUNCH_CHECK();
   return 0;
 }
 
 // how the product is cut: 16 * mf rows x 64 * nf columns a block, or (4-bit x of more than 64 rows) square tiles of `tile`; K over `splits` blocks
 struct LinPlan {
-  int mf, nf, tile, tm, tn, splits, steps_per_split;
+  int mf, nf, tile, s16, tm, tn, splits, steps_per_split;
 };
 static LinPlan lin_plan(int M, int N, int K, int x_kind) {
   LinPlan p;
   const int steps = kb_of(K) / 4;
   p.mf = M <= 16 ? 1 : M <= 32 ? 2 : 4;
   p.nf = p.mf == 1 ? 1 : 2;
-  p.tile = 0;
+  p.tile = p.s16 = 0;
   long long full = 512;                                       // blocks that fill the chip: two a CU
   if (x_kind == IPRGAN_X_MX4 && M > 64) {
     p.tile = (long long)cdiv(M, 256) * cdiv(N, 256) >= 192 ? 256 : 128;
@@ -671,6 +754,10 @@ static LinPlan lin_plan(int M, int N, int K, int x_kind) {
   if (want > steps) want = steps;
   if (want < 1) want = 1;
   p.steps_per_split = cdiv(steps, want);
+  if (p.tile && steps % 4 == 0) {                             // the form that moves the scales of four stages at once
+    p.s16 = 1;
+    p.steps_per_split = rup(p.steps_per_split, 4);
+  }
   p.splits = cdiv(steps, p.steps_per_split);
   return p;
 }
@@ -747,10 +834,13 @@ static int lin_check(const char* who, int M, int N, int K) {
   return 0;
 }
 
-size_t iprgan_mx4_linear_ws_floats(int M, int N, int K, int x_kind) {
+// tanh and the sigmoid are applied by the pass that adds the slabs, also where there is only one
+static bool lin_slab(const LinPlan& p, int act) { return p.splits > 1 || act > IPRGAN_ACT_LRELU; }
+
+size_t iprgan_mx4_linear_ws_floats(int M, int N, int K, int x_kind, int act) {
   if (M < 1 || N < 1 || K < 1) return 0;
   const LinPlan p = lin_plan(M, N, K, x_kind);
-  return p.splits > 1 ? (size_t)p.splits * M * N : 0;
+  return lin_slab(p, act) ? (size_t)p.splits * M * N : 0;
 }
 
 int iprgan_mx4_linear(const void* x, const void* x_scales, const void* w_codes, const void* w_scales, const float* bias, void* y,
@@ -765,19 +855,22 @@ int iprgan_mx4_linear(const void* x, const void* x_scales, const void* w_codes, 
             "mx4_linear: codes must be 16-byte, scales 4-byte aligned");
   const LinPlan p = lin_plan(M, N, K, x_kind);
   IPR_CHECK(p.tm <= 65535 && (long long)p.tm * p.tn < 0x7fffffffll, "mx4_linear: M=%d, N=%d", M, N);
-  IPR_CHECK(p.splits == 1 || (ws && aligned(ws, 16)), "mx4_linear: the workspace of iprgan_mx4_linear_ws_floats is missing");
+  const bool slab = lin_slab(p, act);
+  IPR_CHECK(!slab || (ws && aligned(ws, 16)), "mx4_linear: the workspace of iprgan_mx4_linear_ws_floats is missing");
   hipStream_t st = (hipStream_t)stream;
   LinArgs a;
   a.x = x; a.xs = (const uint8_t*)x_scales; a.w = (const uint8_t*)w_codes; a.ws = (const uint8_t*)w_scales; a.bias = bias; a.y = y;
-  a.slab = p.splits > 1 ? ws : nullptr;
+  a.slab = slab ? ws : nullptr;
   a.M = M; a.N = N; a.K = K; a.KB = kb_of(K); a.steps_per_split = p.steps_per_split;
-  a.act = act; a.slope = slope; a.y_bf16 = y_bf16;
+  a.act = act; a.slope = act == IPRGAN_ACT_LRELU ? slope : 1.f; a.y_bf16 = y_bf16;
   a.vec_x = K % (x_kind == IPRGAN_X_BF16 ? 8 : 4) == 0 && aligned(x, 16);
   a.vec_y = N % 4 == 0 && (a.slab || aligned(y, y_bf16 ? 8 : 16));
+  a.vec8 = y_bf16 && N % 8 == 0 && aligned(y, 16);
   const dim3 grid(p.tn, p.tm, p.splits), blk(256);
   if (x_kind == IPRGAN_X_MX4) {
     if (p.tile) {
-      const int rc = p.tile == 256 ? gemm4_go<256, 256, 2, 4>(a, p.tn, p.tm, p.splits, st) : gemm4_go<128, 128, 2, 2>(a, p.tn, p.tm, p.splits, st);
+      const int rc = p.tile == 256 ? (p.s16 ? gemm4_go<256, 256, 2, 4, true>(a, p.tn, p.tm, p.splits, st) : gemm4_go<256, 256, 2, 4, false>(a, p.tn, p.tm, p.splits, st))
+                                   : (p.s16 ? gemm4_go<128, 128, 2, 2, true>(a, p.tn, p.tm, p.splits, st) : gemm4_go<128, 128, 2, 2, false>(a, p.tn, p.tm, p.splits, st));
       if (rc) return rc;
     } else {
       auto k = p.mf == 1 ? mx4_linear4_kernel<1, 1> : p.mf == 2 ? mx4_linear4_kernel<2, 2> : mx4_linear4_kernel<4, 2>;
@@ -791,7 +884,7 @@ int iprgan_mx4_linear(const void* x, const void* x_scales, const void* w_codes, 
     hipLaunchKernelGGL(k, grid, blk, 0, st, a);
   }
   IPR_LAUNCH_CHECK();
-  return p.splits > 1 ? slab_reduce(ws, p.splits, M, N, bias, y, act, slope, y_bf16, st) : 0;
+  return slab ? slab_reduce(ws, p.splits, M, N, bias, y, act, slope, y_bf16, st) : 0;
 }
 
 size_t iprgan_mx4_linear_bwd_ws_floats(int M, int N, int K) {

@@ -468,7 +468,7 @@ def mx4_linear(x, w, bias=None, act=L.ACT_NONE, slope=0.0, dtype=None):
         xp, xsp = ptr(x), None
     ky = _mx4_out_kind('mx4_linear', dtype)
     y = _new(shape, x, dtype)
-    nws = _ws_floats('iprgan_mx4_linear_ws_floats', M, N, K, k)
+    nws = _ws_floats('iprgan_mx4_linear_ws_floats', M, N, K, k, int(act))
     ws = L.acct_scratch(_new(nws, x, torch.float32)) if nws else None
     L.acct_flops(2.0 * M * N * K)
     wc, wsc = w.ptrs()

@@ -65,8 +65,9 @@ def test_mx4_entries_refuse_bad_calls():
 
 
 def test_workspace_sizes():
-    assert L.query('iprgan_mx4_linear_ws_floats', 0, 8, 8, 0) == 0
-    assert L.query('iprgan_mx4_linear_ws_floats', 4, 64, 8192, 0) % (4 * 64) == 0
+    assert L.query('iprgan_mx4_linear_ws_floats', 0, 8, 8, 0, 0) == 0
+    assert L.query('iprgan_mx4_linear_ws_floats', 4, 64, 8192, 0, 0) % (4 * 64) == 0
+    assert L.query('iprgan_mx4_linear_ws_floats', 4, 64, 32, 0, 3) == 4 * 64 and L.query('iprgan_mx4_linear_ws_floats', 4, 64, 32, 0, 2) == 0
     assert L.query('iprgan_mx8_norm_bwd_ws_floats', 1, 100, 64) >= 5 * 64
     assert L.query('iprgan_mx8_norm_bwd_ws_floats', 0, 100, 64) == 0
 
