@@ -150,10 +150,10 @@ struct LinArgs {
 __device__ __forceinline__ float lin_act(float v, int act, float slope) {
   return v > 0.f ? v : act == IPRGAN_ACT_RELU ? 0.f : v * slope;
 }
-__device__ __forceinline__ void store4(const LinArgs& a, int m, int n, f32x4 v) {
+__device__ __forceinline__ void store4(const LinArgs& a, int z, int m, int n, f32x4 v) {
   if (m >= a.M || n >= a.N) return;
   if (a.slab) {
-    float* o = a.slab + ((size_t)blockIdx.z * a.M + m) * a.N + n;
+    float* o = a.slab + ((size_t)z * a.M + m) * a.N + n;
     if (a.vec_y) {
       *(f32x4*)o = v;
     } else {
@@ -186,16 +186,67 @@ __device__ __forceinline__ void store4(const LinArgs& a, int m, int n, f32x4 v) 
   }
 }
 
+// 8 consecutive elements from column c on of a row that starts `row` bytes into the buffer; zero behind column `cols` and behind the
+// buffer (rows past the last one).  No branches: a load that must not happen gets an offset out of range.  (The first version branched,
+// and every branch waited for its own load: 4096^3 bf16 287 us instead of 183.)
+#define OOB 0xfffffff0u
+template <bool BF, bool VEC>
+__device__ __forceinline__ void buf8(__amdgpu_buffer_rsrc_t rs, unsigned row, int c, int cols, float* v) {
+  if constexpr (BF && VEC) {                                  // (cols % 8 == 0: all or nothing)
+    const bf16x8 h = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rs, c < cols ? row + c * 2u : OOB, 0, 0));
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = (float)h[k];
+  } else if constexpr (VEC) {                                 // (cols % 4 == 0)
+    const f32x4 a = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, c < cols ? row + c * 4u : OOB, 0, 0));
+    const f32x4 b = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, c + 4 < cols ? row + c * 4u + 16u : OOB, 0, 0));
+#pragma unroll
+    for (int k = 0; k < 4; ++k) { v[k] = a[k]; v[k + 4] = b[k]; }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if constexpr (BF) v[k] = (float)__builtin_bit_cast(__bf16, (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(rs, c + k < cols ? row + (c + k) * 2u : OOB, 0, 0));
+      else v[k] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, c + k < cols ? row + (c + k) * 4u : OOB, 0, 0));
+    }
+  }
+}
+// the same as loaded: 8 floats, or 8 bf16
+template <bool BF>
+struct Raw8 {
+  f32x4 a, b;
+};
+template <>
+struct Raw8<true> {
+  bf16x8 h;
+};
+template <bool BF, bool VEC>
+__device__ __forceinline__ Raw8<BF> raw8(__amdgpu_buffer_rsrc_t rs, unsigned row, int c, int cols) {
+  Raw8<BF> r;
+  if constexpr (BF && VEC) {
+    r.h = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rs, c < cols ? row + c * 2u : OOB, 0, 0));
+  } else {
+    float v[8];
+    buf8<BF, VEC>(rs, row, c, cols, v);
+    if constexpr (BF) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) r.h[k] = (__bf16)v[k];
+    } else {
+      r.a = f32x4{v[0], v[1], v[2], v[3]};
+      r.b = f32x4{v[4], v[5], v[6], v[7]};
+    }
+  }
+  return r;
+}
+// the rows [r0, r0 + n) of a [rows][cols] matrix as a buffer of its own (32-bit offsets inside; the base is 64-bit)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t row_buffer(const void* base, int r0, int n, int rows, int cols, unsigned esz) {
+  const unsigned long long bytes = (unsigned long long)min(n, rows - r0) * (unsigned)cols * esz;
+  return __builtin_amdgcn_make_buffer_rsrc((void*)((const uint8_t*)base + (size_t)r0 * cols * esz), 0, (int)(unsigned)bytes, 0x00020000);
+}
+
 // 8 fp4 elements (one word) of a block -> bf16, exact (a 4-bit value times a power of two)
 __device__ __forceinline__ bf16x8 widen_fp4(unsigned w, float scale) {
   const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1),
                c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3);
   const bf16x8 r = {a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
-  return r;
-}
-__device__ __forceinline__ bf16x8 nan8() {
-  const __bf16 q = __builtin_bit_cast(__bf16, (unsigned short)0x7fc0);
-  const bf16x8 r = {q, q, q, q, q, q, q, q};
   return r;
 }
 // x in PL bf16 planes: one (bf16 input) or three (fp32 input: x = h + m + l exactly, so the products with the exactly widened weights
@@ -214,16 +265,160 @@ __device__ __forceinline__ void split_planes(const float* v, bf16x8* p) {
   }
 }
 
-// fp32 / bf16 x.  A block is 4 waves: each owns 16 * NF output columns (weights straight from memory to its registers: a lane reads
+template <int PL, class R>
+__device__ __forceinline__ void split_raw(const R& r, bf16x8* p) {
+  if constexpr (PL == 1) {
+    p[0] = r.h;
+  } else {
+    const float v[8] = {r.a[0], r.a[1], r.a[2], r.a[3], r.b[0], r.b[1], r.b[2], r.b[3]};
+    split_planes<3>(v, p);
+  }
+}
+
+// Which tile and K split a block takes.  The XCDs get contiguous runs of (split, tile) pairs - each has its own L2 - and inside a split the
+// tiles go 4 along n, then down m: blocks that share a K range of x, or rows of W, sit on one XCD (4096^3 fp32: 389 -> 381 us).
+struct Place {
+  int n, m, z;
+};
+__device__ __forceinline__ Place place(int tn, int tm) {
+  const unsigned all = gridDim.x, per = all / 8, rem = all % 8, xcd = blockIdx.x % 8;
+  const unsigned id = xcd * per + min(xcd, rem) + blockIdx.x / 8, tiles = (unsigned)tn * tm;
+  const unsigned z = id / tiles, t = id - z * tiles, grp = t / (4u * tm), in = t - grp * 4u * tm, gw = min(4u, tn - grp * 4u);
+  return Place{(int)(grp * 4 + in % gw), (int)(in / gw), (int)z};
+}
+
+// Few rows: 8 waves, WK along K x 8 / WK along n (16 * NF columns each); both operands straight from memory to registers, no barrier before the
+// end, where the WK partial tiles are added in LDS in fixed order - one launch where a split over blocks takes two.  XT: 0 = 4-bit x
+// (the scaled instruction), 1 = bf16, 3 = fp32 (planes).  Bound by latency, or by the split of fp32 x into planes (176 vector instructions a
+// step and 16 rows, repeated by every wave: why more rows go through LDS below).
+template <int MF, int NF, int XT, bool VX>
+__global__ __launch_bounds__(512) void mx4_direct_kernel(const LinArgs a, int tn, int tm, int wk) {
+  constexpr int PL = XT == 3 ? 3 : 1;
+  __shared__ f32x4 red[8][NF * MF][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+  const Place pl = place(tn, tm);
+  const int kw = wave % wk, nw = wave / wk;
+  const int n0 = (pl.n * (8 / wk) + nw) * 16 * NF, m0 = pl.m * 16 * MF;
+  const int s0 = pl.z * a.steps_per_split + kw, s1 = min(a.KB / 4, (pl.z + 1) * a.steps_per_split);
+  f32x4 acc[NF][MF];
+#pragma unroll
+  for (int n = 0; n < NF; ++n)
+#pragma unroll
+    for (int m = 0; m < MF; ++m) acc[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const i32x4 *wp[NF], *xp[MF];
+  const uint8_t *wsp[NF], *xsp[MF];
+#pragma unroll
+  for (int n = 0; n < NF; ++n) {
+    const size_t r = min(n0 + n * 16 + i, a.N - 1);         // rows past the end repeat the last one; their results are not stored
+    wp[n] = (const i32x4*)(a.w + r * a.KB * 16) + g;
+    wsp[n] = a.ws + r * a.KB + g;
+  }
+  constexpr unsigned ESZ = XT == 1 ? 2 : 4;
+  __amdgpu_buffer_rsrc_t rx;
+  if constexpr (XT == 0) {
+#pragma unroll
+    for (int m = 0; m < MF; ++m) {
+      const size_t r = min(m0 + m * 16 + i, a.M - 1);
+      xp[m] = (const i32x4*)((const uint8_t*)a.x + r * a.KB * 16) + g;
+      xsp[m] = a.xs + r * a.KB + g;
+    }
+  } else {
+    rx = row_buffer(a.x, m0, MF * 16, a.M, a.K, ESZ);
+  }
+  i32x4 wq[2][NF], xq[2][MF];
+  int wsc[2][NF], xsc[2][MF];
+  Raw8<XT == 1> xv[2][XT ? MF : 1][4];
+  auto load = [&](int s, int b) {
+#pragma unroll
+    for (int n = 0; n < NF; ++n) { wq[b][n] = wp[n][s * 4]; wsc[b][n] = wsp[n][s * 4]; }
+#pragma unroll
+    for (int m = 0; m < MF; ++m) {
+      if constexpr (XT == 0) {
+        xq[b][m] = xp[m][s * 4];
+        xsc[b][m] = xsp[m][s * 4];
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) xv[b][m][j] = raw8<XT == 1, VX>(rx, (unsigned)(m * 16 + i) * a.K * ESZ, s * 128 + g * 32 + j * 8, a.K);
+      }
+    }
+  };
+  auto mul = [&](int b) {
+    if constexpr (XT == 0) {
+#pragma unroll
+      for (int n = 0; n < NF; ++n)
+#pragma unroll
+        for (int m = 0; m < MF; ++m) {
+          const i32x4 p = wq[b][n], q = xq[b][m];
+          const i32x8 w8 = {p[0], p[1], p[2], p[3], 0, 0, 0, 0}, x8 = {q[0], q[1], q[2], q[3], 0, 0, 0, 0};
+          acc[n][m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w8, x8, acc[n][m], 4, 4, 0, wsc[b][n], 0, xsc[b][m]);
+        }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        bf16x8 wf[NF];
+#pragma unroll
+        for (int n = 0; n < NF; ++n) wf[n] = widen_fp4((unsigned)wq[b][n][j], mx4_step((unsigned)wsc[b][n]));
+#pragma unroll
+        for (int m = 0; m < MF; ++m) {
+          bf16x8 p[PL];
+          split_raw<PL>(xv[b][m][j], p);
+#pragma unroll
+          for (int q = PL - 1; q >= 0; --q)
+#pragma unroll
+            for (int n = 0; n < NF; ++n) acc[n][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[n], p[q], acc[n][m], 0, 0, 0);
+        }
+      }
+    }
+  };
+  if (s0 < s1) load(s0, 0);
+#pragma unroll 1
+  for (int s = s0; s < s1; s += 2 * wk) {
+    if (s + wk < s1) load(s + wk, 1);
+    __builtin_amdgcn_sched_barrier(0);                      // the next step's loads leave before this one is multiplied
+    mul(0);
+    if (s + wk >= s1) break;
+    if (s + 2 * wk < s1) load(s + 2 * wk, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    mul(1);
+  }
+  if (wk > 1) {
+    if (kw) {
+#pragma unroll
+      for (int n = 0; n < NF; ++n)
+#pragma unroll
+        for (int m = 0; m < MF; ++m) red[wave][n * MF + m][lane] = acc[n][m];
+    }
+    __syncthreads();
+    if (kw) return;
+    for (int k = 1; k < wk; ++k)
+#pragma unroll
+      for (int n = 0; n < NF; ++n)
+#pragma unroll
+        for (int m = 0; m < MF; ++m) acc[n][m] += red[wave + k][n * MF + m][lane];
+  }
+#pragma unroll
+  for (int n = 0; n < NF; ++n)
+#pragma unroll
+    for (int m = 0; m < MF; ++m) store4(a, pl.z, m0 + m * 16 + i, n0 + n * 16 + g * 4, acc[n][m]);
+}
+
+// More rows of fp32 / bf16 x.  A block is 4 waves: each owns 16 * NF output columns (weights straight from memory to its registers: a lane reads
 // whole 16-byte blocks, lane group g block g of the step, and the step's four instructions take 8 elements of each block - the order of
 // K is free as long as both operands agree); the 16 * MF rows of x are shared through LDS, split into planes on the way in.
-template <int MF, int NF, int PL>
-__global__ __launch_bounds__(256) void mx4_linear_kernel(const LinArgs a) {
+// (a barrier for LDS alone: __syncthreads would also wait for the loads in flight)
+__device__ __forceinline__ void lds_sync() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+}
+template <int MF, int NF, int PL, bool VX>
+__global__ __launch_bounds__(256) void mx4_linear_kernel(const LinArgs a, int tn, int tm) {
+  constexpr int AHEAD = PL == 1 && NF < 4 ? 2 : 1;
   constexpr int XP = 136;                                   // LDS row pitch in bf16: 16 rows x 4-bank offset, conflict-free fragment reads
   __shared__ __bf16 xs[PL][MF * 16][XP];                    // one buffer: 52 KB at most, three blocks a CU hide each other's barriers
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * 64 * NF + wave * 16 * NF, m0 = blockIdx.y * 16 * MF;
-  const int s0 = blockIdx.z * a.steps_per_split, s1 = min(a.KB / 4, s0 + a.steps_per_split);
+  const Place pl = place(tn, tm);
+  const int n0 = pl.n * 64 * NF + wave * 16 * NF, m0 = pl.m * 16 * MF;
+  const int s0 = pl.z * a.steps_per_split, s1 = min(a.KB / 4, s0 + a.steps_per_split);
   const int xr = threadIdx.x >> 4, xc = (threadIdx.x & 15) * 8;
   f32x4 acc[NF][MF];
 #pragma unroll
@@ -238,120 +433,72 @@ __global__ __launch_bounds__(256) void mx4_linear_kernel(const LinArgs a) {
     wp[n] = (const u32x4*)(a.w + (size_t)row * a.KB * 16) + g;
     sp[n] = a.ws + (size_t)row * a.KB + g;
   }
-  auto load_x = [&](int s, int t, float* v) {
-    const int m = m0 + xr + t * 16, c = s * 128 + xc;
-    if (m < a.M) {
-      if (a.vec_x) ld8<PL == 1, true>(a.x, m, a.K, c, v);
-      else ld8<PL == 1, false>(a.x, m, a.K, c, v);
-    } else {
+  constexpr unsigned ESZ = PL == 1 ? 2 : 4;
+  const __amdgpu_buffer_rsrc_t rx = row_buffer(a.x, m0, MF * 16, a.M, a.K, ESZ);
+  u32x4 wq[NF], wn[AHEAD][NF];
+  unsigned sq[NF], sn[AHEAD][NF];
+  Raw8<PL == 1> xv[AHEAD][MF];
+  auto load = [&](int s, int b) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = 0.f;
-    }
+    for (int n = 0; n < NF; ++n) { wn[b][n] = wp[n][s * 4]; sn[b][n] = sp[n][s * 4]; }
+#pragma unroll
+    for (int t = 0; t < MF; ++t) xv[b][t] = raw8<PL == 1, VX>(rx, (unsigned)(xr + t * 16) * a.K * ESZ, s * 128 + xc, a.K);
   };
-  u32x4 wq[NF], wn[NF];
-  unsigned sq[NF], sn[NF];
-  float xv[MF][8];
-  auto load = [&](int s) {
 #pragma unroll
-    for (int n = 0; n < NF; ++n) { wn[n] = wp[n][s * 4]; sn[n] = sp[n][s * 4]; }
-#pragma unroll
-    for (int t = 0; t < MF; ++t) load_x(s, t, xv[t]);
-  };
-  if (s0 < s1) load(s0);
-  for (int s = s0; s < s1; ++s) {
-    if (s > s0) __syncthreads();                            // every wave has read the last step's planes
+  for (int b = 0; b < AHEAD; ++b)
+    if (s0 + b < s1) load(s0 + b, b);
+  auto step = [&](int s, int b) {
+    if (s > s0) lds_sync();                                 // every wave has read the last step's planes
 #pragma unroll
     for (int t = 0; t < MF; ++t) {
       bf16x8 p[PL];
-      split_planes<PL>(xv[t], p);
+      split_raw<PL>(xv[b][t], p);
 #pragma unroll
       for (int q = 0; q < PL; ++q) *(bf16x8*)&xs[q][xr + t * 16][xc] = p[q];
     }
 #pragma unroll
-    for (int n = 0; n < NF; ++n) { wq[n] = wn[n]; sq[n] = sn[n]; }
-    __syncthreads();
-    if (s + 1 < s1) load(s + 1);                            // in flight while this step is multiplied
+    for (int n = 0; n < NF; ++n) { wq[n] = wn[b][n]; sq[n] = sn[b][n]; }
+    lds_sync();
+    if (s + AHEAD < s1) load(s + AHEAD, b);                 // in flight while AHEAD steps are multiplied
+    // (8 elements j, plane q) pairs in turn, the smallest plane first; x fragments are read D pairs ahead of their use - left to itself the
+    // compiler waits for every read (2048 x 4096 x 4096 fp32: 225 -> 206 us)
+    constexpr int P = 4 * PL, D = PL == 1 ? 3 : 2;
+    bf16x8 xf[D + 1][MF], wf[NF];
+    auto read = [&](int p) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      bf16x8 wf[NF];
+      for (int m = 0; m < MF; ++m) xf[p % (D + 1)][m] = *(const bf16x8*)&xs[PL - 1 - p % PL][m * 16 + i][g * 32 + p / PL * 8];
+    };
 #pragma unroll
-      for (int n = 0; n < NF; ++n) {
-        wf[n] = widen_fp4(wq[n][j], mx4_step(sq[n]));
-        if (sq[n] == 255u) wf[n] = nan8();
+    for (int p = 0; p < D; ++p) read(p);
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      if (p + D < P) read(p + D);
+      if (p % PL == 0) {
+#pragma unroll
+        for (int n = 0; n < NF; ++n) wf[n] = widen_fp4(wq[n][p / PL], mx4_step(sq[n]));
       }
 #pragma unroll
-      for (int q = PL - 1; q >= 0; --q)
+      for (int m = 0; m < MF; ++m)
 #pragma unroll
-        for (int m = 0; m < MF; ++m) {
-          const bf16x8 xf = *(const bf16x8*)&xs[q][m * 16 + i][g * 32 + j * 8];
-#pragma unroll
-          for (int n = 0; n < NF; ++n) acc[n][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[n], xf, acc[n][m], 0, 0, 0);
-        }
+        for (int n = 0; n < NF; ++n) acc[n][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[n], xf[p % (D + 1)][m], acc[n][m], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
     }
+  };
+#pragma unroll 1
+  for (int s = s0; s < s1; s += AHEAD) {
+#pragma unroll
+    for (int b = 0; b < AHEAD; ++b)
+      if (s + b < s1) step(s + b, b);
   }
 #pragma unroll
   for (int n = 0; n < NF; ++n)
 #pragma unroll
-    for (int m = 0; m < MF; ++m) store4(a, m0 + m * 16 + i, n0 + n * 16 + g * 4, acc[n][m]);
+    for (int m = 0; m < MF; ++m) store4(a, pl.z, m0 + m * 16 + i, n0 + n * 16 + g * 4, acc[n][m]);
 }
 
-// ---- 4-bit x -------------------------------------------------------------------------------------------------------------------
+// ---- many rows of 4-bit x -----------------------------------------------------------------------------------------------------------
 // The scaled matrix instruction multiplies 128 elements of K at once: a lane holds one 16-byte block of its row (i = lane & 15, block
 // g = lane >> 4 of the step) and that block's scale byte, for each operand.
-
-// Few rows (M <= 64): both operands straight from memory, the block's waves side by side along n, K split over blocks.
-template <int MF, int NF>
-__global__ __launch_bounds__(256) void mx4_linear4_kernel(const LinArgs a) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
-  const int n0 = (blockIdx.x * 4 + wave) * 16 * NF, m0 = blockIdx.y * 16 * MF;
-  const int s0 = blockIdx.z * a.steps_per_split, s1 = min(a.KB / 4, s0 + a.steps_per_split);
-  f32x4 acc[NF][MF];
-#pragma unroll
-  for (int n = 0; n < NF; ++n)
-#pragma unroll
-    for (int m = 0; m < MF; ++m) acc[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const i32x4 *wp[NF], *xp[MF];
-  const uint8_t *wsp[NF], *xsp[MF];
-#pragma unroll
-  for (int t = 0; t < NF; ++t) {
-    const size_t r = min(n0 + t * 16 + i, a.N - 1);          // rows past the end repeat the last one; their results are not stored
-    wp[t] = (const i32x4*)(a.w + r * a.KB * 16) + g;
-    wsp[t] = a.ws + r * a.KB + g;
-  }
-#pragma unroll
-  for (int t = 0; t < MF; ++t) {
-    const size_t r = min(m0 + t * 16 + i, a.M - 1);
-    xp[t] = (const i32x4*)((const uint8_t*)a.x + r * a.KB * 16) + g;
-    xsp[t] = a.xs + r * a.KB + g;
-  }
-#pragma unroll 2
-  for (int s = s0; s < s1; ++s) {
-    i32x8 wf[NF], xf[MF];
-    int wsc[NF], xsc[MF];
-#pragma unroll
-    for (int t = 0; t < NF; ++t) {
-      const i32x4 p = wp[t][s * 4];
-      wf[t] = i32x8{p[0], p[1], p[2], p[3], 0, 0, 0, 0};
-      wsc[t] = wsp[t][s * 4];
-    }
-#pragma unroll
-    for (int t = 0; t < MF; ++t) {
-      const i32x4 p = xp[t][s * 4];
-      xf[t] = i32x8{p[0], p[1], p[2], p[3], 0, 0, 0, 0};
-      xsc[t] = xsp[t][s * 4];
-    }
-#pragma unroll
-    for (int n = 0; n < NF; ++n)
-#pragma unroll
-      for (int m = 0; m < MF; ++m)
-        acc[n][m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[n], xf[m], acc[n][m], 4, 4, 0, wsc[n], 0, xsc[m]);
-  }
-#pragma unroll
-  for (int n = 0; n < NF; ++n)
-#pragma unroll
-    for (int m = 0; m < MF; ++m) store4(a, m0 + m * 16 + i, n0 + n * 16 + g * 4, acc[n][m]);
-}
-
 typedef __attribute__((address_space(3))) void lds_void;
 template <int BYTES>
 __device__ __forceinline__ void lds_dma(__amdgpu_buffer_rsrc_t rs, unsigned lds, unsigned voff, unsigned soff) {
@@ -520,7 +667,7 @@ __global__ __launch_bounds__(WN* WM * 64, 2) void mx4_gemm4_kernel(const LinArgs
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) store4(a, m0 + m * 16, n0 + n * 16 + g * 4, acc[n][m]);
+        for (int n = 0; n < NT; ++n) store4(a, blockIdx.z, m0 + m * 16, n0 + n * 16 + g * 4, acc[n][m]);
     }
   }
 }
@@ -589,13 +736,16 @@ struct BwdArgs {
   float* slab;                 // [splits][M][K] when the rows n are split over blocks
   int M, N, K, KB, steps_per_wave, dx_bf16, vec_dy, vec_dx;       // a step is 32 rows of W
 };
-template <int MF, int PL>
-__global__ __launch_bounds__(256) void mx4_linear_bwd_kernel(const BwdArgs a) {
+template <int MF, int PL, bool VX>
+__global__ __launch_bounds__(256) void mx4_linear_bwd_kernel(const BwdArgs a, int tk, int tm) {
   __shared__ float tile[4][16][132];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
-  const int k0 = blockIdx.x * 128, m0 = blockIdx.y * 16 * MF;
+  const Place pl = place(tk, tm);
+  const int k0 = pl.n * 128, m0 = pl.m * 16 * MF;
+  constexpr unsigned ESZ = PL == 1 ? 2 : 4;
+  const __amdgpu_buffer_rsrc_t rd = row_buffer(a.dy, m0, MF * 16, a.M, a.N, ESZ);
   const int steps = (a.N + 31) / 32;
-  const int s0 = (blockIdx.z * 4 + wave) * a.steps_per_wave, s1 = min(steps, s0 + a.steps_per_wave);
+  const int s0 = (pl.z * 4 + wave) * a.steps_per_wave, s1 = min(steps, s0 + a.steps_per_wave);
   f32x4 acc[8][MF];
 #pragma unroll
   for (int j = 0; j < 8; ++j)
@@ -614,14 +764,7 @@ __global__ __launch_bounds__(256) void mx4_linear_bwd_kernel(const BwdArgs a) {
 #pragma unroll
     for (int m = 0; m < MF; ++m) {
       float v[8];
-      const int mm = m0 + m * 16 + i;
-      if (mm < a.M) {
-        if (a.vec_dy) ld8<PL == 1, true>(a.dy, mm, a.N, nb, v);
-        else ld8<PL == 1, false>(a.dy, mm, a.N, nb, v);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = 0.f;
-      }
+      buf8<PL == 1, VX>(rd, (unsigned)(m * 16 + i) * a.N * ESZ, nb, a.N, v);
       split_planes<PL>(v, xf[m]);
     }
 #pragma unroll
@@ -637,7 +780,7 @@ __global__ __launch_bounds__(256) void mx4_linear_bwd_kernel(const BwdArgs a) {
           case 2: t = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(wq[r], step, 2); break;
           default: t = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(wq[r], step, 3); break;
         }
-        p[r] = sc[r] == 255u ? 0x7fc07fc0u : __builtin_bit_cast(unsigned, t);
+        p[r] = __builtin_bit_cast(unsigned, t);
       }
       u32x4 lo, hi;
 #pragma unroll
@@ -670,7 +813,7 @@ __global__ __launch_bounds__(256) void mx4_linear_bwd_kernel(const BwdArgs a) {
       float v[8];
 #pragma unroll
       for (int q = 0; q < 8; ++q) v[q] = (tile[0][mm][kk + q] + tile[1][mm][kk + q]) + (tile[2][mm][kk + q] + tile[3][mm][kk + q]);
-      const size_t o = ((size_t)(a.slab ? blockIdx.z : 0) * a.M + row) * a.K + k;
+      const size_t o = ((size_t)(a.slab ? pl.z : 0) * a.M + row) * a.K + k;
       if (a.slab || !a.dx_bf16) {
         float* d = a.slab ? a.slab : (float*)a.dx;
         if (a.vec_dx && k + 8 <= a.K) {
@@ -728,37 +871,58 @@ static int gemm4_go(const LinArgs& a, int tn, int tm, int splits, hipStream_t st
   return 0;
 }
 
-// how the product is cut: 16 * mf rows x 64 * nf columns a block, or (4-bit x of more than 64 rows) square tiles of `tile`; K over `splits` blocks
+// How the product is cut.
+//   direct (4-bit x: M <= 64; else M <= 16, K <= 4096 and not too many columns): 16 * mf rows x 16 * nf * (8 / wk) columns a block, wk waves along K
+//   tile   (4-bit x of more rows): square tiles, 256 where they fill three quarters of the chip, else 128
+//   LDS    (the rest): 16 * mf rows x 64 * nf columns a block
+// Direct against LDS, wall time: 1 x 4096 x 4096 fp32 13.5 : 19.5 us (one launch instead of two), 8 x 4096 x 16384 bf16 16.3 : 19.0, but
+// 8 x 4096 x 16384 fp32 25.3 : 20.4 (every wave splits x again) and 16 x 18432 x 1024 bf16 26.9 : 18.4 (18 steps in a row).
+// and K over `splits` blocks, chosen by an estimate in us: a block's steps at its measured time a step, against the slabs' traffic at 4 TB/s
+// and a second launch.
 struct LinPlan {
-  int mf, nf, tile, s16, tm, tn, splits, steps_per_split;
+  int mf, nf, wk, tile, s16, tm, tn, splits, steps_per_split;
 };
+static void lin_split(LinPlan& p, int M, int N, int steps, double step_us, int unit) {
+  const double tiles = (double)p.tm * p.tn;
+  double best = 1e30;
+  for (int want = 1; want <= 64 && want <= steps; want = want < 8 ? want + 1 : want + want / 4) {
+    const int per = rup(cdiv(steps, want), unit), splits = cdiv(steps, per);
+    const double load = 0.6 * ((long long)((tiles * splits + 255) / 256));           // blocks a CU: two overlap to 0.6 of their sum
+    const double t = (per * step_us) * (load > 1 ? load : 1) + (splits > 1 ? 5.0 + (double)splits * M * N * 2e-6 : 0.0);
+    if (t < best) {
+      best = t;
+      p.steps_per_split = per;
+      p.splits = splits;
+    }
+  }
+}
 static LinPlan lin_plan(int M, int N, int K, int x_kind) {
   LinPlan p;
+  memset(&p, 0, sizeof(p));
   const int steps = kb_of(K) / 4;
   p.mf = M <= 16 ? 1 : M <= 32 ? 2 : 4;
-  p.nf = p.mf == 1 ? 1 : 2;
-  p.tile = p.s16 = 0;
-  long long full = 512;                                       // blocks that fill the chip: two a CU
-  if (x_kind == IPRGAN_X_MX4 && M > 64) {
+  if (x_kind == IPRGAN_X_MX4 ? M <= 64 : M <= 16 && steps <= 32 && (long long)steps * N <= (x_kind == IPRGAN_X_F32 ? 200000 : 600000)) {
+    p.wk = 1;
+    while (p.wk < 8 && p.wk * 2 <= steps) p.wk *= 2;
+    p.nf = N >= 256 * 32 * (8 / p.wk) ? 2 : 1;              // two fragments a wave once that leaves a block for every CU
+    p.tm = cdiv(M, 16 * p.mf);
+    p.tn = cdiv(N, 16 * p.nf * (8 / p.wk));
+    lin_split(p, M, N, steps, (x_kind == IPRGAN_X_F32 ? 0.6 : 0.35) / p.wk, p.wk);
+  } else if (x_kind == IPRGAN_X_MX4) {
     p.tile = (long long)cdiv(M, 256) * cdiv(N, 256) >= 192 ? 256 : 128;
+    p.s16 = steps % 4 == 0;                                 // the form that moves the scales of four stages at once
     p.tm = cdiv(M, p.tile);
     p.tn = cdiv(N, p.tile);
-    if (p.tile == 256) full = 1;
+    lin_split(p, M, N, steps, p.tile == 256 ? 1.1 : 0.4, p.s16 ? 4 : 1);
   } else {
+    p.nf = p.mf == 1 ? 1 : 2;
+    // four fragments a wave halve the LDS reads a multiplication once two blocks a CU are left: 4096^3 fp32 450 -> 400 us, but 1000 x
+    // 3000 x 5000 (320 blocks) 119 -> 131
+    if (p.mf == 4 && (long long)cdiv(M, 64) * cdiv(N, 256) >= 512) p.nf = 4;
     p.tm = cdiv(M, 16 * p.mf);
     p.tn = cdiv(N, 64 * p.nf);
+    lin_split(p, M, N, steps, x_kind == IPRGAN_X_F32 ? 0.6 + 0.125 * p.mf * p.nf : 0.6 + 0.05 * p.mf * p.nf, 1);
   }
-  const long long tiles = (long long)p.tm * p.tn;
-  int want = tiles >= full ? 1 : (int)(full / tiles);
-  if (want > 64) want = 64;
-  if (want > steps) want = steps;
-  if (want < 1) want = 1;
-  p.steps_per_split = cdiv(steps, want);
-  if (p.tile && steps % 4 == 0) {                             // the form that moves the scales of four stages at once
-    p.s16 = 1;
-    p.steps_per_split = rup(p.steps_per_split, 4);
-  }
-  p.splits = cdiv(steps, p.steps_per_split);
   return p;
 }
 struct BwdPlan {
@@ -830,7 +994,8 @@ int iprgan_mx4_dequant(const void* codes, const void* scales, void* y, int rows,
 
 static int lin_check(const char* who, int M, int N, int K) {
   IPR_CHECK(M > 0 && N > 0 && K > 0, "%s: empty product (M=%d, N=%d, K=%d)", who, M, N, K);
-  IPR_CHECK(K <= (1 << 24) && M <= (1 << 20) && N <= (1 << 28), "%s: M=%d, N=%d, K=%d (at most 2^20, 2^28, 2^24)", who, M, N, K);
+  // 64 rows of x and dy are addressed through 32-bit offsets
+  IPR_CHECK(K < (1 << 24) && M <= (1 << 20) && N < (1 << 24), "%s: M=%d, N=%d, K=%d (M at most 2^20, N and K below 2^24)", who, M, N, K);
   return 0;
 }
 
@@ -854,7 +1019,7 @@ int iprgan_mx4_linear(const void* x, const void* x_scales, const void* w_codes, 
                 (x_kind != IPRGAN_X_MX4 || aligned(x_scales, 4)) && aligned(y, y_bf16 ? 2 : 4),
             "mx4_linear: codes must be 16-byte, scales 4-byte aligned");
   const LinPlan p = lin_plan(M, N, K, x_kind);
-  IPR_CHECK(p.tm <= 65535 && (long long)p.tm * p.tn < 0x7fffffffll, "mx4_linear: M=%d, N=%d", M, N);
+  IPR_CHECK((long long)p.tm * p.tn * p.splits < 0x7fffffffll, "mx4_linear: M=%d, N=%d", M, N);
   const bool slab = lin_slab(p, act);
   IPR_CHECK(!slab || (ws && aligned(ws, 16)), "mx4_linear: the workspace of iprgan_mx4_linear_ws_floats is missing");
   hipStream_t st = (hipStream_t)stream;
@@ -866,22 +1031,24 @@ int iprgan_mx4_linear(const void* x, const void* x_scales, const void* w_codes, 
   a.vec_x = K % (x_kind == IPRGAN_X_BF16 ? 8 : 4) == 0 && aligned(x, 16);
   a.vec_y = N % 4 == 0 && (a.slab || aligned(y, y_bf16 ? 8 : 16));
   a.vec8 = y_bf16 && N % 8 == 0 && aligned(y, 16);
-  const dim3 grid(p.tn, p.tm, p.splits), blk(256);
-  if (x_kind == IPRGAN_X_MX4) {
-    if (p.tile) {
-      const int rc = p.tile == 256 ? (p.s16 ? gemm4_go<256, 256, 2, 4, true>(a, p.tn, p.tm, p.splits, st) : gemm4_go<256, 256, 2, 4, false>(a, p.tn, p.tm, p.splits, st))
-                                   : (p.s16 ? gemm4_go<128, 128, 2, 2, true>(a, p.tn, p.tm, p.splits, st) : gemm4_go<128, 128, 2, 2, false>(a, p.tn, p.tm, p.splits, st));
-      if (rc) return rc;
-    } else {
-      auto k = p.mf == 1 ? mx4_linear4_kernel<1, 1> : p.mf == 2 ? mx4_linear4_kernel<2, 2> : mx4_linear4_kernel<4, 2>;
-      hipLaunchKernelGGL(k, grid, blk, 0, st, a);
-    }
-  } else if (x_kind == IPRGAN_X_BF16) {
-    auto k = p.mf == 1 ? mx4_linear_kernel<1, 1, 1> : p.mf == 2 ? mx4_linear_kernel<2, 2, 1> : mx4_linear_kernel<4, 2, 1>;
-    hipLaunchKernelGGL(k, grid, blk, 0, st, a);
+  const dim3 grid((unsigned)p.tn * p.tm * p.splits);
+  const bool vx = a.vec_x;
+  if (p.tile) {
+    const int rc = p.tile == 256 ? (p.s16 ? gemm4_go<256, 256, 2, 4, true>(a, p.tn, p.tm, p.splits, st) : gemm4_go<256, 256, 2, 4, false>(a, p.tn, p.tm, p.splits, st))
+                                 : (p.s16 ? gemm4_go<128, 128, 2, 2, true>(a, p.tn, p.tm, p.splits, st) : gemm4_go<128, 128, 2, 2, false>(a, p.tn, p.tm, p.splits, st));
+    if (rc) return rc;
+  } else if (p.wk) {
+#define DIRECT(MF, XT, VX) (p.nf == 2 ? mx4_direct_kernel<MF, 2, XT, VX> : mx4_direct_kernel<MF, 1, XT, VX>)
+    auto k = x_kind == IPRGAN_X_F32    ? (vx ? DIRECT(1, 3, true) : DIRECT(1, 3, false))
+             : x_kind == IPRGAN_X_BF16 ? (vx ? DIRECT(1, 1, true) : DIRECT(1, 1, false))
+                                       : (p.mf == 1 ? DIRECT(1, 0, true) : p.mf == 2 ? DIRECT(2, 0, true) : DIRECT(4, 0, true));
+#undef DIRECT
+    hipLaunchKernelGGL(k, grid, dim3(512), 0, st, a, p.tn, p.tm, p.wk);
   } else {
-    auto k = p.mf == 1 ? mx4_linear_kernel<1, 1, 3> : p.mf == 2 ? mx4_linear_kernel<2, 2, 3> : mx4_linear_kernel<4, 2, 3>;
-    hipLaunchKernelGGL(k, grid, blk, 0, st, a);
+#define LDSX(PL, VX) (p.mf == 1 ? mx4_linear_kernel<1, 1, PL, VX> : p.mf == 2 ? mx4_linear_kernel<2, 2, PL, VX> : p.nf == 2 ? mx4_linear_kernel<4, 2, PL, VX> : mx4_linear_kernel<4, 4, PL, VX>)
+    auto k = x_kind == IPRGAN_X_BF16 ? (vx ? LDSX(1, true) : LDSX(1, false)) : (vx ? LDSX(3, true) : LDSX(3, false));
+#undef LDSX
+    hipLaunchKernelGGL(k, grid, dim3(256), 0, st, a, p.tn, p.tm);
   }
   IPR_LAUNCH_CHECK();
   return slab ? slab_reduce(ws, p.splits, M, N, bias, y, act, slope, y_bf16, st) : 0;
@@ -901,7 +1068,7 @@ int iprgan_mx4_linear_bwd(const void* dy, const void* w_codes, const void* w_sca
   IPR_CHECK(aligned(w_codes, 16) && aligned(w_scales, 4) && aligned(dy, dy_bf16 ? 2 : 4) && aligned(dx, dx_bf16 ? 2 : 4),
             "mx4_linear_bwd: codes must be 16-byte, scales 4-byte aligned");
   const BwdPlan p = bwd_plan(M, N, K);
-  IPR_CHECK(p.tm <= 65535, "mx4_linear_bwd: M=%d", M);
+  IPR_CHECK((long long)p.tm * p.tk * p.splits < 0x7fffffffll, "mx4_linear_bwd: M=%d, K=%d", M, K);
   IPR_CHECK(p.splits == 1 || (ws && aligned(ws, 16)), "mx4_linear_bwd: the workspace of iprgan_mx4_linear_bwd_ws_floats is missing");
   hipStream_t st = (hipStream_t)stream;
   BwdArgs a;
@@ -910,10 +1077,12 @@ int iprgan_mx4_linear_bwd(const void* dy, const void* w_codes, const void* w_sca
   a.M = M; a.N = N; a.K = K; a.KB = kb_of(K); a.steps_per_wave = p.steps_per_wave; a.dx_bf16 = dx_bf16;
   a.vec_dy = N % (dy_bf16 ? 8 : 4) == 0 && aligned(dy, 16);
   a.vec_dx = K % (a.slab || !dx_bf16 ? 4 : 8) == 0 && (a.slab || aligned(dx, 16));
-  const dim3 grid(p.tk, p.tm, p.splits), blk(256);
-  auto k = dy_bf16 ? (p.mf == 1 ? mx4_linear_bwd_kernel<1, 1> : mx4_linear_bwd_kernel<2, 1>)
-                   : (p.mf == 1 ? mx4_linear_bwd_kernel<1, 3> : mx4_linear_bwd_kernel<2, 3>);
-  hipLaunchKernelGGL(k, grid, blk, 0, st, a);
+  const dim3 grid((unsigned)p.tk * p.tm * p.splits), blk(256);
+  auto k = dy_bf16 ? (a.vec_dy ? (p.mf == 1 ? mx4_linear_bwd_kernel<1, 1, true> : mx4_linear_bwd_kernel<2, 1, true>)
+                               : (p.mf == 1 ? mx4_linear_bwd_kernel<1, 1, false> : mx4_linear_bwd_kernel<2, 1, false>))
+                   : (a.vec_dy ? (p.mf == 1 ? mx4_linear_bwd_kernel<1, 3, true> : mx4_linear_bwd_kernel<2, 3, true>)
+                               : (p.mf == 1 ? mx4_linear_bwd_kernel<1, 3, false> : mx4_linear_bwd_kernel<2, 3, false>));
+  hipLaunchKernelGGL(k, grid, blk, 0, st, a, p.tk, p.tm);
   IPR_LAUNCH_CHECK();
   return p.splits > 1 ? slab_reduce(ws, p.splits, M, K, nullptr, dx, IPRGAN_ACT_NONE, 0.f, dx_bf16, st) : 0;
 }

@@ -241,7 +241,7 @@ class Mx8(_Packed):
     __slots__ = ('kind', '_n')
 
     def __init__(self, codes, scales, shape, kind=ST_F32):
-        shape = tuple(int(v) for v in shape)
+        shape = tuple(shape)
         n = 1
         for v in shape:
             n *= v
@@ -373,7 +373,7 @@ class Mx4(_Packed):
     __slots__ = ()
 
     def __init__(self, codes, scales, shape):
-        rows, cols = (int(v) for v in shape)
+        rows, cols = shape
         kb = 4 * ((cols + 127) // 128)
         if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
             raise RuntimeError(f'Mx4: uint8 codes and scales expected (got {codes.dtype}, {scales.dtype})')
