@@ -37,6 +37,7 @@ __device__ __forceinline__ unsigned cvt_pk_bf16(float a, float b) {          // 
   return __builtin_bit_cast(unsigned, __builtin_convertvector(v, bf16x2_t));
 }
 __device__ __forceinline__ void split3_pair(float x0, float x1, unsigned& hp, unsigned& mp, unsigned& lp) {
+#pragma clang fp contract(off)      // (x - h is the remainder of the ROUNDED x: not to be fused into a product that formed x)
   hp = cvt_pk_bf16(x0, x1);
   const float r0 = x0 - __builtin_bit_cast(float, hp << 16), r1 = x1 - __builtin_bit_cast(float, hp & 0xffff0000u);
   mp = cvt_pk_bf16(r0, r1);

@@ -110,6 +110,7 @@ __device__ __forceinline__ float4 ld4e(const float* p, size_t i, int b16, size_t
   return *(const float4*)(p + i);
 }
 __device__ __forceinline__ void st4e(float* p, size_t i, float4 v, int b16, size_t ps = 0) {
+#pragma clang fp contract(off)
   if (b16 == 2) {
     typedef __bf16 h4 __attribute__((ext_vector_type(4)));
     __bf16* b = (__bf16*)p + i;
@@ -421,6 +422,7 @@ __device__ __forceinline__ ew_f4 ew_ld(const float* base, size_t e, int st, size
   return *(const ew_f4*)(base + e);
 }
 __device__ __forceinline__ void ew_st(float* base, size_t e, const ew_f4& v, int st, size_t ps) {
+#pragma clang fp contract(off)
   if (st == 2) {
     __bf16* b = (__bf16*)base + e;
     const ew_b4 h = ew_narrow(v);
@@ -765,6 +767,7 @@ __global__ __launch_bounds__(256) void reflect_fold_kernel(const rf_f4* __restri
       for (int k = 0; k < 4; ++k) s[k] *= act_grad_from_out(o[k], prev_act, prev_slope);
     }
     if (okind == 2) {
+#pragma clang fp contract(off)
       const size_t e = (size_t)i * 4;
       if (residual) s += ldb(residual, e) + (ldb(residual, e + ps) + ldb(residual, e + 2 * ps));
       const rf_b4 h = {(__bf16)s.x, (__bf16)s.y, (__bf16)s.z, (__bf16)s.w};
@@ -830,6 +833,7 @@ __global__ __launch_bounds__(256) void reflect_ring_fix_kernel(const rf_f4* __re
       for (int k = 0; k < 4; ++k) s[k] *= act_grad_from_out(o[k], prev_act, prev_slope);
     }
     if (okind == 2) {
+#pragma clang fp contract(off)
       s += ldb(dx, e) + (ldb(dx, e + ps) + ldb(dx, e + 2 * ps));
       const rf_b4 h = {(__bf16)s.x, (__bf16)s.y, (__bf16)s.z, (__bf16)s.w};
       const rf_f4 hf = {(float)h.x, (float)h.y, (float)h.z, (float)h.w};

@@ -71,6 +71,7 @@ __device__ __forceinline__ void ldv(const void* base, size_t e, size_t ps, float
 }
 template <int ST, int V>
 __device__ __forceinline__ void stv(void* base, size_t e, size_t ps, const float* v) {
+#pragma clang fp contract(off)      // v is the fp32 value every storage kind holds: no v - h fused into the product that formed v
   if constexpr (ST == IPRGAN_ST_F32) {
 #pragma unroll
     for (int k = 0; k < V; k += 4) {
@@ -99,6 +100,7 @@ __device__ __forceinline__ float ld1(const void* base, size_t e, size_t ps) {
 }
 template <int ST>
 __device__ __forceinline__ void st1(void* base, size_t e, size_t ps, float v) {
+#pragma clang fp contract(off)
   if constexpr (ST == IPRGAN_ST_F32) { ((float*)base)[e] = v; return; }
   __bf16* b = (__bf16*)base + e;
   const __bf16 h = (__bf16)v;

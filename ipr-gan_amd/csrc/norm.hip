@@ -36,6 +36,7 @@ __device__ __forceinline__ f32x4 ldv(const float* base, size_t e, size_t ps) {
 }
 template <int ST>
 __device__ __forceinline__ void stv(float* base, size_t e, const f32x4& v, size_t ps) {
+#pragma clang fp contract(off)      // v is the fp32 value every storage kind holds: no v - h fused into the product that formed v
   if (ST == 2) {
     __bf16* b = (__bf16*)base + e;
     const nbf16x4 h = narrow4(v);
