@@ -1,6 +1,6 @@
 """Removal attacks of the reference's evaluation scripts, as library functions.
 
-``sign_flip_`` is the loop body of sign_flip.py:59-75, ``prune_`` the one of prune.py:46-57; both act on the
+``quantize_`` is a removal attack the reference does not have (weight compression to 4 bits).  ``sign_flip_`` is the loop body of sign_flip.py:59-75, ``prune_`` the one of prune.py:46-57; both act on the
 generator whose BatchNorm / InstanceNorm scales carry the watermark, and are followed in the reference by
 ``SignLossModel.compute_ber`` (experiments/image_generation.py:161-164) - here the exact int64 count kernel
 ``iprgan_sign_ber``.  ``matching_p_value`` is tools/phash_pvalue.py:34-37 (the hash itself is the third-party
@@ -9,7 +9,7 @@ import numpy as np
 import torch
 import torch.nn as nn
 
-__all__ = ['norm_scales', 'sign_flip_', 'prune_', 'matching_p_value']
+__all__ = ['norm_scales', 'sign_flip_', 'prune_', 'quantize_', 'matching_p_value']
 
 _NORMS = (nn.BatchNorm2d, nn.InstanceNorm2d)
 
@@ -44,6 +44,23 @@ def prune_(state_dict, percent):
     for v in state_dict.values():
         v[v.abs() < threshold] = 0
     return float(threshold)
+
+
+@torch.no_grad()
+def quantize_(net):
+    """Rounds, in place, every weight matrix / kernel of a network on the GPU (parameters of two or more dimensions, seen as
+    [shape[0], rest]) to its microscaled 4-bit values (ops.mx4_quant): removal by compression.  Biases and norm scales - where the
+    sign watermark lives - stay, as in any weight-only compression.  Returns (bytes before, bytes of the 4-bit form)."""
+    from . import ops
+    before = after = 0
+    for p in net.parameters():
+        if p.dim() < 2:
+            continue
+        q = ops.mx4_quant(p.detach().contiguous())
+        p.copy_(ops.mx4_dequant(q, p.dtype).view(p.shape))
+        before += p.numel() * p.element_size()
+        after += q.shape[0] * (17 * 4 * ((q.shape[1] + 127) // 128))
+    return before, after
 
 
 def matching_p_value(hash_x, hash_y):

@@ -48,11 +48,12 @@ class Config(object):
 #     fuse_stats: true       # norm statistics / bias gradients from conv epilogues (IPRGAN_FUSE_STATS)
 #     pair_d: true           # D(real) and D(fake) as one paired pass              (IPRGAN_PAIR_D)
 #     batch_passes: true     # same-network passes of CycleGAN batched             (IPRGAN_BATCH_PASSES)
+#     ckpt8: true            # activations kept for the backward pass in 8 bits       (IPRGAN_CKPT8)
 #     graph: true            # ImageGeneration: the whole step as one captured HIP graph (graphs.py); one rank only, unless
 #     graph_ddp: true        #   ... this opts a data-parallel run in (the exchange through the C ABI's communicator is captured
 #                            #   with the step; every rank captures or every rank stays eager; unproven on real multi-GPU RCCL)
 ENGINE_KEYS = ('math', 'bucket_mb', 'comm', 'comm_timeout', 'tune_cache', 'fuse_stats', 'pair_d', 'batch_passes', 'graph',
-               'graph_ddp')
+               'graph_ddp', 'ckpt8')
 
 
 def apply_engine(config, set_math=True):
@@ -82,7 +83,8 @@ def apply_engine(config, set_math=True):
     from . import engine as _engine, models as _models
     for key, env, mod, attr in (('fuse_stats', 'IPRGAN_FUSE_STATS', _engine, '_FUSE_STATS'),
                                 ('pair_d', 'IPRGAN_PAIR_D', _models, '_PAIR_D'),
-                                ('batch_passes', 'IPRGAN_BATCH_PASSES', _models, '_BATCH_PASSES')):
+                                ('batch_passes', 'IPRGAN_BATCH_PASSES', _models, '_BATCH_PASSES'),
+                                ('ckpt8', 'IPRGAN_CKPT8', _engine, '_CKPT8')):
         if key in blk:
             os.environ[env] = '1' if blk[key] else '0'
             setattr(mod, attr, bool(blk[key]))

@@ -25,6 +25,12 @@ _FUSE_STATS = os.environ.get('IPRGAN_FUSE_STATS', '1') != '0'       # A/B switch
 # 17.68 ms, SRGAN 33.30 -> 33.53 ms, DCGAN-64 11.52 -> 11.53 ms (round 3, same box, back to back).
 _FUSE_BN_BWD = os.environ.get('IPRGAN_FUSE_BN_BWD', '0') != '0'
 _GEMV_PAIR = os.environ.get('IPRGAN_GEMV_PAIR', '1') != '0'        # A/B switch: the head of a paired pass in one launch per kernel
+# Activation checkpoints in 8 bits (`engine: {ckpt8: true}`): what a recorded pass keeps for its backward pass - inputs of convolutions
+# and norm layers, outputs behind activations - is held as ops.Mx8 (1.03 bytes an element instead of 4 or 6).  The norm layers' and
+# the stand-alone activations' backward passes read the codes; the other ops get the tensor back for the time of their own backward.
+# The forward pass is untouched; gradients see activations rounded to 1/127 of their block's maximum.
+_CKPT8 = os.environ.get('IPRGAN_CKPT8', '0') == '1'
+_CKPT8_MIN = 1 << 14        # elements: a smaller tensor stays as it is (64 KB are not worth two launches)
 
 
 class Op:
@@ -286,8 +292,31 @@ class LinearNHWC(Op):
         p = self.m._parameters
         return (p['weight'], p['bias'])
 
+    def _weights_key(self):
+        w, b = self.weight, self.bias
+        return (w._version, w.data_ptr(), b._version, b.data_ptr())
+
+    def quantize(self, on=True):
+        """A 4-bit copy of the weights, rows in NHWC order, for passes in eval mode (networks: quantize_dense)."""
+        if not on:
+            self.__dict__.pop('_mx4', None)
+            return
+        K = self.weight.shape[1]
+        w = ops.permute_021(self.weight, self.C, self.HW, K).view(self.C * self.HW, K)
+        self._mx4 = (self._weights_key(), ops.mx4_quant(w), ops.permute_021(self.bias, self.C, self.HW, 1))
+
     def forward(self, x, st, train):
         B, K = x.shape
+        if not train and '_mx4' in self.__dict__:
+            key, w4, bias = self._mx4
+            if key != self._weights_key():
+                raise RuntimeError('the weights changed after quantize_dense(): its 4-bit copy is out of date (call it again, or quantize_dense(False))')
+            k = ops.act_kind(self.C)
+            y = ops.mx4_linear(x.contiguous(), w4, bias, self.spec.act, self.spec.slope, dtype=torch.bfloat16 if k == ops.ST_BF16 else torch.float32)
+            if k == ops.ST_X3 and y.numel() * 6 < 0x7fffffff:
+                y = ops.to_kind(y, k)
+            st.update(x=x, y=y, mx4=w4)
+            return y
         if x.dtype == torch.float32 and ops.fc_nhwc_ok(B, K, self.C, self.HW):
             # one launch on the parameters as they are (csrc/fc.hip): no permuted copy, no prepared operand, no split of x
             x = x.contiguous()
@@ -312,6 +341,13 @@ class LinearNHWC(Op):
 
     def backward(self, dy, st, need_dx, need_w, prev_act, sink=None):
         sp = self.spec
+        if 'mx4' in st:
+            if need_w:
+                raise RuntimeError('a layer served from its 4-bit copy has no weight gradient: requires_grad_(False) on its parameters, or quantize_dense(False)')
+            if not need_dx:
+                return None, []
+            dz = dy if st.get('dy_is_preact', False) else ops.act_bwd(dy, st['y'], sp.act, sp.slope)
+            return ops.mx4_linear_bwd(ops.f32(dz).view(st['x'].shape[0], -1), st['mx4'], dtype=torch.float32), []
         if st.get('direct'):
             act = L.ACT_NONE if st.get('dy_is_preact', False) else sp.act
             grads = []
@@ -692,13 +728,48 @@ class Chain:
                     break
             if red is not None:
                 red.note_forward()
-        return ChainFn.apply(self, (bool(train), red, bool(pair)), x, *params)
+        return ChainFn.apply(self, (bool(train), red, bool(pair), _CKPT8 and torch.is_grad_enabled()), x, *params)
+
+
+def _pack_saved(ops_list, stash, i, last):
+    """ckpt8: the tensors that ops up to ``i`` saved and the forward pass has finished with -> Mx8.  The output of an op and the input
+    of the next are one tensor: packed once, when its consumer is done.  A max pool keeps its input (and with it that output) exact: its
+    backward pass looks for the position of the maximum, which rounding would move."""
+    st = stash[i]
+    x = st.get('x')
+    if isinstance(x, torch.Tensor) and x.numel() >= _CKPT8_MIN:
+        keep = isinstance(ops_list[i], MaxPool2)
+        q = None if keep else ops.mx8_quant(x)
+        for j in range(i - 1, -1, -1):                 # the producer (views in between hand its storage on)
+            y = stash[j].get('y')
+            if isinstance(y, torch.Tensor):
+                if y.data_ptr() == x.data_ptr() and y.numel() == x.numel() and y.dtype == x.dtype:
+                    stash[j]['y'] = y if keep else q.view(y.shape)
+                break
+        if not keep:
+            st['x'] = q
+    y = st.get('y')
+    if isinstance(y, torch.Tensor):
+        op = ops_list[i]
+        if isinstance(op, (BatchNorm, InstanceNorm)) or (isinstance(op, Conv) and op.spec.act == L.ACT_NONE):
+            st['y'] = None                             # (its backward pass does not read the output)
+        elif last and y.numel() >= _CKPT8_MIN:
+            st['y'] = ops.mx8_quant(y)
+
+
+def _unpack_saved(op, st, need_x):
+    """ckpt8: before ``op``'s backward pass, what it cannot read as codes comes back as a tensor (one layer's worth at a time)."""
+    x, y = st.get('x'), st.get('y')
+    if isinstance(x, ops.Mx8) and not isinstance(op, (BatchNorm, InstanceNorm)):
+        st['x'] = ops.mx8_dequant(x) if need_x else x
+    if isinstance(y, ops.Mx8) and not isinstance(op, Conv):         # (Conv reads its output through ops.act_bwd only)
+        st['y'] = ops.mx8_dequant(y)
 
 
 class ChainFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, chain, opts, x, *params):
-        train, red, pair = opts
+        train, red, pair, ckpt = opts
         h = x.detach()
         if h.dtype != torch.float32:
             raise RuntimeError('iprgan networks take float32 inputs')
@@ -745,6 +816,9 @@ class ChainFn(torch.autograd.Function):
                 st['close_skip'] = True
             h = op.forward(h, st, train)
             shared.pop('conv_stats', None) if not isinstance(op, Conv) else None
+            if ckpt:
+                _pack_saved(chain.ops, stash, i, i + 1 == n_ops)
+        ctx.ckpt = ckpt
         ctx.chain, ctx.stash, ctx.red = chain, stash, red
         ctx.plist = params                  # (the parameter objects of this pass, in op order: backward walks them again)
         # the backward pass reads the live parameters (weights for the data gradients, spectral-norm factors):
@@ -864,7 +938,7 @@ class ChainFn(torch.autograd.Function):
             if (_FUSE_BN_BWD and _FUSE_STATS and need_dx and isinstance(op, Conv) and isinstance(prev, BatchNorm)
                     and prev.prelu is None and stash[i - 1].get('use_batch') and prev.act in (L.ACT_NONE, L.ACT_RELU, L.ACT_LRELU)
                     and 'pair' not in st and not st.get('open_skip') and ops.conv_bwd_data_bn_ok(st['d'])
-                    and i - 1 >= first_needed):
+                    and i - 1 >= first_needed and not ctx.ckpt):
                 pst = stash[i - 1]
                 st['bn_fuse'] = (pst['x'], pst['mean'], pst['invstd'], prev.m.weight, prev.m.bias, prev.act, prev.slope)
             if (isinstance(op, Conv) and need_dx and isinstance(prev, (BatchNorm, InstanceNorm)) and ops._NORM_DYF32
@@ -874,7 +948,11 @@ class ChainFn(torch.autograd.Function):
             if isinstance(op, Conv):
                 st['wg_defer'] = wg_wait
                 st['cs_defer'] = cs_wait
+            if ctx.ckpt:
+                _unpack_saved(op, st, op_need_w[i] or fuse is not None or not isinstance(op, Conv))
             g, pg = op.backward(g, st, need_dx, op_need_w[i], fuse, sink)
+            if ctx.ckpt:                        # (restored tensors live for this op's backward only)
+                st.pop('x', None), st.pop('y', None)
             if 'bn_partials' in st:
                 stash[i - 1]['dz_partials'] = st.pop('bn_partials')
             if 'dx_colsums' in st:

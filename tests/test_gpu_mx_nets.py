@@ -1,0 +1,255 @@
+"""GPU: 8-bit checkpoints inside the chain executor (`engine: {ckpt8: true}`) and 4-bit dense layers of a served generator."""
+import numpy as np
+import pytest
+import torch
+import torch.nn as nn
+
+import mx_reference as R
+from oracle import cases, recipe
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope='module')
+def dev():
+    assert torch.cuda.is_available(), 'gpu tests need a GPU'
+    return torch.device('cuda:0')
+
+
+@pytest.fixture
+def ckpt8(monkeypatch):
+    from iprgan import engine
+    monkeypatch.setattr(engine, '_CKPT8_MIN', 1)
+
+    def switch(on):
+        monkeypatch.setattr(engine, '_CKPT8', on)
+    yield switch
+
+
+@pytest.fixture
+def math(request):
+    from iprgan import _lib
+    before = _lib.get_math()
+    _lib.set_math(request.param)
+    yield request.param
+    _lib.set_math(before)
+
+
+def round8(t):
+    """float64 NCHW tensor rounded as its NHWC (channels padded to 4) checkpoint is"""
+    b, c, h, w = t.shape
+    p = torch.zeros(b, h, w, (c + 3) & ~3, dtype=torch.float64)
+    p[..., :c] = t.permute(0, 2, 3, 1)
+    v = R.mx8_decode(*R.mx8_encode(p.float())).view(p.shape)
+    return v[..., :c].permute(0, 3, 1, 2).contiguous()
+
+
+def test_chain_gradients_are_those_of_the_rounded_activations(dev, ckpt8):
+    """conv + LeakyReLU -> conv -> BatchNorm + ReLU -> conv, backward written out in float64 with every saved activation rounded to its
+    checkpoint.  An activation that two evaluations of the forward pass round to neighbouring codes moves one term of a sum over
+    2 x 16 x 16 positions by 1/127 of its block's maximum: 2e-3 of a gradient's largest entry is several of them."""
+    from iprgan import _lib as L, engine as E
+    from iprgan.ops import ConvSpec
+    torch.manual_seed(3)
+    c1, c2, bn, c3 = nn.Conv2d(3, 32, 3, 1, 1), nn.Conv2d(32, 32, 3, 1, 1), nn.BatchNorm2d(32), nn.Conv2d(32, 8, 3, 1, 1)
+    with torch.no_grad():
+        bn.weight.normal_(1, 0.2)
+        bn.bias.normal_(0, 0.2)
+    x, r = torch.randn(2, 3, 16, 16), torch.randn(2, 8, 16, 16)
+    d = lambda t: t.detach().double()
+    F = nn.functional
+    a1 = F.leaky_relu(F.conv2d(d(x), d(c1.weight), d(c1.bias), padding=1), 0.2)
+    a2 = F.conv2d(a1, d(c2.weight), d(c2.bias), padding=1)
+    mean, var = a2.mean((0, 2, 3), keepdim=True), a2.var((0, 2, 3), unbiased=False, keepdim=True)
+    inv = 1 / torch.sqrt(var + bn.eps)
+    g, b = d(bn.weight).view(1, -1, 1, 1), d(bn.bias).view(1, -1, 1, 1)
+    a3 = F.relu((a2 - mean) * inv * g + b)
+    x8, a1q, a2q, a3q = (round8(t) for t in (d(x), a1, a2, a3))
+    dy = d(r)
+    want = {}
+    want['c3'] = nn.grad.conv2d_weight(a3q, c3.weight.shape, dy, padding=1)
+    g3 = nn.grad.conv2d_input(a3.shape, d(c3.weight), dy, padding=1)
+    t = (a2q - mean) * inv
+    dz = torch.where(t * g + b > 0, g3, torch.zeros_like(g3))
+    want['bn'], want['bnb'] = (dz * t).sum((0, 2, 3)), dz.sum((0, 2, 3))
+    M = 2 * 16 * 16
+    g2 = g * inv * (dz - dz.sum((0, 2, 3), keepdim=True) / M - t * (dz * t).sum((0, 2, 3), keepdim=True) / M)
+    want['c2'] = nn.grad.conv2d_weight(a1q, c2.weight.shape, g2, padding=1)
+    g1 = nn.grad.conv2d_input(a1.shape, d(c2.weight), g2, padding=1) * torch.where(a1q > 0, 1.0, 0.2)
+    want['c1'] = nn.grad.conv2d_weight(x8, c1.weight.shape, g1, padding=1)
+    want['c1b'] = g1.sum((0, 2, 3))
+    want['x'] = nn.grad.conv2d_input(x.shape, d(c1.weight), g1, padding=1)
+    for m in (c1, c2, bn, c3):
+        m.to(dev)
+    plan = [E.ToNHWC(3), E.Conv(ConvSpec(3, 32, 3, 1, 1, act=L.ACT_LRELU, slope=0.2), c1), E.Conv(ConvSpec(32, 32, 3, 1, 1), c2),
+            E.BatchNorm(bn, act=L.ACT_RELU), E.Conv(ConvSpec(32, 8, 3, 1, 1), c3), E.ToNCHW(8)]
+    ckpt8(True)
+    xin = x.to(dev).requires_grad_(True)
+    (E.Chain(plan)(xin, True) * r.to(dev)).sum().backward()
+    got = {'c3': c3.weight.grad, 'bn': bn.weight.grad, 'bnb': bn.bias.grad, 'c2': c2.weight.grad, 'c1': c1.weight.grad, 'c1b': c1.bias.grad,
+           'x': xin.grad}
+    for k, v in want.items():
+        err = float((got[k].cpu().double() - v).abs().max() / v.abs().max())
+        assert err <= 2e-3, (k, err)
+
+
+NETS = ['ConvGenerator32', 'SNDiscriminator32', 'SRResNet', 'Discriminator96', 'Resnet6Blocks', 'ConvDiscriminator', 'VGG19Feature']
+SHAPES = {'ConvGenerator32': (4, 128), 'SNDiscriminator32': (4, 3, 32, 32), 'SRResNet': (2, 3, 24, 24), 'Discriminator96': (2, 3, 96, 96),
+          'Resnet6Blocks': (1, 3, 64, 64), 'ConvDiscriminator': (2, 3, 64, 64), 'VGG19Feature': (1, 3, 64, 64)}
+
+
+@pytest.mark.parametrize('name', NETS)
+@pytest.mark.parametrize('math', ['fp32', 'fp32x3', 'bf16act'], indirect=True)
+def test_every_network_runs_with_checkpoints(dev, ckpt8, name, math):
+    """Outputs are those of the plain pass, bit for bit; gradients point where the plain pass's point.
+
+    How far they may turn: behind a ReLU of normal values a block of 32 has a maximum m of about 2.1 sigma and a step between m / 127.5
+    and m / 63.75, on average m / 90.  A positive value below half a step - 0.0117 sigma, a share of 0.0117 * 0.4 = 0.47 % of all values,
+    0.93 % of the positive ones - is stored as zero and loses its gradient.  n such masks in a row lose a share of 1 - (1 - 0.0093)^n of the
+    gradient's energy and leave a cosine of the root of the rest; twice that share is granted.  (Masks of norm layers and of LeakyReLU lose
+    less, the noise of the values themselves is 1e-5 of the energy.)"""
+    if math == 'bf16act' and name not in ('ConvGenerator32', 'SNDiscriminator32'):
+        pytest.skip('bf16act covers the DCGAN family')
+    from iprgan import networks
+    torch.manual_seed(5)
+    net = getattr(networks, name)(**({'n_block': 2} if name == 'SRResNet' else {})).to(dev)
+    net.train()
+    state = {k: v.clone() for k, v in net.state_dict().items()}
+    x = torch.randn(SHAPES[name], generator=torch.Generator().manual_seed(1)).to(dev)
+    res = []
+    for on in (False, True):
+        net.load_state_dict(state)
+        ckpt8(on)
+        xin = x.clone().requires_grad_(True)
+        for p in net.parameters():
+            p.grad = None
+        y = net(xin)
+        r = torch.randn(y.shape, generator=torch.Generator().manual_seed(2)).to(dev)
+        (y * r).sum().backward()
+        res.append((y.detach().clone(), torch.cat([t.grad.flatten() for t in [xin, *net.parameters()] if t.grad is not None]).double()))
+    assert torch.equal(res[0][0], res[1][0])
+    a, b = res[0][1], res[1][1]
+    assert bool(torch.isfinite(b).all())
+    assert not torch.equal(a, b), 'the checkpoints were not used'
+    cos = float((a * b).sum() / (a.norm() * b.norm()))
+    masks = sum(1 for op in net.chain().ops for a in [getattr(op, 'act', op.out_act[0]), getattr(op, 'prelu', None)] if a)
+    masks += sum(type(op).__name__ in ('PReLU', 'PixelShufflePReLU') for op in net.chain().ops)
+    assert cos > (1 - 2 * (1 - (1 - 0.0093) ** max(masks, 1))) ** 0.5, (cos, masks)
+
+
+def test_checkpoints_lower_the_peak_memory_of_a_pass(dev, ckpt8):
+    from iprgan import engine, networks
+    net = networks.SNDiscriminator64().to(dev)
+    x = torch.randn(64, 3, 64, 64, device=dev)
+    held = []
+    for on in (False, True):
+        ckpt8(on)
+        torch.cuda.synchronize()
+        base = torch.cuda.memory_allocated()
+        y = net(x)
+        held.append(torch.cuda.memory_allocated() - base)       # what the recorded pass keeps for its backward
+        y.sum().backward()
+        del y
+    # fp32 activations to 1 + 1/32 bytes an element; the layers' small tensors stay
+    assert held[1] < 0.35 * held[0], held
+
+
+def test_graphed_step_with_checkpoints_is_bit_identical_to_eager(dev, ckpt8):
+    from iprgan import Config, graphs, models
+    ckpt8(True)
+    runs = []
+    for graphed in (False, True):
+        torch.manual_seed(0)
+        model = models.DCGAN(Config(cases.DCGAN_CFG), device=[dev])
+        recipe.fill(model.G.module, 3)
+        recipe.fill(model.D.module, 4)
+        model.G.to(dev), model.D.to(dev)
+
+        def body(s):
+            model.update_d({'real_sample': s['x'], 'latent': s['z']})
+            model.update_g({'fake_sample': model.fake_sample})
+        first = {'x': torch.zeros(4, 3, 64, 64, device=dev), 'z': torch.zeros(4, 128, device=dev)}
+        step = graphs.GraphedStep(model, body, first, warmup=2) if graphed else body
+        for i in range(6):
+            s = {'x': torch.tanh(recipe.tensor(7, 100 + i, (4, 3, 64, 64))).to(dev), 'z': recipe.tensor(7, 200 + i, (4, 128)).to(dev)}
+            step(s)
+            torch.cuda.synchronize()
+        if graphed:
+            assert step.graph is not None, step.failed
+        runs.append([p.detach().clone() for p in list(model.G.parameters()) + list(model.D.parameters())])
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+@pytest.mark.parametrize('math', ['fp32', 'fp32x3', 'bf16act'], indirect=True)
+@pytest.mark.parametrize('batch', [1, 3, 70])
+def test_generator_served_from_4_bit_dense_weights(dev, math, batch):
+    """quantize_dense(): eval passes equal those of a generator whose Linear holds the rounded values; training passes keep fp32."""
+    from iprgan import networks, ops
+    torch.manual_seed(2)
+    net, ref = networks.ConvGenerator32().to(dev), networks.ConvGenerator32().to(dev)
+    ref.load_state_dict(net.state_dict())
+    with torch.no_grad():
+        w = ref.fc[0].weight
+        w.copy_(ops.mx4_dequant(ops.mx4_quant(w)))
+    z = torch.randn(batch, 128, generator=torch.Generator().manual_seed(1)).to(dev)
+    assert net.quantize_dense() == 1
+    net.eval(), ref.eval()
+    for p in [*net.parameters(), *ref.parameters()]:
+        p.requires_grad_(False)
+    za, zb = z.clone().requires_grad_(True), z.clone().requires_grad_(True)
+    a, b = net(za), ref(zb)
+    tol = 2e-2 if math == 'bf16act' else 5e-4
+    assert float((a - b).detach().abs().max()) <= tol * float(b.detach().abs().max())
+    a.sum().backward(), b.sum().backward()
+    # Two evaluations of the Linear differ by about 1e-6 of sigma.  Behind it a sample passes 8192 + 16384 + 32768 + 65536 = 123 k masks, and a
+    # pre-activation lies within 1e-6 sigma of zero with probability 2e-6 * 0.4: 0.1 flipped masks a sample.  A flip turns one of those
+    # terms of the sample's gradient on or off (1e-2, as everywhere in these tests); 70 samples have 7 expected flips, so a third of the rows
+    # may hold one, the rest are 2e-3.
+    err = (za.grad - zb.grad).abs().amax(1) / zb.grad.abs().max()
+    one, flipped = (5e-2, 5e-2) if math == 'bf16act' else (2e-3, 1e-2)
+    assert float(err.max()) <= flipped and int((err > one).sum()) <= (batch + 2) // 3, err
+    net.train()
+    plain = networks.ConvGenerator32().to(dev)
+    plain.load_state_dict(net.state_dict())
+    with torch.no_grad():
+        assert torch.equal(net(z), plain(z))
+
+
+def test_4_bit_dense_weights_refuse_what_they_cannot_do(dev):
+    from iprgan import networks
+    net = networks.ConvGenerator32().to(dev)
+    z = torch.randn(2, 128, device=dev)
+    net.quantize_dense()
+    net.eval()
+    with pytest.raises(RuntimeError, match='no weight gradient'):
+        net(z).sum().backward()
+    with torch.no_grad():
+        net.fc[0].weight.mul_(2)
+        with pytest.raises(RuntimeError, match='out of date'):
+            net(z)
+        net.quantize_dense()
+        net(z)
+        net.quantize_dense(False)
+        net.fc[0].weight.mul_(2)
+        net(z)
+    with pytest.raises(RuntimeError, match='no dense layer'):
+        networks.SRResNet(n_block=1).to(dev).quantize_dense()
+
+
+def test_compression_attack(dev):
+    from iprgan import Config, attacks, networks, ops, tools
+    net = networks.ConvGenerator32()
+    slm = tools.SignLossModel(net, Config({'gamma_0': 0.1, 'string': 'EXAMPLE A'}))
+    net.to(dev), slm.to(dev)
+    before = {k: v.detach().clone() for k, v in net.named_parameters()}
+    nbytes, small = attacks.quantize_(net)
+    assert nbytes == 4 * sum(v.numel() for v in before.values() if v.dim() >= 2) and small < nbytes / 4
+    for k, p in net.named_parameters():
+        if p.dim() < 2:
+            assert torch.equal(p, before[k])
+        else:
+            w = before[k].cpu()
+            r = R.mx4_decode(*R.mx4_encode(w.reshape(w.shape[0], -1)), w[0].numel())
+            assert np.array_equal(p.detach().cpu().double().view(w.shape[0], -1).numpy(), r.numpy()), k
+    assert float(slm.compute_ber(net)) == 0.0
+    net(torch.randn(2, 128, device=dev))
