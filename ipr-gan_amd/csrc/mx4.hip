@@ -22,6 +22,12 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
+// Rows of odd lengths start on any element: vector accesses that promise no more than the element's own alignment (the memory system takes
+// them at any address).  1281 x 3237 x 2085 fp32: 203 us element by element, 87 like this; nothing changes where rows are aligned.
+typedef f32x4 f32x4u __attribute__((aligned(4)));
+typedef bf16x4 bf16x4u __attribute__((aligned(2)));
+typedef bf16x8 bf16x8u __attribute__((aligned(2)));
+
 // scale byte from the bit pattern of the largest magnitude; see mx8.hip for the same rule with 8-bit codes
 __device__ __forceinline__ unsigned mx4_scale(unsigned amax) {
   if (amax >= 0x7f800000u) return 255u;
@@ -33,23 +39,21 @@ __device__ __forceinline__ float mx4_step(unsigned s) {
   return __uint_as_float(s == 0 ? 0x00400000u : s == 255u ? 0x7fc00000u : s << 23);
 }
 
-// 8 consecutive elements of row `r` from column c on; zero behind the row's end.  VEC: rows start on 16 bytes and 8 elements never straddle an end
-template <bool BF, bool VEC>
+// 8 consecutive elements of row `r` from column c on; zero behind the row's end
+template <bool BF>
 __device__ __forceinline__ void ld8(const void* base, size_t r, int ld, int c, float* v) {
-  if (VEC) {
-    if (c + 8 <= ld) {
-      if (BF) {
-        const bf16x8 h = *(const bf16x8*)((const __bf16*)base + r * ld + c);
+  if (c + 8 <= ld) {
+    if constexpr (BF) {
+      const bf16x8 h = *(const bf16x8u*)((const __bf16*)base + r * ld + c);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = (float)h[k];
-      } else {
-        const float* p = (const float*)base + r * ld + c;
-        const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
+      for (int k = 0; k < 8; ++k) v[k] = (float)h[k];
+    } else {
+      const float* p = (const float*)base + r * ld + c;
+      const f32x4 a = *(const f32x4u*)p, b = *(const f32x4u*)(p + 4);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) { v[k] = a[k]; v[k + 4] = b[k]; }
-      }
-      return;
+      for (int k = 0; k < 4; ++k) { v[k] = a[k]; v[k + 4] = b[k]; }
     }
+    return;
   }
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
@@ -59,14 +63,14 @@ __device__ __forceinline__ void ld8(const void* base, size_t r, int ld, int c, f
 }
 
 // A thread owns 8 consecutive elements (4 bytes of codes); 4 neighbouring lanes share a block.  HBM-bound.
-template <bool BF, bool VEC>
+template <bool BF>
 __global__ __launch_bounds__(256) void mx4_quant_kernel(const void* __restrict__ x, unsigned* __restrict__ codes,
                                                         uint8_t* __restrict__ scales, unsigned groups, int cols, FastDiv d_row) {
   const unsigned stride = gridDim.x * 256;
   for (unsigned i = blockIdx.x * 256 + threadIdx.x; i < groups; i += stride) {       // groups % 16 == 0: a block's lanes stay together
     const unsigned r = fdiv(i, d_row), c = (i - r * d_row.d) * 8;
     float v[8];
-    ld8<BF, VEC>(x, r, cols, (int)c, v);
+    ld8<BF>(x, r, cols, (int)c, v);
     unsigned m = 0;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
@@ -94,7 +98,7 @@ __global__ __launch_bounds__(256) void mx4_quant_kernel(const void* __restrict__
   }
 }
 
-template <bool BF, bool VEC>
+template <bool BF>
 __global__ __launch_bounds__(256) void mx4_dequant_kernel(const unsigned* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                           void* __restrict__ y, unsigned groups, int cols, FastDiv d_row) {
   const unsigned stride = gridDim.x * 256;
@@ -107,17 +111,17 @@ __global__ __launch_bounds__(256) void mx4_dequant_kernel(const unsigned* __rest
     const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 1),
                 p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 2), q = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 3);
     const float v[8] = {a.x * step, a.y * step, b.x * step, b.y * step, p.x * step, p.y * step, q.x * step, q.y * step};
-    if (VEC && (int)c + 8 <= cols) {
+    if ((int)c + 8 <= cols) {
       if (BF) {
         bf16x8 h;
 #pragma unroll
         for (int k = 0; k < 8; ++k) h[k] = (__bf16)v[k];
-        *(bf16x8*)((__bf16*)y + (size_t)r * cols + c) = h;
+        *(bf16x8u*)((__bf16*)y + (size_t)r * cols + c) = h;
       } else {
         float* o = (float*)y + (size_t)r * cols + c;
         const f32x4 lo = {v[0], v[1], v[2], v[3]}, hi = {v[4], v[5], v[6], v[7]};
-        *(f32x4*)o = lo;
-        *(f32x4*)(o + 4) = hi;
+        *(f32x4u*)o = lo;
+        *(f32x4u*)(o + 4) = hi;
       }
     } else {
 #pragma unroll
@@ -141,7 +145,7 @@ struct LinArgs {
   void* y;
   float* slab;                   // [splits][M][N] when the K axis is split
   int M, N, K, KB, steps_per_split;      // a step is 128 elements of K
-  int act, y_bf16, vec_x, vec_y, vec8;      // vec_y: 4 columns at once, vec8: 8 bf16 columns
+  int act, y_bf16, vec8;                 // vec8: 8 bf16 columns at once
   float slope;
 };
 
@@ -152,64 +156,36 @@ __device__ __forceinline__ float lin_act(float v, int act, float slope) {
 }
 __device__ __forceinline__ void store4(const LinArgs& a, int z, int m, int n, f32x4 v) {
   if (m >= a.M || n >= a.N) return;
-  if (a.slab) {
-    float* o = a.slab + ((size_t)z * a.M + m) * a.N + n;
-    if (a.vec_y) {
-      *(f32x4*)o = v;
-    } else {
+  const size_t o = ((size_t)(a.slab ? z : 0) * a.M + m) * a.N + n;
+  if (n + 4 <= a.N) {
+    if (!a.slab) {
+      f32x4 b = {0.f, 0.f, 0.f, 0.f};
+      if (a.bias) b = *(const f32x4u*)(a.bias + n);
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (n + k < a.N) o[k] = v[k];
+      for (int k = 0; k < 4; ++k) v[k] = lin_act(v[k] + b[k], a.act, a.slope);
+      if (a.y_bf16) {
+        const bf16x4 h = {(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+        *(bf16x4u*)((__bf16*)a.y + o) = h;
+        return;
+      }
     }
-    return;
-  }
-  const size_t o = (size_t)m * a.N + n;
-  if (a.vec_y) {
-    f32x4 b = {0.f, 0.f, 0.f, 0.f};
-    if (a.bias) b = f32x4{a.bias[n], a.bias[n + 1], a.bias[n + 2], a.bias[n + 3]};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = lin_act(v[k] + b[k], a.act, a.slope);
-    if (a.y_bf16) {
-      const bf16x4 h = {(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
-      *(bf16x4*)((__bf16*)a.y + o) = h;
-    } else {
-      *(f32x4*)((float*)a.y + o) = v;
-    }
+    *(f32x4u*)((a.slab ? a.slab : (float*)a.y) + o) = v;
     return;
   }
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
+  for (int k = 0; k < 3; ++k) {
     if (n + k >= a.N) continue;
+    if (a.slab) {
+      a.slab[o + k] = v[k];
+      continue;
+    }
     const float r = lin_act(v[k] + (a.bias ? a.bias[n + k] : 0.f), a.act, a.slope);
     if (a.y_bf16) ((__bf16*)a.y)[o + k] = (__bf16)r;
     else ((float*)a.y)[o + k] = r;
   }
 }
 
-// 8 consecutive elements from column c on of a row that starts `row` bytes into the buffer; zero behind column `cols` and behind the
-// buffer (rows past the last one).  No branches: a load that must not happen gets an offset out of range.  (The first version branched,
-// and every branch waited for its own load: 4096^3 bf16 287 us instead of 183.)
-#define OOB 0xfffffff0u
-template <bool BF, bool VEC>
-__device__ __forceinline__ void buf8(__amdgpu_buffer_rsrc_t rs, unsigned row, int c, int cols, float* v) {
-  if constexpr (BF && VEC) {                                  // (cols % 8 == 0: all or nothing)
-    const bf16x8 h = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rs, c < cols ? row + c * 2u : OOB, 0, 0));
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = (float)h[k];
-  } else if constexpr (VEC) {                                 // (cols % 4 == 0)
-    const f32x4 a = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, c < cols ? row + c * 4u : OOB, 0, 0));
-    const f32x4 b = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, c + 4 < cols ? row + c * 4u + 16u : OOB, 0, 0));
-#pragma unroll
-    for (int k = 0; k < 4; ++k) { v[k] = a[k]; v[k + 4] = b[k]; }
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      if constexpr (BF) v[k] = (float)__builtin_bit_cast(__bf16, (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(rs, c + k < cols ? row + (c + k) * 2u : OOB, 0, 0));
-      else v[k] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, c + k < cols ? row + (c + k) * 4u : OOB, 0, 0));
-    }
-  }
-}
-// the same as loaded: 8 floats, or 8 bf16
+// 8 consecutive elements of a row as loaded: 8 floats, or 8 bf16
 template <bool BF>
 struct Raw8 {
   f32x4 a, b;
@@ -218,28 +194,37 @@ template <>
 struct Raw8<true> {
   bf16x8 h;
 };
-template <bool BF, bool VEC>
-__device__ __forceinline__ Raw8<BF> raw8(__amdgpu_buffer_rsrc_t rs, unsigned row, int c, int cols) {
+// ... from column c on; zero behind the row's end, which only the LAST step along the row can meet (`tail`, uniform).  Elsewhere there is no
+// branch: the first version branched on every load, and every branch waited for its own load (4096^3 bf16: 287 us instead of 183).
+template <bool BF>
+__device__ __forceinline__ Raw8<BF> row8(const uint8_t* row, int c, int cols, bool tail) {
   Raw8<BF> r;
-  if constexpr (BF && VEC) {
-    r.h = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rs, c < cols ? row + c * 2u : OOB, 0, 0));
-  } else {
-    float v[8];
-    buf8<BF, VEC>(rs, row, c, cols, v);
+  auto get = [&](int at) {
     if constexpr (BF) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) r.h[k] = (__bf16)v[k];
+      r.h = *(const bf16x8u*)(row + (size_t)at * 2);
     } else {
-      r.a = f32x4{v[0], v[1], v[2], v[3]};
-      r.b = f32x4{v[4], v[5], v[6], v[7]};
+      r.a = *(const f32x4u*)(row + (size_t)at * 4);
+      r.b = *(const f32x4u*)(row + (size_t)at * 4 + 16);
+    }
+  };
+  if (!tail) {
+    get(c);
+    return r;
+  }
+  const bool full = c + 8 <= cols;
+  if (cols >= 8) get(full ? c : 0);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    if constexpr (BF) {
+      if (!full) r.h[k] = c + k < cols ? ((const __bf16*)row)[c + k] : (__bf16)0.f;
+    } else {
+      if (full) continue;
+      const float v = c + k < cols ? ((const float*)row)[c + k] : 0.f;
+      if (k < 4) r.a[k & 3] = v;
+      else r.b[k & 3] = v;
     }
   }
   return r;
-}
-// the rows [r0, r0 + n) of a [rows][cols] matrix as a buffer of its own (32-bit offsets inside; the base is 64-bit)
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t row_buffer(const void* base, int r0, int n, int rows, int cols, unsigned esz) {
-  const unsigned long long bytes = (unsigned long long)min(n, rows - r0) * (unsigned)cols * esz;
-  return __builtin_amdgcn_make_buffer_rsrc((void*)((const uint8_t*)base + (size_t)r0 * cols * esz), 0, (int)(unsigned)bytes, 0x00020000);
 }
 
 // 8 fp4 elements (one word) of a block -> bf16, exact (a 4-bit value times a power of two)
@@ -291,7 +276,7 @@ __device__ __forceinline__ Place place(int tn, int tm) {
 // end, where the WK partial tiles are added in LDS in fixed order - one launch where a split over blocks takes two.  XT: 0 = 4-bit x
 // (the scaled instruction), 1 = bf16, 3 = fp32 (planes).  Bound by latency, or by the split of fp32 x into planes (176 vector instructions a
 // step and 16 rows, repeated by every wave: why more rows go through LDS below).
-template <int MF, int NF, int XT, bool VX>
+template <int MF, int NF, int XT>
 __global__ __launch_bounds__(512) void mx4_direct_kernel(const LinArgs a, int tn, int tm, int wk) {
   constexpr int PL = XT == 3 ? 3 : 1;
   __shared__ f32x4 red[8][NF * MF][64];
@@ -314,16 +299,13 @@ __global__ __launch_bounds__(512) void mx4_direct_kernel(const LinArgs a, int tn
     wsp[n] = a.ws + r * a.KB + g;
   }
   constexpr unsigned ESZ = XT == 1 ? 2 : 4;
-  __amdgpu_buffer_rsrc_t rx;
-  if constexpr (XT == 0) {
+  const uint8_t* xrow[MF];
 #pragma unroll
-    for (int m = 0; m < MF; ++m) {
-      const size_t r = min(m0 + m * 16 + i, a.M - 1);
-      xp[m] = (const i32x4*)((const uint8_t*)a.x + r * a.KB * 16) + g;
-      xsp[m] = a.xs + r * a.KB + g;
-    }
-  } else {
-    rx = row_buffer(a.x, m0, MF * 16, a.M, a.K, ESZ);
+  for (int m = 0; m < MF; ++m) {
+    const size_t r = min(m0 + m * 16 + i, a.M - 1);
+    xp[m] = (const i32x4*)((const uint8_t*)a.x + r * a.KB * 16) + g;
+    xsp[m] = a.xs + r * a.KB + g;
+    xrow[m] = (const uint8_t*)a.x + r * a.K * ESZ;
   }
   i32x4 wq[2][NF], xq[2][MF];
   int wsc[2][NF], xsc[2][MF];
@@ -338,7 +320,7 @@ __global__ __launch_bounds__(512) void mx4_direct_kernel(const LinArgs a, int tn
         xsc[b][m] = xsp[m][s * 4];
       } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) xv[b][m][j] = raw8<XT == 1, VX>(rx, (unsigned)(m * 16 + i) * a.K * ESZ, s * 128 + g * 32 + j * 8, a.K);
+        for (int j = 0; j < 4; ++j) xv[b][m][j] = row8<XT == 1>(xrow[m], s * 128 + g * 32 + j * 8, a.K, s * 128 + 128 > a.K);
       }
     }
   };
@@ -410,7 +392,7 @@ __device__ __forceinline__ void lds_sync() {
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   __builtin_amdgcn_s_barrier();
 }
-template <int MF, int NF, int PL, bool VX>
+template <int MF, int NF, int PL>
 __global__ __launch_bounds__(256) void mx4_linear_kernel(const LinArgs a, int tn, int tm) {
   constexpr int AHEAD = PL == 1 && NF < 4 ? 2 : 1;
   constexpr int XP = 136;                                   // LDS row pitch in bf16: 16 rows x 4-bank offset, conflict-free fragment reads
@@ -433,8 +415,9 @@ __global__ __launch_bounds__(256) void mx4_linear_kernel(const LinArgs a, int tn
     wp[n] = (const u32x4*)(a.w + (size_t)row * a.KB * 16) + g;
     sp[n] = a.ws + (size_t)row * a.KB + g;
   }
-  constexpr unsigned ESZ = PL == 1 ? 2 : 4;
-  const __amdgpu_buffer_rsrc_t rx = row_buffer(a.x, m0, MF * 16, a.M, a.K, ESZ);
+  const uint8_t* xrow[MF];
+#pragma unroll
+  for (int t = 0; t < MF; ++t) xrow[t] = (const uint8_t*)a.x + (size_t)min(m0 + xr + t * 16, a.M - 1) * a.K * (PL == 1 ? 2 : 4);
   u32x4 wq[NF], wn[AHEAD][NF];
   unsigned sq[NF], sn[AHEAD][NF];
   Raw8<PL == 1> xv[AHEAD][MF];
@@ -442,7 +425,7 @@ __global__ __launch_bounds__(256) void mx4_linear_kernel(const LinArgs a, int tn
 #pragma unroll
     for (int n = 0; n < NF; ++n) { wn[b][n] = wp[n][s * 4]; sn[b][n] = sp[n][s * 4]; }
 #pragma unroll
-    for (int t = 0; t < MF; ++t) xv[b][t] = raw8<PL == 1, VX>(rx, (unsigned)(xr + t * 16) * a.K * ESZ, s * 128 + xc, a.K);
+    for (int t = 0; t < MF; ++t) xv[b][t] = row8<PL == 1>(xrow[t], s * 128 + xc, a.K, s * 128 + 128 > a.K);
   };
 #pragma unroll
   for (int b = 0; b < AHEAD; ++b)
@@ -734,18 +717,19 @@ struct BwdArgs {
   const uint8_t *w, *ws;
   void* dx;
   float* slab;                 // [splits][M][K] when the rows n are split over blocks
-  int M, N, K, KB, steps_per_wave, dx_bf16, vec_dy, vec_dx;       // a step is 32 rows of W
+  int M, N, K, KB, steps_per_wave, dx_bf16;       // a step is 32 rows of W
 };
-template <int MF, int PL, bool VX>
+template <int MF, int PL>
 __global__ __launch_bounds__(256) void mx4_linear_bwd_kernel(const BwdArgs a, int tk, int tm) {
   __shared__ float tile[4][16][132];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
   const Place pl = place(tk, tm);
   const int k0 = pl.n * 128, m0 = pl.m * 16 * MF;
-  constexpr unsigned ESZ = PL == 1 ? 2 : 4;
-  const __amdgpu_buffer_rsrc_t rd = row_buffer(a.dy, m0, MF * 16, a.M, a.N, ESZ);
+  const uint8_t* drow[MF];
+#pragma unroll
+  for (int m = 0; m < MF; ++m) drow[m] = (const uint8_t*)a.dy + (size_t)min(m0 + m * 16 + i, a.M - 1) * a.N * (PL == 1 ? 2 : 4);
   const int steps = (a.N + 31) / 32;
-  const int s0 = (pl.z * 4 + wave) * a.steps_per_wave, s1 = min(steps, s0 + a.steps_per_wave);
+  const int s0 = (pl.z * 4 + wave) * a.steps_per_wave, s1 = min(steps, s0 + a.steps_per_wave);         // (a wave may be left without a step)
   f32x4 acc[8][MF];
 #pragma unroll
   for (int j = 0; j < 8; ++j)
@@ -763,9 +747,7 @@ __global__ __launch_bounds__(256) void mx4_linear_bwd_kernel(const BwdArgs a, in
     bf16x8 xf[MF][PL];
 #pragma unroll
     for (int m = 0; m < MF; ++m) {
-      float v[8];
-      buf8<PL == 1, VX>(rd, (unsigned)(m * 16 + i) * a.N * ESZ, nb, a.N, v);
-      split_planes<PL>(v, xf[m]);
+      split_raw<PL>(row8<PL == 1>(drow[m], nb, a.N, s * 32 + 32 > a.N), xf[m]);
     }
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
@@ -816,10 +798,10 @@ __global__ __launch_bounds__(256) void mx4_linear_bwd_kernel(const BwdArgs a, in
       const size_t o = ((size_t)(a.slab ? pl.z : 0) * a.M + row) * a.K + k;
       if (a.slab || !a.dx_bf16) {
         float* d = a.slab ? a.slab : (float*)a.dx;
-        if (a.vec_dx && k + 8 <= a.K) {
+        if (k + 8 <= a.K) {
           const f32x4 lo = {v[0], v[1], v[2], v[3]}, hi = {v[4], v[5], v[6], v[7]};
-          *(f32x4*)(d + o) = lo;
-          *(f32x4*)(d + o + 4) = hi;
+          *(f32x4u*)(d + o) = lo;
+          *(f32x4u*)(d + o + 4) = hi;
         } else {
           for (int q = 0; q < 8 && k + q < a.K; ++q) d[o + q] = v[q];
         }
@@ -827,8 +809,8 @@ __global__ __launch_bounds__(256) void mx4_linear_bwd_kernel(const BwdArgs a, in
         bf16x8 h;
 #pragma unroll
         for (int q = 0; q < 8; ++q) h[q] = (__bf16)v[q];
-        if (a.vec_dx && k + 8 <= a.K) {
-          *(bf16x8*)((__bf16*)a.dx + o) = h;
+        if (k + 8 <= a.K) {
+          *(bf16x8u*)((__bf16*)a.dx + o) = h;
         } else {
           for (int q = 0; q < 8 && k + q < a.K; ++q) ((__bf16*)a.dx)[o + q] = h[q];
         }
@@ -882,13 +864,13 @@ static int gemm4_go(const LinArgs& a, int tn, int tm, int splits, hipStream_t st
 struct LinPlan {
   int mf, nf, wk, tile, s16, tm, tn, splits, steps_per_split;
 };
-static void lin_split(LinPlan& p, int M, int N, int steps, double step_us, int unit) {
-  const double tiles = (double)p.tm * p.tn;
+template <class P>
+static void split_plan(P& p, double tiles, double out, int steps, double step_us, int unit) {
   double best = 1e30;
   for (int want = 1; want <= 64 && want <= steps; want = want < 8 ? want + 1 : want + want / 4) {
     const int per = rup(cdiv(steps, want), unit), splits = cdiv(steps, per);
     const double load = 0.6 * ((long long)((tiles * splits + 255) / 256));           // blocks a CU: two overlap to 0.6 of their sum
-    const double t = (per * step_us) * (load > 1 ? load : 1) + (splits > 1 ? 5.0 + (double)splits * M * N * 2e-6 : 0.0);
+    const double t = (per * step_us) * (load > 1 ? load : 1) + (splits > 1 ? 5.0 + splits * out * 2e-6 : 0.0);
     if (t < best) {
       best = t;
       p.steps_per_split = per;
@@ -907,13 +889,13 @@ static LinPlan lin_plan(int M, int N, int K, int x_kind) {
     p.nf = N >= 256 * 32 * (8 / p.wk) ? 2 : 1;              // two fragments a wave once that leaves a block for every CU
     p.tm = cdiv(M, 16 * p.mf);
     p.tn = cdiv(N, 16 * p.nf * (8 / p.wk));
-    lin_split(p, M, N, steps, (x_kind == IPRGAN_X_F32 ? 0.6 : 0.35) / p.wk, p.wk);
+    split_plan(p, (double)p.tm * p.tn, (double)M * N, steps, (x_kind == IPRGAN_X_F32 ? 0.6 : 0.35) / p.wk, p.wk);
   } else if (x_kind == IPRGAN_X_MX4) {
     p.tile = (long long)cdiv(M, 256) * cdiv(N, 256) >= 192 ? 256 : 128;
     p.s16 = steps % 4 == 0;                                 // the form that moves the scales of four stages at once
     p.tm = cdiv(M, p.tile);
     p.tn = cdiv(N, p.tile);
-    lin_split(p, M, N, steps, p.tile == 256 ? 1.1 : 0.4, p.s16 ? 4 : 1);
+    split_plan(p, (double)p.tm * p.tn, (double)M * N, steps, p.tile == 256 ? 1.1 : 0.4, p.s16 ? 4 : 1);
   } else {
     p.nf = p.mf == 1 ? 1 : 2;
     // four fragments a wave halve the LDS reads a multiplication once two blocks a CU are left: 4096^3 fp32 450 -> 400 us, but 1000 x
@@ -921,26 +903,21 @@ static LinPlan lin_plan(int M, int N, int K, int x_kind) {
     if (p.mf == 4 && (long long)cdiv(M, 64) * cdiv(N, 256) >= 512) p.nf = 4;
     p.tm = cdiv(M, 16 * p.mf);
     p.tn = cdiv(N, 64 * p.nf);
-    lin_split(p, M, N, steps, x_kind == IPRGAN_X_F32 ? 0.6 + 0.125 * p.mf * p.nf : 0.6 + 0.05 * p.mf * p.nf, 1);
+    split_plan(p, (double)p.tm * p.tn, (double)M * N, steps, x_kind == IPRGAN_X_F32 ? 0.6 + 0.125 * p.mf * p.nf : 0.6 + 0.05 * p.mf * p.nf, 1);
   }
   return p;
 }
+// the gradient's reduction: 4 waves a block along N, a step is 32 rows of W a wave; split by the same estimate (1 x 146 x 35 in one launch:
+// 5.4 us instead of 7.5 in two)
 struct BwdPlan {
-  int mf, tm, tk, splits, steps_per_wave;
+  int mf, tm, tk, splits, steps_per_split;
 };
-static BwdPlan bwd_plan(int M, int N, int K) {
+static BwdPlan bwd_plan(int M, int N, int K, int dy_bf16) {
   BwdPlan p;
   p.mf = M <= 16 ? 1 : 2;
   p.tm = cdiv(M, 16 * p.mf);
   p.tk = cdiv(K, 128);
-  const int steps = cdiv(N, 32);
-  const long long tiles = (long long)p.tm * p.tk;
-  int want = tiles >= 512 ? 1 : (int)(512 / tiles);
-  if (want > 64) want = 64;
-  if (want > cdiv(steps, 4)) want = cdiv(steps, 4);
-  if (want < 1) want = 1;
-  p.steps_per_wave = cdiv(steps, want * 4);
-  p.splits = cdiv(steps, p.steps_per_wave * 4);
+  split_plan(p, (double)p.tm * p.tk, (double)M * K, cdiv(cdiv(N, 32), 4), dy_bf16 ? 0.8 : 0.9, 1);
   return p;
 }
 
@@ -966,9 +943,7 @@ int iprgan_mx4_quant(const void* x, void* codes, void* scales, int rows, int col
   IPR_CHECK(x && codes && scales, "mx4_quant: null operand");
   IPR_CHECK(x_bf16 == 0 || x_bf16 == 1, "mx4_quant: storage kind %d (fp32 or bf16)", x_bf16);
   IPR_CHECK(aligned(codes, 16) && aligned(scales, 4) && aligned(x, x_bf16 ? 2 : 4), "mx4_quant: codes must be 16-byte, scales 4-byte aligned");
-  const bool vec = cols % (x_bf16 ? 8 : 4) == 0 && aligned(x, 16);
-  auto k = x_bf16 ? (vec ? mx4_quant_kernel<true, true> : mx4_quant_kernel<true, false>)
-                  : (vec ? mx4_quant_kernel<false, true> : mx4_quant_kernel<false, false>);
+  auto k = x_bf16 ? mx4_quant_kernel<true> : mx4_quant_kernel<false>;
   const unsigned blocks = (groups + 255) / 256;
   hipLaunchKernelGGL(k, dim3(blocks < 8192 ? blocks : 8192), dim3(256), 0, (hipStream_t)stream, x, (unsigned*)codes, (uint8_t*)scales,
                      groups, cols, make_fastdiv((uint32_t)kb_of(cols) * 4));
@@ -982,9 +957,7 @@ int iprgan_mx4_dequant(const void* codes, const void* scales, void* y, int rows,
   IPR_CHECK(y && codes && scales, "mx4_dequant: null operand");
   IPR_CHECK(y_bf16 == 0 || y_bf16 == 1, "mx4_dequant: storage kind %d (fp32 or bf16)", y_bf16);
   IPR_CHECK(aligned(codes, 16) && aligned(scales, 4) && aligned(y, y_bf16 ? 2 : 4), "mx4_dequant: codes must be 16-byte, scales 4-byte aligned");
-  const bool vec = cols % (y_bf16 ? 8 : 4) == 0 && aligned(y, 16);
-  auto k = y_bf16 ? (vec ? mx4_dequant_kernel<true, true> : mx4_dequant_kernel<true, false>)
-                  : (vec ? mx4_dequant_kernel<false, true> : mx4_dequant_kernel<false, false>);
+  auto k = y_bf16 ? mx4_dequant_kernel<true> : mx4_dequant_kernel<false>;
   const unsigned blocks = (groups + 255) / 256;
   hipLaunchKernelGGL(k, dim3(blocks < 8192 ? blocks : 8192), dim3(256), 0, (hipStream_t)stream, (const unsigned*)codes,
                      (const uint8_t*)scales, y, groups, cols, make_fastdiv((uint32_t)kb_of(cols) * 4));
@@ -994,7 +967,6 @@ int iprgan_mx4_dequant(const void* codes, const void* scales, void* y, int rows,
 
 static int lin_check(const char* who, int M, int N, int K) {
   IPR_CHECK(M > 0 && N > 0 && K > 0, "%s: empty product (M=%d, N=%d, K=%d)", who, M, N, K);
-  // 64 rows of x and dy are addressed through 32-bit offsets
   IPR_CHECK(K < (1 << 24) && M <= (1 << 20) && N < (1 << 24), "%s: M=%d, N=%d, K=%d (M at most 2^20, N and K below 2^24)", who, M, N, K);
   return 0;
 }
@@ -1028,25 +1000,20 @@ int iprgan_mx4_linear(const void* x, const void* x_scales, const void* w_codes, 
   a.slab = slab ? ws : nullptr;
   a.M = M; a.N = N; a.K = K; a.KB = kb_of(K); a.steps_per_split = p.steps_per_split;
   a.act = act; a.slope = act == IPRGAN_ACT_LRELU ? slope : 1.f; a.y_bf16 = y_bf16;
-  a.vec_x = K % (x_kind == IPRGAN_X_BF16 ? 8 : 4) == 0 && aligned(x, 16);
-  a.vec_y = N % 4 == 0 && (a.slab || aligned(y, y_bf16 ? 8 : 16));
   a.vec8 = y_bf16 && N % 8 == 0 && aligned(y, 16);
   const dim3 grid((unsigned)p.tn * p.tm * p.splits);
-  const bool vx = a.vec_x;
   if (p.tile) {
     const int rc = p.tile == 256 ? (p.s16 ? gemm4_go<256, 256, 2, 4, true>(a, p.tn, p.tm, p.splits, st) : gemm4_go<256, 256, 2, 4, false>(a, p.tn, p.tm, p.splits, st))
                                  : (p.s16 ? gemm4_go<128, 128, 2, 2, true>(a, p.tn, p.tm, p.splits, st) : gemm4_go<128, 128, 2, 2, false>(a, p.tn, p.tm, p.splits, st));
     if (rc) return rc;
   } else if (p.wk) {
-#define DIRECT(MF, XT, VX) (p.nf == 2 ? mx4_direct_kernel<MF, 2, XT, VX> : mx4_direct_kernel<MF, 1, XT, VX>)
-    auto k = x_kind == IPRGAN_X_F32    ? (vx ? DIRECT(1, 3, true) : DIRECT(1, 3, false))
-             : x_kind == IPRGAN_X_BF16 ? (vx ? DIRECT(1, 1, true) : DIRECT(1, 1, false))
-                                       : (p.mf == 1 ? DIRECT(1, 0, true) : p.mf == 2 ? DIRECT(2, 0, true) : DIRECT(4, 0, true));
+#define DIRECT(MF, XT) (p.nf == 2 ? mx4_direct_kernel<MF, 2, XT> : mx4_direct_kernel<MF, 1, XT>)
+    auto k = x_kind == IPRGAN_X_F32 ? DIRECT(1, 3) : x_kind == IPRGAN_X_BF16 ? DIRECT(1, 1) : p.mf == 1 ? DIRECT(1, 0) : p.mf == 2 ? DIRECT(2, 0) : DIRECT(4, 0);
 #undef DIRECT
     hipLaunchKernelGGL(k, grid, dim3(512), 0, st, a, p.tn, p.tm, p.wk);
   } else {
-#define LDSX(PL, VX) (p.mf == 1 ? mx4_linear_kernel<1, 1, PL, VX> : p.mf == 2 ? mx4_linear_kernel<2, 2, PL, VX> : p.nf == 2 ? mx4_linear_kernel<4, 2, PL, VX> : mx4_linear_kernel<4, 4, PL, VX>)
-    auto k = x_kind == IPRGAN_X_BF16 ? (vx ? LDSX(1, true) : LDSX(1, false)) : (vx ? LDSX(3, true) : LDSX(3, false));
+#define LDSX(PL) (p.mf == 1 ? mx4_linear_kernel<1, 1, PL> : p.mf == 2 ? mx4_linear_kernel<2, 2, PL> : p.nf == 2 ? mx4_linear_kernel<4, 2, PL> : mx4_linear_kernel<4, 4, PL>)
+    auto k = x_kind == IPRGAN_X_BF16 ? LDSX(1) : LDSX(3);
 #undef LDSX
     hipLaunchKernelGGL(k, grid, dim3(256), 0, st, a, p.tn, p.tm);
   }
@@ -1054,9 +1021,9 @@ int iprgan_mx4_linear(const void* x, const void* x_scales, const void* w_codes, 
   return slab ? slab_reduce(ws, p.splits, M, N, bias, y, act, slope, y_bf16, st) : 0;
 }
 
-size_t iprgan_mx4_linear_bwd_ws_floats(int M, int N, int K) {
+size_t iprgan_mx4_linear_bwd_ws_floats(int M, int N, int K, int dy_bf16) {
   if (M < 1 || N < 1 || K < 1) return 0;
-  const BwdPlan p = bwd_plan(M, N, K);
+  const BwdPlan p = bwd_plan(M, N, K, dy_bf16);
   return p.splits > 1 ? (size_t)p.splits * M * K : 0;
 }
 
@@ -1067,21 +1034,17 @@ int iprgan_mx4_linear_bwd(const void* dy, const void* w_codes, const void* w_sca
   IPR_CHECK((dy_bf16 == 0 || dy_bf16 == 1) && (dx_bf16 == 0 || dx_bf16 == 1), "mx4_linear_bwd: storage kinds %d, %d (fp32 or bf16)", dy_bf16, dx_bf16);
   IPR_CHECK(aligned(w_codes, 16) && aligned(w_scales, 4) && aligned(dy, dy_bf16 ? 2 : 4) && aligned(dx, dx_bf16 ? 2 : 4),
             "mx4_linear_bwd: codes must be 16-byte, scales 4-byte aligned");
-  const BwdPlan p = bwd_plan(M, N, K);
+  const BwdPlan p = bwd_plan(M, N, K, dy_bf16);
   IPR_CHECK((long long)p.tm * p.tk * p.splits < 0x7fffffffll, "mx4_linear_bwd: M=%d, K=%d", M, K);
   IPR_CHECK(p.splits == 1 || (ws && aligned(ws, 16)), "mx4_linear_bwd: the workspace of iprgan_mx4_linear_bwd_ws_floats is missing");
   hipStream_t st = (hipStream_t)stream;
   BwdArgs a;
   a.dy = dy; a.w = (const uint8_t*)w_codes; a.ws = (const uint8_t*)w_scales; a.dx = dx;
   a.slab = p.splits > 1 ? ws : nullptr;
-  a.M = M; a.N = N; a.K = K; a.KB = kb_of(K); a.steps_per_wave = p.steps_per_wave; a.dx_bf16 = dx_bf16;
-  a.vec_dy = N % (dy_bf16 ? 8 : 4) == 0 && aligned(dy, 16);
-  a.vec_dx = K % (a.slab || !dx_bf16 ? 4 : 8) == 0 && (a.slab || aligned(dx, 16));
+  a.M = M; a.N = N; a.K = K; a.KB = kb_of(K); a.steps_per_wave = p.steps_per_split; a.dx_bf16 = dx_bf16;
   const dim3 grid((unsigned)p.tk * p.tm * p.splits), blk(256);
-  auto k = dy_bf16 ? (a.vec_dy ? (p.mf == 1 ? mx4_linear_bwd_kernel<1, 1, true> : mx4_linear_bwd_kernel<2, 1, true>)
-                               : (p.mf == 1 ? mx4_linear_bwd_kernel<1, 1, false> : mx4_linear_bwd_kernel<2, 1, false>))
-                   : (a.vec_dy ? (p.mf == 1 ? mx4_linear_bwd_kernel<1, 3, true> : mx4_linear_bwd_kernel<2, 3, true>)
-                               : (p.mf == 1 ? mx4_linear_bwd_kernel<1, 3, false> : mx4_linear_bwd_kernel<2, 3, false>));
+  auto k = dy_bf16 ? (p.mf == 1 ? mx4_linear_bwd_kernel<1, 1> : mx4_linear_bwd_kernel<2, 1>)
+                   : (p.mf == 1 ? mx4_linear_bwd_kernel<1, 3> : mx4_linear_bwd_kernel<2, 3>);
   hipLaunchKernelGGL(k, grid, blk, 0, st, a, p.tk, p.tm);
   IPR_LAUNCH_CHECK();
   return p.splits > 1 ? slab_reduce(ws, p.splits, M, K, nullptr, dx, IPRGAN_ACT_NONE, 0.f, dx_bf16, st) : 0;

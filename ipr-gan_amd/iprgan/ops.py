@@ -492,7 +492,7 @@ def mx4_linear_bwd(dy, w, dtype=None):
     M = dy.numel() // N
     kx = _mx4_out_kind('mx4_linear_bwd', dtype)
     dx = _new((M, K) if dy.dim() == 2 else tuple(dy.shape[:-1]) + (K,), dy, dtype)
-    nws = _ws_floats('iprgan_mx4_linear_bwd_ws_floats', M, N, K)
+    nws = _ws_floats('iprgan_mx4_linear_bwd_ws_floats', M, N, K, k)
     ws = L.acct_scratch(_new(nws, dy, torch.float32)) if nws else None
     L.acct_flops(2.0 * M * N * K)
     wc, wsc = w.ptrs()
