@@ -308,8 +308,10 @@ __global__ __launch_bounds__(256) void mx8_norm_reduce_kernel(const NormArgs a) 
   const int c = (blockIdx.y * TC + tc) * V;
   const bool ok = c < C && tr < TR;
   const size_t gofs = (size_t)grp * a.M * C;
-  __shared__ float sh[3][256][V + 1];
-  float s1[V], s2[V], s3 = 0.f;
+  __shared__ float sh[2][256][V + 1];
+  float s1[V], s2[V];
+  double s3 = 0.;                                        // the slope's gradient is ONE sum over the whole tensor, often much smaller than its
+                                                         // terms: two fused multiply-adds an element in 64 bits, free beside the loads
 #pragma unroll
   for (int k = 0; k < V; ++k) s1[k] = s2[k] = 0.f;
   if (ok) {
@@ -322,6 +324,14 @@ __global__ __launch_bounds__(256) void mx8_norm_reduce_kernel(const NormArgs a) 
 #pragma unroll
       for (int k = 0; k < V; ++k) mask_threshold(m[k], is[k], ga[k], be[k], thr[k], sgn[k]);
     }
+    double va[ACT == 2 ? V : 1], vb[ACT == 2 ? V : 1];  // the activation's input v = x va + vb
+    if (ACT == 2) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        va[k] = (double)is[k] * (double)ga[k];
+        vb[k] = (double)be[k] - (double)m[k] * va[k];
+      }
+    }
     auto accumulate = [&](const float* x, float step, const float* g) {
 #pragma unroll
       for (int k = 0; k < V; ++k) {
@@ -329,7 +339,7 @@ __global__ __launch_bounds__(256) void mx8_norm_reduce_kernel(const NormArgs a) 
         float dz = g[k];
         if (ACT) {
           const bool pos = sgn[k] * xv > thr[k];
-          if (ACT == 2) s3 += pos ? 0.f : g[k] * (t * ga[k] + be[k]);
+          if (ACT == 2) s3 = fma((double)(pos ? 0.f : g[k]), fma((double)xv, va[k], vb[k]), s3);
           dz = pos ? dz : dz * slope;
         }
         s1[k] += dz;
@@ -365,7 +375,12 @@ __global__ __launch_bounds__(256) void mx8_norm_reduce_kernel(const NormArgs a) 
     sh[0][threadIdx.x][k] = s1[k];
     sh[1][threadIdx.x][k] = s2[k];
   }
-  if (ACT == 2) sh[2][threadIdx.x][0] = s3;
+  __shared__ double sh3[4];
+  if (ACT == 2) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s3 += __shfl_xor(s3, o, 64);
+    if ((threadIdx.x & 63) == 0) sh3[threadIdx.x >> 6] = s3;
+  }
   __syncthreads();
   // fixed order: deterministic.  Thread j sums channel j % (TC * V) of sum j / (TC * V)
   const int W = TC * V;
@@ -374,19 +389,23 @@ __global__ __launch_bounds__(256) void mx8_norm_reduce_kernel(const NormArgs a) 
     const int which = j / W, ch = j - which * W, col = ch / V, k = ch - col * V;
     const int cc = blockIdx.y * W + ch;
     if (cc >= C) continue;
-    float s = 0.f;
-    if (which < 2 || k == 0)
-      for (int i = 0; i < TR; ++i) s += sh[which][i * TC + col][which < 2 ? k : 0];
-    p[(size_t)which * C + cc] = s;
+    double s = 0.;                                       // (up to 256 row lanes in a row: in 64 bits)
+    if (which < 2) {
+      for (int i = 0; i < TR; ++i) s += sh[which][i * TC + col][k];
+    } else if (ch < 2) {                                 // the block's one sum, in two parts, in the chunk's first two places; zero in the rest
+      for (int i = 0; i < 4; ++i) s += sh3[i];
+      if (ch) s -= (double)(float)s;
+    }
+    p[(size_t)which * C + cc] = (float)s;
   }
 }
 
 // part [G][NB][W] -> sums [G][W], W = nsum * C: 16 columns x 64 row lanes a block, added in fixed order
 __global__ __launch_bounds__(1024) void mx8_norm_final_kernel(const float* __restrict__ part, int NB, int W, float* __restrict__ sums) {
-  __shared__ float sh[64][17];
+  __shared__ double sh[64][17];
   const int cl = threadIdx.x & 15, rl = threadIdx.x >> 4, w = blockIdx.x * 16 + cl;
   part += (size_t)blockIdx.y * NB * W;
-  float s = 0.f;
+  double s = 0.;
   if (w < W) {
 #pragma unroll 4
     for (int r = rl; r < NB; r += 64) s += part[(size_t)r * W + w];
@@ -394,12 +413,12 @@ __global__ __launch_bounds__(1024) void mx8_norm_final_kernel(const float* __res
   sh[rl][cl] = s;
   __syncthreads();
   if (threadIdx.x < 64) {                               // 4 lanes a column, then their four sums
-    float t = 0.f;
+    double t = 0.;
 #pragma unroll
     for (int i = 0; i < 16; ++i) t += sh[rl * 16 + i][cl];
     t += __shfl_xor(t, 16, 64);
     t += __shfl_xor(t, 32, 64);
-    if (rl == 0 && w < W) sums[(size_t)blockIdx.y * W + w] = t;
+    if (rl == 0 && w < W) sums[(size_t)blockIdx.y * W + w] = (float)t;
   }
 }
 
@@ -477,9 +496,9 @@ __global__ __launch_bounds__(256) void mx8_norm_apply_kernel(const NormArgs a) {
     for (int ch = threadIdx.x; ch < W; ch += 256) {
       const int col = ch / V, k = ch - col * V;
       if (blockIdx.y * W + ch >= C) continue;
-      float s = 0.f;
+      double s = 0.;
       for (int i = 0; i < TR; ++i) s += sh[0][i * TC + col][k];
-      a.colpart[((size_t)grp * gridDim.x + blockIdx.x) * 2 * C + blockIdx.y * W + ch] = s;
+      a.colpart[((size_t)grp * gridDim.x + blockIdx.x) * 2 * C + blockIdx.y * W + ch] = (float)s;
     }
     __syncthreads();
   }
@@ -503,17 +522,17 @@ __global__ __launch_bounds__(256) void mx8_norm_apply_kernel(const NormArgs a) {
     for (int ch = threadIdx.x; ch < W; ch += 256) {
       const int col = ch / V, k = ch - col * V, cc = blockIdx.y * W + ch;
       if (cc >= C) continue;
-      float b = 0.f, g = 0.f;
+      double b = 0., g = 0.;
       for (int i = 0; i < TR; ++i) { b += sh[0][i * TC + col][k]; g += sh[1][i * TC + col][k]; }
-      a.dgamma[cc] = g;
-      a.dbeta[cc] = b;
+      a.dgamma[cc] = (float)g;
+      a.dbeta[cc] = (float)b;
     }
   }
   if (a.dslope && blockIdx.y == 0) {
     __syncthreads();
-    float s = 0.f;
-    for (int j = threadIdx.x; j < C; j += 256) s += a.sums[2 * (size_t)C + j];
-    s = block_sum(s, &sh[0][0][0]);
+    double d = 0.;
+    for (int j = threadIdx.x; j < C; j += 256) d += (double)a.sums[2 * (size_t)C + j];
+    const float s = block_sum((float)d, &sh[0][0][0]);
     if (threadIdx.x == 0) *a.dslope = s;
   }
 }

@@ -237,6 +237,29 @@ def test_norm_backward_mask_is_exact_next_to_zero(dev):
     assert torch.equal(db.cpu().double(), want)
 
 
+@pytest.mark.parametrize('rows', [1 << 9, 1 << 19])
+def test_slope_gradient_keeps_its_precision(dev, rows):
+    """The PReLU slope's gradient is one sum over the whole tensor.  Here the second half of the rows repeats the first with the opposite
+    gradient, all but one row, so that it is far smaller than its parts.  It is taken in 64 bits; a block's sum is stored as two floats
+    (2^-48 of it off), their totals and the result are rounded to one: 3 half steps of the result, 16 allowed; 64-bit sums in
+    chains shorter than 2^12 are off by 2^-41 of the terms' absolute sum, and 2^-40 is allowed."""
+    from iprgan import ops
+    c, half = 64, rows // 2
+    g = torch.Generator(device=dev).manual_seed(5)
+    x = torch.randn(half, c, generator=g, device=dev)
+    dy = torch.rand(half, c, generator=g, device=dev) + 0.5
+    q = ops.mx8_quant(torch.cat([x, x]).view(1, rows // 256, 256, c))
+    dy = torch.cat([dy, -dy])
+    dy[-1] = 1e-3
+    dy = dy.view(1, rows // 256, 256, c)
+    gamma, beta = torch.rand(c, generator=g, device=dev) + 0.5, torch.randn(c, generator=g, device=dev)
+    mean, invstd = 0.1 * torch.randn(c, generator=g, device=dev), torch.rand(c, generator=g, device=dev) + 0.5
+    got = ops.bn_prelu_bwd(q, dy, gamma, beta, mean, invstd, torch.full((1,), 0.25, device=dev))[3]
+    v = (ops.mx8_dequant(q).double() - mean.double()) * invstd.double() * gamma.double() + beta.double()
+    t = v.clamp(max=0) * dy.double()
+    assert abs(float(got) - float(t.sum())) <= 2.0 ** -20 * abs(float(t.sum())) + 2.0 ** -40 * float(t.abs().sum())
+
+
 def test_norm_backward_three_planes(dev, x3_mode):
     """fp32x3: three-plane dy -> three-plane dx; an fp32 dy next to a checkpoint of a splitting layer -> three-plane dx."""
     from iprgan import ops
