@@ -392,11 +392,13 @@ __device__ __forceinline__ void lds_sync() {
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   __builtin_amdgcn_s_barrier();
 }
+// Where a row keeps its 16-byte pieces: piece c at c ^ swz(row).  A 16-byte LDS read serves 16 lanes at a time, lanes 0-3, 12-15, 20-23 and
+// 24-27 the first: rows 0-3 and 12-15 of lane group 0, rows 4-11 of group 1.  This order of the rows (0-15) gives the halves disjoint banks.
+__device__ __forceinline__ int swz(int row) { return (row & 3) | ((row >> 2 & 1) * 2 ^ (row >> 3) * 3) << 2; }
 template <int MF, int NF, int PL>
 __global__ __launch_bounds__(256) void mx4_linear_kernel(const LinArgs a, int tn, int tm) {
   constexpr int AHEAD = PL == 1 && NF < 4 ? 2 : 1;
-  constexpr int XP = 136;                                   // LDS row pitch in bf16: 16 rows x 4-bank offset, conflict-free fragment reads
-  __shared__ __bf16 xs[PL][MF * 16][XP];                    // one buffer: 52 KB at most, three blocks a CU hide each other's barriers
+  __shared__ bf16x8 xs[PL][MF * 16][16];                    // one buffer: 48 KB at most, three blocks a CU hide each other's barriers
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
   const Place pl = place(tn, tm);
   const int n0 = pl.n * 64 * NF + wave * 16 * NF, m0 = pl.m * 16 * MF;
@@ -437,7 +439,7 @@ __global__ __launch_bounds__(256) void mx4_linear_kernel(const LinArgs a, int tn
       bf16x8 p[PL];
       split_raw<PL>(xv[b][t], p);
 #pragma unroll
-      for (int q = 0; q < PL; ++q) *(bf16x8*)&xs[q][xr + t * 16][xc] = p[q];
+      for (int q = 0; q < PL; ++q) xs[q][xr + t * 16][(threadIdx.x & 15) ^ swz(xr)] = p[q];
     }
 #pragma unroll
     for (int n = 0; n < NF; ++n) { wq[n] = wn[b][n]; sq[n] = sn[b][n]; }
@@ -449,7 +451,7 @@ __global__ __launch_bounds__(256) void mx4_linear_kernel(const LinArgs a, int tn
     bf16x8 xf[D + 1][MF], wf[NF];
     auto read = [&](int p) {
 #pragma unroll
-      for (int m = 0; m < MF; ++m) xf[p % (D + 1)][m] = *(const bf16x8*)&xs[PL - 1 - p % PL][m * 16 + i][g * 32 + p / PL * 8];
+      for (int m = 0; m < MF; ++m) xf[p % (D + 1)][m] = xs[PL - 1 - p % PL][m * 16 + i][(g * 4 + p / PL) ^ swz(i)];
     };
 #pragma unroll
     for (int p = 0; p < D; ++p) read(p);
