@@ -27,6 +27,7 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef f32x4 f32x4u __attribute__((aligned(4)));
 typedef bf16x4 bf16x4u __attribute__((aligned(2)));
 typedef bf16x8 bf16x8u __attribute__((aligned(2)));
+typedef bf16x8 bf16x8w __attribute__((aligned(4)));
 
 // scale byte from the bit pattern of the largest magnitude; see mx8.hip for the same rule with 8-bit codes
 __device__ __forceinline__ unsigned mx4_scale(unsigned amax) {
@@ -710,10 +711,10 @@ __global__ __launch_bounds__(256) void mx4_slab_reduce_kernel(const float* __res
 }
 
 // ---- gradient with respect to x: dx[m][k] = sum_n dy[m][n] W[n][k] -----------------------------------------------------------------
-// The reduction runs along the rows of W, so a lane needs 8 rows' values of one k.  It reads one word (8 k) of each of its 8 rows,
-// widens them with the rows' scales and interleaves row pairs: the eight vectors it then holds are its operands for EIGHT instructions
-// j = 0..7, whose row i stands for k = 8 i + j - the 8 x 8 transposition costs 32 permutes and no LDS.  A wave covers 128 k; the
-// block's 4 waves split the rows n and add their tiles through LDS.  The lane's results over j are 8 consecutive k.
+// The reduction runs along the rows of W, so a lane needs 8 rows' values of one k.  It reads KW words (8 KW elements of one block) of each of
+// its 8 rows, widens them with the rows' scales and interleaves row pairs: the eight vectors it then holds per word are its operands for EIGHT
+// instructions j = 0..7, whose row i stands for k = 8 KW i + j - the 8 x 8 transposition costs 32 permutes a word and no LDS.  A wave
+// covers 128 KW k; the block's 4 waves split the rows n and add their tiles through LDS.  The lane's results over j are 8 consecutive k.
 struct BwdArgs {
   const void* dy;
   const uint8_t *w, *ws;
@@ -721,82 +722,135 @@ struct BwdArgs {
   float* slab;                 // [splits][M][K] when the rows n are split over blocks
   int M, N, K, KB, steps_per_wave, dx_bf16;       // a step is 32 rows of W
 };
-template <int MF, int PL>
-__global__ __launch_bounds__(256) void mx4_linear_bwd_kernel(const BwdArgs a, int tk, int tm) {
+template <int KW>
+struct Words {
+  typedef unsigned type __attribute__((ext_vector_type(KW)));
+};
+template <int MF, int KW, int PL, bool ODD>
+__global__ __launch_bounds__(256, 2) void mx4_linear_bwd_kernel(const BwdArgs a, int tk, int tm) {
+  typedef typename Words<KW>::type words;
   __shared__ float tile[4][16][132];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
   const Place pl = place(tk, tm);
-  const int k0 = pl.n * 128, m0 = pl.m * 16 * MF;
+  const int k0 = pl.n * 128 * KW, m0 = pl.m * 16 * MF;
+  const int blk = min(k0 / 32 + i * KW / 4, a.KB - 1);      // (k past the padded row repeat the last block; their results are not stored)
+  const uint8_t* wp = a.w + (size_t)blk * 16 + i * KW % 4 * 4;
+  const uint8_t* sp = a.ws + blk;
   const uint8_t* drow[MF];
 #pragma unroll
   for (int m = 0; m < MF; ++m) drow[m] = (const uint8_t*)a.dy + (size_t)min(m0 + m * 16 + i, a.M - 1) * a.N * (PL == 1 ? 2 : 4);
   const int steps = (a.N + 31) / 32;
   const int s0 = (pl.z * 4 + wave) * a.steps_per_wave, s1 = min(steps, s0 + a.steps_per_wave);         // (a wave may be left without a step)
-  f32x4 acc[8][MF];
+  f32x4 acc[KW][8][MF];
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
+  for (int w = 0; w < KW; ++w)
 #pragma unroll
-    for (int m = 0; m < MF; ++m) acc[j][m] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int s = s0; s < s1; ++s) {
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int m = 0; m < MF; ++m) acc[w][j][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  words wn[8];
+  unsigned sn[8];
+  Raw8<PL == 1> xn[MF];
+  // ODD: bf16 rows of odd length.  Every second one starts in the middle of a 4-byte word, where a vector load takes twice as long, so its elements
+  // are taken from the five words that hold them: 512 x 8193 x 6208 226 -> 151 us (106 with N = 8192).  An instance of its own, for the form of
+  // 64 rows only: the shifts would cost the others more than they give (4 rows: 14.7 -> 15.6 us).
+  unsigned xw[MF], whole = 0;                               // the fifth word; ~0 but for the last step, whose loads look for the row's end
+  auto load = [&](int s) {
     const int nb = s * 32 + g * 8;
-    unsigned wq[8], sc[8];
+    const bool tail = s * 32 + 32 > a.N;
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
       const size_t row = min(nb + r, a.N - 1);              // rows past N meet a zero of dy
-      wq[r] = *(const unsigned*)(a.w + row * a.KB * 16 + k0 / 2 + i * 4);
-      sc[r] = a.ws[row * a.KB + k0 / 32 + (i >> 2)];
+      wn[r] = *(const words*)(wp + row * a.KB * 16);
+      sn[r] = sp[row * a.KB];
     }
-    bf16x8 xf[MF][PL];
 #pragma unroll
     for (int m = 0; m < MF; ++m) {
-      split_raw<PL>(row8<PL == 1>(drow[m], nb, a.N, s * 32 + 32 > a.N), xf[m]);
-    }
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      unsigned p[8];
-#pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        const float step = mx4_step(sc[r]);
-        bf16x2 t;
-        switch (b) {                                        // (the byte number is an immediate)
-          case 0: t = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(wq[r], step, 0); break;
-          case 1: t = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(wq[r], step, 1); break;
-          case 2: t = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(wq[r], step, 2); break;
-          default: t = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(wq[r], step, 3); break;
+      if constexpr (ODD) {
+        xw[m] = 0;
+        if (!tail) {
+          const unsigned half = (unsigned)(uintptr_t)drow[m] & 2;
+          const uint8_t* p = drow[m] + (size_t)nb * 2 - half;
+          xn[m].h = *(const bf16x8w*)p;
+          xw[m] = *(const unsigned*)(p + 12 + half * 2);    // (never past the word of the last element)
+          continue;
         }
-        p[r] = __builtin_bit_cast(unsigned, t);
       }
-      u32x4 lo, hi;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        lo[r] = __builtin_amdgcn_perm(p[2 * r + 1], p[2 * r], 0x05040100u);
-        hi[r] = __builtin_amdgcn_perm(p[2 * r + 1], p[2 * r], 0x07060302u);
-      }
-      const bf16x8 wl = __builtin_bit_cast(bf16x8, lo), wh = __builtin_bit_cast(bf16x8, hi);
-#pragma unroll
-      for (int m = 0; m < MF; ++m)
-#pragma unroll
-        for (int q = PL - 1; q >= 0; --q) {
-          acc[2 * b][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wl, xf[m][q], acc[2 * b][m], 0, 0, 0);
-          acc[2 * b + 1][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wh, xf[m][q], acc[2 * b + 1][m], 0, 0, 0);
-        }
+      xn[m] = row8<PL == 1>(drow[m], nb, a.N, tail);
     }
+    whole = tail ? 0u : ~0u;
+  };
+  if (s0 < s1) load(s0);
+#pragma unroll 1
+  for (int s = s0; s < s1; ++s) {
+    words wq[8];
+    float sc[8];
+    bf16x8 xf[MF][PL];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) { wq[r] = wn[r]; sc[r] = mx4_step(sn[r]); }
+#pragma unroll
+    for (int m = 0; m < MF; ++m) {
+      split_raw<PL>(xn[m], xf[m]);
+      if constexpr (ODD) {
+        const unsigned sh = ((unsigned)(uintptr_t)drow[m] & 2) * 8 & whole;
+        u32x4 d = __builtin_bit_cast(u32x4, xf[m][0]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) d[q] = __builtin_amdgcn_alignbit(q < 3 ? d[q + 1] : xw[m], d[q], sh);
+        xf[m][0] = __builtin_bit_cast(bf16x8, d);
+      }
+    }
+    if (s + 1 < s1) load(s + 1);
+    __builtin_amdgcn_sched_barrier(0);                      // the next step's loads leave before this one is multiplied
+#pragma unroll
+    for (int w = 0; w < KW; ++w)
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        unsigned p[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          bf16x2 t;
+          switch (b) {                                      // (the byte number is an immediate)
+            case 0: t = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(wq[r][w], sc[r], 0); break;
+            case 1: t = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(wq[r][w], sc[r], 1); break;
+            case 2: t = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(wq[r][w], sc[r], 2); break;
+            default: t = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(wq[r][w], sc[r], 3); break;
+          }
+          p[r] = __builtin_bit_cast(unsigned, t);
+        }
+        u32x4 lo, hi;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          lo[r] = __builtin_amdgcn_perm(p[2 * r + 1], p[2 * r], 0x05040100u);
+          hi[r] = __builtin_amdgcn_perm(p[2 * r + 1], p[2 * r], 0x07060302u);
+        }
+        const bf16x8 wl = __builtin_bit_cast(bf16x8, lo), wh = __builtin_bit_cast(bf16x8, hi);
+#pragma unroll
+        for (int q = PL - 1; q >= 0; --q)
+#pragma unroll
+          for (int m = 0; m < MF; ++m) {
+            acc[w][2 * b][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wl, xf[m][q], acc[w][2 * b][m], 0, 0, 0);
+            acc[w][2 * b + 1][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wh, xf[m][q], acc[w][2 * b + 1][m], 0, 0, 0);
+          }
+      }
   }
 #pragma unroll
-  for (int m = 0; m < MF; ++m) {
-    if (m) __syncthreads();
+  for (int m = 0; m < MF; ++m)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const f32x4 lo = {acc[0][m][r], acc[1][m][r], acc[2][m][r], acc[3][m][r]}, hi = {acc[4][m][r], acc[5][m][r], acc[6][m][r], acc[7][m][r]};
-      *(f32x4*)&tile[wave][i][8 * (g * 4 + r)] = lo;
-      *(f32x4*)&tile[wave][i][8 * (g * 4 + r) + 4] = hi;
-    }
-    __syncthreads();
-    const int mm = threadIdx.x >> 4, kk = (threadIdx.x & 15) * 8, row = m0 + m * 16 + mm, k = k0 + kk;
-    if (row < a.M && k < a.K) {
+    for (int w = 0; w < KW; ++w) {
+      if (m || w) __syncthreads();
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const f32x4 lo = {acc[w][0][m][r], acc[w][1][m][r], acc[w][2][m][r], acc[w][3][m][r]},
+                    hi = {acc[w][4][m][r], acc[w][5][m][r], acc[w][6][m][r], acc[w][7][m][r]};
+        *(f32x4*)&tile[wave][i][8 * (g * 4 + r)] = lo;
+        *(f32x4*)&tile[wave][i][8 * (g * 4 + r) + 4] = hi;
+      }
+      __syncthreads();
+      const int mm = threadIdx.x >> 4, kk = threadIdx.x & 15, row = m0 + m * 16 + mm, k = k0 + (kk * KW + w) * 8;
+      if (row >= a.M || k >= a.K) continue;
       float v[8];
 #pragma unroll
-      for (int q = 0; q < 8; ++q) v[q] = (tile[0][mm][kk + q] + tile[1][mm][kk + q]) + (tile[2][mm][kk + q] + tile[3][mm][kk + q]);
+      for (int q = 0; q < 8; ++q) v[q] = (tile[0][mm][kk * 8 + q] + tile[1][mm][kk * 8 + q]) + (tile[2][mm][kk * 8 + q] + tile[3][mm][kk * 8 + q]);
       const size_t o = ((size_t)(a.slab ? pl.z : 0) * a.M + row) * a.K + k;
       if (a.slab || !a.dx_bf16) {
         float* d = a.slab ? a.slab : (float*)a.dx;
@@ -818,7 +872,6 @@ __global__ __launch_bounds__(256) void mx4_linear_bwd_kernel(const BwdArgs a, in
         }
       }
     }
-  }
 }
 
 static inline bool aligned(const void* p, unsigned a) { return ((uintptr_t)p & (a - 1)) == 0; }
@@ -855,72 +908,97 @@ static int gemm4_go(const LinArgs& a, int tn, int tm, int splits, hipStream_t st
   return 0;
 }
 
-// How the product is cut.
-//   direct (4-bit x: M <= 64; else M <= 16, K <= 4096 and not too many columns): 16 * mf rows x 16 * nf * (8 / wk) columns a block, wk waves along K
-//   tile   (4-bit x of more rows): square tiles, 256 where they fill three quarters of the chip, else 128
-//   LDS    (the rest): 16 * mf rows x 64 * nf columns a block
-// Direct against LDS, wall time: 1 x 4096 x 4096 fp32 13.5 : 19.5 us (one launch instead of two), 8 x 4096 x 16384 bf16 16.3 : 19.0, but
-// 8 x 4096 x 16384 fp32 25.3 : 20.4 (every wave splits x again) and 16 x 18432 x 1024 bf16 26.9 : 18.4 (18 steps in a row).
-// and K over `splits` blocks, chosen by an estimate in us: a block's steps at its measured time a step, against the slabs' traffic at 4 TB/s
-// and a second launch.
+// How the products are cut.  A form of a kernel is a tile and what a step along the reduction costs: `step` us for one block a CU (by x: fp32,
+// bf16), `more` of that for each further block beside it, of at most `resident`.  Every form is tried with every split of the reduction: the
+// steps in a row, overlapped with the weights, read once for each row of tiles, at 3.5 TB/s, plus a second launch and the slabs' traffic (8
+// bytes a partial result at 4 TB/s) where it is split.  Fitted to 60 sweeps over 1 to 48 splits, the choice is within 10 % of the fastest split nearly
+// everywhere.  (The largest form only where it fills the chip twice: one block of it alone on a CU waits for its own loads.)
+struct Form {
+  int mf, nf;                    // 16-row fragments of x, fragments (kernels above) or words (gradient) of the weights
+  int resident[2];
+  double step[2], more;
+};
+struct Cut {
+  int form, tm, tn, splits, steps_per_split;
+  double us;
+};
+static Cut cut(const Form* forms, int count, int kind, int rows_f, int cols_f, int M, int N, int steps, int unit, double weights) {
+  Cut best;
+  memset(&best, 0, sizeof(best));
+  best.us = 1e30;
+  for (int f = 0; f < count; ++f) {
+    const Form& q = forms[f];
+    const int tm = cdiv(M, rows_f * q.mf), tn = cdiv(N, cols_f * q.nf), R = q.resident[kind];
+    const double read = weights * tm / 3.5e6;
+    if (q.mf > 1 && rows_f * q.mf >= 2 * M) continue;       // half the tile's rows or more would be empty
+    if (q.mf * q.nf == 16 && (long long)tm * tn < 512) continue;
+    for (int want = 1; want <= 64 && want <= steps; want = want < 8 ? want + 1 : want + want / 4) {
+      const int per = rup(cdiv(steps, want), unit), splits = cdiv(steps, per);
+      const double blocks = (double)tm * tn * splits, b = (double)((long long)((blocks + 255) / 256)), full = (double)((long long)(b / R)), rem = b - full * R;
+      const double row = full * (1 + q.more * (R - 1)) + (rem > 0 ? 1 + q.more * (rem - 1) : 0.);
+      double us = per * q.step[kind] * row;
+      us = sqrt(us * us + read * read);
+      if (splits > 1) us += 5. + splits * (double)M * N * 2e-6;
+      if (us < best.us) best = Cut{f, tm, tn, splits, per, us};
+    }
+  }
+  return best;
+}
+
+//   LDS    : 16 * mf rows x 64 * nf columns a block.  Four fragments a wave halve the LDS reads a multiplication (4096^3 fp32: 450 -> 400 us)
+//   direct : 16 * mf rows x 16 * nf * (8 / wk) columns a block, wk waves along K.  For 4-bit x of up to 64 rows; else for up to 16, where the LDS form
+//            would be split or leaves half the chip idle, K <= 4096 and not too many columns.  Against LDS, wall time: 1 x 4096 x 4096 fp32 13.5 : 19.5
+//            us (one launch instead of two), 8 x 4096 x 16384 bf16 16.3 : 19.0, but fp32 25.3 : 20.4 (every wave splits x again), 16 x 18432 x
+//            1024 bf16 26.9 : 18.4 (18 steps in a row) and 4 x 65536 x 1024 bf16 21.2 : 13.7 (device; 1024 blocks of the LDS form).
+//   tile   : 4-bit x of more rows: square tiles, 256 where they fill three quarters of the chip, else 128
 struct LinPlan {
   int mf, nf, wk, tile, s16, tm, tn, splits, steps_per_split;
 };
-template <class P>
-static void split_plan(P& p, double tiles, double out, int steps, double step_us, int unit) {
-  double best = 1e30;
-  for (int want = 1; want <= 64 && want <= steps; want = want < 8 ? want + 1 : want + want / 4) {
-    const int per = rup(cdiv(steps, want), unit), splits = cdiv(steps, per);
-    const double load = 0.6 * ((long long)((tiles * splits + 255) / 256));           // blocks a CU: two overlap to 0.6 of their sum
-    const double t = (per * step_us) * (load > 1 ? load : 1) + (splits > 1 ? 5.0 + splits * out * 2e-6 : 0.0);
-    if (t < best) {
-      best = t;
-      p.steps_per_split = per;
-      p.splits = splits;
-    }
-  }
-}
 static LinPlan lin_plan(int M, int N, int K, int x_kind) {
+  static const Form lds[4] = {{1, 1, {8, 6}, {0.75, 0.5}, 0.35}, {2, 2, {4, 3}, {1.8, 1.2}, 0.35}, {4, 2, {3, 2}, {2.65, 1.5}, 0.35}, {4, 4, {2, 2}, {5.2, 2.5}, 0.}};
+  static const Form direct = {1, 1, {2, 2}, {0.6, 0.35}, 0.2}, tile = {1, 1, {1, 2}, {1.1, 0.4}, 0.2};      // (tile: by size, 256 or 128)
   LinPlan p;
   memset(&p, 0, sizeof(p));
-  const int steps = kb_of(K) / 4;
-  p.mf = M <= 16 ? 1 : M <= 32 ? 2 : 4;
-  if (x_kind == IPRGAN_X_MX4 ? M <= 64 : M <= 16 && steps <= 32 && (long long)steps * N <= (x_kind == IPRGAN_X_F32 ? 200000 : 600000)) {
+  const int steps = kb_of(K) / 4, kind = x_kind != IPRGAN_X_F32;
+  const double weights = (double)N * K * 0.53;
+  Cut c;
+  bool dir = x_kind == IPRGAN_X_MX4 && M <= 64;
+  if (x_kind != IPRGAN_X_MX4) {
+    c = cut(lds, 4, kind, 16, 64, M, N, steps, 1, weights);
+    p.mf = lds[c.form].mf;
+    p.nf = lds[c.form].nf;
+    dir = M <= 16 && (c.splits > 1 || c.tn < 128) && steps <= 32 && (long long)steps * N <= (kind ? 600000 : 200000);
+  }
+  if (dir) {
+    p.mf = M <= 16 ? 1 : M <= 32 ? 2 : 4;
     p.wk = 1;
     while (p.wk < 8 && p.wk * 2 <= steps) p.wk *= 2;
     p.nf = N >= 256 * 32 * (8 / p.wk) ? 2 : 1;              // two fragments a wave once that leaves a block for every CU
-    p.tm = cdiv(M, 16 * p.mf);
-    p.tn = cdiv(N, 16 * p.nf * (8 / p.wk));
-    split_plan(p, (double)p.tm * p.tn, (double)M * N, steps, (x_kind == IPRGAN_X_F32 ? 0.6 : 0.35) / p.wk, p.wk);
+    Form f = direct;
+    f.step[kind] /= p.wk;
+    c = cut(&f, 1, kind, 16 * p.mf, 16 * p.nf * (8 / p.wk), M, N, steps, p.wk, weights);
   } else if (x_kind == IPRGAN_X_MX4) {
     p.tile = (long long)cdiv(M, 256) * cdiv(N, 256) >= 192 ? 256 : 128;
     p.s16 = steps % 4 == 0;                                 // the form that moves the scales of four stages at once
-    p.tm = cdiv(M, p.tile);
-    p.tn = cdiv(N, p.tile);
-    split_plan(p, (double)p.tm * p.tn, (double)M * N, steps, p.tile == 256 ? 1.1 : 0.4, p.s16 ? 4 : 1);
-  } else {
-    p.nf = p.mf == 1 ? 1 : 2;
-    // four fragments a wave halve the LDS reads a multiplication once two blocks a CU are left: 4096^3 fp32 450 -> 400 us, but 1000 x
-    // 3000 x 5000 (320 blocks) 119 -> 131
-    if (p.mf == 4 && (long long)cdiv(M, 64) * cdiv(N, 256) >= 512) p.nf = 4;
-    p.tm = cdiv(M, 16 * p.mf);
-    p.tn = cdiv(N, 64 * p.nf);
-    split_plan(p, (double)p.tm * p.tn, (double)M * N, steps, x_kind == IPRGAN_X_F32 ? 0.6 + 0.125 * p.mf * p.nf : 0.6 + 0.05 * p.mf * p.nf, 1);
+    c = cut(&tile, 1, p.tile == 128, p.tile, p.tile, M, N, steps, p.s16 ? 4 : 1, weights);
   }
+  p.tm = c.tm;
+  p.tn = c.tn;
+  p.splits = c.splits;
+  p.steps_per_split = c.steps_per_split;
   return p;
 }
-// the gradient's reduction: 4 waves a block along N, a step is 32 rows of W a wave; split by the same estimate (1 x 146 x 35 in one launch:
-// 5.4 us instead of 7.5 in two)
+
+// The gradient's reduction runs along N, 4 waves a block, a step is 32 rows of W a wave.  More words a lane make wider reads of W and share the
+// planes of dy; more rows of dy share the widened W.  1024 x 4096 x 4096: fp32 137 us with (2, 1), 99 with (2, 2); bf16 81, and 57 with (4, 1).
 struct BwdPlan {
-  int mf, tm, tk, splits, steps_per_split;
+  int form, tm, tk, splits, steps_per_split;
 };
 static BwdPlan bwd_plan(int M, int N, int K, int dy_bf16) {
-  BwdPlan p;
-  p.mf = M <= 16 ? 1 : 2;
-  p.tm = cdiv(M, 16 * p.mf);
-  p.tk = cdiv(K, 128);
-  split_plan(p, (double)p.tm * p.tk, (double)M * K, cdiv(cdiv(N, 32), 4), dy_bf16 ? 0.8 : 0.9, 1);
-  return p;
+  static const Form f32[3] = {{1, 1, {4, 4}, {0.82, 0.82}, 0.75}, {1, 2, {2, 2}, {1.03, 1.03}, 0.85}, {2, 2, {2, 2}, {1.75, 1.75}, 0.5}};
+  static const Form b16[3] = {{1, 1, {4, 4}, {0.68, 0.68}, 0.75}, {1, 2, {3, 3}, {0.72, 0.72}, 0.85}, {4, 1, {2, 2}, {1.08, 1.08}, 0.33}};
+  const Cut c = cut(dy_bf16 ? b16 : f32, 3, 0, 16, 128, M, K, cdiv(cdiv(N, 32), 4), 1, (double)N * K * 0.53);
+  return BwdPlan{c.form, c.tm, c.tn, c.splits, c.steps_per_split};
 }
 
 }  // namespace iprgan
@@ -1045,8 +1123,10 @@ int iprgan_mx4_linear_bwd(const void* dy, const void* w_codes, const void* w_sca
   a.slab = p.splits > 1 ? ws : nullptr;
   a.M = M; a.N = N; a.K = K; a.KB = kb_of(K); a.steps_per_wave = p.steps_per_split; a.dx_bf16 = dx_bf16;
   const dim3 grid((unsigned)p.tk * p.tm * p.splits), blk(256);
-  auto k = dy_bf16 ? (p.mf == 1 ? mx4_linear_bwd_kernel<1, 1> : mx4_linear_bwd_kernel<2, 1>)
-                   : (p.mf == 1 ? mx4_linear_bwd_kernel<1, 3> : mx4_linear_bwd_kernel<2, 3>);
+  const bool odd = ((unsigned)(uintptr_t)dy | (unsigned)N * 2) & 2;
+  auto k = !dy_bf16 ? (p.form == 0 ? mx4_linear_bwd_kernel<1, 1, 3, false> : p.form == 1 ? mx4_linear_bwd_kernel<1, 2, 3, false> : mx4_linear_bwd_kernel<2, 2, 3, false>)
+                    : (p.form == 0 ? mx4_linear_bwd_kernel<1, 1, 1, false> : p.form == 1 ? mx4_linear_bwd_kernel<1, 2, 1, false>
+                       : odd ? mx4_linear_bwd_kernel<4, 1, 1, true> : mx4_linear_bwd_kernel<4, 1, 1, false>);
   hipLaunchKernelGGL(k, grid, blk, 0, st, a, p.tk, p.tm);
   IPR_LAUNCH_CHECK();
   return p.splits > 1 ? slab_reduce(ws, p.splits, M, K, nullptr, dx, IPRGAN_ACT_NONE, 0.f, dx_bf16, st) : 0;

@@ -416,6 +416,27 @@ def test_mx4_product_of_many_rows(dev, M, K, N):
     assert bool((err <= tol).all()), float((err / tol).max())
 
 
+@pytest.mark.parametrize('M,K,N', [(2050, 130, 4100), (2050, 77, 4099), (40, 515, 16001), (70, 6000, 1025), (200, 4100, 2049), (300, 4096, 2047), (520, 2050, 640)])
+@pytest.mark.parametrize('kind', ['f32', 'bf16'])
+def test_mx4_linear_and_gradient_large_tiles(dev, M, K, N, kind):
+    """Sizes that reach the tiles of many rows and columns, with rows of odd lengths, and views that start between two 4-byte words
+    (float64 on the device)."""
+    from iprgan import ops
+    t = torch.float32 if kind == 'f32' else torch.bfloat16
+    pl = 3 if kind == 'f32' else 1
+    x, dy = rnd(M * K + 1, seed=1).to(dev, t), rnd(M * N + 1, seed=3).to(dev, t)
+    w4 = ops.mx4_quant(rnd(N, K, seed=2).to(dev))
+    wd = ops.mx4_dequant(w4).double()
+    for o in (0, 1):
+        a, d = x[o: o + M * K].view(M, K), dy[o: o + M * N].view(M, N)
+        y, want = ops.mx4_linear(a, w4, dtype=torch.float32).double(), a.double() @ wd.t().contiguous()
+        err, tol = (y - want).abs(), lin_bound(a.double().abs(), wd.abs().t().contiguous(), K, pl)
+        assert bool((err <= tol).all()), float((err / tol).max())
+        dx, want = ops.mx4_linear_bwd(d, w4, dtype=torch.float32).double(), d.double() @ wd
+        err, tol = (dx - want).abs(), lin_bound(d.double().abs(), wd.abs(), N, pl)
+        assert bool((err <= tol).all()), float((err / tol).max())
+
+
 def test_mx4_linear_leading_dimensions_and_unaligned_views(dev):
     from iprgan import ops
     w4 = ops.mx4_quant(rnd(24, 64, seed=2).to(dev))
