@@ -296,6 +296,7 @@ struct NormArgs {
   float *part, *sums, *dgamma, *dbeta, *dslope, *colpart;
   size_t dyps, dxps;
   int G, M, C, TC, TR, act, nsum;          // nsum: partial sums a channel (2, or 3 with a slope gradient)
+  int RL;                                  // row lanes of the sums in the apply pass; 0: they are in `sums`
   float slope;
 };
 
@@ -422,6 +423,34 @@ __global__ __launch_bounds__(1024) void mx8_norm_final_kernel(const float* __res
   }
 }
 
+// Few partial rows (G NB <= 24 RL): the apply pass adds them itself, every block those of its own channels, RL row lanes x W / 2 quads of the two
+// sums - one launch less.  64x32x32x8 fp32: 13.5 -> 10.6 us, wall 25.2 -> 22.4; 16x24x24x64 PReLU: 12.0 both, wall 27.8 -> 25.1.  Past that the
+// row of loads in every block costs more than the launch.  tot [2][W]: the sums of rows first .. first + rows.
+__device__ __forceinline__ void chunk_sums(const NormArgs& a, int W, int first, int rows, double (*red)[4], float* tot) {
+  const int Q = W / 2, rl = threadIdx.x / Q, q = threadIdx.x - rl * Q, which = q >= W / 4, col = blockIdx.y * W + (q - which * (W / 4)) * 4;
+  if (rl < a.RL) {
+    double d[4] = {0., 0., 0., 0.};
+    if (col < a.C) {
+      const float* p = a.part + ((size_t)first * a.nsum + which) * a.C + col;
+#pragma unroll 4
+      for (int r = rl; r < rows; r += a.RL) {
+        const f32x4 v = *(const f32x4*)(p + (size_t)r * a.nsum * a.C);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) d[k] += v[k];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) red[threadIdx.x][k] = d[k];
+  }
+  __syncthreads();
+  for (int j = threadIdx.x; j < 2 * W; j += 256) {
+    double d = 0.;
+    for (int l = 0; l < a.RL; ++l) d += red[l * Q + j / 4][j & 3];
+    tot[j] = (float)d;
+  }
+  __syncthreads();
+}
+
 template <int SG, int SD, int V, int ACT>
 __global__ __launch_bounds__(256) void mx8_norm_apply_kernel(const NormArgs a) {
   const float slope = a.slope_ptr ? *a.slope_ptr : a.slope;
@@ -433,6 +462,10 @@ __global__ __launch_bounds__(256) void mx8_norm_apply_kernel(const NormArgs a) {
   // the reduction ends at the tensor's end: walking backwards finds its last rows still in the cache
   const int chunks = (a.M + 4 * TR - 1) / (4 * TR);
   __shared__ float sh[2][256][V + 1];
+  __shared__ double red[256][4];
+  __shared__ float tot[2 * 64 * V];
+  const int W = TC * V;
+  if (a.RL) chunk_sums(a, W, grp * gridDim.x, gridDim.x, red, tot);
   float cs[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) cs[k] = 0.f;
@@ -443,8 +476,13 @@ __global__ __launch_bounds__(256) void mx8_norm_apply_kernel(const NormArgs a) {
     ldf<V>(a.invstd + (size_t)grp * C, c, 1.f, is);
     ldf<V>(a.gamma, c, 1.f, ga);
     ldf<V>(a.beta, c, 0.f, be);
-    ldf<V>(su, c, 0.f, s1);
-    ldf<V>(su + C, c, 0.f, s2);
+    if (a.RL) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) { s1[k] = tot[tc * V + k]; s2[k] = tot[W + tc * V + k]; }
+    } else {
+      ldf<V>(su, c, 0.f, s1);
+      ldf<V>(su + C, c, 0.f, s2);
+    }
     if (ACT) {
 #pragma unroll
       for (int k = 0; k < V; ++k) mask_threshold(m[k], is[k], ga[k], be[k], thr[k], sgn[k]);
@@ -488,7 +526,6 @@ __global__ __launch_bounds__(256) void mx8_norm_apply_kernel(const NormArgs a) {
       }
     }
   }
-  const int W = TC * V;
   if (a.colpart) {                                     // column sums of dx: [row of blocks][2][C], as iprgan_colsum_partials reads them
 #pragma unroll
     for (int k = 0; k < V; ++k) sh[0][threadIdx.x][k] = cs[k];
@@ -503,7 +540,18 @@ __global__ __launch_bounds__(256) void mx8_norm_apply_kernel(const NormArgs a) {
     __syncthreads();
   }
   if (blockIdx.x != 0 || grp != 0) return;             // (uniform) one block of each channel chunk sums the groups' parameter gradients
-  if (a.dgamma) {
+  if (a.dgamma && a.RL) {
+    if (a.G > 1) {
+      __syncthreads();
+      chunk_sums(a, W, 0, a.G * gridDim.x, red, tot);
+    }
+    for (int ch = threadIdx.x; ch < W; ch += 256) {
+      const int cc = blockIdx.y * W + ch;
+      if (cc >= C) continue;
+      a.dgamma[cc] = tot[W + ch];
+      a.dbeta[cc] = tot[ch];
+    }
+  } else if (a.dgamma) {
     float d1[V], d2[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) d1[k] = d2[k] = 0.f;
@@ -529,11 +577,21 @@ __global__ __launch_bounds__(256) void mx8_norm_apply_kernel(const NormArgs a) {
     }
   }
   if (a.dslope && blockIdx.y == 0) {
-    __syncthreads();
     double d = 0.;
-    for (int j = threadIdx.x; j < C; j += 256) d += (double)a.sums[2 * (size_t)C + j];
-    const float s = block_sum((float)d, &sh[0][0][0]);
-    if (threadIdx.x == 0) *a.dslope = s;
+    if (a.RL) {
+      for (int j = threadIdx.x; j < (int)(gridDim.x * gridDim.y) * 2; j += 256) {
+        const int r = j / 2 / (int)gridDim.y, y = j / 2 - r * (int)gridDim.y;
+        d += (double)a.part[((size_t)r * a.nsum + 2) * C + y * W + (j & 1)];
+      }
+    } else {
+      for (int j = threadIdx.x; j < C; j += 256) d += (double)a.sums[2 * (size_t)C + j];
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) d += __shfl_xor(d, o, 64);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6][0] = d;
+    __syncthreads();
+    if (threadIdx.x == 0) *a.dslope = (float)((red[0][0] + red[1][0]) + (red[2][0] + red[3][0]));
   }
 }
 
@@ -543,8 +601,10 @@ static int norm_bwd_go(NormArgs a, const NormGeom& g, int act, hipStream_t st) {
   auto red = act == 0 ? mx8_norm_reduce_kernel<SG, V, 0> : act == 1 ? mx8_norm_reduce_kernel<SG, V, 1> : mx8_norm_reduce_kernel<SG, V, 2>;
   hipLaunchKernelGGL(red, grid, blk, 0, st, a);
   IPR_LAUNCH_CHECK();
-  hipLaunchKernelGGL(mx8_norm_final_kernel, dim3(cdiv(a.nsum * a.C, 16), a.G), dim3(1024), 0, st, a.part, g.NB, a.nsum * a.C, a.sums);
-  IPR_LAUNCH_CHECK();
+  if (!a.RL) {
+    hipLaunchKernelGGL(mx8_norm_final_kernel, dim3(cdiv(a.nsum * a.C, 16), a.G), dim3(1024), 0, st, a.part, g.NB, a.nsum * a.C, a.sums);
+    IPR_LAUNCH_CHECK();
+  }
   auto app = act == 0 ? mx8_norm_apply_kernel<SG, SD, V, 0> : mx8_norm_apply_kernel<SG, SD, V, 1>;
   hipLaunchKernelGGL(app, grid, blk, 0, st, a);
   IPR_LAUNCH_CHECK();
@@ -656,6 +716,8 @@ int iprgan_mx8_norm_bwd(const void* codes, const void* scales, const void* dy, c
   a.dgamma = dgamma; a.dbeta = dbeta; a.dslope = dslope; a.dyps = dy_pstride; a.dxps = dx_pstride;
   a.G = G; a.M = M; a.C = C; a.TC = g.TC; a.TR = g.TR; a.act = act; a.slope = act == IPRGAN_ACT_RELU ? 0.f : slope;
   a.nsum = dslope ? 3 : 2;
+  const int quads = g.TC * (wide ? 8 : 4) / 2, lanes = 256 / quads < 16 ? 256 / quads : 16;
+  a.RL = (long long)G * g.NB <= 24 * lanes ? lanes : 0;
   a.part = ws;
   a.sums = ws + (size_t)G * g.NB * a.nsum * C;
   float* colpart = a.sums + (size_t)G * a.nsum * C;
