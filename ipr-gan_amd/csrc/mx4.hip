@@ -493,31 +493,35 @@ __device__ __forceinline__ void lds_dma(__amdgpu_buffer_rsrc_t rs, unsigned lds,
   else __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(uintptr_t)lds, 4, voff, soff, 0, 0);
 #endif
 }
-template <int L>
-__device__ __forceinline__ void wait_ring(int stages) {
-  if (stages >= 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(L) : "memory");
-  else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+// (the barrier alone is no fence to the compiler)
+__device__ __forceinline__ void block_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 }
 
-// Many rows: TN x TM tiles, WN x WM waves, codes and scales of both operands through an LDS ring of four stages (128 elements of K each)
-// filled by LDS-DMA; the first half of the waves loads W, the second half x.
-//   * The stages of ALL tiles a block computes form one stream (a block walks tiles blockIdx.x, + gridDim.x, ..): the next tile's first
-//     stages are in flight while a tile's results are stored.  In the middle of a stage's multiplications a wave waits for its share of
-//     the next stage (counted; a full drain behind an epilogue, whose stores share the counter), then ONE barrier - every wave's share
-//     has landed, and every wave is done with the previous stage, whose slot is refilled.
-//   * Rows are 64 bytes a stage = 4 blocks; block c of row r sits at position c ^ ((r >> 1) & 3): 8 lanes of a fragment read then touch all 32
-//     banks (at r >> 2 the conflicts doubled the LDS time).  A DMA lane's place in LDS is fixed, so the swizzle is in its address.
-//   * S16 (rows of whole 512-element groups): the scales of four stages travel as one 16-byte piece a row; one 4-byte piece a row and
-//     stage costs the intake as much as a third of the codes (64 cache lines an instruction): 375 -> 352 us at 8192^3.
+// Many rows: TN x TM tiles, WN x WM waves, codes and scales of both operands through two LDS slots filled by LDS-DMA, a stage of 256
+// elements of K (two steps of the instruction) in each; the first half of the waves loads W, the second half x.
+//   * A row is 128 bytes a stage, a whole cache line: 25 M L2 requests at 8192^3, where stages of 128 elements made 42 M of half a line
+//     each (2048 x 4096 x 4096: 38 -> 35 us; 8192^3 300 -> 290).
+//   * The stages of ALL tiles a block computes form one stream (a block walks tiles blockIdx.x, + gridDim.x, ..), and the fragments of the
+//     next step are read while the last D of this one are multiplied, so the matrix pipe does not wait at a step's or a tile's start.
+//     Where a stage ends, a wave waits for its share of the next, then ONE barrier - every wave's share has landed, and every wave is
+//     done with this stage's slot, which is refilled.
+//   * Piece c (16 bytes) of row r sits at position c ^ ((r >> 1) & 7): the 16 lanes that an LDS read serves together then touch all
+//     banks.  A DMA lane's place in LDS is fixed, so the swizzle is in its address.
+//   * S16 (rows of whole 512-element groups): the scales of two stages travel as one 16-byte piece a row; 4-byte pieces, two a row and
+//     stage, cost the intake as much as a third of the codes (64 cache lines an instruction).
 //   * Tile order: the XCDs take contiguous runs (each has its own L2), and a run walks 4 tiles along n, then down m.
-// What bounds it: 256 x 256, 8192^3: the DMA intake alone takes 0.63 us a stage, the multiplications 0.67 at the sustained clock.
+// What bounds it, 256 x 256 at 8192^3, 290 us: the multiplications alone take 175 at the clock the chip sustains under them (it falls from 2.4 to
+// 1.9 GHz), the loop without its DMA 226: LDS serves the fragments and the DMA's writes for 60 % of the time, in the matrix pipe's way.
 template <int TN, int TM, int WN, int WM, bool S16>
 __global__ __launch_bounds__(WN* WM * 64, 2) void mx4_gemm4_kernel(const LinArgs a, int tn, int tm) {
-  constexpr int WAVES = WN * WM, NT = TN / WN / 16, MT = TM / WM / 16, NST = 4, D = 2;        // D: W fragments read ahead
-  constexpr int PC = (TN + TM) / 16 / WAVES, PS = (TN + TM) / 64 / WAVES, L = PC + (S16 ? 0 : PS);      // DMA pieces a wave and stage
-  constexpr int XC = TN * 64, WS = XC + TM * 64, XS = WS + (S16 ? 0 : TN * 4), STAGE = XS + (S16 ? 0 : TM * 4);
-  constexpr int RING = NST * STAGE, SSLOT = (TN + TM) * 16, SR = S16 ? 16 : 4;                 // SR: scale bytes of a row in LDS
-  static_assert(TN == TM && WAVES % 2 == 0 && PS >= 1 && NST == 4, "each half of the waves loads one operand");
+  constexpr int WAVES = WN * WM, NT = TN / WN / 16, MT = TM / WM / 16, D = 3;       // D: W fragments read ahead
+  constexpr int PC = (TN + TM) / 8 / WAVES, PS = (TN + TM) / 64 / WAVES, L = PC + (S16 ? 0 : 2 * PS);      // DMA pieces a wave and stage
+  constexpr int XC = TN * 128, WS = XC + TM * 128, XS = WS + (S16 ? 0 : TN * 8), STAGE = XS + (S16 ? 0 : TM * 8);
+  constexpr int RING = 2 * STAGE, SSLOT = (TN + TM) * 16, SR = S16 ? 16 : 4;                   // SR: scale bytes of a row in LDS
+  static_assert(TN == TM && WAVES % 2 == 0 && PS >= 1 && NT % (D + 1) == 0 && MT == 4, "each half of the waves loads one operand");
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   const unsigned ring = (unsigned)(uintptr_t)(lds_void*)smem;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
@@ -529,13 +533,15 @@ __global__ __launch_bounds__(WN* WM * 64, 2) void mx4_gemm4_kernel(const LinArgs
     n0 = (int)(grp * 4 + in % gw) * TN;
     m0 = (int)(in / gw) * TM;
   };
-  const int tiles = (int)((total - blockIdx.x + gridDim.x - 1) / gridDim.x), stages = tiles * steps;      // blockIdx.x < total
+  const int tiles = (int)((total - blockIdx.x + gridDim.x - 1) / gridDim.x);            // blockIdx.x < total
+  const int turns = (steps + 1) / 2, stages = tiles * turns;                            // the last stage of an odd number of steps holds one
 
   // the loading side: cursor (it, is) = tile and stage of the next piece, the tile's addresses
   const bool mine_w = wave < WAVES / 2;
   const int sub = mine_w ? wave : wave - WAVES / 2;
   __amdgpu_buffer_rsrc_t rc, rs;
   unsigned vc[PC], vs[PS];
+  const unsigned piece = (lane & 7) ^ (lane >> 4);                                       // of even p; p odd: ^ 4
   int it = 0, is = 0;
   auto aim = [&](int k) {
     int n0, m0;
@@ -544,42 +550,65 @@ __global__ __launch_bounds__(WN* WM * 64, 2) void mx4_gemm4_kernel(const LinArgs
     rc = __builtin_amdgcn_make_buffer_rsrc((void*)((mine_w ? a.w : (const uint8_t*)a.x) + (size_t)base * a.KB * 16), 0, -1, 0x00020000);
     rs = __builtin_amdgcn_make_buffer_rsrc((void*)((mine_w ? a.ws : a.xs) + (size_t)base * a.KB), 0, -1, 0x00020000);
 #pragma unroll
-    for (int p = 0; p < PC; ++p) {
-      const int r = (sub * PC + p) * 16 + (lane >> 2);
-      vc[p] = (unsigned)min(r, last) * a.KB * 16 + (((lane & 3) ^ ((r >> 1) & 3)) * 16);
-    }
+    for (int p = 0; p < PC; ++p) vc[p] = (unsigned)min((sub * PC + p) * 8 + (lane >> 3), last) * a.KB * 16 + (piece ^ (p & 1) * 4) * 16;
 #pragma unroll
     for (int p = 0; p < PS; ++p) vs[p] = (unsigned)min((sub * PS + p) * 64 + lane, last) * a.KB;
   };
   const unsigned lc = ring + (mine_w ? 0 : XC) + sub * PC * 1024;
   const unsigned ls = S16 ? ring + RING + (mine_w ? 0 : TN * 16) + sub * PS * 1024 : ring + (mine_w ? WS : XS) + sub * PS * 256;
-  auto issue = [&](int q) {                             // stage q of the stream (S16: every tile has a multiple of 4 stages)
-    const unsigned slot = (unsigned)(q & 3) * STAGE, s = s0 + is;
+  auto issue = [&](int d) {                             // stage d of the stream (S16: every tile has a multiple of 2 stages)
+    const unsigned slot = (unsigned)(d & 1) * STAGE, s = s0 + is * 2;
+    const bool one = is * 2 + 1 == steps;               // the second half would lie behind the rows: the first again, not read from LDS
     if constexpr (S16) {
-      if ((q & 3) == 0) {
+      if ((d & 1) == 0) {
 #pragma unroll
-        for (int p = 0; p < PS; ++p) lds_dma<16>(rs, ls + ((q >> 2) & 1) * SSLOT + p * 1024, vs[p], s * 4);
+        for (int p = 0; p < PS; ++p) lds_dma<16>(rs, ls + ((d >> 1) & 1) * SSLOT + p * 1024, vs[p], s * 4);
       }
     }
 #pragma unroll
-    for (int p = 0; p < PC; ++p) lds_dma<16>(rc, lc + slot + p * 1024, vc[p], s * 64);
+    for (int p = 0; p < PC; ++p) lds_dma<16>(rc, lc + slot + p * 1024, one && (piece ^ (p & 1) * 4) >= 4 ? vc[p] - 64 : vc[p], s * 64);
     if constexpr (!S16) {
 #pragma unroll
-      for (int p = 0; p < PS; ++p) lds_dma<4>(rs, ls + slot + p * 256, vs[p], s * 4);
+      for (int p = 0; p < PS; ++p) {
+        lds_dma<4>(rs, ls + slot + p * 256, vs[p], s * 4);
+        lds_dma<4>(rs, ls + slot + (mine_w ? TN : TM) * 4 + p * 256, vs[p], one ? s * 4 : s * 4 + 4);
+      }
     }
-    if (++is == steps) {
+    if (++is == turns) {
       is = 0;
       if (++it < tiles) aim(it);
     }
   };
   const int wn = wave % WN, wm = wave / WN;
-  const int fr = i * 64 + (g ^ ((i >> 1) & 3)) * 16;                                        // fragment read: row i, block g
+  i32x4 xf[2][MT], wf[D + 1];
+  int xsc[2][MT], wsc[D + 1];
+  const uint8_t *wl, *xl, *wsl, *xsl;                   // where this lane reads the fragments and scales of a step
+  auto look = [&](int d, int u) {
+    const uint8_t* st = smem + (d & 1) * STAGE;
+    const int f = i * 128 + ((u * 4 + g) ^ (i >> 1)) * 16;
+    wl = st + wn * (NT * 2048) + f;
+    xl = st + XC + wm * (MT * 2048) + f;
+    const uint8_t* sc = S16 ? smem + RING + ((d >> 1) & 1) * SSLOT + ((d & 1) * 2 + u) * 4 + g : st + WS + u * (TN * 4) + g;
+    wsl = sc + (wn * NT * 16 + i) * SR;
+    xsl = sc + TN * (S16 ? 16 : 8) + (wm * MT * 16 + i) * SR;
+  };
+  auto read_w = [&](int n, int f) { wf[f] = *(const i32x4*)(wl + n * 2048); wsc[f] = wsl[n * 16 * SR]; };
+  auto read_x = [&](int u, int m) { xf[u][m] = *(const i32x4*)(xl + m * 2048); xsc[u][m] = xsl[m * 16 * SR]; };
   aim(0);
-  for (int q = 0; q < NST - 1 && q < stages; ++q) issue(q);
-  if (stages >= 3) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * L) : "memory");             // (S16: the scale piece is issued first)
-  else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  int q = 0;
+  issue(0);
+  if (stages > 1) {
+    issue(1);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(L) : "memory");
+  } else {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  }
+  block_barrier();
+  look(0, 0);
+#pragma unroll
+  for (int m = 0; m < MT; ++m) read_x(0, m);
+#pragma unroll
+  for (int n = 0; n < D; ++n) read_w(n, n);
+  int d = 0;
 #pragma unroll 1
   for (int k = 0; k < tiles; ++k) {
     f32x4 acc[NT][MT];
@@ -588,34 +617,45 @@ __global__ __launch_bounds__(WN* WM * 64, 2) void mx4_gemm4_kernel(const LinArgs
 #pragma unroll
       for (int m = 0; m < MT; ++m) acc[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
-    for (int t = 0; t < steps; ++t, ++q) {
-      const uint8_t* st = smem + (q & 3) * STAGE;
-      const uint8_t *wl = st + wn * (NT * 16 * 64) + fr, *xl = st + XC + wm * (MT * 16 * 64) + fr;
-      const uint8_t* sc = S16 ? smem + RING + ((q >> 2) & 1) * SSLOT + (q & 3) * 4 + g : st + WS + g;
-      const uint8_t *wsl = sc + (wn * NT * 16 + i) * SR, *xsl = sc + TN * SR + (wm * MT * 16 + i) * SR;
-      i32x4 xf[MT], wf[D + 1];
-      int xsc[MT], wsc[D + 1];
+    for (int t = 0; t < turns; ++t, ++d) {
+      const bool one = t * 2 + 1 == steps;
 #pragma unroll
-      for (int m = 0; m < MT; ++m) { xf[m] = *(const i32x4*)(xl + m * 1024); xsc[m] = xsl[m * 16 * SR]; }
+      for (int u = 0; u < 2; ++u) {
+        if (u && one) {                                 // the next stage's x went to xf[1]
 #pragma unroll
-      for (int n = 0; n < D; ++n) { wf[n] = *(const i32x4*)(wl + n * 1024); wsc[n] = wsl[n * 16 * SR]; }
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        if (n == NT / 2 - 1 && q + 1 < stages) {
-          if (t == 0 && k) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-          else wait_ring<L>(stages - 2 - q);
-          __builtin_amdgcn_s_barrier();
-          if (q + NST - 1 < stages) issue(q + NST - 1);
+          for (int m = 0; m < MT; ++m) { xf[0][m] = xf[1][m]; xsc[0][m] = xsc[1][m]; }
+          break;
         }
-        if (n + D < NT) { wf[(n + D) % (D + 1)] = *(const i32x4*)(wl + (n + D) * 1024); wsc[(n + D) % (D + 1)] = wsl[(n + D) * 16 * SR]; }
-        const i32x4 wq = wf[n % (D + 1)];
-        const i32x8 w8 = {wq[0], wq[1], wq[2], wq[3], 0, 0, 0, 0};
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          const i32x8 x8 = {xf[m][0], xf[m][1], xf[m][2], xf[m][3], 0, 0, 0, 0};
-          acc[n][m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w8, x8, acc[n][m], 4, 4, 0, wsc[n % (D + 1)], 0, xsc[m]);
+        for (int n = 0; n < NT; ++n) {
+          if (n == NT - D) {                            // everything of this step has been read
+            if (u || one) {
+              if (d + 1 < stages) {
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                block_barrier();
+                if (d + 2 < stages) issue(d + 2);
+              }
+              look(d + 1, 0);                           // (behind the last stage: read, not used)
+            } else {
+              look(d, 1);
+            }
+          }
+          read_w((n + D) % NT, (n + D) % (D + 1));
+          if (n == NT - 3) { read_x(u ^ 1, 0); read_x(u ^ 1, 1); }
+          if (n == NT - 2) read_x(u ^ 1, 2);
+          if (n == NT - 1) read_x(u ^ 1, 3);
+          const i32x4 wq = wf[n % (D + 1)];
+          const i32x8 w8 = {wq[0], wq[1], wq[2], wq[3], 0, 0, 0, 0};
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            const i32x8 x8 = {xf[u][m][0], xf[u][m][1], xf[u][m][2], xf[u][m][3], 0, 0, 0, 0};
+            acc[n][m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w8, x8, acc[n][m], 4, 4, 0, wsc[n % (D + 1)], 0, xsc[u][m]);
+          }
+          // (an empty read of each result: left to itself the compiler moves the multiplications behind the branches, past all reads)
+#pragma unroll
+          for (int m = 0; m < MT; ++m) asm volatile("" : "+v"(acc[n][m]));
+          __builtin_amdgcn_sched_barrier(0);            // the reads stay D fragments ahead of the multiplications
         }
-        __builtin_amdgcn_sched_barrier(0);              // the reads stay D fragments ahead of the multiplications
       }
     }
     int n0, m0;
@@ -892,7 +932,7 @@ static int slab_reduce(const float* slab, int splits, int M, int N, const float*
 
 template <int TN, int TM, int WN, int WM, bool S16>
 static int gemm4_go(const LinArgs& a, int tn, int tm, int splits, hipStream_t st) {
-  constexpr int LDS = S16 ? (TN + TM) * (4 * 64 + 2 * 16) : (TN + TM) * 4 * 68;
+  constexpr int LDS = (TN + TM) * (S16 ? 2 * 128 + 2 * 16 : 2 * 136);
   auto k = mx4_gemm4_kernel<TN, TM, WN, WM, S16>;
   static std::atomic<unsigned long long> ready{0};           // one bit a device: more than 64 KB of dynamic LDS has to be allowed once
   int dev = 0;
@@ -980,7 +1020,7 @@ static LinPlan lin_plan(int M, int N, int K, int x_kind) {
   } else if (x_kind == IPRGAN_X_MX4) {
     p.tile = (long long)cdiv(M, 256) * cdiv(N, 256) >= 192 ? 256 : 128;
     p.s16 = steps % 4 == 0;                                 // the form that moves the scales of four stages at once
-    c = cut(&tile, 1, p.tile == 128, p.tile, p.tile, M, N, steps, p.s16 ? 4 : 1, weights);
+    c = cut(&tile, 1, p.tile == 128, p.tile, p.tile, M, N, steps, p.s16 ? 4 : 2, weights);
   }
   p.tm = c.tm;
   p.tn = c.tn;
