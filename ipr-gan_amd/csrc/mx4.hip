@@ -411,22 +411,23 @@ __global__ __launch_bounds__(256) void mx4_linear_kernel(const LinArgs a, int tn
 #pragma unroll
     for (int m = 0; m < MF; ++m) acc[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
   const u32x4* wp[NF];
-  const uint8_t* sp[NF];
 #pragma unroll
   for (int n = 0; n < NF; ++n) {
     const int row = min(n0 + n * 16 + i, a.N - 1);          // columns past N repeat the last row; their results are not stored
     wp[n] = (const u32x4*)(a.w + (size_t)row * a.KB * 16) + g;
-    sp[n] = a.ws + (size_t)row * a.KB + g;
   }
+  // a step's four scale bytes of one column a lane: 64 cache accesses an instruction, where a byte a lane and fragment takes 64 for each
+  const unsigned* sp = (const unsigned*)(a.ws + (size_t)min(n0 + (lane & (16 * NF - 1)), a.N - 1) * a.KB);
   const uint8_t* xrow[MF];
 #pragma unroll
   for (int t = 0; t < MF; ++t) xrow[t] = (const uint8_t*)a.x + (size_t)min(m0 + xr + t * 16, a.M - 1) * a.K * (PL == 1 ? 2 : 4);
   u32x4 wq[NF], wn[AHEAD][NF];
-  unsigned sq[NF], sn[AHEAD][NF];
+  unsigned sq[NF], sn[AHEAD];
   Raw8<PL == 1> xv[AHEAD][MF];
   auto load = [&](int s, int b) {
 #pragma unroll
-    for (int n = 0; n < NF; ++n) { wn[b][n] = wp[n][s * 4]; sn[b][n] = sp[n][s * 4]; }
+    for (int n = 0; n < NF; ++n) wn[b][n] = wp[n][s * 4];
+    if (NF == 4 || lane < 16 * NF) sn[b] = sp[s];
 #pragma unroll
     for (int t = 0; t < MF; ++t) xv[b][t] = row8<PL == 1>(xrow[t], s * 128 + xc, a.K, s * 128 + 128 > a.K);
   };
@@ -443,7 +444,10 @@ __global__ __launch_bounds__(256) void mx4_linear_kernel(const LinArgs a, int tn
       for (int q = 0; q < PL; ++q) xs[q][xr + t * 16][(threadIdx.x & 15) ^ swz(xr)] = p[q];
     }
 #pragma unroll
-    for (int n = 0; n < NF; ++n) { wq[n] = wn[b][n]; sq[n] = sn[b][n]; }
+    for (int n = 0; n < NF; ++n) {
+      wq[n] = wn[b][n];
+      sq[n] = (unsigned)__builtin_amdgcn_ds_bpermute((n * 16 + i) * 4, (int)sn[b]) >> (g * 8) & 255u;
+    }
     lds_sync();
     if (s + AHEAD < s1) load(s + AHEAD, b);                 // in flight while AHEAD steps are multiplied
     // (8 elements j, plane q) pairs in turn, the smallest plane first; x fragments are read D pairs ahead of their use - left to itself the
