@@ -278,7 +278,7 @@ __device__ __forceinline__ Place place(int tn, int tm) {
 // (the scaled instruction), 1 = bf16, 3 = fp32 (planes).  Bound by latency, or by the split of fp32 x into planes (176 vector instructions a
 // step and 16 rows, repeated by every wave: why more rows go through LDS below).
 template <int MF, int NF, int XT>
-__global__ __launch_bounds__(512) void mx4_direct_kernel(const LinArgs a, int tn, int tm, int wk) {
+__global__ __launch_bounds__(512, NF == 1 && XT != 3 ? 4 : 2) void mx4_direct_kernel(const LinArgs a, int tn, int tm, int wk) {
   constexpr int PL = XT == 3 ? 3 : 1;
   __shared__ f32x4 red[8][NF * MF][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
@@ -292,12 +292,13 @@ __global__ __launch_bounds__(512) void mx4_direct_kernel(const LinArgs a, int tn
 #pragma unroll
     for (int m = 0; m < MF; ++m) acc[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
   const i32x4 *wp[NF], *xp[MF];
-  const uint8_t *wsp[NF], *xsp[MF];
+  // (the four scale bytes of a row and step by one lane each, handed round: byte loads by all lanes cost as many cache accesses as the codes)
+  const unsigned* wsp = (const unsigned*)(a.ws + (size_t)min(n0 + (lane & (16 * NF - 1)), a.N - 1) * a.KB);
+  const unsigned* xsp = (const unsigned*)(a.xs + (size_t)min(m0 + (lane & (16 * MF - 1)), a.M - 1) * a.KB);
 #pragma unroll
   for (int n = 0; n < NF; ++n) {
     const size_t r = min(n0 + n * 16 + i, a.N - 1);         // rows past the end repeat the last one; their results are not stored
     wp[n] = (const i32x4*)(a.w + r * a.KB * 16) + g;
-    wsp[n] = a.ws + r * a.KB + g;
   }
   constexpr unsigned ESZ = XT == 1 ? 2 : 4;
   const uint8_t* xrow[MF];
@@ -305,20 +306,20 @@ __global__ __launch_bounds__(512) void mx4_direct_kernel(const LinArgs a, int tn
   for (int m = 0; m < MF; ++m) {
     const size_t r = min(m0 + m * 16 + i, a.M - 1);
     xp[m] = (const i32x4*)((const uint8_t*)a.x + r * a.KB * 16) + g;
-    xsp[m] = a.xs + r * a.KB + g;
     xrow[m] = (const uint8_t*)a.x + r * a.K * ESZ;
   }
   i32x4 wq[2][NF], xq[2][MF];
-  int wsc[2][NF], xsc[2][MF];
+  int wsn[2], xsn[2];
   Raw8<XT == 1> xv[2][XT ? MF : 1][4];
   auto load = [&](int s, int b) {
 #pragma unroll
-    for (int n = 0; n < NF; ++n) { wq[b][n] = wp[n][s * 4]; wsc[b][n] = wsp[n][s * 4]; }
+    for (int n = 0; n < NF; ++n) wq[b][n] = wp[n][s * 4];
+    if (lane < 16 * NF) wsn[b] = (int)wsp[s];
+    if (XT == 0 && (MF == 4 || lane < 16 * MF)) xsn[b] = (int)xsp[s];
 #pragma unroll
     for (int m = 0; m < MF; ++m) {
       if constexpr (XT == 0) {
         xq[b][m] = xp[m][s * 4];
-        xsc[b][m] = xsp[m][s * 4];
       } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j) xv[b][m][j] = row8<XT == 1>(xrow[m], s * 128 + g * 32 + j * 8, a.K, s * 128 + 128 > a.K);
@@ -326,6 +327,11 @@ __global__ __launch_bounds__(512) void mx4_direct_kernel(const LinArgs a, int tn
     }
   };
   auto mul = [&](int b) {
+    int wsc[NF], xsc[MF];
+#pragma unroll
+    for (int n = 0; n < NF; ++n) wsc[n] = __builtin_amdgcn_ds_bpermute((n * 16 + i) * 4, wsn[b]) >> (g * 8) & 255;
+#pragma unroll
+    for (int m = 0; m < MF; ++m) xsc[m] = XT == 0 ? __builtin_amdgcn_ds_bpermute((m * 16 + i) * 4, xsn[b]) >> (g * 8) & 255 : 0;
     if constexpr (XT == 0) {
 #pragma unroll
       for (int n = 0; n < NF; ++n)
@@ -333,14 +339,14 @@ __global__ __launch_bounds__(512) void mx4_direct_kernel(const LinArgs a, int tn
         for (int m = 0; m < MF; ++m) {
           const i32x4 p = wq[b][n], q = xq[b][m];
           const i32x8 w8 = {p[0], p[1], p[2], p[3], 0, 0, 0, 0}, x8 = {q[0], q[1], q[2], q[3], 0, 0, 0, 0};
-          acc[n][m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w8, x8, acc[n][m], 4, 4, 0, wsc[b][n], 0, xsc[b][m]);
+          acc[n][m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w8, x8, acc[n][m], 4, 4, 0, wsc[n], 0, xsc[m]);
         }
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         bf16x8 wf[NF];
 #pragma unroll
-        for (int n = 0; n < NF; ++n) wf[n] = widen_fp4((unsigned)wq[b][n][j], mx4_step((unsigned)wsc[b][n]));
+        for (int n = 0; n < NF; ++n) wf[n] = widen_fp4((unsigned)wq[b][n][j], mx4_step((unsigned)wsc[n]));
 #pragma unroll
         for (int m = 0; m < MF; ++m) {
           bf16x8 p[PL];
@@ -385,6 +391,14 @@ __global__ __launch_bounds__(512) void mx4_direct_kernel(const LinArgs a, int tn
     for (int m = 0; m < MF; ++m) store4(a, pl.z, m0 + m * 16 + i, n0 + n * 16 + g * 4, acc[n][m]);
 }
 
+typedef __attribute__((address_space(3))) void lds_void;
+template <int BYTES>
+__device__ __forceinline__ void lds_dma(__amdgpu_buffer_rsrc_t rs, unsigned lds, unsigned voff, unsigned soff) {
+#if defined(__HIP_DEVICE_COMPILE__)      // (an error that the host pass defers silently, dropping the kernel's stub)
+  if constexpr (BYTES == 16) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(uintptr_t)lds, 16, voff, soff, 0, 0);
+  else __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(uintptr_t)lds, 4, voff, soff, 0, 0);
+#endif
+}
 // More rows of fp32 / bf16 x.  A block is 4 waves: each owns 16 * NF output columns (weights straight from memory to its registers: a lane reads
 // whole 16-byte blocks, lane group g block g of the step, and the step's four instructions take 8 elements of each block - the order of
 // K is free as long as both operands agree); the 16 * MF rows of x are shared through LDS, split into planes on the way in.
@@ -399,8 +413,10 @@ __device__ __forceinline__ int swz(int row) { return (row & 3) | ((row >> 2 & 1)
 template <int MF, int NF, int PL>
 __global__ __launch_bounds__(256) void mx4_linear_kernel(const LinArgs a, int tn, int tm) {
   constexpr int AHEAD = PL == 1 && NF < 4 ? 2 : 1;
-  __shared__ bf16x8 xs[PL][MF * 16][16];                    // one buffer: 48 KB at most, three blocks a CU hide each other's barriers
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+  constexpr bool DMA = !(MF == 4 && NF == 2 && PL == 3);
+  __shared__ u32x4 ws[DMA ? AHEAD : 1][4][DMA ? NF * 64 : 1];
+  __shared__ bf16x8 xs[PL][MF * 16][16];                    // one buffer: 48 KB at most, blocks beside it hide the barriers
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
   const Place pl = place(tn, tm);
   const int n0 = pl.n * 64 * NF + wave * 16 * NF, m0 = pl.m * 16 * MF;
   const int s0 = pl.z * a.steps_per_split, s1 = min(a.KB / 4, s0 + a.steps_per_split);
@@ -410,23 +426,34 @@ __global__ __launch_bounds__(256) void mx4_linear_kernel(const LinArgs a, int tn
   for (int n = 0; n < NF; ++n)
 #pragma unroll
     for (int m = 0; m < MF; ++m) acc[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const u32x4* wp[NF];
+  // W goes through LDS by DMA: four neighbouring lanes fetch a row's 64 bytes, where the fragments' own order (neighbours in different rows) takes
+  // an access a lane (4096^3: bf16 149 -> 140 us, fp32 328 -> 318).  Piece c of row r at c ^ ((r >> 1) & 3): no conflicts.  Not for fp32 in 64 x
+  // 128 tiles, where the 8 KB more leave two blocks a CU instead of three (64 x 8192 x 16384: 67 -> 73).  Columns past N repeat the last row;
+  // their results are not stored.
+  const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc((void*)(a.w + (size_t)min(n0, a.N - 1) * a.KB * 16), 0, -1, 0x00020000);
+  unsigned wo[NF];
 #pragma unroll
   for (int n = 0; n < NF; ++n) {
-    const int row = min(n0 + n * 16 + i, a.N - 1);          // columns past N repeat the last row; their results are not stored
-    wp[n] = (const u32x4*)(a.w + (size_t)row * a.KB * 16) + g;
+    const int row = DMA ? lane >> 2 : i, piece = DMA ? (lane & 3) ^ ((lane >> 3) & 3) : g;
+    wo[n] = (unsigned)max(min(n * 16 + row, a.N - 1 - n0), 0) * a.KB * 16 + piece * 16;
   }
+  const unsigned wbase = (unsigned)(uintptr_t)(lds_void*)&ws[0][wave][0];
+  const int fr = i * 4 + (g ^ ((i >> 1) & 3));
   // a step's four scale bytes of one column a lane: 64 cache accesses an instruction, where a byte a lane and fragment takes 64 for each
   const unsigned* sp = (const unsigned*)(a.ws + (size_t)min(n0 + (lane & (16 * NF - 1)), a.N - 1) * a.KB);
   const uint8_t* xrow[MF];
 #pragma unroll
   for (int t = 0; t < MF; ++t) xrow[t] = (const uint8_t*)a.x + (size_t)min(m0 + xr + t * 16, a.M - 1) * a.K * (PL == 1 ? 2 : 4);
-  u32x4 wq[NF], wn[AHEAD][NF];
+  u32x4 wq[NF], wn[DMA ? 1 : NF];
   unsigned sq[NF], sn[AHEAD];
   Raw8<PL == 1> xv[AHEAD][MF];
   auto load = [&](int s, int b) {
 #pragma unroll
-    for (int n = 0; n < NF; ++n) wn[b][n] = wp[n][s * 4];
+    for (int n = 0; n < NF; ++n) {
+      if constexpr (DMA) lds_dma<16>(rw, wbase + b * (4 * NF * 1024) + n * 1024, wo[n], s * 64);
+      else wn[n] = __builtin_amdgcn_raw_buffer_load_b128(rw, wo[n], s * 64, 0);
+    }
+    asm volatile("" ::: "memory");                            // (x is loaded after W: once x is there, W is)
     if (NF == 4 || lane < 16 * NF) sn[b] = sp[s];
 #pragma unroll
     for (int t = 0; t < MF; ++t) xv[b][t] = row8<PL == 1>(xrow[t], s * 128 + xc, a.K, s * 128 + 128 > a.K);
@@ -435,6 +462,11 @@ __global__ __launch_bounds__(256) void mx4_linear_kernel(const LinArgs a, int tn
   for (int b = 0; b < AHEAD; ++b)
     if (s0 + b < s1) load(s0 + b, b);
   auto step = [&](int s, int b) {
+#pragma unroll
+    for (int t = 0; t < MF; ++t) {
+      if constexpr (PL == 1) asm volatile("" ::"v"(xv[b][t].h) : "memory");
+      else asm volatile("" ::"v"(xv[b][t].a), "v"(xv[b][t].b) : "memory");
+    }
     if (s > s0) lds_sync();                                 // every wave has read the last step's planes
 #pragma unroll
     for (int t = 0; t < MF; ++t) {
@@ -445,7 +477,8 @@ __global__ __launch_bounds__(256) void mx4_linear_kernel(const LinArgs a, int tn
     }
 #pragma unroll
     for (int n = 0; n < NF; ++n) {
-      wq[n] = wn[b][n];
+      if constexpr (DMA) wq[n] = ws[b][wave][n * 64 + fr];
+      else wq[n] = wn[n];
       sq[n] = (unsigned)__builtin_amdgcn_ds_bpermute((n * 16 + i) * 4, (int)sn[b]) >> (g * 8) & 255u;
     }
     lds_sync();
@@ -489,14 +522,6 @@ __global__ __launch_bounds__(256) void mx4_linear_kernel(const LinArgs a, int tn
 // ---- many rows of 4-bit x -----------------------------------------------------------------------------------------------------------
 // The scaled matrix instruction multiplies 128 elements of K at once: a lane holds one 16-byte block of its row (i = lane & 15, block
 // g = lane >> 4 of the step) and that block's scale byte, for each operand.
-typedef __attribute__((address_space(3))) void lds_void;
-template <int BYTES>
-__device__ __forceinline__ void lds_dma(__amdgpu_buffer_rsrc_t rs, unsigned lds, unsigned voff, unsigned soff) {
-#if defined(__HIP_DEVICE_COMPILE__)      // (an error that the host pass defers silently, dropping the kernel's stub)
-  if constexpr (BYTES == 16) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(uintptr_t)lds, 16, voff, soff, 0, 0);
-  else __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(uintptr_t)lds, 4, voff, soff, 0, 0);
-#endif
-}
 // (the barrier alone is no fence to the compiler)
 __device__ __forceinline__ void block_barrier() {
   asm volatile("" ::: "memory");
@@ -773,18 +798,39 @@ struct Words {
 template <int MF, int KW, int PL, bool ODD>
 __global__ __launch_bounds__(256, 2) void mx4_linear_bwd_kernel(const BwdArgs a, int tk, int tm) {
   typedef typename Words<KW>::type words;
-  __shared__ float tile[4][16][132];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+  constexpr int RB = PL == 1 ? 64 : 128;                    // bytes of a dy row in a step
+  constexpr bool DMA = MF > 1 && !ODD;
+  __shared__ union {
+    float tile[4][16][132];
+    u32x4 dy[4][DMA ? MF * RB : 1];                                   // [wave]: MF * 16 rows of RB / 16 pieces
+  } sh;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
   const Place pl = place(tk, tm);
   const int k0 = pl.n * 128 * KW, m0 = pl.m * 16 * MF;
   const int blk = min(k0 / 32 + i * KW / 4, a.KB - 1);      // (k past the padded row repeat the last block; their results are not stored)
   const uint8_t* wp = a.w + (size_t)blk * 16 + i * KW % 4 * 4;
-  const uint8_t* sp = a.ws + blk;
+  // the scales of a step: lane l holds four of row l % 32 (KW = 2: lanes from 32 on the next four), handed round
+  const uint8_t* sp = a.ws + min(k0 / 32 + (lane >> 5) * 4, a.KB - 4);
+  const int sl = ((KW == 2 ? (i >> 3) * 32 : 0) + g * 8) * 4, sb = (i * KW / 4 & 3) * 8;
   const uint8_t* drow[MF];
 #pragma unroll
   for (int m = 0; m < MF; ++m) drow[m] = (const uint8_t*)a.dy + (size_t)min(m0 + m * 16 + i, a.M - 1) * a.N * (PL == 1 ? 2 : 4);
   const int steps = (a.N + 31) / 32;
   const int s0 = (pl.z * 4 + wave) * a.steps_per_wave, s1 = min(steps, s0 + a.steps_per_wave);         // (a wave may be left without a step)
+  // Several fragments of dy go through LDS by DMA, a wave's own rows: neighbouring lanes fetch a row's bytes, where the fragments' order takes an
+  // access a lane (512 x 4096 x 4096: bf16 42 -> 36 us, fp32 67 -> 62; one fragment is not worth its waits, 32 x 8192 x 16384 33 -> 36).
+  // Piece c of row r at c ^ swz_dy(r): no bank conflicts.  Row ends are met by the last step alone, which loads to registers; so do rows of
+  // odd length.
+  constexpr int PR = RB / 16, DP = DMA ? MF * 16 * RB / 1024 : 1;     // pieces a row; DMA instructions a step
+  auto swz_dy = [](int r) { return PR == 4 ? r >> 1 & 3 : (r >> 1 & 1) | ((r >> 2 & 1) * 2 ^ (r >> 3 & 1) * 3) << 1; };
+  unsigned dofs[DP];
+  const __amdgpu_buffer_rsrc_t rd = __builtin_amdgcn_make_buffer_rsrc((void*)((const uint8_t*)a.dy + (size_t)m0 * a.N * (RB / 32)), 0, -1, 0x00020000);
+#pragma unroll
+  for (int p = 0; p < DP; ++p) {
+    const int r = p * (64 / PR) + lane / PR;
+    dofs[p] = (unsigned)min(r, a.M - 1 - m0) * (unsigned)a.N * (RB / 32) + ((lane % PR) ^ swz_dy(r)) * 16;
+  }
+  const unsigned dbase = (unsigned)(uintptr_t)(lds_void*)&sh.dy[wave][0];
   f32x4 acc[KW][8][MF];
 #pragma unroll
   for (int w = 0; w < KW; ++w)
@@ -793,7 +839,7 @@ __global__ __launch_bounds__(256, 2) void mx4_linear_bwd_kernel(const BwdArgs a,
 #pragma unroll
       for (int m = 0; m < MF; ++m) acc[w][j][m] = f32x4{0.f, 0.f, 0.f, 0.f};
   words wn[8];
-  unsigned sn[8];
+  unsigned sn = 0;
   Raw8<PL == 1> xn[MF];
   // ODD: bf16 rows of odd length.  Every second one starts in the middle of a 4-byte word, where a vector load takes twice as long, so its elements
   // are taken from the five words that hold them: 512 x 8193 x 6208 226 -> 151 us (106 with N = 8192).  An instance of its own, for the form of
@@ -802,25 +848,29 @@ __global__ __launch_bounds__(256, 2) void mx4_linear_bwd_kernel(const BwdArgs a,
   auto load = [&](int s) {
     const int nb = s * 32 + g * 8;
     const bool tail = s * 32 + 32 > a.N;
+    if (DMA && !tail) {
 #pragma unroll
-    for (int r = 0; r < 8; ++r) {
-      const size_t row = min(nb + r, a.N - 1);              // rows past N meet a zero of dy
-      wn[r] = *(const words*)(wp + row * a.KB * 16);
-      sn[r] = sp[row * a.KB];
+      for (int p = 0; p < DP; ++p) lds_dma<16>(rd, dbase + p * 1024, dofs[p], s * RB);
     }
+    if (DMA) asm volatile("" ::: "memory");                 // (W is loaded after dy: once W is there, dy is)
+    if (KW == 2 || lane < 32) sn = *(const unsigned*)(sp + (size_t)min(s * 32 + (lane & 31), a.N - 1) * a.KB);
 #pragma unroll
-    for (int m = 0; m < MF; ++m) {
-      if constexpr (ODD) {
-        xw[m] = 0;
-        if (!tail) {
-          const unsigned half = (unsigned)(uintptr_t)drow[m] & 2;
-          const uint8_t* p = drow[m] + (size_t)nb * 2 - half;
-          xn[m].h = *(const bf16x8w*)p;
-          xw[m] = *(const unsigned*)(p + 12 + half * 2);    // (never past the word of the last element)
-          continue;
+    for (int r = 0; r < 8; ++r) wn[r] = *(const words*)(wp + (size_t)min(nb + r, a.N - 1) * a.KB * 16);      // rows past N meet a zero of dy
+    if (!DMA || tail) {
+#pragma unroll
+      for (int m = 0; m < MF; ++m) {
+        if constexpr (ODD) {
+          xw[m] = 0;
+          if (!tail) {
+            const unsigned half = (unsigned)(uintptr_t)drow[m] & 2;
+            const uint8_t* p = drow[m] + (size_t)nb * 2 - half;
+            xn[m].h = *(const bf16x8w*)p;
+            xw[m] = *(const unsigned*)(p + 12 + half * 2);  // (never past the word of the last element)
+            continue;
+          }
         }
+        xn[m] = row8<PL == 1>(drow[m], nb, a.N, tail);
       }
-      xn[m] = row8<PL == 1>(drow[m], nb, a.N, tail);
     }
     whole = tail ? 0u : ~0u;
   };
@@ -831,7 +881,24 @@ __global__ __launch_bounds__(256, 2) void mx4_linear_bwd_kernel(const BwdArgs a,
     float sc[8];
     bf16x8 xf[MF][PL];
 #pragma unroll
-    for (int r = 0; r < 8; ++r) { wq[r] = wn[r]; sc[r] = mx4_step(sn[r]); }
+    for (int r = 0; r < 8; ++r) {
+      if constexpr (DMA && KW == 1) asm volatile("" ::"v"(wn[r][0]) : "memory");
+      if constexpr (DMA && KW > 1) asm volatile("" ::"v"(wn[r]) : "memory");
+      wq[r] = wn[r];
+      sc[r] = mx4_step((unsigned)__builtin_amdgcn_ds_bpermute(sl + r * 4, (int)sn) >> sb & 255u);
+    }
+    if (DMA && whole) {
+#pragma unroll
+      for (int m = 0; m < MF; ++m) {
+        const u32x4* d = &sh.dy[wave][(m * 16 + i) * PR];
+        if constexpr (PL == 1) {
+          xn[m].h = __builtin_bit_cast(bf16x8, d[g ^ swz_dy(i)]);
+        } else {
+          xn[m].a = __builtin_bit_cast(f32x4, d[(2 * g) ^ swz_dy(i)]);
+          xn[m].b = __builtin_bit_cast(f32x4, d[(2 * g + 1) ^ swz_dy(i)]);
+        }
+      }
+    }
 #pragma unroll
     for (int m = 0; m < MF; ++m) {
       split_raw<PL>(xn[m], xf[m]);
@@ -843,6 +910,7 @@ __global__ __launch_bounds__(256, 2) void mx4_linear_bwd_kernel(const BwdArgs a,
         xf[m][0] = __builtin_bit_cast(bf16x8, d);
       }
     }
+    if (DMA) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");        // dy has been read
     if (s + 1 < s1) load(s + 1);
     __builtin_amdgcn_sched_barrier(0);                      // the next step's loads leave before this one is multiplied
 #pragma unroll
@@ -881,20 +949,20 @@ __global__ __launch_bounds__(256, 2) void mx4_linear_bwd_kernel(const BwdArgs a,
   for (int m = 0; m < MF; ++m)
 #pragma unroll
     for (int w = 0; w < KW; ++w) {
-      if (m || w) __syncthreads();
+      __syncthreads();                                      // (before the first: the tiles lie where dy lay)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const f32x4 lo = {acc[w][0][m][r], acc[w][1][m][r], acc[w][2][m][r], acc[w][3][m][r]},
                     hi = {acc[w][4][m][r], acc[w][5][m][r], acc[w][6][m][r], acc[w][7][m][r]};
-        *(f32x4*)&tile[wave][i][8 * (g * 4 + r)] = lo;
-        *(f32x4*)&tile[wave][i][8 * (g * 4 + r) + 4] = hi;
+        *(f32x4*)&sh.tile[wave][i][8 * (g * 4 + r)] = lo;
+        *(f32x4*)&sh.tile[wave][i][8 * (g * 4 + r) + 4] = hi;
       }
       __syncthreads();
       const int mm = threadIdx.x >> 4, kk = threadIdx.x & 15, row = m0 + m * 16 + mm, k = k0 + (kk * KW + w) * 8;
       if (row >= a.M || k >= a.K) continue;
       float v[8];
 #pragma unroll
-      for (int q = 0; q < 8; ++q) v[q] = (tile[0][mm][kk * 8 + q] + tile[1][mm][kk * 8 + q]) + (tile[2][mm][kk * 8 + q] + tile[3][mm][kk * 8 + q]);
+      for (int q = 0; q < 8; ++q) v[q] = (sh.tile[0][mm][kk * 8 + q] + sh.tile[1][mm][kk * 8 + q]) + (sh.tile[2][mm][kk * 8 + q] + sh.tile[3][mm][kk * 8 + q]);
       const size_t o = ((size_t)(a.slab ? pl.z : 0) * a.M + row) * a.K + k;
       if (a.slab || !a.dx_bf16) {
         float* d = a.slab ? a.slab : (float*)a.dx;
