@@ -514,14 +514,15 @@ int iprgan_mx4_pitch(int cols);
 int iprgan_mx4_quant(const void* x, void* codes, void* scales, int rows, int cols, int x_bf16, void* stream);
 int iprgan_mx4_dequant(const void* codes, const void* scales, void* y, int rows, int cols, int y_bf16, void* stream);
 /* y [M][N] = act(x W^T + bias), W [N][K] in 4 bits.  x [M][K]: fp32 (multiplied as three bf16 planes: products exact, fp32
- * accumulation), bf16, or 4-bit itself (x = codes with K columns, x_scales; the scaled matrix instruction).  bias [N] fp32 or
+ * accumulation; an infinity, or a magnitude that rounds to one in bf16 - above 3.39e38 -, gives NaN), bf16, or 4-bit itself (x = codes with K columns, x_scales; the scaled matrix instruction).  bias [N] fp32 or
  * NULL; y fp32 or bf16, rounded once.  ws: 16-byte aligned, iprgan_mx4_linear_ws_floats floats (0: may be NULL); sums over a
  * split K are added in fixed order. */
 enum { IPRGAN_X_F32 = 0, IPRGAN_X_BF16 = 1, IPRGAN_X_MX4 = 2 };
 size_t iprgan_mx4_linear_ws_floats(int M, int N, int K, int x_kind, int act);
 int iprgan_mx4_linear(const void* x, const void* x_scales, const void* w_codes, const void* w_scales, const float* bias, void* y,
                       float* ws, int M, int N, int K, int x_kind, int act, float slope, int y_bf16, void* stream);
-/* dx [M][K] = dy [M][N] W (M at most 2^20, N and K below 2^24, here and above): the gradient with respect to x through the frozen 4-bit weights */
+/* dx [M][K] = dy [M][N] W: the gradient with respect to x through the frozen 4-bit weights.  (M at most 2^20, N and K below
+ * 2^24, here and above.) */
 size_t iprgan_mx4_linear_bwd_ws_floats(int M, int N, int K, int dy_bf16);
 int iprgan_mx4_linear_bwd(const void* dy, const void* w_codes, const void* w_scales, void* dx, float* ws, int M, int N, int K,
                           int dy_bf16, int dx_bf16, void* stream);

@@ -1,6 +1,7 @@
-"""Removal attacks of the reference's evaluation scripts, as library functions (SURVEY.md section 8f rank 3).
+"""Removal attacks of the reference's evaluation scripts, as library functions.
 
-``quantize_`` is a removal attack the reference does not have (weight compression to 4 bits).  ``sign_flip_`` is the loop body of sign_flip.py:59-75, ``prune_`` the one of prune.py:46-57; both act on the
+``quantize_`` is a removal attack the reference does not have (weight compression to 4 bits).
+``sign_flip_`` is the loop body of sign_flip.py:59-75, ``prune_`` the one of prune.py:46-57; both act on the
 generator whose BatchNorm / InstanceNorm scales carry the watermark, and are followed in the reference by
 ``SignLossModel.compute_ber`` (experiments/image_generation.py:161-164) - here the exact int64 count kernel
 ``iprgan_sign_ber``.  ``matching_p_value`` is tools/phash_pvalue.py:34-37 (the hash itself is the third-party

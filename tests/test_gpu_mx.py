@@ -404,6 +404,24 @@ def test_mx4_linear_gradient_against_differences(dev):
     assert abs(float(num - ana)) <= 2.0 ** -23 * 100 * float(scale)
 
 
+@pytest.mark.parametrize('M,K,N', [(1000, 1024, 700), (2304, 2048, 5888), (100, 20000, 70), (70, 33000, 200), (257, 128, 300), (129, 256, 40)])
+def test_mx4_product_stages_and_splits(dev, M, K, N):
+    """Both operands in 4 bits: K in whole and odd numbers of stages, split over blocks, one tile and several a block, repeated (float64 on
+    the device)."""
+    from iprgan import ops
+    xq = ops.mx4_quant(rnd(M, K, seed=1).to(dev))
+    wq = ops.mx4_quant((rnd(N, K, seed=2) / K ** 0.5).to(dev))
+    bias = rnd(N, seed=3).to(dev)
+    xd, wd = ops.mx4_dequant(xq).double(), ops.mx4_dequant(wq).double().t().contiguous()
+    want = xd @ wd + bias.double()
+    tol = lin_bound(xd.abs(), wd.abs(), K, 1) + 2.0 ** -23 * want.abs()
+    first = ops.mx4_linear(xq, wq, bias, dtype=torch.float32)
+    err = (first.double() - want).abs()
+    assert bool((err <= tol).all()), float((err / tol).max())
+    for _ in range(3):
+        assert torch.equal(first, ops.mx4_linear(xq, wq, bias, dtype=torch.float32))
+
+
 @pytest.mark.parametrize('M,K,N', [(4099, 300, 3101), (2304, 1700, 5888)])
 def test_mx4_product_of_many_rows(dev, M, K, N):
     """More tiles than the chip runs at once, ragged edges, both operands in 4 bits (float64 on the device)."""

@@ -115,3 +115,12 @@ def test_shapes_are_checked():
         ops.bn_bwd(q, None, torch.zeros(4, 31), None, torch.zeros(32), torch.zeros(32), 0)
     with pytest.raises(RuntimeError, match='norm backward'):
         ops.bn_bwd(q, None, torch.zeros(4, 32), torch.zeros(31), torch.zeros(32), torch.zeros(32), 0)
+
+
+def test_ckpt8_engine_key(monkeypatch):
+    from iprgan import configs, engine
+    monkeypatch.setenv('IPRGAN_CKPT8', '0')
+    monkeypatch.setattr(engine, '_CKPT8', False)
+    assert configs.apply_engine({'engine': {'ckpt8': True}}, set_math=False) == {'ckpt8': True} and engine._CKPT8
+    configs.apply_engine({'engine': {'ckpt8': False}}, set_math=False)
+    assert not engine._CKPT8
