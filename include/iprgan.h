@@ -515,7 +515,7 @@ int iprgan_mx4_quant(const void* x, void* codes, void* scales, int rows, int col
 int iprgan_mx4_dequant(const void* codes, const void* scales, void* y, int rows, int cols, int y_bf16, void* stream);
 /* y [M][N] = act(x W^T + bias), W [N][K] in 4 bits.  x [M][K]: fp32 (multiplied as three bf16 planes: products exact, fp32
  * accumulation; an infinity, or a magnitude that rounds to one in bf16 - above 3.39e38 -, gives NaN), bf16, or 4-bit itself (x = codes with K columns, x_scales; the scaled matrix instruction).  bias [N] fp32 or
- * NULL; y fp32 or bf16, rounded once.  ws: 16-byte aligned, iprgan_mx4_linear_ws_floats floats (0: may be NULL); sums over a
+ * NULL; act as everywhere here (a NaN behind a ReLU is 0); y fp32 or bf16, rounded once.  ws: 16-byte aligned, iprgan_mx4_linear_ws_floats floats (0: may be NULL); sums over a
  * split K are added in fixed order. */
 enum { IPRGAN_X_F32 = 0, IPRGAN_X_BF16 = 1, IPRGAN_X_MX4 = 2 };
 size_t iprgan_mx4_linear_ws_floats(int M, int N, int K, int x_kind, int act);

@@ -399,13 +399,22 @@ __device__ __forceinline__ void lds_dma(__amdgpu_buffer_rsrc_t rs, unsigned lds,
   else __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(uintptr_t)lds, 4, voff, soff, 0, 0);
 #endif
 }
-// More rows of fp32 / bf16 x.  A block is 4 waves: each owns 16 * NF output columns (weights straight from memory to its registers: a lane reads
-// whole 16-byte blocks, lane group g block g of the step, and the step's four instructions take 8 elements of each block - the order of
-// K is free as long as both operands agree); the 16 * MF rows of x are shared through LDS, split into planes on the way in.
+// (the barrier alone is no fence to the compiler)
+__device__ __forceinline__ void block_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// More rows of fp32 / bf16 x.  A block is 4 waves: each owns 16 * NF output columns (their weights come through a part of LDS that is the wave's
+// own: a lane holds whole 16-byte blocks, lane group g block g of the step, and the step's four instructions take 8 elements of each block -
+// the order of K is free as long as both operands agree); the 16 * MF rows of x are shared through LDS, split into planes on the way in.
+// What bounds it at 4096^3: bf16 136 us, 1010 TFLOP/s - two blocks a CU, whose loads, LDS traffic and multiplications overlap to about 45 % of
+// the matrix pipe; fp32 318 us, three products each.
 // (a barrier for LDS alone: __syncthreads would also wait for the loads in flight)
 __device__ __forceinline__ void lds_sync() {
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  __builtin_amdgcn_s_barrier();
+  block_barrier();
 }
 // Where a row keeps its 16-byte pieces: piece c at c ^ swz(row).  A 16-byte LDS read serves 16 lanes at a time, lanes 0-3, 12-15, 20-23 and
 // 24-27 the first: rows 0-3 and 12-15 of lane group 0, rows 4-11 of group 1.  This order of the rows (0-15) gives the halves disjoint banks.
@@ -522,13 +531,6 @@ __global__ __launch_bounds__(256) void mx4_linear_kernel(const LinArgs a, int tn
 // ---- many rows of 4-bit x -----------------------------------------------------------------------------------------------------------
 // The scaled matrix instruction multiplies 128 elements of K at once: a lane holds one 16-byte block of its row (i = lane & 15, block
 // g = lane >> 4 of the step) and that block's scale byte, for each operand.
-// (the barrier alone is no fence to the compiler)
-__device__ __forceinline__ void block_barrier() {
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-}
-
 // Many rows: TN x TM tiles, WN x WM waves, codes and scales of both operands through two LDS slots filled by LDS-DMA, a stage of 256
 // elements of K (two steps of the instruction) in each; the first half of the waves loads W, the second half x.
 //   * A row is 128 bytes a stage, a whole cache line: 25 M L2 requests at 8192^3, where stages of 128 elements made 42 M of half a line
@@ -1046,7 +1048,9 @@ static Cut cut(const Form* forms, int count, int kind, int rows_f, int cols_f, i
     if (q.mf * q.nf == 16 && (long long)tm * tn < 512) continue;
     for (int want = 1; want <= 64 && want <= steps; want = want < 8 ? want + 1 : want + want / 4) {
       const int per = rup(cdiv(steps, want), unit), splits = cdiv(steps, per);
-      const double blocks = (double)tm * tn * splits, b = (double)((long long)((blocks + 255) / 256)), full = (double)((long long)(b / R)), rem = b - full * R;
+      const double blocks = (double)tm * tn * splits;
+      if (want > 1 && blocks > 256. * 3 * R) break;         // the chip is full three times over: no further split shortens anything
+      const double b = (double)((long long)((blocks + 255) / 256)), full = (double)((long long)(b / R)), rem = b - full * R;
       const double row = full * (1 + q.more * (R - 1)) + (rem > 0 ? 1 + q.more * (rem - 1) : 0.);
       double us = per * q.step[kind] * row;
       us = sqrt(us * us + read * read);
