@@ -420,11 +420,13 @@ __device__ __forceinline__ void lds_sync() {
 // 24-27 the first: rows 0-3 and 12-15 of lane group 0, rows 4-11 of group 1.  This order of the rows (0-15) gives the halves disjoint banks.
 __device__ __forceinline__ int swz(int row) { return (row & 3) | ((row >> 2 & 1) * 2 ^ (row >> 3) * 3) << 2; }
 template <int MF, int NF, int PL>
-__global__ __launch_bounds__(256) void mx4_linear_kernel(const LinArgs a, int tn, int tm) {
+__global__ __launch_bounds__(256, NF < 4 ? 2 : 1) void mx4_linear_kernel(const LinArgs a, int tn, int tm) {
   constexpr int AHEAD = PL == 1 && NF < 4 ? 2 : 1;
   constexpr bool DMA = !(MF == 4 && NF == 2 && PL == 3);
   __shared__ u32x4 ws[DMA ? AHEAD : 1][4][DMA ? NF * 64 : 1];
-  __shared__ bf16x8 xs[PL][MF * 16][16];                    // one buffer: 48 KB at most, blocks beside it hide the barriers
+  constexpr int XB = PL == 1 ? 2 : 1;                       // planes of x: two buffers of bf16 (one barrier a step: 4096^3 143 -> 137 us), one of
+                                                            // fp32, 48 KB at most, where blocks beside it hide the barriers
+  __shared__ bf16x8 xs[XB][PL][MF * 16][16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
   const Place pl = place(tn, tm);
   const int n0 = pl.n * 64 * NF + wave * 16 * NF, m0 = pl.m * 16 * MF;
@@ -476,13 +478,14 @@ __global__ __launch_bounds__(256) void mx4_linear_kernel(const LinArgs a, int tn
       if constexpr (PL == 1) asm volatile("" ::"v"(xv[b][t].h) : "memory");
       else asm volatile("" ::"v"(xv[b][t].a), "v"(xv[b][t].b) : "memory");
     }
-    if (s > s0) lds_sync();                                 // every wave has read the last step's planes
+    if (XB == 1 && s > s0) lds_sync();                      // every wave has read the last step's planes
+    bf16x8(*xb)[MF * 16][16] = xs[XB == 2 ? (s - s0) & 1 : 0];
 #pragma unroll
     for (int t = 0; t < MF; ++t) {
       bf16x8 p[PL];
       split_raw<PL>(xv[b][t], p);
 #pragma unroll
-      for (int q = 0; q < PL; ++q) xs[q][xr + t * 16][(threadIdx.x & 15) ^ swz(xr)] = p[q];
+      for (int q = 0; q < PL; ++q) xb[q][xr + t * 16][(threadIdx.x & 15) ^ swz(xr)] = p[q];
     }
 #pragma unroll
     for (int n = 0; n < NF; ++n) {
@@ -498,7 +501,7 @@ __global__ __launch_bounds__(256) void mx4_linear_kernel(const LinArgs a, int tn
     bf16x8 xf[D + 1][MF], wf[NF];
     auto read = [&](int p) {
 #pragma unroll
-      for (int m = 0; m < MF; ++m) xf[p % (D + 1)][m] = xs[PL - 1 - p % PL][m * 16 + i][(g * 4 + p / PL) ^ swz(i)];
+      for (int m = 0; m < MF; ++m) xf[p % (D + 1)][m] = xb[PL - 1 - p % PL][m * 16 + i][(g * 4 + p / PL) ^ swz(i)];
     };
 #pragma unroll
     for (int p = 0; p < D; ++p) read(p);
@@ -1071,7 +1074,7 @@ struct LinPlan {
   int mf, nf, wk, tile, s16, tm, tn, splits, steps_per_split;
 };
 static LinPlan lin_plan(int M, int N, int K, int x_kind) {
-  static const Form lds[4] = {{1, 1, {8, 6}, {0.75, 0.5}, 0.35}, {2, 2, {4, 3}, {1.8, 1.2}, 0.35}, {4, 2, {3, 2}, {2.65, 1.5}, 0.35}, {4, 4, {2, 2}, {5.2, 2.5}, 0.}};
+  static const Form lds[4] = {{1, 1, {8, 6}, {0.75, 0.5}, 0.35}, {2, 2, {4, 3}, {1.8, 1.2}, 0.35}, {4, 2, {3, 3}, {2.65, 1.5}, 0.35}, {4, 4, {2, 2}, {5.2, 2.5}, 0.}};
   static const Form direct = {1, 1, {2, 2}, {0.6, 0.35}, 0.2}, tile = {1, 1, {1, 2}, {1.1, 0.4}, 0.2};      // (tile: by size, 256 or 128)
   LinPlan p;
   memset(&p, 0, sizeof(p));
