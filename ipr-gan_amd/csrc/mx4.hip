@@ -1027,13 +1027,13 @@ static int gemm4_go(const LinArgs& a, int tn, int tm, int splits, hipStream_t st
 
 // How the products are cut.  A form of a kernel is a tile and what a step along the reduction costs: `step` us for one block a CU (by x: fp32,
 // bf16), `more` of that for each further block beside it, of at most `resident`.  Every form is tried with every split of the reduction: the
-// steps in a row, overlapped with the weights, read once for each row of tiles, at 3.5 TB/s, plus a second launch and the slabs' traffic (8
+// steps in a row, overlapped with the weights, read once for each row of tiles, at 4 TB/s, plus a second launch and the slabs' traffic (8
 // bytes a partial result at 4 TB/s) where it is split.  Fitted to 60 sweeps over 1 to 48 splits, the choice is within 10 % of the fastest split nearly
 // everywhere.  (The largest form only where it fills the chip twice: one block of it alone on a CU waits for its own loads.)
 struct Form {
   int mf, nf;                    // 16-row fragments of x, fragments (kernels above) or words (gradient) of the weights
   int resident[2];
-  double step[2], more;
+  double step[2], more[2];
 };
 struct Cut {
   int form, tm, tn, splits, steps_per_split;
@@ -1046,15 +1046,15 @@ static Cut cut(const Form* forms, int count, int kind, int rows_f, int cols_f, i
   for (int f = 0; f < count; ++f) {
     const Form& q = forms[f];
     const int tm = cdiv(M, rows_f * q.mf), tn = cdiv(N, cols_f * q.nf), R = q.resident[kind];
-    const double read = weights * tm / 3.5e6;
+    const double read = weights * tm / 4e6;
     if (q.mf > 1 && rows_f * q.mf >= 2 * M) continue;       // half the tile's rows or more would be empty
-    if (q.mf * q.nf == 16 && (long long)tm * tn < 512) continue;
     for (int want = 1; want <= 64 && want <= steps; want = want < 8 ? want + 1 : want + want / 4) {
       const int per = rup(cdiv(steps, want), unit), splits = cdiv(steps, per);
       const double blocks = (double)tm * tn * splits;
+      if (q.mf * q.nf == 16 && blocks < 512.) continue;
       if (want > 1 && blocks > 256. * 3 * R) break;         // the chip is full three times over: no further split shortens anything
       const double b = (double)((long long)((blocks + 255) / 256)), full = (double)((long long)(b / R)), rem = b - full * R;
-      const double row = full * (1 + q.more * (R - 1)) + (rem > 0 ? 1 + q.more * (rem - 1) : 0.);
+      const double row = full * (1 + q.more[kind] * (R - 1)) + (rem > 0 ? 1 + q.more[kind] * (rem - 1) : 0.);
       double us = per * q.step[kind] * row;
       us = sqrt(us * us + read * read);
       if (splits > 1) us += 5. + splits * (double)M * N * 2e-6;
@@ -1066,7 +1066,7 @@ static Cut cut(const Form* forms, int count, int kind, int rows_f, int cols_f, i
 
 //   LDS    : 16 * mf rows x 64 * nf columns a block.  Four fragments a wave halve the LDS reads a multiplication (4096^3 fp32: 450 -> 400 us)
 //   direct : 16 * mf rows x 16 * nf * (8 / wk) columns a block, wk waves along K.  For 4-bit x of up to 64 rows; else for up to 16, where the LDS form
-//            would be split or leaves half the chip idle, K <= 4096 and not too many columns.  Against LDS, wall time: 1 x 4096 x 4096 fp32 13.5 : 19.5
+//            would be split or leaves half the chip idle and the estimate is 2 us lower, K <= 4096 and not too many columns.  Against LDS, wall time: 1 x 4096 x 4096 fp32 13.5 : 19.5
 //            us (one launch instead of two), 8 x 4096 x 16384 bf16 16.3 : 19.0, but fp32 25.3 : 20.4 (every wave splits x again), 16 x 18432 x
 //            1024 bf16 26.9 : 18.4 (18 steps in a row) and 4 x 65536 x 1024 bf16 21.2 : 13.7 (device; 1024 blocks of the LDS form).
 //   tile   : 4-bit x of more rows: square tiles, 256 where they fill three quarters of the chip, else 128
@@ -1074,29 +1074,35 @@ struct LinPlan {
   int mf, nf, wk, tile, s16, tm, tn, splits, steps_per_split;
 };
 static LinPlan lin_plan(int M, int N, int K, int x_kind) {
-  static const Form lds[4] = {{1, 1, {8, 6}, {0.75, 0.5}, 0.35}, {2, 2, {4, 3}, {1.8, 1.2}, 0.35}, {4, 2, {3, 3}, {2.65, 1.5}, 0.35}, {4, 4, {2, 2}, {5.2, 2.5}, 0.}};
-  static const Form direct = {1, 1, {2, 2}, {0.6, 0.35}, 0.2}, tile = {1, 1, {1, 2}, {1.1, 0.4}, 0.2};      // (tile: by size, 256 or 128)
+  static const Form lds[4] = {{1, 1, {8, 8}, {0.46, 0.28}, {0.65, 0.4}}, {2, 2, {4, 4}, {1.1, 0.5}, {0.65, 0.6}}, {4, 2, {3, 3}, {2.1, 0.75}, {0.45, 0.55}}, {4, 4, {2, 2}, {3.6, 1.5}, {0.35, 0.3}}};
+  static const Form direct = {1, 1, {2, 2}, {0.6, 0.35}, {0.2, 0.2}}, tile = {1, 1, {1, 2}, {1.1, 0.4}, {0., 0.2}};      // (tile: by size, 256 or 128)
   LinPlan p;
   memset(&p, 0, sizeof(p));
   const int steps = kb_of(K) / 4, kind = x_kind != IPRGAN_X_F32;
   const double weights = (double)N * K * 0.53;
-  Cut c;
+  Cut c, d;
   bool dir = x_kind == IPRGAN_X_MX4 && M <= 64;
-  if (x_kind != IPRGAN_X_MX4) {
-    c = cut(lds, 4, kind, 16, 64, M, N, steps, 1, weights);
-    p.mf = lds[c.form].mf;
-    p.nf = lds[c.form].nf;
-    dir = M <= 16 && (c.splits > 1 || c.tn < 128) && steps <= 32 && (long long)steps * N <= (kind ? 600000 : 200000);
-  }
-  if (dir) {
-    p.mf = M <= 16 ? 1 : M <= 32 ? 2 : 4;
+  if (M <= 64) {
     p.wk = 1;
     while (p.wk < 8 && p.wk * 2 <= steps) p.wk *= 2;
+    p.mf = M <= 16 ? 1 : M <= 32 ? 2 : 4;
     p.nf = N >= 256 * 32 * (8 / p.wk) ? 2 : 1;              // two fragments a wave once that leaves a block for every CU
     Form f = direct;
     f.step[kind] /= p.wk;
-    c = cut(&f, 1, kind, 16 * p.mf, 16 * p.nf * (8 / p.wk), M, N, steps, p.wk, weights);
-  } else if (x_kind == IPRGAN_X_MX4) {
+    d = cut(&f, 1, kind, 16 * p.mf, 16 * p.nf * (8 / p.wk), M, N, steps, p.wk, weights);
+  }
+  if (x_kind != IPRGAN_X_MX4) {
+    c = cut(lds, 4, kind, 16, 64, M, N, steps, 1, weights);
+    dir = M <= 16 && (c.splits > 1 || c.tn < 128) && d.us + 2. < c.us && steps <= 32 && (long long)steps * N <= (kind ? 600000 : 200000);
+  }
+  if (dir) {
+    c = d;
+  } else if (x_kind != IPRGAN_X_MX4) {
+    p.wk = 0;
+    p.mf = lds[c.form].mf;
+    p.nf = lds[c.form].nf;
+  } else {
+    p.wk = 0;
     p.tile = (long long)cdiv(M, 256) * cdiv(N, 256) >= 192 ? 256 : 128;
     p.s16 = steps % 4 == 0;                                 // the form that moves the scales of four stages at once
     c = cut(&tile, 1, p.tile == 128, p.tile, p.tile, M, N, steps, p.s16 ? 4 : 2, weights);
@@ -1114,9 +1120,9 @@ struct BwdPlan {
   int form, tm, tk, splits, steps_per_split;
 };
 static BwdPlan bwd_plan(int M, int N, int K, int dy_bf16) {
-  static const Form f32[3] = {{1, 1, {4, 4}, {0.82, 0.82}, 0.75}, {1, 2, {2, 2}, {1.03, 1.03}, 0.85}, {2, 2, {2, 2}, {1.75, 1.75}, 0.5}};
-  static const Form b16[3] = {{1, 1, {4, 4}, {0.68, 0.68}, 0.75}, {1, 2, {3, 3}, {0.72, 0.72}, 0.85}, {4, 1, {2, 2}, {1.08, 1.08}, 0.33}};
-  const Cut c = cut(dy_bf16 ? b16 : f32, 3, 0, 16, 128, M, K, cdiv(cdiv(N, 32), 4), 1, (double)N * K * 0.53);
+  static const Form f32[3] = {{1, 1, {4, 4}, {0.82, 0.82}, {0.75, 0.75}}, {1, 2, {2, 2}, {1.03, 1.03}, {0.85, 0.85}}, {2, 2, {2, 2}, {1.75, 1.75}, {0.5, 0.5}}};
+  static const Form b16[3] = {{1, 1, {4, 4}, {0.68, 0.72}, {0.75, 0.75}}, {1, 2, {3, 3}, {0.72, 0.8}, {0.85, 0.85}}, {4, 1, {2, 2}, {1.08, 1.75}, {0.33, 0.33}}};
+  const Cut c = cut(dy_bf16 ? b16 : f32, 3, dy_bf16 ? N & 1 : 0, 16, 128, M, K, cdiv(cdiv(N, 32), 4), 1, (double)N * K * 0.53);      // (bf16: rows of even, odd length)
   return BwdPlan{c.form, c.tm, c.tn, c.splits, c.steps_per_split};
 }
 
