@@ -1027,9 +1027,10 @@ static int gemm4_go(const LinArgs& a, int tn, int tm, int splits, hipStream_t st
 
 // How the products are cut.  A form of a kernel is a tile and what a step along the reduction costs: `step` us for one block a CU (by x: fp32,
 // bf16), `more` of that for each further block beside it, of at most `resident`.  Every form is tried with every split of the reduction: the
-// steps in a row, overlapped with the weights, read once for each row of tiles, at 4 TB/s, plus a second launch and the slabs' traffic (8
-// bytes a partial result at 4 TB/s) where it is split.  Fitted to 60 sweeps over 1 to 48 splits, the choice is within 10 % of the fastest split nearly
-// everywhere.  (The largest form only where it fills the chip twice: one block of it alone on a CU waits for its own loads.)
+// steps in a row, overlapped with the weights at 4 TB/s, read `again` times for each further row of tiles, plus a second launch and the slabs' traffic (8
+// bytes a partial result at 4 TB/s) where it is split.  Fitted to sweeps of 140 sizes over all forms and 1 to 48 splits: within 10 % of the fastest
+// in nine of ten, at worst 25 % (few blocks on an idle chip step faster than the estimate knows).  The largest form only where it fills the
+// chip twice: one block of it alone on a CU waits for its own loads.
 struct Form {
   int mf, nf;                    // 16-row fragments of x, fragments (kernels above) or words (gradient) of the weights
   int resident[2];
@@ -1039,14 +1040,14 @@ struct Cut {
   int form, tm, tn, splits, steps_per_split;
   double us;
 };
-static Cut cut(const Form* forms, int count, int kind, int rows_f, int cols_f, int M, int N, int steps, int unit, double weights) {
+static Cut cut(const Form* forms, int count, int kind, int rows_f, int cols_f, int M, int N, int steps, int unit, double weights, double again) {
   Cut best;
   memset(&best, 0, sizeof(best));
   best.us = 1e30;
   for (int f = 0; f < count; ++f) {
     const Form& q = forms[f];
     const int tm = cdiv(M, rows_f * q.mf), tn = cdiv(N, cols_f * q.nf), R = q.resident[kind];
-    const double read = weights * tm / 4e6;
+    const double read = weights * (1 + again * (tm - 1)) / 4e6;
     if (q.mf > 1 && rows_f * q.mf >= 2 * M) continue;       // half the tile's rows or more would be empty
     for (int want = 1; want <= 64 && want <= steps; want = want < 8 ? want + 1 : want + want / 4) {
       const int per = rup(cdiv(steps, want), unit), splits = cdiv(steps, per);
@@ -1066,9 +1067,10 @@ static Cut cut(const Form* forms, int count, int kind, int rows_f, int cols_f, i
 
 //   LDS    : 16 * mf rows x 64 * nf columns a block.  Four fragments a wave halve the LDS reads a multiplication (4096^3 fp32: 450 -> 400 us)
 //   direct : 16 * mf rows x 16 * nf * (8 / wk) columns a block, wk waves along K.  For 4-bit x of up to 64 rows; else for up to 16, where the LDS form
-//            would be split or leaves half the chip idle and the estimate is 2 us lower, K <= 4096 and not too many columns.  Against LDS, wall time: 1 x 4096 x 4096 fp32 13.5 : 19.5
-//            us (one launch instead of two), 8 x 4096 x 16384 bf16 16.3 : 19.0, but fp32 25.3 : 20.4 (every wave splits x again), 16 x 18432 x
-//            1024 bf16 26.9 : 18.4 (18 steps in a row) and 4 x 65536 x 1024 bf16 21.2 : 13.7 (device; 1024 blocks of the LDS form).
+//            would be split or leaves half the chip idle and the estimate is 2 us lower (4 x 2000 x 300 fp32: 8.8 : 6.2 us for LDS), K <= 4096 and
+//            not too many columns.  Against LDS, wall time: 1 x 4096 x 4096 fp32 13.5 : 19.5 us (one launch instead of two), 8 x 4096 x
+//            16384 bf16 16.3 : 19.0, but fp32 25.3 : 20.4 (every wave splits x again), 16 x 18432 x 1024 bf16 26.9 : 18.4 (18 steps in a row)
+//            and 4 x 65536 x 1024 bf16 21.2 : 13.7 (device; 1024 blocks of the LDS form).
 //   tile   : 4-bit x of more rows: square tiles, 256 where they fill three quarters of the chip, else 128
 struct LinPlan {
   int mf, nf, wk, tile, s16, tm, tn, splits, steps_per_split;
@@ -1089,10 +1091,10 @@ static LinPlan lin_plan(int M, int N, int K, int x_kind) {
     p.nf = N >= 256 * 32 * (8 / p.wk) ? 2 : 1;              // two fragments a wave once that leaves a block for every CU
     Form f = direct;
     f.step[kind] /= p.wk;
-    d = cut(&f, 1, kind, 16 * p.mf, 16 * p.nf * (8 / p.wk), M, N, steps, p.wk, weights);
+    d = cut(&f, 1, kind, 16 * p.mf, 16 * p.nf * (8 / p.wk), M, N, steps, p.wk, weights, 1.);
   }
   if (x_kind != IPRGAN_X_MX4) {
-    c = cut(lds, 4, kind, 16, 64, M, N, steps, 1, weights);
+    c = cut(lds, 4, kind, 16, 64, M, N, steps, 1, weights, 1.);
     dir = M <= 16 && (c.splits > 1 || c.tn < 128) && d.us + 2. < c.us && steps <= 32 && (long long)steps * N <= (kind ? 600000 : 200000);
   }
   if (dir) {
@@ -1105,7 +1107,7 @@ static LinPlan lin_plan(int M, int N, int K, int x_kind) {
     p.wk = 0;
     p.tile = (long long)cdiv(M, 256) * cdiv(N, 256) >= 192 ? 256 : 128;
     p.s16 = steps % 4 == 0;                                 // the form that moves the scales of four stages at once
-    c = cut(&tile, 1, p.tile == 128, p.tile, p.tile, M, N, steps, p.s16 ? 4 : 2, weights);
+    c = cut(&tile, 1, p.tile == 128, p.tile, p.tile, M, N, steps, p.s16 ? 4 : 2, weights, 1.);
   }
   p.tm = c.tm;
   p.tn = c.tn;
@@ -1122,7 +1124,7 @@ struct BwdPlan {
 static BwdPlan bwd_plan(int M, int N, int K, int dy_bf16) {
   static const Form f32[3] = {{1, 1, {4, 4}, {0.82, 0.82}, {0.75, 0.75}}, {1, 2, {2, 2}, {1.03, 1.03}, {0.85, 0.85}}, {2, 2, {2, 2}, {1.75, 1.75}, {0.5, 0.5}}};
   static const Form b16[3] = {{1, 1, {4, 4}, {0.68, 0.72}, {0.75, 0.75}}, {1, 2, {3, 3}, {0.72, 0.8}, {0.85, 0.85}}, {4, 1, {2, 2}, {1.08, 1.75}, {0.33, 0.33}}};
-  const Cut c = cut(dy_bf16 ? b16 : f32, 3, dy_bf16 ? N & 1 : 0, 16, 128, M, K, cdiv(cdiv(N, 32), 4), 1, (double)N * K * 0.53);      // (bf16: rows of even, odd length)
+  const Cut c = cut(dy_bf16 ? b16 : f32, 3, dy_bf16 ? N & 1 : 0, 16, 128, M, K, cdiv(cdiv(N, 32), 4), 1, (double)N * K * 0.53, 0.4);      // (bf16: rows of even, odd length)
   return BwdPlan{c.form, c.tm, c.tn, c.splits, c.steps_per_split};
 }
 
