@@ -20,10 +20,6 @@ typedef __bf16 nbf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 nbf16x8 __attribute__((ext_vector_type(8)));
 
 // ---- V consecutive elements (V = 4 or 8) of a tensor of storage kind ST (IPRGAN_ST_*): 16-byte accesses per plane where possible
-template <int ST, int V>
-struct Vec {
-  float v[V];
-};
 template <int V>
 __device__ __forceinline__ void ldbf(const __bf16* b, float* v) {
   if constexpr (V == 8) {
@@ -147,7 +143,8 @@ __device__ __forceinline__ void ldcodes(const int8_t* q, size_t e, float* v) {  
 }
 
 // Quantise: a thread owns V consecutive elements, 32 / V neighbouring lanes share a block and its maximum.  n is the element count;
-// lanes past the end contribute zeros.  Bound by HBM (reads sizeof(x), writes 1 + 1/32 bytes an element).
+// lanes past the end contribute zeros.  Bound by HBM (reads sizeof(x), writes 1 + 1/32 bytes an element): 256x128x128x64 bf16 156 us = 5.2
+// TB/s, the rate of a copy; two or four pieces in flight a thread are slower (173, 179 us).
 template <int ST, int V>
 __global__ __launch_bounds__(256) void mx8_quant_kernel(const void* __restrict__ x, int8_t* __restrict__ q,
                                                         uint8_t* __restrict__ scales, size_t n, size_t ps) {
@@ -195,6 +192,7 @@ __global__ __launch_bounds__(256) void mx8_quant_kernel(const void* __restrict__
   }
 }
 
+// Restore: the same bytes the other way, 151 us at the same size (5.4 TB/s).  Small tensors are bound by the launch (27 540 elements: 2.4 us).
 template <int ST, int V>
 __global__ __launch_bounds__(256) void mx8_dequant_kernel(const int8_t* __restrict__ q, const uint8_t* __restrict__ scales,
                                                           void* __restrict__ y, size_t n, size_t ps) {
@@ -214,7 +212,7 @@ __global__ __launch_bounds__(256) void mx8_dequant_kernel(const int8_t* __restri
   }
 }
 
-// dz = dy * act'(out), out read from its checkpoint
+// dz = dy * act'(out), out read from its checkpoint: one pass, HBM (sizeof(dy) twice and 1 + 1/32 bytes an element)
 template <int ST, int V>
 __global__ __launch_bounds__(256) void mx8_act_bwd_kernel(const void* __restrict__ dy, const int8_t* __restrict__ q,
                                                           const uint8_t* __restrict__ scales, void* __restrict__ dz, size_t n,
@@ -248,6 +246,8 @@ __global__ __launch_bounds__(256) void mx8_act_bwd_kernel(const void* __restrict
 // Rows go to the blocks in chunks of 4 * TR, chunk by chunk round the grid: all blocks together sweep the tensor.  (One contiguous
 // run of rows a block puts the blocks a power of two apart and on the same memory channels: 208 us instead of 89 for the reduction
 // over 256x64x64x128 bf16.)
+// Bound by HBM: the statistics need all of dy and the codes before the first dx, so both are read twice - 16.3 + 23.9 us for 128x32x32x128 fp32
+// (5.2 and 6.3 TB/s: the second pass walks backwards and finds part of them cached), 90 + 110 us for 256x64x64x128 bf16.
 struct NormGeom {
   int TC, TR, gy, NB;
 };
@@ -295,7 +295,7 @@ struct NormArgs {
   const float *gamma, *beta, *mean, *invstd, *slope_ptr;
   float *part, *sums, *dgamma, *dbeta, *dslope, *colpart;
   size_t dyps, dxps;
-  int G, M, C, TC, TR, act, nsum;          // nsum: partial sums a channel (2, or 3 with a slope gradient)
+  int G, M, C, TC, TR, nsum;          // nsum: partial sums a channel (2, or 3 with a slope gradient)
   int RL;                                  // row lanes of the sums in the apply pass; 0: they are in `sums`
   float slope;
 };
@@ -714,7 +714,7 @@ int iprgan_mx8_norm_bwd(const void* codes, const void* scales, const void* dy, c
   a.q = (const int8_t*)codes; a.scales = (const uint8_t*)scales; a.dy = dy; a.dx = dx;
   a.gamma = gamma; a.beta = beta; a.mean = save_mean; a.invstd = save_invstd; a.slope_ptr = slope_dev;
   a.dgamma = dgamma; a.dbeta = dbeta; a.dslope = dslope; a.dyps = dy_pstride; a.dxps = dx_pstride;
-  a.G = G; a.M = M; a.C = C; a.TC = g.TC; a.TR = g.TR; a.act = act; a.slope = act == IPRGAN_ACT_RELU ? 0.f : slope;
+  a.G = G; a.M = M; a.C = C; a.TC = g.TC; a.TR = g.TR; a.slope = act == IPRGAN_ACT_RELU ? 0.f : slope;
   a.nsum = dslope ? 3 : 2;
   const int quads = g.TC * (wide ? 8 : 4) / 2, lanes = 256 / quads < 16 ? 256 / quads : 16;
   a.RL = (long long)G * g.NB <= 24 * lanes ? lanes : 0;
