@@ -422,7 +422,7 @@ __device__ __forceinline__ void lds_sync() {
 __device__ __forceinline__ int swz(int row) { return (row & 3) | ((row >> 2 & 1) * 2 ^ (row >> 3) * 3) << 2; }
 template <int MF, int NF, int PL>
 __global__ __launch_bounds__(256, NF < 4 ? 2 : 1) void mx4_linear_kernel(const LinArgs a, int tn, int tm) {
-  constexpr int AHEAD = PL == 1 && NF < 4 ? 2 : 1;
+  constexpr int AHEAD = (PL == 1 ? NF < 4 : MF <= 2) ? 2 : 1;      // (three: 1 to 15 % slower; two elsewhere: no gain)
   constexpr bool DMA = !(MF == 4 && NF == 2 && PL == 3);
   __shared__ u32x4 ws[DMA ? AHEAD : 1][4][DMA ? NF * 64 : 1];
   constexpr int XB = PL == 1 ? 2 : 1;                       // planes of x: two buffers of bf16 (one barrier a step: 4096^3 143 -> 137 us), one of
