@@ -492,7 +492,7 @@ int iprgan_mx8_quant(const void* x, void* codes, void* scales, size_t n, int kin
 int iprgan_mx8_dequant(const void* codes, const void* scales, void* y, size_t n, int kind, size_t pstride, void* stream);
 /* dz = dy * act'(out), out read from its checkpoint (iprgan_act_bwd; dy and dz fp32 or bf16) */
 int iprgan_mx8_act_bwd(const void* dy, const void* codes, const void* scales, void* dz, size_t n, int act, float slope, int kind,
-                       size_t dy_pstride, size_t dz_pstride, void* stream);
+                       void* stream);
 /* Norm backward with the layer's INPUT read from its checkpoint: iprgan_bn_bwd (G = 1), iprgan_instnorm_bwd (G = batch, M = HW;
  * mean / invstd [G][C]), iprgan_bn_prelu_bwd (slope_dev: the PReLU slope on the device, dslope its gradient; act LRELU).  Activation none,
  * ReLU or LeakyReLU: the mask gamma * (x - mean) * invstd + beta > 0 is one comparison of x with a threshold formed in 64 bits.

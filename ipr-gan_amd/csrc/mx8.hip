@@ -216,20 +216,20 @@ __global__ __launch_bounds__(256) void mx8_dequant_kernel(const int8_t* __restri
 template <int ST, int V>
 __global__ __launch_bounds__(256) void mx8_act_bwd_kernel(const void* __restrict__ dy, const int8_t* __restrict__ q,
                                                           const uint8_t* __restrict__ scales, void* __restrict__ dz, size_t n,
-                                                          size_t dps, size_t zps, int act, float slope) {
+                                                          int act, float slope) {
   const size_t stride = (size_t)gridDim.x * 256 * V;
   for (size_t e = ((size_t)blockIdx.x * 256 + threadIdx.x) * V; e < n; e += stride) {
     const float step = mx8_step(scales[e >> 5]);
     if (e + V <= n) {
       float v[V], g[V];
       ldcodes<V>(q, e, v);
-      ldv<ST, V>(dy, e, dps, g);
+      ldv<ST, V>(dy, e, 0, g);
 #pragma unroll
       for (int k = 0; k < V; ++k) g[k] *= act_grad_from_out(v[k] * step, act, slope);
-      stv<ST, V>(dz, e, zps, g);
+      stv<ST, V>(dz, e, 0, g);
     } else {
       for (int k = 0; k < V; ++k)
-        if (e + k < n) st1<ST>(dz, e + k, zps, ld1<ST>(dy, e + k, dps) * act_grad_from_out((float)q[e + k] * step, act, slope));
+        if (e + k < n) st1<ST>(dz, e + k, 0, ld1<ST>(dy, e + k, 0) * act_grad_from_out((float)q[e + k] * step, act, slope));
     }
   }
 }
@@ -658,16 +658,17 @@ int iprgan_mx8_dequant(const void* codes, const void* scales, void* y, size_t n,
 }
 
 int iprgan_mx8_act_bwd(const void* dy, const void* codes, const void* scales, void* dz, size_t n, int act, float slope, int kind,
-                       size_t dy_pstride, size_t dz_pstride, void* stream) {
+                       void* stream) {
   IPR_CHECK(n > 0, "mx8_act_bwd: empty input");
   IPR_CHECK(dy && dz && codes && scales, "mx8_act_bwd: null operand");
   IPR_CHECK(kind == IPRGAN_ST_F32 || kind == IPRGAN_ST_BF16, "mx8_act_bwd: storage kind %d (fp32 or bf16)", kind);
+  IPR_CHECK(act >= IPRGAN_ACT_NONE && act <= IPRGAN_ACT_SIGMOID_PM1, "mx8_act_bwd: activation %d", act);
   IPR_CHECK((kind == IPRGAN_ST_F32 ? al16(dy) && al16(dz) : al8(dy) && al8(dz)) && al16(codes),
             "mx8_act_bwd: operands must be 16-byte aligned (8: bf16)");
   const bool wide = kind == IPRGAN_ST_BF16 && al16(dy) && al16(dz);
   auto k = kind == IPRGAN_ST_F32 ? mx8_act_bwd_kernel<0, 4> : wide ? mx8_act_bwd_kernel<1, 8> : mx8_act_bwd_kernel<1, 4>;
   hipLaunchKernelGGL(k, dim3(flat_grid(n, wide ? 8 : 4)), dim3(256), 0, (hipStream_t)stream, dy, (const int8_t*)codes,
-                     (const uint8_t*)scales, dz, n, dy_pstride, dz_pstride, act, slope);
+                     (const uint8_t*)scales, dz, n, act, slope);
   IPR_LAUNCH_CHECK();
   return 0;
 }

@@ -136,7 +136,7 @@ SIGNATURES = {
     'iprgan_prof_get_layer': (_I, [_I, C.c_char_p, _I, C.POINTER(C.c_longlong), C.POINTER(C.c_double), C.POINTER(C.c_double)]),
     'iprgan_mx8_quant': (_I, [_P, _P, _P, _Z, _I, _Z, _P]),
     'iprgan_mx8_dequant': (_I, [_P, _P, _P, _Z, _I, _Z, _P]),
-    'iprgan_mx8_act_bwd': (_I, [_P, _P, _P, _P, _Z, _I, _F, _I, _Z, _Z, _P]),
+    'iprgan_mx8_act_bwd': (_I, [_P, _P, _P, _P, _Z, _I, _F, _I, _P]),
     'iprgan_mx8_norm_bwd_ws_floats': (_Z, [_I, _I, _I]),
     'iprgan_mx8_norm_bwd': (_I, [_P] * 13 + [_I, _I, _I, _I, _F, _P, _I, _F, _I, _Z, _I, _Z, _P]),
     'iprgan_mx4_pitch': (_I, [_I]),

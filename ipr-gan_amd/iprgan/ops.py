@@ -558,7 +558,7 @@ def act_bwd(dy, out, act, slope=0.0):
         keep = []
         pdy, dz = _vptr(dy, keep), _new(dy.shape, dy, dy.dtype)
         c, s = out.ptrs()
-        call('iprgan_mx8_act_bwd', pdy, c, s, ptr(dz), dy.numel(), act, float(slope), is16(dy), 0, 0, stream())
+        call('iprgan_mx8_act_bwd', pdy, c, s, ptr(dz), dy.numel(), act, float(slope), is16(dy), stream())
         return dz
     if ST_X3 in (is16(dy), is16(out)):          # (no three-plane form: a stand-alone activation backward is rare)
         dy, out = f32(dy), f32(out)

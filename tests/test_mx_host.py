@@ -25,8 +25,9 @@ def test_mx8_entries_refuse_bad_calls():
     refused('iprgan_mx8_dequant', P, P, P, 0, 0, 0, None)
     refused('iprgan_mx8_dequant', P, P, ODD, 8, 0, 0, None)
     refused('iprgan_mx8_dequant', P, P, P, 8, 2, 6, None)
-    refused('iprgan_mx8_act_bwd', P, P, P, P, 8, 1, 0.0, 2, 0, 0, None)
-    refused('iprgan_mx8_act_bwd', P, P, P, P, 0, 1, 0.0, 0, 0, 0, None)
+    refused('iprgan_mx8_act_bwd', P, P, P, P, 8, 1, 0.0, 2, None)
+    refused('iprgan_mx8_act_bwd', P, P, P, P, 0, 1, 0.0, 0, None)
+    refused('iprgan_mx8_act_bwd', P, P, P, P, 8, 99, 0.0, 0, None)
 
 
 def norm(codes=P, dy=P, gamma=P, beta=P, slope=None, dx=P, dgamma=P, dbeta=P, dslope=None, ws=P, G=1, M=8, C_=8, act=1, dbias=None, nb=0,
