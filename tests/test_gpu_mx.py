@@ -512,3 +512,111 @@ def test_operators_under_capture_and_on_another_stream(dev):
         torch.cuda.current_stream().wait_stream(side)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(other, eager))
+
+
+# ---- offsets past 32 bits (about 25 GB at a time; all but the ends of each tensor is zero) ------------------------------------------
+def test_checkpoint_past_32_bits(dev):
+    """2^32 + 4 113 elements: the end of the tensor is quantised and restored as it is by itself; a restore in fp32 passes 2^34 bytes."""
+    from iprgan import ops
+    n, k = (1 << 32) + 4113, 4096 + 17
+    end = awkward(k, 5).bfloat16().to(dev)
+    x = torch.zeros(n, dtype=torch.bfloat16, device=dev)
+    x[-k:] = end
+    q, own = ops.mx8_quant(x), ops.mx8_quant(end)
+    assert torch.equal(q.codes[-k:], own.codes) and torch.equal(q.scales[(n - k) // 32:], own.scales)
+    assert int(q.codes[:n - k].count_nonzero()) == 0
+    del x
+    for kind in (ops.ST_BF16, ops.ST_F32):
+        y = ops.mx8_dequant(q, kind)
+        assert same(y[-k:], ops.mx8_dequant(own, kind))
+        assert int(y[:n - k].count_nonzero()) == 0
+        del y
+    dy = torch.zeros(n, dtype=torch.bfloat16, device=dev)
+    dy[-k:] = rnd(k, seed=6).bfloat16()
+    dz = ops.act_bwd(dy, q, 2, 0.25)
+    assert same(dz[-k:], ops.act_bwd(dy[-k:].clone(), own, 2, 0.25))
+
+
+def test_norm_backward_past_32_bits(dev):
+    """2^26 + 5 rows of 64 channels; only the first and the last 1000 rows have gradients.  Sums: 2000 additions that are not of a zero, each off by
+    at most half a step of the sum of the magnitudes, and 8 roundings a term; dx: 8 fp32 roundings of its terms and one to bf16."""
+    from iprgan import ops
+    M, C, k = (1 << 26) + 5, 64, 1000
+    x = torch.zeros(M, C, dtype=torch.bfloat16, device=dev)
+    dy = torch.zeros(M, C, dtype=torch.bfloat16, device=dev)
+    for s, rows in ((1, slice(0, k)), (2, slice(M - k, M))):
+        x[rows] = rnd(k, C, seed=s).bfloat16().to(dev)
+        dy[rows] = rnd(k, C, seed=s + 10).bfloat16().to(dev)
+    mean, invstd = 0.1 * rnd(C, seed=3), 1 + 0.1 * rnd(C, seed=4).abs()
+    gamma, beta = rnd(C, seed=5), rnd(C, seed=6)
+    ends = [ops.mx8_dequant(ops.mx8_quant(t.clone())).double().cpu() for t in (x[:k], x[M - k:])]
+    q = ops.mx8_quant(x)
+    g = torch.cat([dy[:k], dy[M - k:]]).double().cpu()
+    del x
+    dx, dgamma, dbeta = ops.bn_bwd(q, None, dy, gamma.to(dev), mean.to(dev), invstd.to(dev), 1, beta=beta.to(dev))
+    t = (torch.cat(ends) - mean.double()) * invstd.double()
+    dz = torch.where(t * gamma.double() + beta.double() > 0, g, 0.0)
+    u = 2.0 ** -24
+    for got, terms in ((dbeta, dz), (dgamma, dz * t)):
+        mag = terms.abs().sum(0) + (dz.abs() * (mean * invstd).abs().double()).sum(0)
+        assert bool(((got.cpu().double() - terms.sum(0)).abs() <= 2008 * u * mag).all())
+    gi = gamma.double() * invstd.double()
+    s1, s2 = dbeta.cpu().double() / M, dgamma.cpu().double() / M
+    want = gi * (dz - s1 - t * s2)
+    bound = want.abs() * 2.0 ** -8 + 16 * u * gi.abs() * (dz.abs() + s1.abs() + (t.abs() + (mean * invstd).abs().double()) * s2.abs())
+    got = torch.cat([dx[:k], dx[M - k:]]).cpu().double()
+    assert bool(((got - want).abs() <= bound).all())
+
+
+def test_weights_past_32_bits(dev):
+    """65 600 x 65 536 weights (2.15 GB of codes), whole numbers small enough that every product and sum is exact."""
+    from iprgan import ops
+    N, K, k = 65600, 65536, 5
+    gen = torch.Generator().manual_seed(3)
+    end = torch.tensor([0., 1, 2, 3, 4, 6, -1, -2, -6])[torch.randint(0, 9, (k, K), generator=gen)]
+    end[:, ::32] = 6.                                            # (block maximum 6: scale 1, values are codes)
+    x = torch.zeros(N, K, dtype=torch.bfloat16, device=dev)
+    x[-k:] = end.to(dev)
+    w = ops.mx4_quant(x)
+    del x
+    back = ops.mx4_dequant(w, torch.bfloat16)
+    assert torch.equal(back[-k:].float().cpu(), end) and int(back[:N - k].count_nonzero()) == 0
+    del back
+    for M in (2, 70):
+        xs = torch.randint(-2, 3, (M, K), generator=gen).float()
+        xs[:, ::32] = 0.
+        want = xs.double() @ end.double().t()
+        assert float((xs.abs().double() @ end.abs().double().t()).max()) < 2 ** 24
+        for a in (xs.to(dev), xs.bfloat16().to(dev), ops.mx4_quant(xs.to(dev))):
+            y = ops.mx4_linear(a, w, dtype=torch.float32)
+            assert torch.equal(y[:, -k:].double().cpu(), want) and int(y[:, :N - k].count_nonzero()) == 0
+        dy = torch.zeros(M, N)
+        dy[:, -k:] = torch.randint(-8, 9, (M, k), generator=gen).float()
+        for d in (dy.to(dev), dy.bfloat16().to(dev)):
+            assert torch.equal(ops.mx4_linear_bwd(d, w, torch.float32).double().cpu(), dy[:, -k:].double() @ end.double())
+
+
+def test_results_past_32_bits(dev):
+    """40 000 x 65 600 results (2.6e9) of short whole-number sums, the product's and the gradient's."""
+    from iprgan import ops
+    M, N, K = 40000, 65600, 96
+    gen = torch.Generator().manual_seed(4)
+    x = torch.randint(-2, 3, (M, K), generator=gen).float().to(dev)
+    wt = torch.randint(-2, 3, (N, K), generator=gen).float()
+    wt[:, ::32] = 6.
+    w = ops.mx4_quant(wt.to(dev))
+    rows = torch.tensor([0, 16384, 32735, 32736, M - 1])         # (row 32 736 passes 2^31 elements)
+    xq = x.clone()
+    xq[:, ::32] = 6.
+    for a, src in ((x, x), (x.bfloat16(), x), (ops.mx4_quant(xq), xq)):
+        y = ops.mx4_linear(a, w, dtype=torch.bfloat16)
+        want = (src.cpu()[rows].double() @ wt.double().t()).bfloat16()
+        assert torch.equal(y[rows.to(dev)].cpu(), want)
+        del y
+    wb = torch.randint(-2, 3, (K, N), generator=gen).float()
+    wb[:, ::32] = 6.
+    w = ops.mx4_quant(wb.to(dev))
+    for d in (x, x.bfloat16()):
+        dx = ops.mx4_linear_bwd(d, w, torch.bfloat16)
+        assert torch.equal(dx[rows.to(dev)].cpu(), (x.cpu()[rows].double() @ wb.double()).bfloat16())
+        del dx
