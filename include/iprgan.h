@@ -34,7 +34,7 @@
 extern "C" {
 #endif
 
-#define IPRGAN_VERSION 227
+#define IPRGAN_VERSION 228
 
 enum { IPRGAN_ACT_NONE = 0, IPRGAN_ACT_RELU = 1, IPRGAN_ACT_LRELU = 2, IPRGAN_ACT_TANH = 3,
        IPRGAN_ACT_SIGMOID_PM1 = 4 };   /* sigmoid(x)*2-1: nn.Sigmoid + Decoder32.Normalize (networks/decoder.py:14-16,31-32) */
@@ -497,12 +497,14 @@ int iprgan_mx8_act_bwd(const void* dy, const void* codes, const void* scales, vo
  * mean / invstd [G][C]), iprgan_bn_prelu_bwd (slope_dev: the PReLU slope on the device, dslope its gradient; act LRELU).  Activation none,
  * ReLU or LeakyReLU: the mask gamma * (x - mean) * invstd + beta > 0 is one comparison of x with a threshold formed in 64 bits.
  * gamma / beta (when there is an activation) and dgamma / dbeta: both or neither.  dx_kind = dy_kind, or three planes from an fp32 dy.  ws: 16-byte aligned,
- * iprgan_mx8_norm_bwd_ws_floats(G, M, C) floats.  dbias_prev / dbias_n / dbias_beta as for iprgan_bn_bwd. */
-size_t iprgan_mx8_norm_bwd_ws_floats(int G, int M, int C);
+ * iprgan_mx8_norm_bwd_ws_floats(G, M, C) floats.  dbias_prev / dbias_n / dbias_beta as for iprgan_bn_bwd.  (Sizes come in 64 bits, here and
+ * below: one past the limits is refused, or a size query answers 0, where an int would have been cut to a small one.) */
+size_t iprgan_mx8_norm_bwd_ws_floats(long long G, long long M, long long C);
 int iprgan_mx8_norm_bwd(const void* codes, const void* scales, const void* dy, const float* gamma, const float* beta,
                         const float* save_mean, const float* save_invstd, const float* slope_dev, void* dx, float* dgamma,
-                        float* dbeta, float* dslope, float* ws, int G, int M, int C, int act, float slope, float* dbias_prev,
-                        int dbias_n, float dbias_beta, int dy_kind, size_t dy_pstride, int dx_kind, size_t dx_pstride, void* stream);
+                        float* dbeta, float* dslope, float* ws, long long G, long long M, long long C, int act, float slope,
+                        float* dbias_prev, long long dbias_n, float dbias_beta, int dy_kind, size_t dy_pstride, int dx_kind,
+                        size_t dx_pstride, void* stream);
 
 /* ---- microscaled 4-bit floating point (csrc/mx4.hip): compressed weights and their product -----------------------------------
  * A matrix [rows][cols] in blocks of 32 elements along a row: E2M1 codes (0, .5, 1, 1.5, 2, 3, 4, 6 and a sign), one E8M0
@@ -510,22 +512,22 @@ int iprgan_mx8_norm_bwd(const void* codes, const void* scales, const void* dy, c
  * ties to the even code.  A block that holds a NaN or an infinity stores scale byte 255 and reads back as NaN.  Rows are padded with
  * zero codes to whole groups of 128 elements: KB = iprgan_mx4_pitch(cols) = 4 * ceil(cols / 128) blocks a row; codes
  * [rows][KB * 16] bytes (element 2i in the low half of byte i; 16-byte aligned), scales [rows][KB] bytes (4-byte aligned). */
-int iprgan_mx4_pitch(int cols);
-int iprgan_mx4_quant(const void* x, void* codes, void* scales, int rows, int cols, int x_bf16, void* stream);
-int iprgan_mx4_dequant(const void* codes, const void* scales, void* y, int rows, int cols, int y_bf16, void* stream);
+int iprgan_mx4_pitch(long long cols);
+int iprgan_mx4_quant(const void* x, void* codes, void* scales, long long rows, long long cols, int x_bf16, void* stream);
+int iprgan_mx4_dequant(const void* codes, const void* scales, void* y, long long rows, long long cols, int y_bf16, void* stream);
 /* y [M][N] = act(x W^T + bias), W [N][K] in 4 bits.  x [M][K]: fp32 (multiplied as three bf16 planes: products exact, fp32
  * accumulation; an infinity, or a magnitude that rounds to one in bf16 - above 3.39e38 -, gives NaN), bf16, or 4-bit itself (x = codes with K columns, x_scales; the scaled matrix instruction).  bias [N] fp32 or
  * NULL; act as everywhere here (a NaN behind a ReLU is 0); y fp32 or bf16, rounded once.  ws: 16-byte aligned, iprgan_mx4_linear_ws_floats floats (0: may be NULL); sums over a
  * split K are added in fixed order. */
 enum { IPRGAN_X_F32 = 0, IPRGAN_X_BF16 = 1, IPRGAN_X_MX4 = 2 };
-size_t iprgan_mx4_linear_ws_floats(int M, int N, int K, int x_kind, int act);
+size_t iprgan_mx4_linear_ws_floats(long long M, long long N, long long K, int x_kind, int act);
 int iprgan_mx4_linear(const void* x, const void* x_scales, const void* w_codes, const void* w_scales, const float* bias, void* y,
-                      float* ws, int M, int N, int K, int x_kind, int act, float slope, int y_bf16, void* stream);
+                      float* ws, long long M, long long N, long long K, int x_kind, int act, float slope, int y_bf16, void* stream);
 /* dx [M][K] = dy [M][N] W: the gradient with respect to x through the frozen 4-bit weights.  (M at most 2^20, N and K below
  * 2^24, here and above.) */
-size_t iprgan_mx4_linear_bwd_ws_floats(int M, int N, int K, int dy_bf16);
-int iprgan_mx4_linear_bwd(const void* dy, const void* w_codes, const void* w_scales, void* dx, float* ws, int M, int N, int K,
-                          int dy_bf16, int dx_bf16, void* stream);
+size_t iprgan_mx4_linear_bwd_ws_floats(long long M, long long N, long long K, int dy_bf16);
+int iprgan_mx4_linear_bwd(const void* dy, const void* w_codes, const void* w_scales, void* dx, float* ws, long long M, long long N,
+                          long long K, int dy_bf16, int dx_bf16, void* stream);
 
 /* ---- misc elementwise ----------------------------------------------------------------------- */
 int iprgan_fill(float* p, float v, size_t n, void* stream);

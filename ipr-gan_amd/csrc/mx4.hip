@@ -996,6 +996,7 @@ __global__ __launch_bounds__(256, 2) void mx4_linear_bwd_kernel(const BwdArgs a,
 
 static inline bool aligned(const void* p, unsigned a) { return ((uintptr_t)p & (a - 1)) == 0; }
 static inline int kb_of(int cols) { return 4 * cdiv(cols, 128); }
+constexpr long long MAX_COLS = 0x7fffff80;      // of a row: its padded length is an int
 
 static int slab_reduce(const float* slab, int splits, int M, int N, const float* bias, void* out, int act, float slope, int out_bf16,
                        hipStream_t st) {
@@ -1137,17 +1138,17 @@ using namespace iprgan;
 
 extern "C" {
 
-int iprgan_mx4_pitch(int cols) { return cols > 0 && cols <= 0x7fffff80 ? kb_of(cols) : 0; }
+int iprgan_mx4_pitch(long long cols) { return cols > 0 && cols <= MAX_COLS ? kb_of((int)cols) : 0; }
 
-static int mx4_rows_check(const char* who, int rows, int cols, unsigned* groups) {
-  IPR_CHECK(rows > 0 && cols > 0, "%s: empty input (%d rows of %d)", who, rows, cols);
-  const size_t g = (size_t)rows * cdivz((size_t)cols, 128) * 16;
-  IPR_CHECK(g < 0x7fff0000ull, "%s: %d rows of %d are too many elements", who, rows, cols);
+static int mx4_rows_check(const char* who, long long rows, long long cols, unsigned* groups) {
+  IPR_CHECK(rows > 0 && cols > 0, "%s: empty input (%lld rows of %lld)", who, rows, cols);
+  const size_t g = rows < 0x7fff0000ll && cols <= MAX_COLS ? (size_t)rows * cdivz((size_t)cols, 128) * 16 : ~(size_t)0;
+  IPR_CHECK(g < 0x7fff0000ull, "%s: %lld rows of %lld are too many elements", who, rows, cols);
   *groups = (unsigned)g;
   return 0;
 }
 
-int iprgan_mx4_quant(const void* x, void* codes, void* scales, int rows, int cols, int x_bf16, void* stream) {
+int iprgan_mx4_quant(const void* x, void* codes, void* scales, long long rows, long long cols, int x_bf16, void* stream) {
   unsigned groups;
   if (mx4_rows_check("mx4_quant", rows, cols, &groups)) return 1;
   IPR_CHECK(x && codes && scales, "mx4_quant: null operand");
@@ -1156,12 +1157,12 @@ int iprgan_mx4_quant(const void* x, void* codes, void* scales, int rows, int col
   auto k = x_bf16 ? mx4_quant_kernel<true> : mx4_quant_kernel<false>;
   const unsigned blocks = (groups + 255) / 256;
   hipLaunchKernelGGL(k, dim3(blocks < 8192 ? blocks : 8192), dim3(256), 0, (hipStream_t)stream, x, (unsigned*)codes, (uint8_t*)scales,
-                     groups, cols, make_fastdiv((uint32_t)kb_of(cols) * 4));
+                     groups, (int)cols, make_fastdiv((uint32_t)kb_of((int)cols) * 4));
   IPR_LAUNCH_CHECK();
   return 0;
 }
 
-int iprgan_mx4_dequant(const void* codes, const void* scales, void* y, int rows, int cols, int y_bf16, void* stream) {
+int iprgan_mx4_dequant(const void* codes, const void* scales, void* y, long long rows, long long cols, int y_bf16, void* stream) {
   unsigned groups;
   if (mx4_rows_check("mx4_dequant", rows, cols, &groups)) return 1;
   IPR_CHECK(y && codes && scales, "mx4_dequant: null operand");
@@ -1170,29 +1171,33 @@ int iprgan_mx4_dequant(const void* codes, const void* scales, void* y, int rows,
   auto k = y_bf16 ? mx4_dequant_kernel<true> : mx4_dequant_kernel<false>;
   const unsigned blocks = (groups + 255) / 256;
   hipLaunchKernelGGL(k, dim3(blocks < 8192 ? blocks : 8192), dim3(256), 0, (hipStream_t)stream, (const unsigned*)codes,
-                     (const uint8_t*)scales, y, groups, cols, make_fastdiv((uint32_t)kb_of(cols) * 4));
+                     (const uint8_t*)scales, y, groups, (int)cols, make_fastdiv((uint32_t)kb_of((int)cols) * 4));
   IPR_LAUNCH_CHECK();
   return 0;
 }
 
-static int lin_check(const char* who, int M, int N, int K) {
-  IPR_CHECK(M > 0 && N > 0 && K > 0, "%s: empty product (M=%d, N=%d, K=%d)", who, M, N, K);
-  IPR_CHECK(K < (1 << 24) && M <= (1 << 20) && N < (1 << 24), "%s: M=%d, N=%d, K=%d (M at most 2^20, N and K below 2^24)", who, M, N, K);
+static bool lin_sizes_ok(long long M, long long N, long long K) {
+  return M > 0 && N > 0 && K > 0 && M <= (1 << 20) && N < (1 << 24) && K < (1 << 24);
+}
+static int lin_check(const char* who, long long M, long long N, long long K) {
+  IPR_CHECK(M > 0 && N > 0 && K > 0, "%s: empty product (M=%lld, N=%lld, K=%lld)", who, M, N, K);
+  IPR_CHECK(lin_sizes_ok(M, N, K), "%s: M=%lld, N=%lld, K=%lld (M at most 2^20, N and K below 2^24)", who, M, N, K);
   return 0;
 }
 
 // tanh and the sigmoid are applied by the pass that adds the slabs, also where there is only one
 static bool lin_slab(const LinPlan& p, int act) { return p.splits > 1 || act > IPRGAN_ACT_LRELU; }
 
-size_t iprgan_mx4_linear_ws_floats(int M, int N, int K, int x_kind, int act) {
-  if (M < 1 || N < 1 || K < 1) return 0;
-  const LinPlan p = lin_plan(M, N, K, x_kind);
+size_t iprgan_mx4_linear_ws_floats(long long M, long long N, long long K, int x_kind, int act) {
+  if (!lin_sizes_ok(M, N, K)) return 0;
+  const LinPlan p = lin_plan((int)M, (int)N, (int)K, x_kind);
   return lin_slab(p, act) ? (size_t)p.splits * M * N : 0;
 }
 
 int iprgan_mx4_linear(const void* x, const void* x_scales, const void* w_codes, const void* w_scales, const float* bias, void* y,
-                      float* ws, int M, int N, int K, int x_kind, int act, float slope, int y_bf16, void* stream) {
-  if (lin_check("mx4_linear", M, N, K)) return 1;
+                      float* ws, long long rows, long long outs, long long ins, int x_kind, int act, float slope, int y_bf16, void* stream) {
+  if (lin_check("mx4_linear", rows, outs, ins)) return 1;
+  const int M = (int)rows, N = (int)outs, K = (int)ins;
   IPR_CHECK(x_kind == IPRGAN_X_F32 || x_kind == IPRGAN_X_BF16 || x_kind == IPRGAN_X_MX4, "mx4_linear: kind %d of x", x_kind);
   IPR_CHECK(x && w_codes && w_scales && y && (x_kind != IPRGAN_X_MX4 || x_scales), "mx4_linear: null operand");
   IPR_CHECK(y_bf16 == 0 || y_bf16 == 1, "mx4_linear: storage kind %d of y (fp32 or bf16)", y_bf16);
@@ -1231,15 +1236,16 @@ int iprgan_mx4_linear(const void* x, const void* x_scales, const void* w_codes, 
   return slab ? slab_reduce(ws, p.splits, M, N, bias, y, act, slope, y_bf16, st) : 0;
 }
 
-size_t iprgan_mx4_linear_bwd_ws_floats(int M, int N, int K, int dy_bf16) {
-  if (M < 1 || N < 1 || K < 1) return 0;
-  const BwdPlan p = bwd_plan(M, N, K, dy_bf16);
+size_t iprgan_mx4_linear_bwd_ws_floats(long long M, long long N, long long K, int dy_bf16) {
+  if (!lin_sizes_ok(M, N, K)) return 0;
+  const BwdPlan p = bwd_plan((int)M, (int)N, (int)K, dy_bf16);
   return p.splits > 1 ? (size_t)p.splits * M * K : 0;
 }
 
-int iprgan_mx4_linear_bwd(const void* dy, const void* w_codes, const void* w_scales, void* dx, float* ws, int M, int N, int K,
-                          int dy_bf16, int dx_bf16, void* stream) {
-  if (lin_check("mx4_linear_bwd", M, N, K)) return 1;
+int iprgan_mx4_linear_bwd(const void* dy, const void* w_codes, const void* w_scales, void* dx, float* ws, long long rows, long long outs,
+                          long long ins, int dy_bf16, int dx_bf16, void* stream) {
+  if (lin_check("mx4_linear_bwd", rows, outs, ins)) return 1;
+  const int M = (int)rows, N = (int)outs, K = (int)ins;
   IPR_CHECK(dy && w_codes && w_scales && dx, "mx4_linear_bwd: null operand");
   IPR_CHECK((dy_bf16 == 0 || dy_bf16 == 1) && (dx_bf16 == 0 || dx_bf16 == 1), "mx4_linear_bwd: storage kinds %d, %d (fp32 or bf16)", dy_bf16, dx_bf16);
   IPR_CHECK(aligned(w_codes, 16) && aligned(w_scales, 4) && aligned(dy, dy_bf16 ? 2 : 4) && aligned(dx, dx_bf16 ? 2 : 4),

@@ -258,9 +258,14 @@ static NormGeom norm_geom(int G, int M, int C, int V) {
   g.TC = cdiv(cq, g.gy);
   g.TR = 256 / g.TC;
   int nb = cdiv(M, g.TR * 4);
-  const int cap = cdiv(1024, g.gy * G);         // four blocks a CU in all
+  const int cap = (int)cdivz(1024, (size_t)g.gy * G);         // four blocks a CU in all
   g.NB = nb < cap ? nb : cap;
   return g;
+}
+
+// int row numbers, and the grid's limits: 65535 groups, as many chunks of 64 V channels
+static bool norm_sizes_ok(long long G, long long M, long long C) {
+  return G > 0 && G <= 65535 && M > 0 && M <= (1 << 30) && C >= 4 && C <= 65535 * 512;
 }
 
 // threshold form of the mask: v > 0  <=>  sgn * x > thr
@@ -674,19 +679,22 @@ int iprgan_mx8_act_bwd(const void* dy, const void* codes, const void* scales, vo
 }
 
 // the most partial rows either vector width asks for
-size_t iprgan_mx8_norm_bwd_ws_floats(int G, int M, int C) {
-  if (G < 1 || M < 1 || C < 4) return 0;
-  const NormGeom a = norm_geom(G, M, C, 4), b = norm_geom(G, M, C, 8);
+size_t iprgan_mx8_norm_bwd_ws_floats(long long G, long long M, long long C) {
+  if (!norm_sizes_ok(G, M, C)) return 0;
+  const NormGeom a = norm_geom((int)G, (int)M, (int)C, 4), b = norm_geom((int)G, (int)M, (int)C, 8);
   const size_t nb = (size_t)G * (a.NB > b.NB ? a.NB : b.NB);
   return nb * 3 * C + (size_t)G * 3 * C + (nb + 64) * 2 * C;         // partials, sums, column sums of dx and their compacted rows
 }
 
 int iprgan_mx8_norm_bwd(const void* codes, const void* scales, const void* dy, const float* gamma, const float* beta,
                         const float* save_mean, const float* save_invstd, const float* slope_dev, void* dx, float* dgamma,
-                        float* dbeta, float* dslope, float* ws, int G, int M, int C, int act, float slope, float* dbias_prev,
-                        int dbias_n, float dbias_beta, int dy_kind, size_t dy_pstride, int dx_kind, size_t dx_pstride, void* stream) {
-  IPR_CHECK(G > 0 && M > 0 && C > 0, "mx8_norm_bwd: empty input (%d groups of %d rows, %d channels)", G, M, C);
-  IPR_CHECK(C % 4 == 0, "mx8_norm_bwd: C=%d must be a multiple of 4", C);
+                        float* dbeta, float* dslope, float* ws, long long groups, long long rows, long long channels, int act, float slope,
+                        float* dbias_prev, long long dbias_n, float dbias_beta, int dy_kind, size_t dy_pstride, int dx_kind,
+                        size_t dx_pstride, void* stream) {
+  IPR_CHECK(groups > 0 && rows > 0 && channels > 0, "mx8_norm_bwd: empty input (%lld groups of %lld rows, %lld channels)", groups, rows, channels);
+  IPR_CHECK(channels % 4 == 0, "mx8_norm_bwd: C=%lld must be a multiple of 4", channels);
+  IPR_CHECK(norm_sizes_ok(groups, rows, channels), "mx8_norm_bwd: %lld groups of %lld rows, %lld channels (at most 65535, 2^30, 65535 * 512)", groups, rows, channels);
+  const int G = (int)groups, M = (int)rows, C = (int)channels;
   IPR_CHECK(codes && scales && dy && dx && save_mean && save_invstd && ws, "mx8_norm_bwd: null operand");
   IPR_CHECK(act == IPRGAN_ACT_NONE || !gamma == !beta, "mx8_norm_bwd: the mask is recomputed from x: gamma and beta are both needed (or both absent)");
   IPR_CHECK(!beta || gamma, "mx8_norm_bwd: beta without gamma");
@@ -697,9 +705,7 @@ int iprgan_mx8_norm_bwd(const void* codes, const void* scales, const void* dy, c
   IPR_CHECK(!slope_dev || act == IPRGAN_ACT_LRELU, "mx8_norm_bwd: a device slope belongs to IPRGAN_ACT_LRELU");
   IPR_CHECK(dy_kind >= IPRGAN_ST_F32 && dy_kind <= IPRGAN_ST_X3, "mx8_norm_bwd: dy kind %d", dy_kind);
   IPR_CHECK(dx_kind == dy_kind || (dy_kind == IPRGAN_ST_F32 && dx_kind == IPRGAN_ST_X3), "mx8_norm_bwd: dx kind %d from dy kind %d", dx_kind, dy_kind);
-  IPR_CHECK(G <= 65535, "mx8_norm_bwd: %d groups (at most 65535)", G);
-  IPR_CHECK(M <= (1 << 30), "mx8_norm_bwd: %d rows (at most 2^30)", M);
-  IPR_CHECK(!dbias_prev || (dbias_n > 0 && dbias_n <= C), "mx8_norm_bwd: %d bias gradients for %d channels", dbias_n, C);
+  IPR_CHECK(!dbias_prev || (dbias_n > 0 && dbias_n <= C), "mx8_norm_bwd: %lld bias gradients for %d channels", dbias_n, C);
   const size_t n = (size_t)G * M * C;
   if (!dy_pstride) dy_pstride = n;
   if (!dx_pstride) dx_pstride = n;
@@ -710,6 +716,7 @@ int iprgan_mx8_norm_bwd(const void* codes, const void* scales, const void* dy, c
   hipStream_t st = (hipStream_t)stream;
   const bool wide = dy_kind != IPRGAN_ST_F32 && C % 8 == 0 && al16(dy) && al16(dx) && (dy_kind != IPRGAN_ST_X3 || (dy_pstride % 8 == 0 && dx_pstride % 8 == 0));
   const NormGeom g = norm_geom(G, M, C, wide ? 8 : 4);
+  IPR_CHECK(g.gy <= 65535, "mx8_norm_bwd: %d channels in chunks of %d", C, g.TC * (wide ? 8 : 4));
   NormArgs a;
   memset(&a, 0, sizeof(a));
   a.q = (const int8_t*)codes; a.scales = (const uint8_t*)scales; a.dy = dy; a.dx = dx;
@@ -733,7 +740,7 @@ int iprgan_mx8_norm_bwd(const void* codes, const void* scales, const void* dy, c
     rc = wide ? norm_bwd_go<2, 2, 8>(a, g, am, st) : norm_bwd_go<2, 2, 4>(a, g, am, st);
   }
   if (rc) return rc;
-  if (dbias_prev) return iprgan_colsum_partials(colpart, G * g.NB, C, dbias_n, dbias_prev, dbias_beta, stream);
+  if (dbias_prev) return iprgan_colsum_partials(colpart, G * g.NB, C, (int)dbias_n, dbias_prev, dbias_beta, stream);
   return 0;
 }
 

@@ -137,15 +137,15 @@ SIGNATURES = {
     'iprgan_mx8_quant': (_I, [_P, _P, _P, _Z, _I, _Z, _P]),
     'iprgan_mx8_dequant': (_I, [_P, _P, _P, _Z, _I, _Z, _P]),
     'iprgan_mx8_act_bwd': (_I, [_P, _P, _P, _P, _Z, _I, _F, _I, _P]),
-    'iprgan_mx8_norm_bwd_ws_floats': (_Z, [_I, _I, _I]),
-    'iprgan_mx8_norm_bwd': (_I, [_P] * 13 + [_I, _I, _I, _I, _F, _P, _I, _F, _I, _Z, _I, _Z, _P]),
-    'iprgan_mx4_pitch': (_I, [_I]),
-    'iprgan_mx4_quant': (_I, [_P, _P, _P, _I, _I, _I, _P]),
-    'iprgan_mx4_dequant': (_I, [_P, _P, _P, _I, _I, _I, _P]),
-    'iprgan_mx4_linear_ws_floats': (_Z, [_I, _I, _I, _I, _I]),
-    'iprgan_mx4_linear': (_I, [_P] * 7 + [_I, _I, _I, _I, _I, _F, _I, _P]),
-    'iprgan_mx4_linear_bwd_ws_floats': (_Z, [_I, _I, _I, _I]),
-    'iprgan_mx4_linear_bwd': (_I, [_P] * 5 + [_I, _I, _I, _I, _I, _P]),
+    'iprgan_mx8_norm_bwd_ws_floats': (_Z, [_LL, _LL, _LL]),
+    'iprgan_mx8_norm_bwd': (_I, [_P] * 13 + [_LL, _LL, _LL, _I, _F, _P, _LL, _F, _I, _Z, _I, _Z, _P]),
+    'iprgan_mx4_pitch': (_I, [_LL]),
+    'iprgan_mx4_quant': (_I, [_P, _P, _P, _LL, _LL, _I, _P]),
+    'iprgan_mx4_dequant': (_I, [_P, _P, _P, _LL, _LL, _I, _P]),
+    'iprgan_mx4_linear_ws_floats': (_Z, [_LL, _LL, _LL, _I, _I]),
+    'iprgan_mx4_linear': (_I, [_P] * 7 + [_LL, _LL, _LL, _I, _I, _F, _I, _P]),
+    'iprgan_mx4_linear_bwd_ws_floats': (_Z, [_LL, _LL, _LL, _I]),
+    'iprgan_mx4_linear_bwd': (_I, [_P] * 5 + [_LL, _LL, _LL, _I, _I, _P]),
     'iprgan_fill': (_I, [_P, _F, _Z, _P]),
     'iprgan_axpy': (_I, [_P, _P, _F, _Z, _P]),
     'iprgan_axpy_multi': (_I, [_P, _P, _P, _I, _F, _P]),

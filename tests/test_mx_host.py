@@ -125,3 +125,31 @@ def test_ckpt8_engine_key(monkeypatch):
     assert configs.apply_engine({'engine': {'ckpt8': True}}, set_math=False) == {'ckpt8': True} and engine._CKPT8
     configs.apply_engine({'engine': {'ckpt8': False}}, set_math=False)
     assert not engine._CKPT8
+
+
+WRAP = 1 << 32          # added to a size: what an int would cut off
+
+
+def refused_size(name, *args):
+    """refused() by the entry's own checks: behind them there is no GPU here, and a launch fails too."""
+    with pytest.raises(RuntimeError, match=name) as e:
+        L.call(name, *args)
+    assert 'launch' not in str(e.value), e.value
+
+
+def test_sizes_past_an_int_are_not_cut():
+    """A dimension of 2^32 + k is refused (or priced) as itself, never taken for k."""
+    assert L.query('iprgan_mx4_pitch', WRAP + 128) == 0
+    refused_size('iprgan_mx4_quant', P, P, P, 1, WRAP + 128, 0, None)
+    refused_size('iprgan_mx4_quant', P, P, P, WRAP + 1, 128, 0, None)
+    refused_size('iprgan_mx4_dequant', P, P, P, 1, WRAP + 128, 0, None)
+    refused_size('iprgan_mx4_dequant', P, P, P, WRAP + 1, 128, 0, None)
+    for i in range(3):
+        d = [8, 8, 8]
+        d[i] += WRAP
+        refused_size('iprgan_mx4_linear', P, None, P, P, None, P, P, *d, 0, 0, 0.0, 0, None)
+        refused_size('iprgan_mx4_linear_bwd', P, P, P, P, P, *d, 0, 0, None)
+        assert L.query('iprgan_mx4_linear_ws_floats', *d, 0, 3) == 0 and L.query('iprgan_mx4_linear_bwd_ws_floats', *d, 0) == 0
+    for bad in (dict(G=WRAP + 1), dict(M=WRAP + 8), dict(C_=WRAP + 8), dict(dbias=P, nb=WRAP + 8)):
+        refused_size(*norm(**bad))
+    assert L.query('iprgan_mx8_norm_bwd_ws_floats', 1, WRAP + 8, 8) == 0
