@@ -523,8 +523,8 @@ enum { IPRGAN_X_F32 = 0, IPRGAN_X_BF16 = 1, IPRGAN_X_MX4 = 2 };
 size_t iprgan_mx4_linear_ws_floats(long long M, long long N, long long K, int x_kind, int act);
 int iprgan_mx4_linear(const void* x, const void* x_scales, const void* w_codes, const void* w_scales, const float* bias, void* y,
                       float* ws, long long M, long long N, long long K, int x_kind, int act, float slope, int y_bf16, void* stream);
-/* dx [M][K] = dy [M][N] W: the gradient with respect to x through the frozen 4-bit weights.  (M at most 2^20, N and K below
- * 2^24, here and above.) */
+/* dx [M][K] = dy [M][N] W: the gradient with respect to x through the frozen 4-bit weights.  (M below 2^30, N and K below 2^24, here
+ * and above; a launch's 2^24 tiles of at most 64 x 256 results may be the nearer limit: past it the call is refused.) */
 size_t iprgan_mx4_linear_bwd_ws_floats(long long M, long long N, long long K, int dy_bf16);
 int iprgan_mx4_linear_bwd(const void* dy, const void* w_codes, const void* w_scales, void* dx, float* ws, long long M, long long N,
                           long long K, int dy_bf16, int dx_bf16, void* stream);

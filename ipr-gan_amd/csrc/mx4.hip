@@ -998,15 +998,27 @@ static inline bool aligned(const void* p, unsigned a) { return ((uintptr_t)p & (
 static inline int kb_of(int cols) { return 4 * cdiv(cols, 128); }
 constexpr long long MAX_COLS = 0x7fffff80;      // of a row: its padded length is an int
 
+// a launch has fewer than 2^32 threads along x
+static inline bool grid_ok(size_t blocks, unsigned threads) { return blocks * threads <= 0xffffffffull; }
+
+struct SlabGrid {
+  bool vec, deep;                // 4 outputs a group; 8 lanes a group, which pay for themselves from 8 splits on
+  size_t blocks;
+};
+static SlabGrid slab_grid(int splits, int M, int N, const void* out, int out_bf16) {
+  SlabGrid g;
+  g.vec = N % 4 == 0 && aligned(out, out_bf16 ? 8 : 16);
+  g.deep = splits >= 8;
+  g.blocks = cdivz((size_t)M * N, (g.vec ? 4 : 1) * (g.deep ? 32 : 256));
+  return g;
+}
 static int slab_reduce(const float* slab, int splits, int M, int N, const float* bias, void* out, int act, float slope, int out_bf16,
                        hipStream_t st) {
   const size_t total = (size_t)M * N;
-  const bool vec = N % 4 == 0 && aligned(out, out_bf16 ? 8 : 16);
-  const bool deep = splits >= 8;                             // 8 lanes a group pay for themselves from 8 splits on
-  const size_t blocks = cdivz(total, (vec ? 4 : 1) * (deep ? 32 : 256));
-  IPR_CHECK(blocks < 0x7fffffffull, "mx4: %zu outputs are too many", total);
+  const SlabGrid g = slab_grid(splits, M, N, out, out_bf16);      // (grid_ok: the entry points look before they launch the product)
+  const bool vec = g.vec, deep = g.deep;
   auto k = vec ? (deep ? mx4_slab_reduce_kernel<4, 8> : mx4_slab_reduce_kernel<4, 1>) : (deep ? mx4_slab_reduce_kernel<1, 8> : mx4_slab_reduce_kernel<1, 1>);
-  hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(256), 0, st, slab, splits, total, N, bias, out, act, slope, out_bf16);
+  hipLaunchKernelGGL(k, dim3((unsigned)g.blocks), dim3(256), 0, st, slab, splits, total, N, bias, out, act, slope, out_bf16);
   IPR_LAUNCH_CHECK();
   return 0;
 }
@@ -1177,11 +1189,11 @@ int iprgan_mx4_dequant(const void* codes, const void* scales, void* y, long long
 }
 
 static bool lin_sizes_ok(long long M, long long N, long long K) {
-  return M > 0 && N > 0 && K > 0 && M <= (1 << 20) && N < (1 << 24) && K < (1 << 24);
+  return M > 0 && N > 0 && K > 0 && M < (1 << 30) && N < (1 << 24) && K < (1 << 24);      // M: 2 M and every tile's rows are ints
 }
 static int lin_check(const char* who, long long M, long long N, long long K) {
   IPR_CHECK(M > 0 && N > 0 && K > 0, "%s: empty product (M=%lld, N=%lld, K=%lld)", who, M, N, K);
-  IPR_CHECK(lin_sizes_ok(M, N, K), "%s: M=%lld, N=%lld, K=%lld (M at most 2^20, N and K below 2^24)", who, M, N, K);
+  IPR_CHECK(lin_sizes_ok(M, N, K), "%s: M=%lld, N=%lld, K=%lld (M below 2^30, N and K below 2^24)", who, M, N, K);
   return 0;
 }
 
@@ -1206,8 +1218,10 @@ int iprgan_mx4_linear(const void* x, const void* x_scales, const void* w_codes, 
                 (x_kind != IPRGAN_X_MX4 || aligned(x_scales, 4)) && aligned(y, y_bf16 ? 2 : 4),
             "mx4_linear: codes must be 16-byte, scales 4-byte aligned");
   const LinPlan p = lin_plan(M, N, K, x_kind);
-  IPR_CHECK((long long)p.tm * p.tn * p.splits < 0x7fffffffll, "mx4_linear: M=%d, N=%d", M, N);
   const bool slab = lin_slab(p, act);
+  IPR_CHECK(p.tile || grid_ok((size_t)p.tm * p.tn * p.splits, p.wk ? 512 : 256), "mx4_linear: M=%d, N=%d are too many tiles for a launch", M, N);
+  IPR_CHECK((long long)p.tm * p.tn < 0x7fffffffll && (!slab || grid_ok(slab_grid(p.splits, M, N, y, y_bf16).blocks, 256)),
+            "mx4_linear: M=%d, N=%d are too many results", M, N);
   IPR_CHECK(!slab || (ws && aligned(ws, 16)), "mx4_linear: the workspace of iprgan_mx4_linear_ws_floats is missing");
   hipStream_t st = (hipStream_t)stream;
   LinArgs a;
@@ -1251,7 +1265,8 @@ int iprgan_mx4_linear_bwd(const void* dy, const void* w_codes, const void* w_sca
   IPR_CHECK(aligned(w_codes, 16) && aligned(w_scales, 4) && aligned(dy, dy_bf16 ? 2 : 4) && aligned(dx, dx_bf16 ? 2 : 4),
             "mx4_linear_bwd: codes must be 16-byte, scales 4-byte aligned");
   const BwdPlan p = bwd_plan(M, N, K, dy_bf16);
-  IPR_CHECK((long long)p.tm * p.tk * p.splits < 0x7fffffffll, "mx4_linear_bwd: M=%d, K=%d", M, K);
+  IPR_CHECK(grid_ok((size_t)p.tm * p.tk * p.splits, 256) && (p.splits == 1 || grid_ok(slab_grid(p.splits, M, K, dx, dx_bf16).blocks, 256)),
+            "mx4_linear_bwd: M=%d, K=%d are too many tiles for a launch", M, K);
   IPR_CHECK(p.splits == 1 || (ws && aligned(ws, 16)), "mx4_linear_bwd: the workspace of iprgan_mx4_linear_bwd_ws_floats is missing");
   hipStream_t st = (hipStream_t)stream;
   BwdArgs a;

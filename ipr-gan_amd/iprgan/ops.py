@@ -466,7 +466,8 @@ X_MX4 = 2           # include/iprgan.h: IPRGAN_X_MX4
 
 def mx4_linear(x, w, bias=None, act=L.ACT_NONE, slope=0.0, dtype=None):
     """y = act(x W^T + bias): ``w`` an Mx4 of shape (N, K); ``x`` [..., K] fp32 or bf16 (unrounded: fp32 goes through three bf16
-    planes) or an Mx4 of shape (M, K).  y in ``dtype`` (default: x's; float32 for a 4-bit x)."""
+    planes, an infinity gives NaN) or an Mx4 of shape (M, K).  y in ``dtype`` (default: x's; float32 for a 4-bit x).  Fewer than 2^30 rows, N
+    and K below 2^24."""
     if not isinstance(w, Mx4):
         raise RuntimeError('mx4_linear: the weights must be an Mx4 (mx4_quant)')
     N, K = w.shape
@@ -501,7 +502,7 @@ def mx4_linear(x, w, bias=None, act=L.ACT_NONE, slope=0.0, dtype=None):
 
 def mx4_linear_bwd(dy, w, dtype=None):
     """dx = dy W: the gradient with respect to x through the frozen 4-bit weights; dy [..., N] fp32 or bf16, dx in ``dtype``
-    (default: dy's)."""
+    (default: dy's).  The sizes of mx4_linear."""
     if not isinstance(w, Mx4):
         raise RuntimeError('mx4_linear_bwd: the weights must be an Mx4 (mx4_quant)')
     N, K = w.shape

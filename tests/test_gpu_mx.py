@@ -620,3 +620,29 @@ def test_results_past_32_bits(dev):
         dx = ops.mx4_linear_bwd(d, w, torch.bfloat16)
         assert torch.equal(dx[rows.to(dev)].cpu(), (x.cpu()[rows].double() @ wb.double()).bfloat16())
         del dx
+
+
+@pytest.mark.parametrize('M', [(1 << 20) + 5, 256 * 128 * 128 + 1])
+def test_more_than_a_million_rows(dev, M):
+    """Every position of a batch of maps as a row: whole numbers small enough that products and sums are exact."""
+    from iprgan import ops
+    K, N = 32, 12
+    gen = torch.Generator().manual_seed(4)
+    wt = torch.randint(-2, 3, (N, K), generator=gen).float()
+    wt[:, 0] = 6.                                                # (scale 1: the values are the codes)
+    w = ops.mx4_quant(wt.to(dev))
+    x = torch.randint(-2, 3, (M, K), generator=gen).float().to(dev)
+    x[:, 0] = 6.
+    want = torch.zeros(M, N, device=dev)
+    for k in range(K):
+        want += x[:, k:k + 1] * wt[:, k].to(dev)
+    for a in (x, x.bfloat16(), ops.mx4_quant(x)):
+        assert torch.equal(ops.mx4_linear(a, w, dtype=torch.float32), want)
+    got = ops.mx4_linear(x, w, act=3)
+    assert torch.equal(got[-70:], ops.mx4_linear(x[-70:].clone(), w, act=3))
+    dy = torch.randint(-8, 9, (M, N), generator=gen).float().to(dev)
+    want = torch.zeros(M, K, device=dev)
+    for n in range(N):
+        want += dy[:, n:n + 1] * wt[n].to(dev)
+    for d in (dy, dy.bfloat16()):
+        assert torch.equal(ops.mx4_linear_bwd(d, w, torch.float32), want)

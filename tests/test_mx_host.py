@@ -134,7 +134,7 @@ def refused_size(name, *args):
     """refused() by the entry's own checks: behind them there is no GPU here, and a launch fails too."""
     with pytest.raises(RuntimeError, match=name) as e:
         L.call(name, *args)
-    assert 'launch' not in str(e.value), e.value
+    assert 'launch failed' not in str(e.value), e.value
 
 
 def test_sizes_past_an_int_are_not_cut():
@@ -153,3 +153,15 @@ def test_sizes_past_an_int_are_not_cut():
     for bad in (dict(G=WRAP + 1), dict(M=WRAP + 8), dict(C_=WRAP + 8), dict(dbias=P, nb=WRAP + 8)):
         refused_size(*norm(**bad))
     assert L.query('iprgan_mx8_norm_bwd_ws_floats', 1, WRAP + 8, 8) == 0
+
+
+def test_rows_of_a_map_are_within_the_limits():
+    """All positions of a batch of maps are rows of one product: more than 2^20 are ordinary, 2^30 are refused, and so is a grid past a launch."""
+    rows = 256 * 128 * 128
+    assert L.query('iprgan_mx4_linear_ws_floats', rows, 4, 32, 0, 3) == rows * 4             # (tanh goes through the workspace)
+    refused_size('iprgan_mx4_linear', P, None, P, P, None, P, P, 1 << 30, 8, 8, 0, 0, 0.0, 0, None)
+    refused_size('iprgan_mx4_linear_bwd', P, P, P, P, P, 1 << 30, 8, 8, 0, 0, None)
+    refused_size('iprgan_mx4_linear', P, None, P, P, None, P, P, 1 << 29, 1 << 20, 8, 0, 0, 0.0, 0, None)
+    refused_size('iprgan_mx4_linear', P, None, P, P, None, P, P, 1 << 29, 255, 8, 0, 3, 0.0, 0, None)
+    refused_size('iprgan_mx4_linear_bwd', P, P, P, P, P, 1 << 29, 8, 1 << 20, 0, 0, None)
+    refused_size('iprgan_mx4_linear', P, P, P, P, None, P, P, 1 << 29, 1 << 23, 8, 2, 0, 0.0, 0, None)
