@@ -44,12 +44,17 @@ class _HipNet(nn.Module):
     def run(self, x):
         return self.chain()(x, self.training)
 
+    def _dense_ops(self):
+        ch = self.chain()
+        chains = [ch] if isinstance(ch, E.Chain) else [ch[0], *ch[1]]        # (the encoder: a body and its heads)
+        return [op for c in chains for op in c.ops if isinstance(op, E.LinearNHWC)]
+
     def quantize_dense(self, on=True):
-        """Serve the net's dense layers (the generators' first Linear: 4.2 of DCGAN-64's 7 million parameters, 16.8 of DCGAN-128's 19.5)
-        from a 4-bit copy of their weights (ops.Mx4: 0.53 bytes a weight) in eval mode; training passes keep the fp32 weights.
+        """Serve the net's dense layers (the generators' first Linear: 4.2 of DCGAN-64's 7 million parameters, 16.8 of DCGAN-128's 19.5; the
+        encoder's two heads) from a 4-bit copy of their weights (ops.Mx4: 0.53 bytes a weight) in eval mode; training passes keep the fp32 weights.
         The input's gradient is available (latent inversion), the weights' is not.  Weights that change afterwards make the next eval
         pass raise; call again to requantise, ``quantize_dense(False)`` drops the copies.  Returns the number of layers."""
-        dense = [op for op in self.chain().ops if isinstance(op, E.LinearNHWC)]
+        dense = self._dense_ops()
         if on and not dense:
             raise RuntimeError(f'{type(self).__name__} has no dense layer to quantise')
         for op in dense:

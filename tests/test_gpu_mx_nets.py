@@ -253,3 +253,22 @@ def test_compression_attack(dev):
             assert np.array_equal(p.detach().cpu().double().view(w.shape[0], -1).numpy(), r.numpy()), k
     assert float(slm.compute_ber(net)) == 0.0
     net(torch.randn(2, 128, device=dev))
+
+
+def test_encoder_heads_served_from_4_bit_weights(dev):
+    """Two dense layers behind the encoder's body; K = 2048 is one sum of 2048 terms: 2048 half steps of the terms' magnitude."""
+    from iprgan import networks, ops
+    torch.manual_seed(4)
+    net, ref = networks.Encoder32().to(dev).eval(), networks.Encoder32().to(dev).eval()
+    ref.load_state_dict(net.state_dict())
+    assert net.quantize_dense() == 2
+    with torch.no_grad():
+        for m in (ref.q_mean, ref.q_logvar):
+            m.weight.copy_(ops.mx4_dequant(ops.mx4_quant(m.weight)))
+        x = torch.randn(5, 3, 32, 32, generator=torch.Generator().manual_seed(1)).to(dev)
+        got, q = net(x)[1], ref.chain()[0](x, False).double()
+        for a, m in zip(got, (ref.q_mean, ref.q_logvar)):
+            w = m.weight.detach().double()
+            want, mag = q @ w.t().contiguous() + m.bias.detach().double(), q.abs() @ w.abs().t().contiguous() + m.bias.detach().double().abs()
+            assert bool(((a.double() - want).abs() <= 2048 * 2.0 ** -24 * mag).all())
+    assert net.quantize_dense(False) == 2

@@ -165,3 +165,12 @@ def test_rows_of_a_map_are_within_the_limits():
     refused_size('iprgan_mx4_linear', P, None, P, P, None, P, P, 1 << 29, 255, 8, 0, 3, 0.0, 0, None)
     refused_size('iprgan_mx4_linear_bwd', P, P, P, P, P, 1 << 29, 8, 1 << 20, 0, 0, None)
     refused_size('iprgan_mx4_linear', P, P, P, P, None, P, P, 1 << 29, 1 << 23, 8, 2, 0, 0.0, 0, None)
+
+
+@pytest.mark.parametrize('name,layers', [('ConvGenerator32', 1), ('ConvGenerator64', 1), ('Decoder32', 1), ('Encoder32', 2), ('SRResNet', 0)])
+def test_quantize_dense_finds_the_dense_layers_of_every_network(name, layers):
+    from iprgan import networks
+    net = getattr(networks, name)()
+    assert net.quantize_dense(False) == layers
+    with pytest.raises(RuntimeError, match='GPU tensors' if layers else 'no dense layer'):
+        net.quantize_dense()
