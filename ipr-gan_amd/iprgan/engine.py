@@ -296,6 +296,32 @@ class LinearNHWC(Op):
         w, b = self.weight, self.bias
         return (w._version, w.data_ptr(), b._version, b.data_ptr())
 
+    # The 4-bit copy (_mx4: key, Mx4, bias) is keyed on the weights' storage and version.  Where the op or its module is copied, pickled or
+    # moved, the storage changes and the weights do not: a copy that was current is keyed anew, one that was out of date stays so.
+    def quantized_current(self):
+        ent = self.__dict__.get('_mx4')
+        return ent is not None and ent[0] == self._weights_key()
+
+    def rekey_quantized(self):
+        _, w4, bias = self._mx4
+        if self.weight.dtype != torch.float32:
+            self._mx4 = (None, w4, bias)               # (no key: out of date)
+            return
+        d = self.weight.device
+        self._mx4 = (self._weights_key(), ops.Mx4(w4.codes.to(d), w4.scales.to(d), w4.shape), bias.to(d))
+
+    def __getstate__(self):
+        d = dict(self.__dict__)
+        if '_mx4' in d:
+            d['_mx4'] = (self.quantized_current(),) + d['_mx4'][1:]
+        return d
+
+    def __setstate__(self, d):
+        self.__dict__.update(d)
+        if '_mx4' in d:
+            current, w4, bias = d['_mx4']
+            self._mx4 = (self._weights_key() if current else None, w4, bias)
+
     def quantize(self, on=True):
         """A 4-bit copy of the weights, rows in NHWC order, for passes in eval mode (networks: quantize_dense)."""
         if not on:

@@ -49,11 +49,20 @@ class _HipNet(nn.Module):
         chains = [ch] if isinstance(ch, E.Chain) else [ch[0], *ch[1]]        # (the encoder: a body and its heads)
         return [op for c in chains for op in c.ops if isinstance(op, E.LinearNHWC)]
 
+    def _apply(self, fn, recurse=True):
+        """.to(), .cuda(), .cpu(): the dense layers' 4-bit copies go along."""
+        current = [op for op in self._dense_ops() if op.quantized_current()] if '_chain' in self.__dict__ else []
+        super()._apply(fn, recurse)
+        for op in current:
+            op.rekey_quantized()
+        return self
+
     def quantize_dense(self, on=True):
         """Serve the net's dense layers (the generators' first Linear: 4.2 of DCGAN-64's 7 million parameters, 16.8 of DCGAN-128's 19.5; the
         encoder's two heads) from a 4-bit copy of their weights (ops.Mx4: 0.53 bytes a weight) in eval mode; training passes keep the fp32 weights.
-        The input's gradient is available (latent inversion), the weights' is not.  Weights that change afterwards make the next eval
-        pass raise; call again to requantise, ``quantize_dense(False)`` drops the copies.  Returns the number of layers."""
+        The input's gradient is available (latent inversion), the weights' is not.  The copies follow a net that is copied,
+        pickled or moved.  Weights that change afterwards make the next eval pass raise; call again to requantise,
+        ``quantize_dense(False)`` drops the copies.  Returns the number of layers."""
         dense = self._dense_ops()
         if on and not dense:
             raise RuntimeError(f'{type(self).__name__} has no dense layer to quantise')

@@ -246,6 +246,9 @@ class _Packed:
     def get_device(self):
         return self._dev
 
+    def __reduce__(self):                              # (copies and pickles: through the constructor and its checks)
+        return type(self), (self.codes, self.scales, self.shape)
+
     def ptrs(self):
         """(codes, scales) as device pointers."""
         if self._buf is None:
@@ -279,6 +282,9 @@ class Mx8(_Packed):
             raise RuntimeError(f'Mx8: storage kind {kind}')
         self._adopt(codes, scales)
         self.shape, self.kind, self._n = shape, kind, n
+
+    def __reduce__(self):
+        return Mx8, (self.codes, self.scales, self.shape, self.kind)
 
     @property
     def codes(self):

@@ -272,3 +272,24 @@ def test_encoder_heads_served_from_4_bit_weights(dev):
             want, mag = q @ w.t().contiguous() + m.bias.detach().double(), q.abs() @ w.abs().t().contiguous() + m.bias.detach().double().abs()
             assert bool(((a.double() - want).abs() <= 2048 * 2.0 ** -24 * mag).all())
     assert net.quantize_dense(False) == 2
+
+
+def test_a_copied_or_moved_generator_is_served_as_before(dev):
+    import copy
+    from iprgan import networks
+    torch.manual_seed(6)
+    net = networks.ConvGenerator32().to(dev).eval()
+    net.quantize_dense()
+    z = torch.randn(3, 128, generator=torch.Generator().manual_seed(1)).to(dev)
+    with torch.no_grad():
+        want = net(z)
+        twin = copy.deepcopy(net)
+        assert torch.equal(twin(z), want)
+        twin.fc[0].weight.mul_(2)
+        with pytest.raises(RuntimeError, match='out of date'):
+            twin(z)
+        assert torch.equal(net.cpu().to(dev)(z), want)
+        net.fc[0].weight.mul_(2)
+        net.cpu().to(dev)
+        with pytest.raises(RuntimeError, match='out of date'):
+            net(z)

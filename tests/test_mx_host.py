@@ -174,3 +174,53 @@ def test_quantize_dense_finds_the_dense_layers_of_every_network(name, layers):
     assert net.quantize_dense(False) == layers
     with pytest.raises(RuntimeError, match='GPU tensors' if layers else 'no dense layer'):
         net.quantize_dense()
+
+
+def test_a_copied_or_moved_net_keeps_its_4_bit_copy():
+    """The copy is keyed on the weights' storage and version: copying or moving a net changes the storage, not the weights.  A copy that was
+    out of date stays so.  (Made by hand: quantising needs a GPU.)"""
+    import copy
+    import io
+    from iprgan import networks
+    net = networks.ConvGenerator32()
+    op = net.chain().ops[0]
+
+    def serve():
+        n, k = op.weight.shape
+        w4 = ops.Mx4(torch.randint(0, 256, (n, 64 * (k // 128)), dtype=torch.uint8), torch.full((n, k // 32), 120, dtype=torch.uint8), (n, k))
+        op._mx4 = (op._weights_key(), w4, op.bias.detach().clone())
+        return w4
+
+    def pickled(n):
+        f = io.BytesIO()
+        torch.save(n, f)
+        f.seek(0)
+        return torch.load(f, weights_only=False)            # (a file this test has just written)
+
+    w4 = serve()
+    for twin in (copy.deepcopy(net), pickled(net)):
+        t = twin.chain().ops[0]
+        assert t.weight is not op.weight and t._mx4[0] == t._weights_key() != op._mx4[0]
+        assert torch.equal(t._mx4[1].codes, w4.codes) and t._mx4[1].codes.data_ptr() != w4.codes.data_ptr() and t._mx4[1].shape == w4.shape
+    with torch.no_grad():
+        twin.fc[0].weight.mul_(2)
+    assert t._mx4[0] != t._weights_key()
+    again = copy.deepcopy(twin).chain().ops[0]
+    assert again._mx4[0] != again._weights_key(), 'an outdated copy must not become valid'
+    net._apply(lambda p: p.clone())                          # what .to() / .cuda() do
+    assert op._mx4[0] == op._weights_key() and torch.equal(op._mx4[1].codes, w4.codes)
+    with torch.no_grad():
+        net.fc[0].weight.mul_(2)
+    net._apply(lambda p: p.clone())
+    assert op._mx4[0] != op._weights_key(), 'an outdated copy must not become valid'
+    assert op._weights_key() == op._weights_key()
+    serve()
+    net.double()
+    assert op._mx4[0] != op._weights_key(), 'another type: other weights'
+
+
+def test_containers_are_rebuilt_through_their_checks():
+    import copy
+    q = ops.Mx8(torch.arange(64, dtype=torch.int8), torch.full((2,), 120, dtype=torch.uint8), (4, 16), ops.ST_BF16)
+    t = copy.deepcopy(q)
+    assert torch.equal(t.codes, q.codes) and torch.equal(t.scales, q.scales) and (t.shape, t.kind, t.get_device()) == ((4, 16), ops.ST_BF16, -1)
