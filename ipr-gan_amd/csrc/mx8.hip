@@ -305,6 +305,20 @@ struct NormArgs {
   float slope;
 };
 
+// A thread's sums over the rows it walks are fp32 for 64 chunks (256 rows) at a time, then added to a 64-bit sum in its own place in LDS: a
+// chain of rounded additions has 256 links however long the tensor (an InstanceNorm of many groups leaves a group to one block: thousands of
+// rows a thread).  In registers the wide sums cost the loop its fourth block a CU: 104 us for the reduction over 256x64x64x128 bf16 instead of 92.
+constexpr int FOLD = 64;
+template <int V>
+__device__ __forceinline__ void fold(double* mine, float* s, bool first) {
+  asm volatile("" ::: "memory");       // (left to itself the compiler keeps them in registers over the loop)
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    mine[k] = first ? (double)s[k] : mine[k] + (double)s[k];
+    s[k] = 0.f;
+  }
+}
+
 // ACT: 0 none, 1 mask with a slope (ReLU: slope 0), 2 the same plus the slope gradient (PReLU)
 template <int SG, int V, int ACT>
 __global__ __launch_bounds__(256) void mx8_norm_reduce_kernel(const NormArgs a) {
@@ -314,7 +328,7 @@ __global__ __launch_bounds__(256) void mx8_norm_reduce_kernel(const NormArgs a) 
   const int c = (blockIdx.y * TC + tc) * V;
   const bool ok = c < C && tr < TR;
   const size_t gofs = (size_t)grp * a.M * C;
-  __shared__ float sh[2][256][V + 1];
+  __shared__ double sh[2][256][V + 1];
   float s1[V], s2[V];
   double s3 = 0.;                                        // the slope's gradient is ONE sum over the whole tensor, often much smaller than its
                                                          // terms: two fused multiply-adds an element in 64 bits, free beside the loads
@@ -352,34 +366,35 @@ __global__ __launch_bounds__(256) void mx8_norm_reduce_kernel(const NormArgs a) 
         s2[k] += dz * t;
       }
     };
-    for (int r0 = blockIdx.x * 4 * TR; r0 < a.M; r0 += gridDim.x * 4 * TR) {
-      const int r = r0 + tr;
-      if (r0 + 4 * TR <= a.M) {                          // four rows in flight
-        float x[4][V], g[4][V], st[4];
+    const int start = blockIdx.x * 4 * TR, step = gridDim.x * 4 * TR;      // (every block has a chunk)
+#pragma unroll 1
+    for (int lo = start; lo < a.M; lo += FOLD * step) {
+      for (int r0 = lo; r0 < min(a.M, lo + FOLD * step); r0 += step) {
+        const int r = r0 + tr;
+        if (r0 + 4 * TR <= a.M) {                          // four rows in flight
+          float x[4][V], g[4][V], st[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const size_t e = gofs + (size_t)(r + u * TR) * C + c;
-          ldcodes<V>(a.q, e, x[u]);
-          st[u] = mx8_step(a.scales[e >> 5]);
-          ldv<SG, V>(a.dy, e, a.dyps, g[u]);
-        }
+          for (int u = 0; u < 4; ++u) {
+            const size_t e = gofs + (size_t)(r + u * TR) * C + c;
+            ldcodes<V>(a.q, e, x[u]);
+            st[u] = mx8_step(a.scales[e >> 5]);
+            ldv<SG, V>(a.dy, e, a.dyps, g[u]);
+          }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) accumulate(x[u], st[u], g[u]);
-      } else {
-        for (int q = r; q < a.M; q += TR) {
-          float x[V], g[V];
-          const size_t e = gofs + (size_t)q * C + c;
-          ldcodes<V>(a.q, e, x);
-          ldv<SG, V>(a.dy, e, a.dyps, g);
-          accumulate(x, mx8_step(a.scales[e >> 5]), g);
+          for (int u = 0; u < 4; ++u) accumulate(x[u], st[u], g[u]);
+        } else {
+          for (int q = r; q < a.M; q += TR) {
+            float x[V], g[V];
+            const size_t e = gofs + (size_t)q * C + c;
+            ldcodes<V>(a.q, e, x);
+            ldv<SG, V>(a.dy, e, a.dyps, g);
+            accumulate(x, mx8_step(a.scales[e >> 5]), g);
+          }
         }
       }
+      fold<V>(sh[0][threadIdx.x], s1, lo == start);
+      fold<V>(sh[1][threadIdx.x], s2, lo == start);
     }
-  }
-#pragma unroll
-  for (int k = 0; k < V; ++k) {
-    sh[0][threadIdx.x][k] = s1[k];
-    sh[1][threadIdx.x][k] = s2[k];
   }
   __shared__ double sh3[4];
   if (ACT == 2) {
@@ -466,7 +481,10 @@ __global__ __launch_bounds__(256) void mx8_norm_apply_kernel(const NormArgs a) {
   const size_t gofs = (size_t)grp * a.M * C;
   // the reduction ends at the tensor's end: walking backwards finds its last rows still in the cache
   const int chunks = (a.M + 4 * TR - 1) / (4 * TR);
-  __shared__ float sh[2][256][V + 1];
+  __shared__ union {
+    double cs[256][V + 1];
+    float g[2][256][V + 1];
+  } sh;
   __shared__ double red[256][4];
   __shared__ float tot[2 * 64 * V];
   const int W = TC * V;
@@ -507,39 +525,42 @@ __global__ __launch_bounds__(256) void mx8_norm_apply_kernel(const NormArgs a) {
       }
       stv<SD, V>(a.dx, e, a.dxps, o);
     };
-    for (int q = chunks - 1 - (int)blockIdx.x; q >= 0; q -= gridDim.x) {
-      const int r0 = q * 4 * TR, r = r0 + tr;
-      if (r0 + 4 * TR <= a.M) {
-        float x[4][V], g[4][V], st[4];
+    const int start = chunks - 1 - (int)blockIdx.x, nb = (int)gridDim.x;
+#pragma unroll 1
+    for (int hi = start; hi >= 0; hi -= FOLD * nb) {
+      for (int q = hi; q >= 0 && q > hi - FOLD * nb; q -= nb) {
+        const int r0 = q * 4 * TR, r = r0 + tr;
+        if (r0 + 4 * TR <= a.M) {
+          float x[4][V], g[4][V], st[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const size_t e = gofs + (size_t)(r + u * TR) * C + c;
-          ldcodes<V>(a.q, e, x[u]);
-          st[u] = mx8_step(a.scales[e >> 5]);
-          ldv<SG, V>(a.dy, e, a.dyps, g[u]);
-        }
+          for (int u = 0; u < 4; ++u) {
+            const size_t e = gofs + (size_t)(r + u * TR) * C + c;
+            ldcodes<V>(a.q, e, x[u]);
+            st[u] = mx8_step(a.scales[e >> 5]);
+            ldv<SG, V>(a.dy, e, a.dyps, g[u]);
+          }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) body(gofs + (size_t)(r + u * TR) * C + c, x[u], st[u], g[u]);
-      } else {
-        for (int z = r; z < a.M; z += TR) {
-          float x[V], g[V];
-          const size_t e = gofs + (size_t)z * C + c;
-          ldcodes<V>(a.q, e, x);
-          ldv<SG, V>(a.dy, e, a.dyps, g);
-          body(e, x, mx8_step(a.scales[e >> 5]), g);
+          for (int u = 0; u < 4; ++u) body(gofs + (size_t)(r + u * TR) * C + c, x[u], st[u], g[u]);
+        } else {
+          for (int z = r; z < a.M; z += TR) {
+            float x[V], g[V];
+            const size_t e = gofs + (size_t)z * C + c;
+            ldcodes<V>(a.q, e, x);
+            ldv<SG, V>(a.dy, e, a.dyps, g);
+            body(e, x, mx8_step(a.scales[e >> 5]), g);
+          }
         }
       }
+      if (a.colpart) fold<V>(sh.cs[threadIdx.x], cs, hi == start);
     }
   }
   if (a.colpart) {                                     // column sums of dx: [row of blocks][2][C], as iprgan_colsum_partials reads them
-#pragma unroll
-    for (int k = 0; k < V; ++k) sh[0][threadIdx.x][k] = cs[k];
     __syncthreads();
     for (int ch = threadIdx.x; ch < W; ch += 256) {
       const int col = ch / V, k = ch - col * V;
       if (blockIdx.y * W + ch >= C) continue;
       double s = 0.;
-      for (int i = 0; i < TR; ++i) s += sh[0][i * TC + col][k];
+      for (int i = 0; i < TR; ++i) s += sh.cs[i * TC + col][k];
       a.colpart[((size_t)grp * gridDim.x + blockIdx.x) * 2 * C + blockIdx.y * W + ch] = (float)s;
     }
     __syncthreads();
@@ -557,9 +578,9 @@ __global__ __launch_bounds__(256) void mx8_norm_apply_kernel(const NormArgs a) {
       a.dbeta[cc] = tot[ch];
     }
   } else if (a.dgamma) {
-    float d1[V], d2[V];
+    double d1[V], d2[V];
 #pragma unroll
-    for (int k = 0; k < V; ++k) d1[k] = d2[k] = 0.f;
+    for (int k = 0; k < V; ++k) d1[k] = d2[k] = 0.;
     if (ok) {
       for (int g = tr; g < a.G; g += TR) {
         float t1[V], t2[V];
@@ -569,14 +590,15 @@ __global__ __launch_bounds__(256) void mx8_norm_apply_kernel(const NormArgs a) {
         for (int k = 0; k < V; ++k) { d1[k] += t1[k]; d2[k] += t2[k]; }
       }
     }
+    __syncthreads();
 #pragma unroll
-    for (int k = 0; k < V; ++k) { sh[0][threadIdx.x][k] = d1[k]; sh[1][threadIdx.x][k] = d2[k]; }
+    for (int k = 0; k < V; ++k) { sh.g[0][threadIdx.x][k] = (float)d1[k]; sh.g[1][threadIdx.x][k] = (float)d2[k]; }
     __syncthreads();
     for (int ch = threadIdx.x; ch < W; ch += 256) {
       const int col = ch / V, k = ch - col * V, cc = blockIdx.y * W + ch;
       if (cc >= C) continue;
       double b = 0., g = 0.;
-      for (int i = 0; i < TR; ++i) { b += sh[0][i * TC + col][k]; g += sh[1][i * TC + col][k]; }
+      for (int i = 0; i < TR; ++i) { b += sh.g[0][i * TC + col][k]; g += sh.g[1][i * TC + col][k]; }
       a.dgamma[cc] = (float)g;
       a.dbeta[cc] = (float)b;
     }

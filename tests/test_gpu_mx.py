@@ -646,3 +646,37 @@ def test_more_than_a_million_rows(dev, M):
         want += dy[:, n:n + 1] * wt[n].to(dev)
     for d in (dy, dy.bfloat16()):
         assert torch.equal(ops.mx4_linear_bwd(d, w, torch.float32), want)
+
+
+@pytest.mark.parametrize('form,G,M,C', [('inst', 1024, 1 << 17, 4), ('inst', 64, 4096, 4096), ('bn', 1, 1 << 20, 2048)])
+@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+def test_norm_sums_of_long_runs_of_rows(dev, form, G, M, C, dtype):
+    """Tensors of which one thread walks 256 to 1024 rows or more.  A large gradient in the first rows and ones behind it: an fp32 sum that
+    is not handed on to a wider one in time drops every one of them (a thousand of them: 2^-14 of the sum).  A sum in 64 bits of fp32 sums of
+    256 rows is off by 256 half steps of the magnitudes, by 4 more for the stored partial sums and the result; every term here is exact.  The
+    column sums of dx: gamma = invstd = 1, s1 / M and s2 / M the rounded sums, 8 roundings a dx, 256 + 4 of the sum."""
+    from iprgan import ops
+    n = G * M * C
+    codes = torch.full((n,), 1, dtype=torch.int8, device=dev)
+    scales = torch.full((n // 32,), 127, dtype=torch.uint8, device=dev)
+    dy = torch.ones(G, M, 1, C, dtype=torch.float32 if dtype == 'f32' else torch.bfloat16, device=dev)
+    dy[:, :256] = 2.0 ** 24
+    mean, inv, gamma, beta = torch.zeros(G, C, device=dev), torch.ones(G, C, device=dev), torch.ones(C, device=dev), torch.ones(C, device=dev)
+    q = ops.Mx8(codes, scales, dy.shape)
+    db = torch.zeros(C, device=dev)
+    f = (lambda *a, **k: ops.bn_bwd(*a[:4], a[4].view(C), a[5].view(C), *a[6:], **k)) if form == 'bn' else ops.instnorm_bwd
+    dx, dgamma, dbeta = f(q, None, dy, gamma, mean, inv, 1, beta=beta, dbias=db)
+    one = 256 * 2.0 ** 24 + (M - 256)                                      # a group's sum; x = 1: both sums are the same
+    u = 2.0 ** -24
+    for got in (dgamma, dbeta):
+        assert float((got.double() - G * one).abs().max()) <= (256 + 4) * u * G * one
+    s = torch.tensor(one).float().double()
+    want = dx.double().sum((0, 1, 2)) if dtype == 'f32' else None
+    if want is not None:                                                    # (bf16: dx is rounded again behind the sum)
+        mag = dx.double().abs().sum((0, 1, 2))
+        assert bool(((db.double() - want).abs() <= (256 + 4) * u * mag).all())
+    big, rest = (2.0 ** 24 - 2 * float(s) / M), (1 - 2 * float(s) / M)
+    tol = u * 264 * (2.0 ** 24 + 2 * float(s) / M) + (2.0 ** -8 * 2.0 ** 24 if dtype == 'bf16' else 0)
+    assert float((dx[:, :256].double() - big).abs().max()) <= tol
+    tol = u * 264 * (1 + 2 * float(s) / M) + (2.0 ** -8 * abs(rest) if dtype == 'bf16' else 0)
+    assert float((dx[:, 256:].double() - rest).abs().max()) <= tol
