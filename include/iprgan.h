@@ -487,7 +487,10 @@ int iprgan_tune_import(const int* records, size_t n_records, int replace);
  * [-127, 121]; code = rint(x * 2^-e) (ties to even), scale byte = e + 127, value = code * 2^e.  Off by at most half a step
  * 2^(e-1) <= m / 127.5 (above 127.5 * 2^121 an element saturates: less than one step).  A block that holds a NaN or an infinity
  * stores scale byte 255 and reads back as NaN.  codes: n bytes, 16-byte aligned; scales: ceil(n / 32) bytes.
- * kind / pstride: storage kind of the tensor (IPRGAN_ST_F32 / _BF16 / _X3) and plane stride of a three-plane one (0 = n). */
+ * kind / pstride: storage kind of the tensor (IPRGAN_ST_F32 / _BF16 / _X3) and plane stride of a three-plane one (0 = n).
+ * iprgan_mx8_quant: kind | IPRGAN_MX8_SIGNS for a tensor that is read as a mask (x > 0: the output of a ReLU or LeakyReLU, the input of a
+ * PReLU): a positive element below half a step is stored as code 1 instead of 0 (off by less than one step), so that value > 0 where x > 0. */
+enum { IPRGAN_MX8_SIGNS = 16 };
 int iprgan_mx8_quant(const void* x, void* codes, void* scales, size_t n, int kind, size_t pstride, void* stream);
 int iprgan_mx8_dequant(const void* codes, const void* scales, void* y, size_t n, int kind, size_t pstride, void* stream);
 /* dz = dy * act'(out), out read from its checkpoint (iprgan_act_bwd; dy and dz fp32 or bf16) */

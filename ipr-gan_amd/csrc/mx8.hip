@@ -7,7 +7,8 @@
 // e is the smallest exponent for which nothing rounds past 127, so every element is off by at most half a step (2^(e-1), at most
 // m / 127.5); x * 2^-e is exact, which leaves ONE rounding.  The cap keeps 127 * 2^e finite: only above 127.5 * 2^121 =
 // 3.39e38 does an element saturate (off by less than one step).  A block with a NaN or an infinity stores scale byte 255 and reads back
-// as NaN: a diverged run stays non-finite.  Why int8 and a power of two: at 1.03 bytes an element the noise is 43 dB under a
+// as NaN: a diverged run stays non-finite.  What is rounded to zero loses its sign, and with it the mask of a ReLU or LeakyReLU that is read off the
+// checkpoint: IPRGAN_MX8_SIGNS keeps it (mx8_code), at the price of an error below one step instead of half a step for those elements.  Why int8 and a power of two: at 1.03 bytes an element the noise is 43 dB under a
 // normally distributed signal (an 8-bit float's 3-bit mantissa: 31 dB), and the scale costs no multiplication error.
 #include "common.h"
 
@@ -122,12 +123,17 @@ __device__ __forceinline__ float mx8_step(unsigned s) {
   return __uint_as_float(s == 0 ? 0x00400000u : s == 255u ? 0x7fc00000u : s << 23);
 }
 // int8 code in the low byte: adding 1.5 * 2^23 rounds to an integer, ties to even; the clamp acts above 127.5 * 2^121 only
+// SIGNS: a positive value is never stored as zero but as one step at least - what reads x > 0 off the codes reads it off x.  (A negative one may
+// still be stored as zero: neither is positive.)
+template <bool SIGNS>
 __device__ __forceinline__ unsigned mx8_code(float x, float inv) {
-  const float t = fminf(fmaxf(x * inv, -127.f), 127.f);
+  float t = fminf(fmaxf(x * inv, -127.f), 127.f);
+  if (SIGNS) t = x > 0.f ? fmaxf(t, 1.f) : t;
   return __float_as_uint(t + 12582912.f) & 0xffu;
 }
+template <bool SIGNS>
 __device__ __forceinline__ unsigned pack4(const float* v, float inv) {
-  return mx8_code(v[0], inv) | mx8_code(v[1], inv) << 8 | mx8_code(v[2], inv) << 16 | mx8_code(v[3], inv) << 24;
+  return mx8_code<SIGNS>(v[0], inv) | mx8_code<SIGNS>(v[1], inv) << 8 | mx8_code<SIGNS>(v[2], inv) << 16 | mx8_code<SIGNS>(v[3], inv) << 24;
 }
 template <int V>
 __device__ __forceinline__ void ldcodes(const int8_t* q, size_t e, float* v) {          // codes as floats, not yet scaled
@@ -145,7 +151,7 @@ __device__ __forceinline__ void ldcodes(const int8_t* q, size_t e, float* v) {  
 // Quantise: a thread owns V consecutive elements, 32 / V neighbouring lanes share a block and its maximum.  n is the element count;
 // lanes past the end contribute zeros.  Bound by HBM (reads sizeof(x), writes 1 + 1/32 bytes an element): 256x128x128x64 bf16 156 us = 5.2
 // TB/s, the rate of a copy; two or four pieces in flight a thread are slower (173, 179 us).
-template <int ST, int V>
+template <int ST, int V, bool SIGNS>
 __global__ __launch_bounds__(256) void mx8_quant_kernel(const void* __restrict__ x, int8_t* __restrict__ q,
                                                         uint8_t* __restrict__ scales, size_t n, size_t ps) {
   constexpr int L = 32 / V;                     // lanes of a block
@@ -179,14 +185,14 @@ __global__ __launch_bounds__(256) void mx8_quant_kernel(const void* __restrict__
     const float inv = s == 255u ? 1.f : mx8_inv(s);
     if (full) {
       if constexpr (V == 8) {
-        *(uint2*)(q + e) = make_uint2(pack4(v, inv), pack4(v + 4, inv));
+        *(uint2*)(q + e) = make_uint2(pack4<SIGNS>(v, inv), pack4<SIGNS>(v + 4, inv));
       } else {
-        *(unsigned*)(q + e) = pack4(v, inv);
+        *(unsigned*)(q + e) = pack4<SIGNS>(v, inv);
       }
     } else {
 #pragma unroll
       for (int k = 0; k < V; ++k)
-        if (e + k < n) q[e + k] = (int8_t)mx8_code(v[k], inv);
+        if (e + k < n) q[e + k] = (int8_t)mx8_code<SIGNS>(v[k], inv);
     }
     if ((threadIdx.x & (L - 1)) == 0 && e < n) scales[e >> 5] = (uint8_t)s;
   }
@@ -654,6 +660,8 @@ extern "C" {
 int iprgan_mx8_quant(const void* x, void* codes, void* scales, size_t n, int kind, size_t pstride, void* stream) {
   IPR_CHECK(n > 0, "mx8_quant: empty input");
   IPR_CHECK(x && codes && scales, "mx8_quant: null operand");
+  const bool signs = kind & IPRGAN_MX8_SIGNS;
+  kind &= ~IPRGAN_MX8_SIGNS;
   IPR_CHECK(kind >= IPRGAN_ST_F32 && kind <= IPRGAN_ST_X3, "mx8_quant: storage kind %d", kind);
   IPR_CHECK((kind == IPRGAN_ST_F32 ? al16(x) : al8(x)) && al16(codes), "mx8_quant: operands must be 16-byte aligned (8: bf16 and three planes)");
   if (kind == IPRGAN_ST_X3 && !pstride) pstride = n;
@@ -661,8 +669,9 @@ int iprgan_mx8_quant(const void* x, void* codes, void* scales, size_t n, int kin
   hipStream_t st = (hipStream_t)stream;
   const bool wide = kind != IPRGAN_ST_F32 && al16(x) && (kind != IPRGAN_ST_X3 || pstride % 8 == 0);
   IPR_CHECK(kind != IPRGAN_ST_X3 || pstride % 4 == 0, "mx8_quant: plane stride %zu is not a multiple of 4", pstride);
-  auto k = kind == IPRGAN_ST_F32 ? mx8_quant_kernel<0, 4> : kind == IPRGAN_ST_BF16 ? (wide ? mx8_quant_kernel<1, 8> : mx8_quant_kernel<1, 4>)
-           : wide ? mx8_quant_kernel<2, 8> : mx8_quant_kernel<2, 4>;
+#define QUANT(ST, V) (signs ? mx8_quant_kernel<ST, V, true> : mx8_quant_kernel<ST, V, false>)
+  auto k = kind == IPRGAN_ST_F32 ? QUANT(0, 4) : kind == IPRGAN_ST_BF16 ? (wide ? QUANT(1, 8) : QUANT(1, 4)) : wide ? QUANT(2, 8) : QUANT(2, 4);
+#undef QUANT
   hipLaunchKernelGGL(k, dim3(flat_grid(n, wide ? 8 : 4)), dim3(256), 0, st, x, (int8_t*)codes, (uint8_t*)scales, n, pstride);
   IPR_LAUNCH_CHECK();
   return 0;

@@ -49,11 +49,12 @@ class Config(object):
 #     pair_d: true           # D(real) and D(fake) as one paired pass              (IPRGAN_PAIR_D)
 #     batch_passes: true     # same-network passes of CycleGAN batched             (IPRGAN_BATCH_PASSES)
 #     ckpt8: true            # activations kept for the backward pass in 8 bits       (IPRGAN_CKPT8)
+#     ckpt8_signs: true      # ... masks (x > 0) kept exact through the rounding; as ckpt8 unless set  (IPRGAN_CKPT8_SIGNS)
 #     graph: true            # ImageGeneration: the whole step as one captured HIP graph (graphs.py); one rank only, unless
 #     graph_ddp: true        #   ... this opts a data-parallel run in (the exchange through the C ABI's communicator is captured
 #                            #   with the step; every rank captures or every rank stays eager; unproven on real multi-GPU RCCL)
 ENGINE_KEYS = ('math', 'bucket_mb', 'comm', 'comm_timeout', 'tune_cache', 'fuse_stats', 'pair_d', 'batch_passes', 'graph',
-               'graph_ddp', 'ckpt8')
+               'graph_ddp', 'ckpt8', 'ckpt8_signs')
 
 
 def apply_engine(config, set_math=True):
@@ -84,8 +85,11 @@ def apply_engine(config, set_math=True):
     for key, env, mod, attr in (('fuse_stats', 'IPRGAN_FUSE_STATS', _engine, '_FUSE_STATS'),
                                 ('pair_d', 'IPRGAN_PAIR_D', _models, '_PAIR_D'),
                                 ('batch_passes', 'IPRGAN_BATCH_PASSES', _models, '_BATCH_PASSES'),
-                                ('ckpt8', 'IPRGAN_CKPT8', _engine, '_CKPT8')):
+                                ('ckpt8', 'IPRGAN_CKPT8', _engine, '_CKPT8'),
+                                ('ckpt8_signs', 'IPRGAN_CKPT8_SIGNS', _engine, '_CKPT8_SIGNS')):
         if key in blk:
             os.environ[env] = '1' if blk[key] else '0'
             setattr(mod, attr, bool(blk[key]))
+    if 'ckpt8' in blk and 'ckpt8_signs' not in blk:
+        _engine._CKPT8_SIGNS = os.environ.get('IPRGAN_CKPT8_SIGNS', os.environ['IPRGAN_CKPT8']) == '1'
     return blk

@@ -30,6 +30,11 @@ _GEMV_PAIR = os.environ.get('IPRGAN_GEMV_PAIR', '1') != '0'        # A/B switch:
 # the stand-alone activations' backward passes read the codes; the other ops get the tensor back for the time of their own backward.
 # The forward pass is untouched; gradients see activations rounded to 1/127 of their block's maximum.
 _CKPT8 = os.environ.get('IPRGAN_CKPT8', '0') == '1'
+# ... and masks that are those of the activations: what is rounded to zero would count as not positive, so a tensor that is read as a mask (outputs
+# of a convolution or dense layer with ReLU / LeakyReLU, inputs of a PReLU) is stored with no positive element rounded to zero.  Without it
+# (`ckpt8_signs: false`) about 1 % of a ReLU's positive elements lose their gradient, always in that direction, and a channel 250 times
+# smaller than the largest of its 32 neighbours loses all of it.  Unless set, it goes with ckpt8.
+_CKPT8_SIGNS = os.environ.get('IPRGAN_CKPT8_SIGNS', os.environ.get('IPRGAN_CKPT8', '0')) == '1'
 _CKPT8_MIN = 1 << 14        # elements: a smaller tensor stays as it is (64 KB are not worth two launches)
 
 
@@ -757,6 +762,11 @@ class Chain:
         return ChainFn.apply(self, (bool(train), red, bool(pair), _CKPT8 and torch.is_grad_enabled()), x, *params)
 
 
+def _is_mask(op):
+    """The derivative of the activation behind ``op`` is read off the sign of its output."""
+    return op.out_act[0] in (L.ACT_RELU, L.ACT_LRELU)
+
+
 def _pack_saved(ops_list, stash, i, last):
     """ckpt8: the tensors that ops up to ``i`` saved and the forward pass has finished with -> Mx8.  The output of an op and the input
     of the next are one tensor: packed once, when its consumer is done.  A max pool keeps its input (and with it that output) exact: its
@@ -764,23 +774,26 @@ def _pack_saved(ops_list, stash, i, last):
     st = stash[i]
     x = st.get('x')
     if isinstance(x, torch.Tensor) and x.numel() >= _CKPT8_MIN:
-        keep = isinstance(ops_list[i], MaxPool2)
-        q = None if keep else ops.mx8_quant(x)
-        for j in range(i - 1, -1, -1):                 # the producer (views in between hand its storage on)
+        made = None                                    # the producer (views in between hand its storage on)
+        for j in range(i - 1, -1, -1):
             y = stash[j].get('y')
             if isinstance(y, torch.Tensor):
                 if y.data_ptr() == x.data_ptr() and y.numel() == x.numel() and y.dtype == x.dtype:
-                    stash[j]['y'] = y if keep else q.view(y.shape)
+                    made = j
                 break
-        if not keep:
+        if not isinstance(ops_list[i], MaxPool2):
+            q = ops.mx8_quant(x, _CKPT8_SIGNS and (isinstance(ops_list[i], (PReLU, PixelShufflePReLU))
+                                                   or (made is not None and _is_mask(ops_list[made]))))
             st['x'] = q
+            if made is not None:
+                stash[made]['y'] = q.view(stash[made]['y'].shape)
     y = st.get('y')
     if isinstance(y, torch.Tensor):
         op = ops_list[i]
         if isinstance(op, (BatchNorm, InstanceNorm)) or (isinstance(op, Conv) and op.spec.act == L.ACT_NONE):
             st['y'] = None                             # (its backward pass does not read the output)
         elif last and y.numel() >= _CKPT8_MIN:
-            st['y'] = ops.mx8_quant(y)
+            st['y'] = ops.mx8_quant(y, _CKPT8_SIGNS and _is_mask(op))
 
 
 def _unpack_saved(op, st, need_x):

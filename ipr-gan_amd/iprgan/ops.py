@@ -320,8 +320,12 @@ class Mx8(_Packed):
         return q
 
 
-def mx8_quant(x):
-    """``x`` (any storage kind) saved in 8 bits."""
+MX8_SIGNS = 16      # include/iprgan.h: IPRGAN_MX8_SIGNS
+
+
+def mx8_quant(x, signs=False):
+    """``x`` (any storage kind) saved in 8 bits.  ``signs``: for a tensor that is read as a mask (x > 0): no positive element is rounded to
+    zero, those below half a step are stored as one step."""
     _one_device('mx8_quant', x)
     keep = []
     p, n, k = _vptr(x, keep), x.numel(), is16(x)
@@ -333,7 +337,7 @@ def mx8_quant(x):
     c = buf.data_ptr()
     if L._acct is not None:
         L._acct_note(buf)
-    call('iprgan_mx8_quant', p, c, c + split, n, k, pstride(x) if k == ST_X3 else 0, stream())
+    call('iprgan_mx8_quant', p, c, c + split, n, k | MX8_SIGNS if signs else k, pstride(x) if k == ST_X3 else 0, stream())
     return q
 
 

@@ -76,3 +76,11 @@ def act(v, kind, slope):
     if kind == 4:
         return torch.sigmoid(v) * 2 - 1
     return v
+
+
+def mx8_encode_signs(x):
+    """mx8_encode with no positive element rounded to zero (a block that holds a NaN or an infinity: all zero codes, as there)."""
+    codes, s = mx8_encode(x)
+    v = x.detach().cpu().double().reshape(-1)
+    lost = (v > 0) & (codes == 0) & (s.repeat_interleave(32)[:v.numel()] != 255)
+    return torch.where(lost, torch.ones_like(codes), codes), s

@@ -680,3 +680,30 @@ def test_norm_sums_of_long_runs_of_rows(dev, form, G, M, C, dtype):
     assert float((dx[:, :256].double() - big).abs().max()) <= tol
     tol = u * 264 * (1 + 2 * float(s) / M) + (2.0 ** -8 * abs(rest) if dtype == 'bf16' else 0)
     assert float((dx[:, 256:].double() - rest).abs().max()) <= tol
+
+
+@pytest.mark.parametrize('kind,n', [(k, n) for k in ('f32', 'bf16') for n in (1, 31, 32, 33, 1000, 40001)] + [('x3', 32), ('x3', 1000), ('x3', 40004)])
+def test_mx8_signs(dev, kind, n, request):
+    """Codes, scales and values as stated; value > 0 exactly where x > 0; act_bwd's mask is that of x."""
+    from iprgan import ops
+    x = awkward(n, n)
+    x[n // 2] = 1e-45                                            # the smallest subnormal beside whatever its block holds
+    if kind == 'x3':
+        request.getfixturevalue('x3_mode')
+        x = (rnd(n, seed=n) * torch.exp2(-8 * rnd(n, seed=n + 1).abs())).clamp(-4, 4)
+        t = ops.to_kind(x.to(dev), ops.ST_X3)
+    else:
+        x = x if kind == 'f32' else x.bfloat16()
+        t = x.to(dev)
+    q = ops.mx8_quant(t, signs=True)
+    codes, scales = R.mx8_encode_signs(x)
+    assert torch.equal(q.scales.cpu(), scales) and torch.equal(q.codes.cpu(), codes)
+    f = ops.mx8_dequant(q, ops.ST_F32).cpu()
+    assert same(f, R.mx8_decode(codes, scales))
+    fine = scales.repeat_interleave(32)[:n] != 255
+    assert torch.equal((f > 0)[fine], (x > 0)[fine])
+    back = ops.mx8_dequant(q)
+    assert torch.equal((ops.f32(back) > 0).cpu()[fine], (x > 0)[fine])
+    dy = rnd(n, seed=3)
+    dz = ops.act_bwd(dy.to(dev), q, 1).cpu()
+    assert torch.equal(dz[fine], torch.where(x > 0, dy, torch.zeros(n))[fine])

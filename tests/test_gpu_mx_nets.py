@@ -293,3 +293,165 @@ def test_a_copied_or_moved_generator_is_served_as_before(dev):
         net.cpu().to(dev)
         with pytest.raises(RuntimeError, match='out of date'):
             net(z)
+
+
+def test_a_small_channel_keeps_its_gradient(dev, ckpt8, monkeypatch):
+    """conv + LeakyReLU -> conv, the channels of the first scaled over three decades, in blocks of 32: with `engine: {ckpt8: true}` the masks
+    are those of the activations, so the first convolution's gradients, channel by channel, are those of the exact pass but for the
+    rounding of its input: sum |g| |x - x8|, written out below, and 2^-14 of the magnitudes for the fp32 arithmetic, 288 + 512 roundings
+    in a row at most, each half a step.  Of the second's gradients a channel's are off by at most a step of its blocks."""
+    from iprgan import _lib as L, configs, engine as E
+    from iprgan.ops import ConvSpec
+    torch.manual_seed(9)
+    c1, c2 = nn.Conv2d(4, 64, 3, 1, 1), nn.Conv2d(64, 32, 3, 1, 1)
+    s = torch.logspace(0, -3, 64)[torch.randperm(64, generator=torch.Generator().manual_seed(1))]
+    with torch.no_grad():
+        c1.weight.mul_(s.view(-1, 1, 1, 1))
+        c1.bias.mul_(s)
+        c2.weight.div_(s.view(1, -1, 1, 1))                      # every channel matters to the second layer
+    x, r = torch.randn(2, 4, 16, 16), torch.randn(2, 32, 16, 16)
+    d = lambda t: t.detach().double()
+    F = nn.functional
+    a1 = F.leaky_relu(F.conv2d(d(x), d(c1.weight), d(c1.bias), padding=1), 0.2)
+    dy = d(r)
+    g1 = nn.grad.conv2d_input(a1.shape, d(c2.weight), dy, padding=1) * torch.where(a1 > 0, 1.0, 0.2)
+    mag = nn.grad.conv2d_input(a1.shape, d(c2.weight).abs(), dy.abs(), padding=1)
+    wantw, wantb = nn.grad.conv2d_weight(d(x), c1.weight.shape, g1, padding=1), g1.sum((0, 2, 3))
+    x8 = round8(d(x))
+    tolw = nn.grad.conv2d_weight((d(x) - x8).abs(), c1.weight.shape, g1.abs(), padding=1)
+    tolw = tolw + 2.0 ** -14 * nn.grad.conv2d_weight(d(x).abs(), c1.weight.shape, mag, padding=1)
+    tolb = 2.0 ** -14 * mag.sum((0, 2, 3))
+    p = a1.permute(0, 2, 3, 1).reshape(-1, 32)
+    _, sc = R.mx8_encode(p.float())
+    step = torch.exp2(sc.double() - 127).repeat_interleave(32).view(2, 16, 16, 64).permute(0, 3, 1, 2)
+    want2 = nn.grad.conv2d_weight(a1, c2.weight.shape, dy, padding=1)
+    tol2 = nn.grad.conv2d_weight(step, c2.weight.shape, dy.abs(), padding=1) + 2.0 ** -14 * nn.grad.conv2d_weight(a1.abs(), c2.weight.shape, dy.abs(), padding=1)
+    c1.to(dev), c2.to(dev)
+    plan = [E.ToNHWC(4), E.Conv(ConvSpec(4, 64, 3, 1, 1, act=L.ACT_LRELU, slope=0.2), c1), E.Conv(ConvSpec(64, 32, 3, 1, 1), c2), E.ToNCHW(32)]
+    for k in ('IPRGAN_CKPT8', 'IPRGAN_CKPT8_SIGNS'):             # (put back, with the module's switches, when the test ends)
+        monkeypatch.setenv(k, '0')
+    monkeypatch.delenv('IPRGAN_CKPT8_SIGNS')
+    monkeypatch.setattr(E, '_CKPT8_SIGNS', False)
+    ckpt8(False)
+    configs.apply_engine({'engine': {'ckpt8': True}}, set_math=False)
+    assert E._CKPT8 and E._CKPT8_SIGNS
+    (E.Chain(plan)(x.to(dev), True) * r.to(dev)).sum().backward()
+    for got, want, tol in ((c1.weight.grad, wantw, tolw), (c1.bias.grad, wantb, tolb), (c2.weight.grad, want2, tol2)):
+        err = (got.cpu().double() - want).abs()
+        assert bool((err <= tol).all()), float((err / tol).max())
+
+
+@pytest.mark.parametrize('name,math', [('SNDiscriminator32', 'fp32'), ('SNDiscriminator32', 'fp32x3'), ('SNDiscriminator32', 'bf16act'),
+                                       ('VGG19Feature', 'fp32'), ('VGG19Feature', 'fp32x3')], indirect=['math'])
+@pytest.mark.parametrize('least', [1, None])
+def test_data_gradients_without_norm_layers_are_those_of_the_plain_pass(dev, ckpt8, monkeypatch, name, math, least):
+    """Where every mask is read off an output and no layer's data gradient reads its input, a checkpoint with exact masks changes weight gradients
+    only: the input's and the biases' are bit-identical, with every tensor packed and with the default threshold (some packed, some not).
+    A weight gradient is off by the rounding of its layer's input: at most half a step of a block, m / 127.5 of its maximum m, a third of that on
+    average, where the values' average is m / 4 and more: 2 % of a tensor's gradient if it is as incoherent as the rounding; 5 % granted."""
+    from iprgan import engine, networks
+    if least is None:
+        monkeypatch.setattr(engine, '_CKPT8_MIN', 1 << 14)
+    monkeypatch.setattr(engine, '_CKPT8_SIGNS', True)
+    torch.manual_seed(5)
+    net = getattr(networks, name)().to(dev)
+    net.train()
+    state = {k: v.clone() for k, v in net.state_dict().items()}
+    x = torch.randn(SHAPES[name], generator=torch.Generator().manual_seed(1)).to(dev)
+    res = []
+    for on in (False, True):
+        net.load_state_dict(state)
+        ckpt8(on)
+        xin = x.clone().requires_grad_(True)
+        for p in net.parameters():
+            p.grad = None
+        y = net(xin)
+        r = torch.randn(y.shape, generator=torch.Generator().manual_seed(2)).to(dev)
+        (y * r).sum().backward()
+        res.append({'x': xin.grad, **{k: p.grad for k, p in net.named_parameters() if p.grad is not None}})
+    moved = 0
+    for k, a in res[0].items():
+        b = res[1][k]
+        if k == 'x' or k.endswith('bias'):
+            assert torch.equal(a, b), k
+        else:
+            moved += not torch.equal(a, b)
+            assert float((a - b).norm()) <= 0.05 * float(a.norm()), k
+    assert moved > 0 or len(res[0]) == 1, 'the checkpoints were not used'
+
+
+def test_chain_of_packed_and_plain_tensors(dev, ckpt8, monkeypatch):
+    """The default threshold in the middle of a chain: conv + LeakyReLU (16 384 elements: packed, masks kept) -> conv -> BatchNorm + ReLU (8 192: its
+    input stays, its output is dropped all the same) -> conv, written out in float64.  Bounds as in the chain test above."""
+    from iprgan import _lib as L, engine as E
+    from iprgan.ops import ConvSpec
+    torch.manual_seed(3)
+    c1, c2, bn, c3 = nn.Conv2d(3, 32, 3, 1, 1), nn.Conv2d(32, 16, 3, 1, 1), nn.BatchNorm2d(16), nn.Conv2d(16, 8, 3, 1, 1)
+    with torch.no_grad():
+        bn.weight.normal_(1, 0.2)
+        bn.bias.normal_(0, 0.2)
+    x, r = torch.randn(2, 3, 16, 16), torch.randn(2, 8, 16, 16)
+    d = lambda t: t.detach().double()
+    F = nn.functional
+    a1 = F.leaky_relu(F.conv2d(d(x), d(c1.weight), d(c1.bias), padding=1), 0.2)
+    p = a1.permute(0, 2, 3, 1).contiguous()
+    a1q = R.mx8_decode(*R.mx8_encode_signs(p.float())).view(p.shape).permute(0, 3, 1, 2).contiguous()
+    a2 = F.conv2d(a1, d(c2.weight), d(c2.bias), padding=1)
+    inv = 1 / torch.sqrt(a2.var((0, 2, 3), unbiased=False, keepdim=True) + bn.eps)
+    t = (a2 - a2.mean((0, 2, 3), keepdim=True)) * inv
+    g, b = d(bn.weight).view(1, -1, 1, 1), d(bn.bias).view(1, -1, 1, 1)
+    a3 = F.relu(t * g + b)
+    dy = d(r)
+    want = {'c3': nn.grad.conv2d_weight(a3, c3.weight.shape, dy, padding=1)}
+    dz = torch.where(t * g + b > 0, nn.grad.conv2d_input(a3.shape, d(c3.weight), dy, padding=1), 0.0)
+    want['bn'], want['bnb'] = (dz * t).sum((0, 2, 3)), dz.sum((0, 2, 3))
+    M = 2 * 16 * 16
+    g2 = g * inv * (dz - dz.sum((0, 2, 3), keepdim=True) / M - t * (dz * t).sum((0, 2, 3), keepdim=True) / M)
+    want['c2'] = nn.grad.conv2d_weight(a1q, c2.weight.shape, g2, padding=1)
+    g1 = nn.grad.conv2d_input(a1.shape, d(c2.weight), g2, padding=1) * torch.where(a1 > 0, 1.0, 0.2)
+    want['c1'], want['c1b'] = nn.grad.conv2d_weight(d(x), c1.weight.shape, g1, padding=1), g1.sum((0, 2, 3))
+    want['x'] = nn.grad.conv2d_input(x.shape, d(c1.weight), g1, padding=1)
+    for m in (c1, c2, bn, c3):
+        m.to(dev)
+    plan = [E.ToNHWC(3), E.Conv(ConvSpec(3, 32, 3, 1, 1, act=L.ACT_LRELU, slope=0.2), c1), E.Conv(ConvSpec(32, 16, 3, 1, 1), c2),
+            E.BatchNorm(bn, act=L.ACT_RELU), E.Conv(ConvSpec(16, 8, 3, 1, 1), c3), E.ToNCHW(8)]
+    ckpt8(True)
+    monkeypatch.setattr(E, '_CKPT8_MIN', 1 << 14)
+    monkeypatch.setattr(E, '_CKPT8_SIGNS', True)
+    xin = x.to(dev).requires_grad_(True)
+    (E.Chain(plan)(xin, True) * r.to(dev)).sum().backward()
+    got = {'c3': c3.weight.grad, 'bn': bn.weight.grad, 'bnb': bn.bias.grad, 'c2': c2.weight.grad, 'c1': c1.weight.grad, 'c1b': c1.bias.grad,
+           'x': xin.grad}
+    for k, v in want.items():
+        err = float((got[k].cpu().double() - v).abs().max() / v.abs().max())
+        assert err <= 2e-3, (k, err)
+
+
+@pytest.mark.parametrize('shuffle', [False, True])
+def test_prelu_masks_are_those_of_the_plain_pass(dev, ckpt8, monkeypatch, shuffle):
+    """conv -> (pixel shuffle) PReLU -> conv: the mask is read off the PReLU's input.  With exact masks the data gradient and the first convolution's
+    gradients of it are bit-identical, the slope's is off by the rounding of x: sum |dy| step over the negative half at most."""
+    from iprgan import engine as E
+    from iprgan.ops import ConvSpec
+    monkeypatch.setattr(E, '_CKPT8_SIGNS', True)
+    torch.manual_seed(11)
+    c1, pr, c2 = nn.Conv2d(4, 64, 3, 1, 1).to(dev), nn.PReLU().to(dev), nn.Conv2d(16 if shuffle else 64, 8, 3, 1, 1).to(dev)
+    plan = [E.ToNHWC(4), E.Conv(ConvSpec(4, 64, 3, 1, 1), c1), E.PixelShufflePReLU(pr) if shuffle else E.PReLU(pr),
+            E.Conv(ConvSpec(16 if shuffle else 64, 8, 3, 1, 1), c2), E.ToNCHW(8)]
+    side = 32 if shuffle else 16
+    x, r = torch.randn(2, 4, 16, 16).to(dev), torch.randn(2, 8, side, side).to(dev)
+    res = []
+    for on in (False, True):
+        ckpt8(on)
+        for m in (c1, pr, c2):
+            m.zero_grad()
+        xin = x.clone().requires_grad_(True)
+        (E.Chain(plan)(xin, True) * r).sum().backward()
+        res.append((xin.grad, c1.bias.grad, pr.weight.grad, c2.weight.grad))
+    (xa, ba, sa, wa), (xb, bb, sb, wb) = res
+    assert torch.equal(xa, xb) and torch.equal(ba, bb) and not torch.equal(wa, wb)
+    with torch.no_grad():
+        h = nn.functional.conv2d(x.double().cpu(), c1.weight.double().cpu(), c1.bias.double().cpu(), padding=1)
+        g = nn.grad.conv2d_input((2, c2.in_channels, side, side), c2.weight.double().cpu(), r.double().cpu(), padding=1)
+        bound = float(h.abs().max()) / 63.75 * float(g.abs().sum())
+    assert abs(float(sa - sb)) <= bound

@@ -224,3 +224,26 @@ def test_containers_are_rebuilt_through_their_checks():
     q = ops.Mx8(torch.arange(64, dtype=torch.int8), torch.full((2,), 120, dtype=torch.uint8), (4, 16), ops.ST_BF16)
     t = copy.deepcopy(q)
     assert torch.equal(t.codes, q.codes) and torch.equal(t.scales, q.scales) and (t.shape, t.kind, t.get_device()) == ((4, 16), ops.ST_BF16, -1)
+
+
+def test_ckpt8_signs_go_with_ckpt8_unless_set(monkeypatch):
+    import os
+    from iprgan import configs, engine
+    monkeypatch.setenv('IPRGAN_CKPT8', '0')
+    monkeypatch.delenv('IPRGAN_CKPT8_SIGNS', raising=False)
+    monkeypatch.setattr(engine, '_CKPT8', False)
+    monkeypatch.setattr(engine, '_CKPT8_SIGNS', False)
+    for blk, want in (({'ckpt8': True}, True), ({'ckpt8': False}, False), ({'graph': False}, False)):
+        configs.apply_engine({'engine': blk}, set_math=False)
+        assert engine._CKPT8_SIGNS == want and 'IPRGAN_CKPT8_SIGNS' not in os.environ
+    monkeypatch.setenv('IPRGAN_CKPT8_SIGNS', '0')
+    configs.apply_engine({'engine': {'ckpt8': True}}, set_math=False)
+    assert engine._CKPT8 and not engine._CKPT8_SIGNS
+    configs.apply_engine({'engine': {'ckpt8': True, 'ckpt8_signs': True}}, set_math=False)
+    assert engine._CKPT8_SIGNS
+
+
+def test_mx8_quant_takes_the_signs_flag_beside_a_storage_kind():
+    refused_size('iprgan_mx8_quant', P, P, P, 8, 16 | 3, 0, None)
+    refused_size('iprgan_mx8_quant', P, P, P, 8, 32, 0, None)
+    refused_size('iprgan_mx8_dequant', P, P, P, 8, 16, 0, None)
