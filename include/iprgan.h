@@ -531,6 +531,10 @@ int iprgan_mx4_linear(const void* x, const void* x_scales, const void* w_codes, 
 size_t iprgan_mx4_linear_bwd_ws_floats(long long M, long long N, long long K, int dy_bf16);
 int iprgan_mx4_linear_bwd(const void* dy, const void* w_codes, const void* w_scales, void* dx, float* ws, long long M, long long N,
                           long long K, int dy_bf16, int dx_bf16, void* stream);
+/* Which form of the kernels a product (gradient 0) or its gradient (gradient 1; x_kind = dy's) of these sizes takes, for tests and tuning:
+ * form[0] 0 tiles through LDS, 1 operands straight to registers, 2 4-bit tiles, 3 gradient; [1] rows of a tile; [2] columns of a tile (of K for the
+ * gradient); [3] waves along K (form 1), 4 stages' scales at once (form 2), rows of odd length (form 3); [4] splits of the sum over blocks. */
+int iprgan_mx4_form(long long M, long long N, long long K, int x_kind, int gradient, int* form);
 
 /* ---- misc elementwise ----------------------------------------------------------------------- */
 int iprgan_fill(float* p, float v, size_t n, void* stream);

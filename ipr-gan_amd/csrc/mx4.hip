@@ -1137,10 +1137,13 @@ static LinPlan lin_plan(int M, int N, int K, int x_kind) {
 struct BwdPlan {
   int form, tm, tk, splits, steps_per_split;
 };
-static BwdPlan bwd_plan(int M, int N, int K, int dy_bf16) {
+static const Form* bwd_forms(int dy_bf16) {
   static const Form f32[3] = {{1, 1, {4, 4}, {0.82, 0.82}, {0.75, 0.75}}, {1, 2, {2, 2}, {1.03, 1.03}, {0.85, 0.85}}, {2, 2, {2, 2}, {1.75, 1.75}, {0.5, 0.5}}};
   static const Form b16[3] = {{1, 1, {4, 4}, {0.68, 0.72}, {0.75, 0.75}}, {1, 2, {3, 3}, {0.72, 0.8}, {0.85, 0.85}}, {4, 1, {2, 2}, {1.08, 1.75}, {0.33, 0.33}}};
-  const Cut c = cut(dy_bf16 ? b16 : f32, 3, dy_bf16 ? N & 1 : 0, 16, 128, M, K, cdiv(cdiv(N, 32), 4), 1, (double)N * K * 0.53, 0.4);      // (bf16: rows of even, odd length)
+  return dy_bf16 ? b16 : f32;
+}
+static BwdPlan bwd_plan(int M, int N, int K, int dy_bf16) {
+  const Cut c = cut(bwd_forms(dy_bf16), 3, dy_bf16 ? N & 1 : 0, 16, 128, M, K, cdiv(cdiv(N, 32), 4), 1, (double)N * K * 0.53, 0.4);      // (bf16: rows of even, odd length)
   return BwdPlan{c.form, c.tm, c.tn, c.splits, c.steps_per_split};
 }
 
@@ -1248,6 +1251,22 @@ int iprgan_mx4_linear(const void* x, const void* x_scales, const void* w_codes, 
   }
   IPR_LAUNCH_CHECK();
   return slab ? slab_reduce(ws, p.splits, M, N, bias, y, act, slope, y_bf16, st) : 0;
+}
+
+int iprgan_mx4_form(long long M, long long N, long long K, int x_kind, int gradient, int* form) {
+  if (lin_check("mx4_form", M, N, K)) return 1;
+  IPR_CHECK(form && x_kind >= IPRGAN_X_F32 && x_kind <= (gradient ? IPRGAN_X_BF16 : IPRGAN_X_MX4), "mx4_form: kind %d", x_kind);
+  if (gradient) {
+    const BwdPlan p = bwd_plan((int)M, (int)N, (int)K, x_kind);
+    const Form& f = bwd_forms(x_kind)[p.form];
+    const int v[5] = {3, 16 * f.mf, 128 * f.nf, x_kind && f.mf == 4 && (N & 1), p.splits};
+    memcpy(form, v, sizeof(v));
+  } else {
+    const LinPlan p = lin_plan((int)M, (int)N, (int)K, x_kind);
+    const int v[5] = {p.tile ? 2 : p.wk ? 1 : 0, p.tile ? p.tile : 16 * p.mf, p.tile ? p.tile : 16 * p.nf * (p.wk ? 8 / p.wk : 4), p.tile ? p.s16 : p.wk, p.splits};
+    memcpy(form, v, sizeof(v));
+  }
+  return 0;
 }
 
 size_t iprgan_mx4_linear_bwd_ws_floats(long long M, long long N, long long K, int dy_bf16) {

@@ -146,6 +146,7 @@ SIGNATURES = {
     'iprgan_mx4_linear': (_I, [_P] * 7 + [_LL, _LL, _LL, _I, _I, _F, _I, _P]),
     'iprgan_mx4_linear_bwd_ws_floats': (_Z, [_LL, _LL, _LL, _I]),
     'iprgan_mx4_linear_bwd': (_I, [_P] * 5 + [_LL, _LL, _LL, _I, _I, _P]),
+    'iprgan_mx4_form': (_I, [_LL, _LL, _LL, _I, _I, _P]),
     'iprgan_fill': (_I, [_P, _F, _Z, _P]),
     'iprgan_axpy': (_I, [_P, _P, _F, _Z, _P]),
     'iprgan_axpy_multi': (_I, [_P, _P, _P, _I, _F, _P]),

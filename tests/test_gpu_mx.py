@@ -6,6 +6,7 @@ pipe's accumulator one step (2^-23, it truncates)."""
 import pytest
 import torch
 
+import mx_forms
 import mx_reference as R
 
 pytestmark = pytest.mark.gpu
@@ -707,3 +708,43 @@ def test_mx8_signs(dev, kind, n, request):
     dy = rnd(n, seed=3)
     dz = ops.act_bwd(dy.to(dev), q, 1).cpu()
     assert torch.equal(dz[fine], torch.where(x > 0, dy, torch.zeros(n))[fine])
+
+
+@pytest.mark.parametrize('kind,size,form', mx_forms.PRODUCT)
+def test_every_form_of_the_product(dev, kind, size, form):
+    """bias, LeakyReLU and both result types; K and N odd, the last rows and columns of a tile empty (float64 on the device)."""
+    from iprgan import ops
+    M, K, N = size
+    g = torch.Generator(device=dev).manual_seed(7)
+    x = torch.randn(M, K, generator=g, device=dev).to(torch.bfloat16 if kind == 'bf16' else torch.float32)
+    w4 = ops.mx4_quant(torch.randn(N, K, generator=g, device=dev) / K ** 0.5)
+    bias = torch.randn(N, generator=g, device=dev)
+    xin = ops.mx4_quant(x) if kind == 'mx4' else x
+    xd = ops.mx4_dequant(xin).double() if kind == 'mx4' else x.double()
+    wd = ops.mx4_dequant(w4).double().t().contiguous()
+    pre = xd @ wd + bias.double()
+    want = torch.where(pre > 0, pre, pre * float(torch.tensor(0.2)))
+    tol = lin_bound(xd.abs(), wd.abs(), K, 3 if kind == 'f32' else 1) + 4 * 2.0 ** -24 * pre.abs()
+    for dt in (torch.float32, torch.bfloat16):
+        y = ops.mx4_linear(xin, w4, bias, 2, 0.2, dtype=dt)
+        err = (y.double() - want).abs()
+        t = tol + (2.0 ** -8 * want.abs() if dt == torch.bfloat16 else 0)
+        assert bool((err <= t).all()), (form, dt, float((err / t).max()))
+        assert torch.equal(y, ops.mx4_linear(xin, w4, bias, 2, 0.2, dtype=dt)), 'not deterministic'
+
+
+@pytest.mark.parametrize('kind,size,form', mx_forms.GRADIENT)
+def test_every_form_of_the_gradient(dev, kind, size, form):
+    from iprgan import ops
+    M, K, N = size
+    g = torch.Generator(device=dev).manual_seed(8)
+    dy = torch.randn(M, N, generator=g, device=dev).to(torch.bfloat16 if kind == 'bf16' else torch.float32)
+    w4 = ops.mx4_quant(torch.randn(N, K, generator=g, device=dev))
+    wd = ops.mx4_dequant(w4).double()
+    want, tol = dy.double() @ wd, lin_bound(dy.double().abs(), wd.abs(), N, 3 if kind == 'f32' else 1)
+    for dt in (torch.float32, torch.bfloat16):
+        dx = ops.mx4_linear_bwd(dy, w4, dtype=dt)
+        err = (dx.double() - want).abs()
+        t = tol + (2.0 ** -8 * want.abs() if dt == torch.bfloat16 else 0)
+        assert bool((err <= t).all()), (form, dt, float((err / t).max()))
+        assert torch.equal(dx, ops.mx4_linear_bwd(dy, w4, dtype=dt)), 'not deterministic'

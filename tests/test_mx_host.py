@@ -4,6 +4,7 @@ import ctypes as C
 import pytest
 import torch
 
+import mx_forms
 from iprgan import _lib as L
 from iprgan import ops
 
@@ -247,3 +248,15 @@ def test_mx8_quant_takes_the_signs_flag_beside_a_storage_kind():
     refused_size('iprgan_mx8_quant', P, P, P, 8, 16 | 3, 0, None)
     refused_size('iprgan_mx8_quant', P, P, P, 8, 32, 0, None)
     refused_size('iprgan_mx8_dequant', P, P, P, 8, 16, 0, None)
+
+
+@pytest.mark.parametrize('gradient', [0, 1])
+def test_sizes_of_the_form_tests_take_their_forms(gradient):
+    kinds = {'f32': 0, 'bf16': 1, 'mx4': 2}
+    form = (C.c_int * 5)()
+    for kind, (M, K, N), want in mx_forms.GRADIENT if gradient else mx_forms.PRODUCT:
+        L.call('iprgan_mx4_form', M, N, K, kinds[kind], gradient, form)
+        assert tuple(form[:4]) + (form[4] > 1,) == want, (kind, M, K, N, tuple(form))
+    refused_size('iprgan_mx4_form', 8, 8, 0, 0, gradient, form)
+    refused_size('iprgan_mx4_form', 8, 8, 8, 3 - gradient, gradient, form)
+    refused_size('iprgan_mx4_form', 8, 8, 8, 0, gradient, None)
