@@ -1083,10 +1083,10 @@ static Cut cut(const Form* forms, int count, int kind, int rows_f, int cols_f, i
 
 //   LDS    : 16 * mf rows x 64 * nf columns a block.  Four fragments a wave halve the LDS reads a multiplication (4096^3 fp32: 450 -> 400 us)
 //   direct : 16 * mf rows x 16 * nf * (8 / wk) columns a block, wk waves along K.  For 4-bit x of up to 64 rows; else for up to 16, where the LDS form
-//            would be split or leaves half the chip idle and the estimate is 2 us lower (4 x 2000 x 300 fp32: 8.8 : 6.2 us for LDS), K <= 4096 and
-//            not too many columns.  Against LDS, wall time: 1 x 4096 x 4096 fp32 13.5 : 19.5 us (one launch instead of two), 8 x 4096 x
-//            16384 bf16 16.3 : 19.0, but fp32 25.3 : 20.4 (every wave splits x again), 16 x 18432 x 1024 bf16 26.9 : 18.4 (18 steps in a row)
-//            and 4 x 65536 x 1024 bf16 21.2 : 13.7 (device; 1024 blocks of the LDS form).
+//            would be split or leaves half the chip idle and the estimate is 2 us lower, K <= 4096 and not too many columns.  Against LDS, device
+//            time, M x N x K: 8 x 1024 x 1024 fp32 4.3 : 6.4 us, bf16 3.4 : 4.2; 1 x 4096 x 4096 bf16 4.8 : 6.7, fp32 8.7 : 7.9 (one launch less
+//            for the host); outside the rule 4 x 2000 x 300 fp32 6.6 : 4.4, 16 x 1024 x 18432 bf16 23.5 : 8.1 (18 steps in a row),
+//            4 x 65536 x 1024 bf16 16.5 : 8.1, 8 x 16384 x 4096 fp32 23.2 : 21.5 (every wave splits x again).  Two fragments of bf16 x: no size.
 //   tile   : 4-bit x of more rows: square tiles, 256 where they fill three quarters of the chip, else 128
 struct LinPlan {
   int mf, nf, wk, tile, s16, tm, tn, splits, steps_per_split;
@@ -1111,7 +1111,7 @@ static LinPlan lin_plan(int M, int N, int K, int x_kind) {
   }
   if (x_kind != IPRGAN_X_MX4) {
     c = cut(lds, 4, kind, 16, 64, M, N, steps, 1, weights, 1.);
-    dir = M <= 16 && (c.splits > 1 || c.tn < 128) && d.us + 2. < c.us && steps <= 32 && (long long)steps * N <= (kind ? 600000 : 200000);
+    dir = M <= 16 && (kind == 0 || p.nf == 1) && (c.splits > 1 || c.tn < 128) && d.us + 2. < c.us && steps <= 32 && (long long)steps * N <= (kind ? 600000 : 200000);
   }
   if (dir) {
     c = d;
@@ -1240,7 +1240,7 @@ int iprgan_mx4_linear(const void* x, const void* x_scales, const void* w_codes, 
     if (rc) return rc;
   } else if (p.wk) {
 #define DIRECT(MF, XT) (p.nf == 2 ? mx4_direct_kernel<MF, 2, XT> : mx4_direct_kernel<MF, 1, XT>)
-    auto k = x_kind == IPRGAN_X_F32 ? DIRECT(1, 3) : x_kind == IPRGAN_X_BF16 ? DIRECT(1, 1) : p.mf == 1 ? DIRECT(1, 0) : p.mf == 2 ? DIRECT(2, 0) : DIRECT(4, 0);
+    auto k = x_kind == IPRGAN_X_F32 ? DIRECT(1, 3) : x_kind == IPRGAN_X_BF16 ? mx4_direct_kernel<1, 1, 1> : p.mf == 1 ? DIRECT(1, 0) : p.mf == 2 ? DIRECT(2, 0) : DIRECT(4, 0);
 #undef DIRECT
     hipLaunchKernelGGL(k, grid, dim3(512), 0, st, a, p.tn, p.tm, p.wk);
   } else {
