@@ -195,6 +195,14 @@ def _one_device(who, first, *rest):
         raise RuntimeError(f'{who}: operands on cuda:{d}, which is not the current device')
 
 
+def _kind_of(who, t):
+    """is16() of a tensor a user hands in: in 'fp32x3' mode a bf16 tensor is read as three planes, which an ordinary one does not have."""
+    k = is16(t)
+    if k == ST_X3 and (t.storage_offset() + 2 * pstride(t) + t.numel()) * 2 > t.untyped_storage().nbytes():
+        raise RuntimeError(f'{who}: in this math mode a bfloat16 tensor is the first of three planes, and the storage of this one ends with it')
+    return k
+
+
 def _vptr(t, keep):
     """ptr() for vector accesses: a contiguous view that starts off a 16-byte boundary (a row of an odd-sized tensor, a slice of a
     flat buffer) is copied; the copy lives in ``keep`` until the launch is enqueued.  (Three-plane tensors stay: a copy of the h plane
@@ -326,9 +334,10 @@ MX8_SIGNS = 16      # include/iprgan.h: IPRGAN_MX8_SIGNS
 def mx8_quant(x, signs=False):
     """``x`` (any storage kind) saved in 8 bits.  ``signs``: for a tensor that is read as a mask (x > 0): no positive element is rounded to
     zero, those below half a step are stored as one step."""
+    k = _kind_of('mx8_quant', x)
     _one_device('mx8_quant', x)
     keep = []
-    p, n, k = _vptr(x, keep), x.numel(), is16(x)
+    p, n = _vptr(x, keep), x.numel()
     split = (n + 15) & ~15
     q = object.__new__(Mx8)
     q._buf = buf = torch.empty(split + (n + 31) // 32, dtype=torch.uint8, device=x.device)
@@ -375,8 +384,8 @@ def _mx8_norm_bwd(q, dy, gamma, beta, mean, invstd, act, slope, groups, slope_t=
     if mean.numel() != groups * C_ or invstd.numel() != groups * C_ or (gamma is not None and gamma.numel() != C_) \
             or (beta is not None and beta.numel() != C_):
         raise RuntimeError(f'norm backward: a parameter or statistic does not fit {groups} group(s) of {C_} channels')
+    k = _kind_of('norm backward', dy)
     _one_device('norm backward', q, dy, gamma, beta, mean, invstd, slope_t, dbias)
-    k = is16(dy)
     kx = k
     if k == ST_F32 and L.act_x3() and (q.kind == ST_X3 or (q.kind == ST_F32 and _NORM_DYF32 and _norm_splits_here(q))):
         kx = ST_X3
@@ -427,8 +436,8 @@ class Mx4(_Packed):
 
 def mx4_quant(x):
     """A matrix (or a tensor seen as [shape[0], rest]) rounded to 4 bits; fp32 or bf16."""
+    k = _kind_of('mx4_quant', x)
     _one_device('mx4_quant', x)
-    k = is16(x)
     if k == ST_X3:
         x, k = f32(x), ST_F32
     n = x.numel()
@@ -482,7 +491,7 @@ def mx4_linear(x, w, bias=None, act=L.ACT_NONE, slope=0.0, dtype=None):
         raise RuntimeError('mx4_linear: the weights must be an Mx4 (mx4_quant)')
     N, K = w.shape
     quantised = isinstance(x, Mx4)
-    k = X_MX4 if quantised else is16(x)
+    k = X_MX4 if quantised else _kind_of('mx4_linear', x)
     if k == ST_X3 and not quantised:
         x, k = f32(x), ST_F32
     if len(x.shape) < 1 or x.shape[-1] != K:
@@ -516,7 +525,7 @@ def mx4_linear_bwd(dy, w, dtype=None):
     if not isinstance(w, Mx4):
         raise RuntimeError('mx4_linear_bwd: the weights must be an Mx4 (mx4_quant)')
     N, K = w.shape
-    k = is16(dy)
+    k = _kind_of('mx4_linear_bwd', dy)
     if k == ST_X3:
         dy, k = f32(dy), ST_F32
     if dy.dim() < 1 or dy.shape[-1] != N:
@@ -564,12 +573,14 @@ def act_bwd(dy, out, act, slope=0.0):
     if isinstance(out, Mx8):
         if dy.numel() != out.numel():
             raise RuntimeError(f'act_bwd: checkpoint of shape {out.shape}, gradient of shape {tuple(dy.shape)}')
+        k = _kind_of('act_bwd', dy)
         _one_device('act_bwd', dy, out)
-        dy = f32(dy) if is16(dy) == ST_X3 else dy
+        if k == ST_X3:
+            dy, k = f32(dy), ST_F32
         keep = []
         pdy, dz = _vptr(dy, keep), _new(dy.shape, dy, dy.dtype)
         c, s = out.ptrs()
-        call('iprgan_mx8_act_bwd', pdy, c, s, ptr(dz), dy.numel(), act, float(slope), is16(dy), stream())
+        call('iprgan_mx8_act_bwd', pdy, c, s, ptr(dz), dy.numel(), act, float(slope), k, stream())
         return dz
     if ST_X3 in (is16(dy), is16(out)):          # (no three-plane form: a stand-alone activation backward is rare)
         dy, out = f32(dy), f32(out)

@@ -260,3 +260,27 @@ def test_sizes_of_the_form_tests_take_their_forms(gradient):
     refused_size('iprgan_mx4_form', 8, 8, 0, 0, gradient, form)
     refused_size('iprgan_mx4_form', 8, 8, 8, 3 - gradient, gradient, form)
     refused_size('iprgan_mx4_form', 8, 8, 8, 0, gradient, None)
+
+
+def test_a_plain_bf16_tensor_is_not_taken_for_three_planes():
+    """In 'fp32x3' mode a bf16 tensor is the first of three planes in one storage; one whose storage ends behind its own elements is refused before
+    anything reads on."""
+    before = L.get_math()
+    L.set_math('fp32x3')
+    try:
+        x = torch.zeros(6, 32, dtype=torch.bfloat16)
+        w4 = ops.Mx4(torch.zeros(32, 64, dtype=torch.uint8), torch.zeros(32, 4, dtype=torch.uint8), (32, 32))
+        q = ops.Mx8(torch.zeros(192, dtype=torch.int8), torch.zeros(6, dtype=torch.uint8), (6, 32))
+        v = torch.zeros(32)
+        calls = (lambda t: ops.mx8_quant(t), lambda t: ops.mx4_quant(t), lambda t: ops.mx4_linear(t, w4), lambda t: ops.mx4_linear_bwd(t, w4),
+                 lambda t: ops.act_bwd(t, q, 1), lambda t: ops.bn_bwd(q, None, t, v, v, v, 1, beta=v))
+        whole = torch.zeros(3, 6, 32, dtype=torch.bfloat16)[0]
+        slice_ = torch.zeros(3, 9, 32, dtype=torch.bfloat16)[0][3:]
+        for f in calls:
+            with pytest.raises(RuntimeError, match='three planes'):
+                f(x)
+            for t in (whole, slice_):
+                with pytest.raises(RuntimeError, match='GPU tensors'):
+                    f(t)
+    finally:
+        L.set_math(before)
