@@ -492,6 +492,11 @@ int iprgan_tune_import(const int* records, size_t n_records, int replace);
  * PReLU): a positive element below half a step is stored as code 1 instead of 0 (off by less than one step), so that value > 0 where x > 0. */
 enum { IPRGAN_MX8_SIGNS = 16 };
 int iprgan_mx8_quant(const void* x, void* codes, void* scales, size_t n, int kind, size_t pstride, void* stream);
+/* ... of a norm layer's input (G groups of M rows, C channels, C % 4 = 0; iprgan_mx8_norm_bwd's gamma, beta, save_mean, save_invstd): the layer's mask
+ * gamma * (x - mean) * invstd + beta > 0 is the same for x and for its value; an element that rounding would carry over that border is stored one
+ * code further on its own side (off by less than one step; where that code would be 128 it stays).  ws: 16-byte aligned, G C floats. */
+int iprgan_mx8_quant_norm(const void* x, void* codes, void* scales, const float* gamma, const float* beta, const float* save_mean,
+                          const float* save_invstd, float* ws, long long G, long long M, long long C, int kind, size_t pstride, void* stream);
 int iprgan_mx8_dequant(const void* codes, const void* scales, void* y, size_t n, int kind, size_t pstride, void* stream);
 /* dz = dy * act'(out), out read from its checkpoint (iprgan_act_bwd; dy and dz fp32 or bf16) */
 int iprgan_mx8_act_bwd(const void* dy, const void* codes, const void* scales, void* dz, size_t n, int act, float slope, int kind,

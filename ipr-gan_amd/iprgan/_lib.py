@@ -135,6 +135,7 @@ SIGNATURES = {
     'iprgan_prof_num_layers': (_I, []),
     'iprgan_prof_get_layer': (_I, [_I, C.c_char_p, _I, C.POINTER(C.c_longlong), C.POINTER(C.c_double), C.POINTER(C.c_double)]),
     'iprgan_mx8_quant': (_I, [_P, _P, _P, _Z, _I, _Z, _P]),
+    'iprgan_mx8_quant_norm': (_I, [_P] * 8 + [_LL, _LL, _LL, _I, _Z, _P]),
     'iprgan_mx8_dequant': (_I, [_P, _P, _P, _Z, _I, _Z, _P]),
     'iprgan_mx8_act_bwd': (_I, [_P, _P, _P, _P, _Z, _I, _F, _I, _P]),
     'iprgan_mx8_norm_bwd_ws_floats': (_Z, [_LL, _LL, _LL]),

@@ -31,9 +31,10 @@ _GEMV_PAIR = os.environ.get('IPRGAN_GEMV_PAIR', '1') != '0'        # A/B switch:
 # The forward pass is untouched; gradients see activations rounded to 1/127 of their block's maximum.
 _CKPT8 = os.environ.get('IPRGAN_CKPT8', '0') == '1'
 # ... and masks that are those of the activations: what is rounded to zero would count as not positive, so a tensor that is read as a mask (outputs
-# of a convolution or dense layer with ReLU / LeakyReLU, inputs of a PReLU) is stored with no positive element rounded to zero.  Without it
-# (`ckpt8_signs: false`) about 1 % of a ReLU's positive elements lose their gradient, always in that direction, and a channel 250 times
-# smaller than the largest of its 32 neighbours loses all of it.  Unless set, it goes with ckpt8.
+# of a convolution or dense layer with ReLU / LeakyReLU, inputs of a PReLU) is stored with no positive element rounded to zero, and the input
+# of a norm layer with an activation with none carried across the border of its mask.  Without it (`ckpt8_signs: false`) about 1 % of a ReLU's
+# positive elements lose their gradient, always in that direction, a channel 250 times smaller than the largest of its 32
+# neighbours loses all of it, and 0.3 % of a norm layer's masks turn.  Unless set, it goes with ckpt8.
 _CKPT8_SIGNS = os.environ.get('IPRGAN_CKPT8_SIGNS', os.environ.get('IPRGAN_CKPT8', '0')) == '1'
 _CKPT8_MIN = 1 << 14        # elements: a smaller tensor stays as it is (64 KB are not worth two launches)
 
@@ -782,9 +783,12 @@ def _pack_saved(ops_list, stash, i, last):
                     made = j
                 break
         if not isinstance(ops_list[i], MaxPool2):
-            q = ops.mx8_quant(x, _CKPT8_SIGNS and (isinstance(ops_list[i], (PReLU, PixelShufflePReLU))
-                                                   or (made is not None and _is_mask(ops_list[made]))))
-            st['x'] = q
+            op = ops_list[i]
+            signs = _CKPT8_SIGNS and (isinstance(op, (PReLU, PixelShufflePReLU)) or (made is not None and _is_mask(ops_list[made])))
+            norm = None
+            if _CKPT8_SIGNS and not signs and isinstance(op, (BatchNorm, InstanceNorm)) and (op.act or getattr(op, 'prelu', None) is not None):
+                norm = (op.m.weight, op.m.bias, st['mean'], st['invstd'])
+            st['x'] = q = ops.mx8_quant(x, signs, norm)
             if made is not None:
                 stash[made]['y'] = q.view(stash[made]['y'].shape)
     y = st.get('y')

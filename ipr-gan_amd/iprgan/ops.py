@@ -331,9 +331,13 @@ class Mx8(_Packed):
 MX8_SIGNS = 16      # include/iprgan.h: IPRGAN_MX8_SIGNS
 
 
-def mx8_quant(x, signs=False):
+def mx8_quant(x, signs=False, norm=None):
     """``x`` (any storage kind) saved in 8 bits.  ``signs``: for a tensor that is read as a mask (x > 0): no positive element is rounded to
-    zero, those below half a step are stored as one step."""
+    zero, those below half a step are stored as one step.  ``norm``: for the input of a norm layer with an activation, (gamma, beta, mean,
+    invstd) of its backward pass (gamma and beta both None without affine parameters; mean and invstd [groups, channels]): no element is
+    rounded across the border of the layer's mask."""
+    if norm is not None and signs:
+        raise RuntimeError('mx8_quant: signs or the mask of a norm layer, not both')
     k = _kind_of('mx8_quant', x)
     _one_device('mx8_quant', x)
     keep = []
@@ -346,6 +350,18 @@ def mx8_quant(x, signs=False):
     c = buf.data_ptr()
     if L._acct is not None:
         L._acct_note(buf)
+    if norm is not None:
+        gamma, beta, mean, invstd = norm
+        C_ = x.shape[-1] if x.dim() else 0
+        groups = mean.numel() // C_ if C_ else 0
+        if not groups or n % (groups * C_) or mean.numel() != groups * C_ or invstd.numel() != mean.numel() \
+                or any(t is not None and t.numel() != C_ for t in (gamma, beta)):
+            raise RuntimeError(f'mx8_quant: parameters and statistics of a norm layer do not fit an input of shape {tuple(x.shape)}')
+        _one_device('mx8_quant', x, gamma, beta, mean, invstd)
+        ws = L.acct_scratch(_new(groups * C_, mean, torch.float32))
+        call('iprgan_mx8_quant_norm', p, c, c + split, ptr32(gamma), ptr32(beta), ptr32(mean), ptr32(invstd), ws.data_ptr(), groups, n // (groups * C_),
+             C_, k, pstride(x) if k == ST_X3 else 0, stream())
+        return q
     call('iprgan_mx8_quant', p, c, c + split, n, k | MX8_SIGNS if signs else k, pstride(x) if k == ST_X3 else 0, stream())
     return q
 

@@ -84,3 +84,20 @@ def mx8_encode_signs(x):
     v = x.detach().cpu().double().reshape(-1)
     lost = (v > 0) & (codes == 0) & (s.repeat_interleave(32)[:v.numel()] != 255)
     return torch.where(lost, torch.ones_like(codes), codes), s
+
+
+def mx8_encode_norm(x, gamma, beta, mean, invstd):
+    """mx8_encode of a norm layer's input [G, M, C] with no element carried across v = 0, v = gamma (x - mean) invstd + beta: such an element goes one
+    code further on its own side.  -> codes, scales, v > 0"""
+    codes, s = mx8_encode(x)
+    G, M, C = x.shape
+    step = torch.exp2(s.double() - 127).repeat_interleave(32)[:codes.numel()].view(x.shape)
+    k = (gamma.double() if gamma is not None else torch.ones(C, dtype=torch.float64)).view(1, 1, C) * invstd.double().view(G, 1, C)
+    b = (beta.double() if beta is not None else torch.zeros(C, dtype=torch.float64)).view(1, 1, C)
+    v = lambda t: (t - mean.double().view(G, 1, C)) * k + b
+    q = codes.double().view(x.shape)
+    want, got = v(x.double()) > 0, v(q * step) > 0
+    up = torch.where(k < 0, -1.0, 1.0).expand(x.shape)
+    q = torch.where(want & ~got, q + up, torch.where(got & ~want, q - up, q)).clamp(-127, 127)
+    q = torch.where((s == 255).repeat_interleave(32)[:codes.numel()].view(x.shape), 0.0, q)
+    return q.to(torch.int8).reshape(-1), s, want

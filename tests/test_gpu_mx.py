@@ -748,3 +748,73 @@ def test_every_form_of_the_gradient(dev, kind, size, form):
         t = tol + (2.0 ** -8 * want.abs() if dt == torch.bfloat16 else 0)
         assert bool((err <= t).all()), (form, dt, float((err / t).max()))
         assert torch.equal(dx, ops.mx4_linear_bwd(dy, w4, dtype=dt)), 'not deterministic'
+
+
+@pytest.mark.parametrize('form,shape,affine', [(f, s, a) for f, s, a in [
+    ('bn', (4, 9, 7, 64), True), ('bn', (3, 5, 5, 36), True), ('bn', (2, 3, 3, 4), True), ('bn', (1, 1, 17, 260), True), ('bn', (2, 4, 4, 1024), True),
+    ('bn', (16, 33, 31, 20), True), ('inst', (4, 9, 7, 64), True), ('inst', (4, 9, 7, 64), False), ('inst', (70, 4, 5, 12), True),
+    ('inst', (1, 17, 1, 516), True), ('inst', (2, 1, 1, 8), True), ('inst', (600, 5, 5, 132), False), ('bn', (9, 129, 129, 128), True)]])
+@pytest.mark.parametrize('kind', ['f32', 'bf16', 'x3'])
+def test_norm_inputs_keep_their_masks(dev, form, shape, affine, kind, request):
+    """Codes and scales as stated; the mask read off the codes is that of x, counted by a gradient of ones (whole numbers: exact); nothing is off by a
+    step or more.  The last shapes are walked in several strides, over several groups a stride."""
+    from iprgan import ops
+    if kind == 'x3':
+        request.getfixturevalue('x3_mode')
+    b, h, w, c = shape
+    G = b if form == 'inst' else 1
+    M = b * h * w // G
+    x = rnd(*shape, seed=1) * torch.exp(0.3 * rnd(c, seed=2)) + rnd(c, seed=3)
+    x = x.bfloat16() if kind == 'bf16' else x
+    xg = x.float().view(G, M, c)
+    mean, invstd = xg.mean(1), 1 / torch.sqrt(xg.var(1, unbiased=False) + 1e-5)
+    gamma = (1 + 0.3 * rnd(c, seed=4)) if affine else None
+    if affine:
+        gamma[0], gamma[1] = -gamma[0].abs(), 0.0
+    beta = 0.3 * rnd(c, seed=5) if affine else None
+    codes, scales, mask = R.mx8_encode_norm(xg, gamma, beta, mean, invstd)
+    to = lambda t: None if t is None else t.to(dev)
+    t = ops.to_kind(x.to(dev), ops.ST_X3) if kind == 'x3' else x.to(dev)
+    q = ops.mx8_quant(t, norm=(to(gamma), to(beta), to(mean if form == 'inst' else mean.view(c)), to(invstd if form == 'inst' else invstd.view(c))))
+    assert torch.equal(q.scales.cpu(), scales) and torch.equal(q.codes.cpu(), codes)
+    val = R.mx8_decode(codes, scales).view(xg.shape)
+    step = torch.exp2(scales.double() - 127).repeat_interleave(32)[:codes.numel()].view(xg.shape)
+    assert bool(((val - xg.double()).abs() < step).all())
+    edge = codes.view(xg.shape).abs() == 127                     # (its neighbour on the other side would be 128: may have stayed)
+    k = (gamma if affine else torch.ones(c)).double() * invstd.double().view(G, 1, c)
+    got = (val - mean.double().view(G, 1, c)) * k + (beta if affine else torch.zeros(c)).double() > 0
+    assert torch.equal(got[~edge], mask[~edge])
+    if affine:
+        f = ops.bn_bwd if form == 'bn' else ops.instnorm_bwd
+        ms = [to(mean), to(invstd)] if form == 'inst' else [to(mean.view(c)), to(invstd.view(c))]
+        db = f(q, None, torch.ones(shape, device=dev), to(gamma), *ms, 1, beta=to(beta))[2]
+        assert torch.equal(db.cpu().double(), got.double().sum((0, 1)))
+
+
+def test_norm_input_masks_refuse_what_does_not_fit(dev):
+    from iprgan import ops
+    x, v = torch.zeros(2, 3, 3, 8, device=dev), torch.ones(8, device=dev)
+    for bad in ((v[:4], v[:4], v, v), (v, v, v[:4], v), (v, v, v, torch.ones(16, device=dev)), (v, v, torch.ones(40, device=dev), torch.ones(40, device=dev)),
+                (v, None, v, v)):
+        with pytest.raises(RuntimeError, match='mx8_quant'):
+            ops.mx8_quant(x, norm=bad)
+    with pytest.raises(RuntimeError, match='not both'):
+        ops.mx8_quant(x, signs=True, norm=(v, v, v, v))
+    with pytest.raises(RuntimeError, match='one device'):
+        ops.mx8_quant(x, norm=(v.cpu(), v.cpu(), v, v))
+
+
+def test_norm_input_masks_past_32_bits(dev):
+    """2^32 + 512 elements and more in groups of 2^31 and of 128 channels: the end of the tensor as it is by itself."""
+    from iprgan import ops
+    C, M, G = 128, (1 << 24) + 4, 2
+    tail = 40
+    x = torch.zeros(G, M, 1, C, dtype=torch.bfloat16, device=dev)
+    end = rnd(tail, C, seed=1).bfloat16().to(dev)
+    x[1, -tail:, 0] = end
+    mean, inv = 0.1 * rnd(G, C, seed=2).to(dev), 1 + 0.1 * rnd(G, C, seed=3).abs().to(dev)
+    gamma, beta = rnd(C, seed=4).to(dev), 0.3 * rnd(C, seed=5).to(dev)
+    q = ops.mx8_quant(x, norm=(gamma, beta, mean, inv))
+    own = ops.mx8_quant(end.view(1, tail, 1, C), norm=(gamma, beta, mean[1:], inv[1:]))
+    assert torch.equal(q.codes[-tail * C:], own.codes) and torch.equal(q.scales[-tail * C // 32:], own.scales)
+    assert bool((q.scales[:-tail * C // 32] == 0).all())

@@ -284,3 +284,10 @@ def test_a_plain_bf16_tensor_is_not_taken_for_three_planes():
                     f(t)
     finally:
         L.set_math(before)
+
+
+def test_mx8_quant_norm_refuses_bad_calls():
+    args = dict(x=P, codes=P, scales=P, gamma=P, beta=P, mean=P, invstd=P, ws=P, G=1, M=8, C=8, kind=0, ps=0)
+    for bad in (dict(x=None), dict(ws=None), dict(mean=None), dict(gamma=None), dict(beta=None), dict(x=ODD), dict(codes=ODD), dict(ws=ODD), dict(M=0), dict(C=6),
+                dict(kind=3), dict(kind=16), dict(kind=2, ps=8), dict(G=70000), dict(M=WRAP + 8), dict(C=WRAP + 8), dict(G=WRAP + 1)):
+        refused_size('iprgan_mx8_quant_norm', *{**args, **bad}.values(), None)
