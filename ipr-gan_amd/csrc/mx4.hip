@@ -8,6 +8,8 @@
 //   e = floor(log2 max|x|) - 2, one more when max|x| * 2^-e >= 7, clamped to [-127, 125]; round to nearest, ties to the even code
 // e is the smallest exponent for which nothing rounds past 6: an element is off by at most half the distance of its neighbours.
 // x * 2^-e is exact, so this is ONE rounding.  A block with a NaN or an infinity stores scale byte 255 and reads back as NaN.
+//
+// Sizes in the comments below are M x N x K (x [M][K], W [N][K]) throughout, times the device's.
 #include "common.h"
 
 #include <atomic>
@@ -23,7 +25,7 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 // Rows of odd lengths start on any element: vector accesses that promise no more than the element's own alignment (the memory system takes
-// them at any address).  1281 x 3237 x 2085 fp32: 203 us element by element, 87 like this; nothing changes where rows are aligned.
+// them at any address).  1281 x 2085 x 3237 fp32: 203 us element by element, 79 like this; nothing changes where rows are aligned.
 typedef f32x4 f32x4u __attribute__((aligned(4)));
 typedef bf16x4 bf16x4u __attribute__((aligned(2)));
 typedef bf16x8 bf16x8u __attribute__((aligned(2)));
@@ -274,7 +276,7 @@ __device__ __forceinline__ Place place(int tn, int tm) {
   return Place{(int)(grp * 4 + in % gw), (int)(in / gw), (int)z};
 }
 
-// Few rows (1 x 8192 x 16384 with 4-bit x 14.9 us, 4.5 TB/s of weights; 1 x 4096 x 4096 bf16 6 us): 8 waves, WK along K x 8 / WK along n (16 *
+// Few rows (1 x 16384 x 8192 with 4-bit x 13.9 us, 5.1 TB/s of weights; 1 x 4096 x 4096 bf16 4.7 us): 8 waves, WK along K x 8 / WK along n (16 *
 // NF columns each); both operands straight from memory to registers, no barrier before the end, where the WK partial tiles are added in LDS in fixed order - one launch where a split over blocks takes two.  XT: 0 = 4-bit x
 // (the scaled instruction), 1 = bf16, 3 = fp32 (planes).  Bound by latency, or by the split of fp32 x into planes (176 vector instructions a
 // step and 16 rows, repeated by every wave: why more rows go through LDS below).
@@ -411,7 +413,7 @@ __device__ __forceinline__ void block_barrier() {
 // own: a lane holds whole 16-byte blocks, lane group g block g of the step, and the step's four instructions take 8 elements of each block -
 // the order of K is free as long as both operands agree); the 16 * MF rows of x are shared through LDS, split into planes on the way in.
 // What bounds it at 4096^3: bf16 136 us, 1010 TFLOP/s - two blocks a CU, whose loads, LDS traffic and multiplications overlap to about 45 % of
-// the matrix pipe; fp32 318 us, three products each.
+// the matrix pipe; fp32 309 to 318 us, three products each.
 // (a barrier for LDS alone: __syncthreads would also wait for the loads in flight)
 __device__ __forceinline__ void lds_sync() {
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -440,7 +442,7 @@ __global__ __launch_bounds__(256, NF < 4 ? 2 : 1) void mx4_linear_kernel(const L
     for (int m = 0; m < MF; ++m) acc[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
   // W goes through LDS by DMA: four neighbouring lanes fetch a row's 64 bytes, where the fragments' own order (neighbours in different rows) takes
   // an access a lane (4096^3: bf16 149 -> 140 us, fp32 328 -> 318).  Piece c of row r at c ^ ((r >> 1) & 3): no conflicts.  Not for fp32 in 64 x
-  // 128 tiles, where the 8 KB more leave two blocks a CU instead of three (64 x 8192 x 16384: 67 -> 73).  Columns past N repeat the last row;
+  // 128 tiles, where the 8 KB more leave two blocks a CU instead of three (64 x 16384 x 8192, either way round: 67 -> 73).  Columns past N repeat the last row;
   // their results are not stored.
   const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc((void*)(a.w + (size_t)min(n0, a.N - 1) * a.KB * 16), 0, -1, 0x00020000);
   unsigned wo[NF];
@@ -548,7 +550,7 @@ __global__ __launch_bounds__(256, NF < 4 ? 2 : 1) void mx4_linear_kernel(const L
 //   * S16 (rows of whole 512-element groups): the scales of two stages travel as one 16-byte piece a row; 4-byte pieces, two a row and
 //     stage, cost the intake as much as a third of the codes (64 cache lines an instruction).
 //   * Tile order: the XCDs take contiguous runs (each has its own L2), and a run walks 4 tiles along n, then down m.
-// What bounds it, 256 x 256 at 8192^3, 290 us: the multiplications alone take 175 at the clock the chip sustains under them (it falls from 2.4 to
+// What bounds it, 256 x 256 at 8192^3, 281 to 302 us: the multiplications alone take 160 to 196 at the clock the chip sustains under them (it falls from 2.4 to
 // 1.9 GHz), the loop without its DMA 226: LDS serves the fragments and the DMA's writes for 60 % of the time, in the matrix pipe's way.
 template <int TN, int TM, int WN, int WM, bool S16>
 __global__ __launch_bounds__(WN* WM * 64, 2) void mx4_gemm4_kernel(const LinArgs a, int tn, int tm) {
@@ -790,8 +792,8 @@ __global__ __launch_bounds__(256) void mx4_slab_reduce_kernel(const float* __res
 // its 8 rows, widens them with the rows' scales and interleaves row pairs: the eight vectors it then holds per word are its operands for EIGHT
 // instructions j = 0..7, whose row i stands for k = 8 KW i + j - the 8 x 8 transposition costs 32 permutes a word and no LDS.  A wave
 // covers 128 KW k; the block's 4 waves split the rows n and add their tiles through LDS.  The lane's results over j are 8 consecutive k.
-// Few rows of dy stream the weights: 4 x 8192 x 16384 bf16 20 us, 3.4 TB/s.  Many are bound by the vector instructions that widen W and split dy
-// beside the multiplications: 1024 x 8192 x 4096 bf16 97 us, 710 TFLOP/s, fp32 195 us, 1 060 over its three planes.
+// Few rows of dy stream the weights: 4 x 8192 x 16384 bf16 18.6 us, 3.8 TB/s.  Many are bound by the vector instructions that widen W and split dy
+// beside the multiplications: 1024 x 8192 x 4096 bf16 93 us, 740 TFLOP/s, fp32 183 us, 1 130 over its three planes.
 struct BwdArgs {
   const void* dy;
   const uint8_t *w, *ws;
@@ -826,7 +828,7 @@ __global__ __launch_bounds__(256, 2) void mx4_linear_bwd_kernel(const BwdArgs a,
   const int steps = (a.N + 31) / 32;
   const int s0 = (pl.z * 4 + wave) * a.steps_per_wave, s1 = min(steps, s0 + a.steps_per_wave);         // (a wave may be left without a step)
   // Several fragments of dy go through LDS by DMA, a wave's own rows: neighbouring lanes fetch a row's bytes, where the fragments' order takes an
-  // access a lane (512 x 4096 x 4096: bf16 42 -> 36 us, fp32 67 -> 62; one fragment is not worth its waits, 32 x 8192 x 16384 33 -> 36).
+  // access a lane (512 x 4096 x 4096: bf16 42 -> 36 us, fp32 67 -> 62; one fragment is not worth its waits, 32 rows by 8192 and 16384 33 -> 36).
   // Piece c of row r at c ^ swz_dy(r): no bank conflicts.  Row ends are met by the last step alone, which loads to registers; so do rows of
   // odd length.
   constexpr int PR = RB / 16, DP = DMA ? MF * 16 * RB / 1024 : 1;     // pieces a row; DMA instructions a step

@@ -149,8 +149,8 @@ __device__ __forceinline__ void ldcodes(const int8_t* q, size_t e, float* v) {  
 }
 
 // Quantise: a thread owns V consecutive elements, 32 / V neighbouring lanes share a block and its maximum.  n is the element count;
-// lanes past the end contribute zeros.  Bound by HBM (reads sizeof(x), writes 1 + 1/32 bytes an element): 256x128x128x64 bf16 156 us = 5.2
-// TB/s, the rate of a copy; two or four pieces in flight a thread are slower (173, 179 us).
+// lanes past the end contribute zeros.  Bound by HBM (reads sizeof(x), writes 1 + 1/32 bytes an element): 256x128x128x64 bf16 156 to 169 us =
+// 4.8 to 5.2 TB/s, the rate of a copy; two or four pieces in flight a thread are slower (173, 179 us).
 template <int ST, int V, bool SIGNS>
 __global__ __launch_bounds__(256) void mx8_quant_kernel(const void* __restrict__ x, int8_t* __restrict__ q,
                                                         uint8_t* __restrict__ scales, size_t n, size_t ps) {
@@ -288,7 +288,8 @@ __global__ __launch_bounds__(256) void mx8_quant_norm_kernel(const void* __restr
   }
 }
 
-// Restore: the same bytes the other way, 151 us at the same size (5.4 TB/s).  Small tensors are bound by the launch (27 540 elements: 2.4 us).
+// Restore: the same bytes the other way, 146 us at the same size (5.6 TB/s); half as many elements in fp32 174 (3.9 TB/s).  Small tensors are bound by
+// the launch (27 540 elements: 2.4 us).
 template <int ST, int V>
 __global__ __launch_bounds__(256) void mx8_dequant_kernel(const int8_t* __restrict__ q, const uint8_t* __restrict__ scales,
                                                           void* __restrict__ y, size_t n, size_t ps) {
@@ -342,8 +343,8 @@ __global__ __launch_bounds__(256) void mx8_act_bwd_kernel(const void* __restrict
 // Rows go to the blocks in chunks of 4 * TR, chunk by chunk round the grid: all blocks together sweep the tensor.  (One contiguous
 // run of rows a block puts the blocks a power of two apart and on the same memory channels: 208 us instead of 89 for the reduction
 // over 256x64x64x128 bf16.)
-// Bound by HBM: the statistics need all of dy and the codes before the first dx, so both are read twice - 16.3 + 23.9 us for 128x32x32x128 fp32
-// (5.2 and 6.3 TB/s: the second pass walks backwards and finds part of them cached), 90 + 110 us for 256x64x64x128 bf16.
+// Bound by HBM: the statistics need all of dy and the codes before the first dx, so both are read twice - 16.1 + 24.0 us for 128x32x32x128 fp32
+// (5.2 and 6.3 TB/s: the second pass walks backwards and finds part of them cached), 93 + 111 us for 256x64x64x128 bf16, three planes 189 + 316.
 struct NormGeom {
   int TC, TR, gy, NB;
 };
