@@ -8,7 +8,8 @@
 // m / 127.5); x * 2^-e is exact, which leaves ONE rounding.  The cap keeps 127 * 2^e finite: only above 127.5 * 2^121 =
 // 3.39e38 does an element saturate (off by less than one step).  A block with a NaN or an infinity stores scale byte 255 and reads back
 // as NaN: a diverged run stays non-finite.  What is rounded to zero loses its sign, and with it the mask of a ReLU or LeakyReLU that is read off the
-// checkpoint: IPRGAN_MX8_SIGNS keeps it (mx8_code), at the price of an error below one step instead of half a step for those elements.  Why int8 and a power of two: at 1.03 bytes an element the noise is 43 dB under a
+// checkpoint: IPRGAN_MX8_SIGNS keeps it (mx8_code), at the price of an error below one step instead of half a step for those elements.
+// Why int8 and a power of two: at 1.03 bytes an element the noise is 43 dB under a
 // normally distributed signal (an 8-bit float's 3-bit mantissa: 31 dB), and the scale costs no multiplication error.
 #include "common.h"
 
